@@ -26,6 +26,22 @@ class AttnSeq(C.Structure):
 assert C.sizeof(SeqInfo) == 48 and C.sizeof(AttnSeq) == 40
 
 
+class Kv4Seq(C.Structure):
+    """A sequence over a 4-bit key/value cache (64 bytes)."""
+    _fields_ = [("q_start", i32), ("q_len", i32), ("kv_start", i32), ("kv_len", i32), ("ext_len", i32),
+                ("ext_cap", i32), ("k4", p), ("v4", p), ("kp", p), ("vp", p), ("mass", p)]
+
+
+class Kv4Evict(C.Structure):
+    """A 4-bit cache to thin out (112 bytes)."""
+    _fields_ = [("len", i32), ("cap", i32), ("keep", i32), ("recent", i32), ("dst_cap", i32), ("_pad", i32),
+                ("k4", p), ("v4", p), ("kp", p), ("vp", p), ("mass", p), ("dst_k4", p), ("dst_v4", p), ("dst_kp", p),
+                ("dst_vp", p), ("dst_mass", p), ("kept", p)]
+
+
+assert C.sizeof(Kv4Seq) == 64 and C.sizeof(Kv4Evict) == 112
+
+
 class TrunkLayer(C.Structure):
     _fields_ = [("is_attn", i32), ("in_proj", p), ("out_proj", p), ("convw", p), ("qkv", p), ("out", p),
                 ("qn", p), ("kn", p), ("op_norm", p), ("ffn_norm", p), ("gate_up", p), ("down", p), ("ffn", i32)]
@@ -159,6 +175,12 @@ EXTENSIONS = {
     "d1_conformer_dw_clips": (i32, [p, p, p, p, p, p, p, p, i32, i32, i32, i32, p]),
     "d1_gemm_noalloc": (i32, [i32, i32, i32, p, i32, p, i32, p, i32, i32, p]),
     "d1_gemm_noalloc_error": (i32, []),
+    "d1_kv4_append": (i32, [p, p, i32, p, i32, i32, i32, p]),
+    "d1_kv4_load": (i32, [p, i32, i32, i32, p, p, i32, p]),
+    "d1_flash_attn_kv4": (i32, [p, i32, p, p, i32, p, i32, p, i32, p, i32, i32, i32, i32, i32, f32, i32, i32, p]),
+    "d1_kv4_mass": (i32, [p, i32, p, i32, p, i32, i32, i32, i32, i32, f32, i32, i32, p]),
+    "d1_kv4_evict": (i32, [p, i32, i32, i32, p]),
+    "d1_kv4_error": (i32, []),
     "d1_lt_destroy": (None, [p]),
     "d1_build_id": (C.c_char_p, []),
 }

@@ -329,6 +329,104 @@ int d1_gemm_noalloc(int M, int N, int K, const d1_half* X, int ldx, const d1_hal
  * word could not be read). Waits for the device's outstanding work. */
 int d1_gemm_noalloc_error(void);
 
+/* ------------------------------------------------------------------------ extensions: 4-bit key/value caches */
+
+/* extension, no reference counterpart — key/value caches held in 4 bits (the reference keeps media prefixes in fp16,
+ * src/model.rs:70-104): 34 bytes for each vector of 64 dimensions instead of 128, so that 3.76 times as many prefix
+ * positions fit a media cache and an attention over a long prefix reads 3.76 times fewer bytes.
+ *
+ * A cache of one attention layer and one sequence is four arrays, head after head, ext_cap rows for each kv head:
+ *   k4, v4  codes, uint8 [kv head][ext_cap][32]; element 8w + 2n of a vector is bits 4n .. 4n+3 of its 32-bit word w,
+ *           element 8w + 2n + 1 bits 16+4n .. 19+4n
+ *   kp, vp  parameters, 16 bits [kv head][ext_cap]: the fp16 bits of `step`, whose low 4 bits hold `zero`
+ * A vector x[64] is stored as follows (fp32 arithmetic, round half to even):
+ *   lo = min(0, min x), hi = max(0, max x); step = (hi - lo) / 15, rounded up to 7 significant bits and to a multiple
+ *   of 2^-20, so that its low 4 fp16 bits are zero; zero = round(-lo / step) in 0 .. 15 (step 0: zero 0, codes 0)
+ *   code = round(x / step) + zero in 0 .. 15, moved towards zero where |code - zero| * step would exceed 65504
+ * and stands for (code - zero) * step, which fp16 holds exactly: |x - value| <= step / 2 (step, beside 65504). A vector
+ * with a NaN or an infinity reads as NaN in every element.
+ *
+ * ext_cap must be a multiple of 8 and the four pointers 16-byte aligned; ext_cap = 0 with null pointers is a sequence
+ * without a cache. The tables below are read on the device when the kernel runs. An entry that breaks these rules or
+ * reaches outside the rows that the call names is skipped, its outputs left as they were, and d1_kv4_error() tells.
+ * The launchers keep no state and no workspace: calls on several streams, and captured ones, do not affect each other
+ * as long as what they write does not overlap. */
+typedef struct D1Kv4Seq {
+    int q_start, q_len;    /* query rows */
+    int kv_start, kv_len;  /* the sequence's own fp16 key/value rows */
+    int ext_len, ext_cap;  /* cached keys, which come before the own ones; rows per kv head in the cache's arrays */
+    uint8_t* k4;
+    uint8_t* v4;
+    d1_half* kp;
+    d1_half* vp;
+    float* mass;           /* [kv head][ext_cap], d1_kv4_mass only (NULL: not wanted) */
+} D1Kv4Seq;
+
+/* One cache to thin out (d1_kv4_evict). */
+typedef struct D1Kv4Evict {
+    int len, cap;          /* cached keys; rows per kv head of the source arrays */
+    int keep, recent;      /* keys to keep of each kv head, and how many of them are the last ones whatever their mass */
+    int dst_cap, _pad;     /* rows per kv head of the destination arrays, at least min(keep, len) */
+    const uint8_t* k4;
+    const uint8_t* v4;
+    const d1_half* kp;
+    const d1_half* vp;
+    const float* mass;     /* [kv head][cap] */
+    uint8_t* dst_k4;
+    uint8_t* dst_v4;
+    d1_half* dst_kp;
+    d1_half* dst_vp;
+    float* dst_mass;       /* [kv head][dst_cap], or NULL */
+    int* kept;             /* [kv head][dst_cap]: the kept keys' source indices, or NULL */
+} D1Kv4Evict;
+
+#ifdef __cplusplus
+static_assert(sizeof(D1Kv4Seq) == 64 && offsetof(D1Kv4Seq, k4) == 24, "D1Kv4Seq layout");
+static_assert(sizeof(D1Kv4Evict) == 112 && offsetof(D1Kv4Evict, k4) == 24, "D1Kv4Evict layout");
+#endif
+
+/* extension — stores the own rows of every sequence behind its cached ones: rows kv_start .. kv_start + kv_len - 1 of
+ * K and V (fp16, kv_heads * 64 columns, row pitch ldkv) at cache rows ext_len .. ext_len + kv_len - 1, which must fit
+ * ext_cap. The caller then counts them in ext_len. max_rows: the longest kv_len, by which the grid is chosen (results
+ * do not depend on it). K, V 16-byte aligned, ldkv a multiple of 8. */
+int d1_kv4_append(const d1_half* K, const d1_half* V, int ldkv, const D1Kv4Seq* seqs, int n_seqs, int max_rows,
+                  int kv_heads, cudaStream_t stream);
+
+/* extension — the inverse of d1_kv4_append with the same table: cache rows ext_len .. ext_len + kv_len - 1 of every
+ * sequence as fp16 rows kv_start .. of K and V, the layout in which d1_flash_attn reads a prefix (ext_len = 0 and
+ * kv_len = the cache's length for all of it). */
+int d1_kv4_load(const D1Kv4Seq* seqs, int n_seqs, int max_rows, int kv_heads, d1_half* K, d1_half* V, int ldkv,
+                cudaStream_t stream);
+
+/* extension — d1_flash_attn over 4-bit caches: for every sequence, row q and head h,
+ *   O[q] = softmax(scale * Q[q] K^T) V over the keys [cached | own], kv head h / group, fp32 softmax
+ * and, with lse != NULL, lse[h * lse_ld + row] = ln(sum exp(scale * Q[q] K^T)) in fp32. Rows without any key get O = 0
+ * and lse = -inf. Bidirectional, as d1_flash_attn. max_q, max_keys: the longest q_len and the longest ext_len + kv_len,
+ * by which the kernel and the split over the keys are chosen (results differ only by rounding; lengths beyond them are
+ * computed all the same). q_rows / kv_rows: rows of Q and O (lse: q_rows <= lse_ld) and of K and V. Q, K, V, O 16-byte
+ * aligned, leading dimensions multiples of 8; K and V may be NULL with kv_rows = 0. scale > 0. */
+int d1_flash_attn_kv4(const d1_half* Q, int ldq, const d1_half* K, const d1_half* V, int ldkv, d1_half* O, int ldo,
+                      float* lse, int lse_ld, const D1Kv4Seq* seqs, int n_seqs, int max_q, int max_keys, int heads,
+                      int group, float scale, int q_rows, int kv_rows, cudaStream_t stream);
+
+/* extension — the attention weight that every cached key received: for every kv head g and key k of a sequence's cache
+ *   mass[g][k] (+)= sum over its rows q and the heads h of g of exp(scale * Q[q] . K[k] - lse[h][q])
+ * with lse as d1_flash_attn_kv4 gave it (-inf: the row adds nothing). accumulate = 0 overwrites mass[g][0 .. ext_len-1],
+ * 1 adds to it. Sequences with the same `mass` must share their cache; their weights are added up in the table's order,
+ * always in the same order for the same call. max_q, max_len: the longest q_len and ext_len (see above). */
+int d1_kv4_mass(const d1_half* Q, int ldq, const float* lse, int lse_ld, const D1Kv4Seq* seqs, int n_seqs, int max_q,
+                int max_len, int heads, int group, float scale, int accumulate, int q_rows, cudaStream_t stream);
+
+/* extension — eviction by accumulated attention weight: of each kv head, the last min(recent, keep) keys and those of
+ * the others with the largest mass (equal ones: the lowest index; NaN counts as -inf), min(keep, len) in all, move in
+ * their order to the destination's rows 0 .. , with their codes, parameters, mass and source indices; rows behind them
+ * are left as they were. Source and destination must not overlap. max_len: the longest len (see above). */
+int d1_kv4_evict(const D1Kv4Evict* items, int n_items, int max_len, int kv_heads, cudaStream_t stream);
+
+/* extension — reads and clears the error word of the d1_kv4_* and d1_flash_attn_kv4 kernels on the current device
+ * (nonzero: a table entry was refused and skipped, or a kernel gave up on a bounded wait). Waits for the device. */
+int d1_kv4_error(void);
+
 /* extension — releases a context made by d1_lt_init (the reference never frees it). */
 void d1_lt_destroy(void* ctx);
 
