@@ -1,5 +1,6 @@
 // Attention over key/value caches held in 4 bits (format: include/d1kernels.h, D1Kv4Seq), and the attention weight that
 // every cached key received. Head dim 64, packed variable-length sequences, bidirectional.
+#include "attn_tc.cuh"
 #include "kv4.cuh"
 #include "warp_mma.cuh"
 
@@ -17,14 +18,47 @@ struct Kv4Args {
     float* lse;
     const D1Kv4Seq* seqs;
     int* err;
-    int ldq, ldkv, ldo, lse_ld, n_seqs, group, q_rows, kv_rows, accumulate;
+    int ldq, ldkv, ldo, lse_ld, n_seqs, heads, group, q_rows, kv_rows, accumulate;
+    int n_blocks;  // tcgen05 form: blocks of rows per sequence, by max_q
     float scale_log2;
 };
 
-__device__ __forceinline__ float ex2f(float x) {
-    float y;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
+__device__ __forceinline__ float fmax_nan(float a, float b) {  // NaN if either is
+    float d;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
+    return d;
+}
+__device__ __forceinline__ uint64_t f2_mul(uint64_t a, uint64_t b) {
+    uint64_t d;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+    return d;
+}
+
+// 2^x of two numbers without the SFU: x = n + f, n whole by adding and taking away 1.5 * 2^23 (the sum's low bits, with
+// 127 added, are 2^n's exponent), |f| <= 1/2, 2^f by a polynomial fitted here for the smallest relative error: 7.5e-5 of
+// degree 3 (below P's rounding to fp16), 2.1e-7 of degree 5 evaluated in fp32. x below -126 counts as -126; NaN stays.
+template <int DEG>
+__device__ __forceinline__ void ex2_fma2(float x0, float x1, float& p0, float& p1) {
+    static_assert(DEG == 3 || DEG == 5, "fitted degrees");
+    const uint64_t x = f2_pack(fmax_nan(x0, -126.f), fmax_nan(x1, -126.f));
+    const uint64_t t = f2_add(x, f2_pack(12583039.f, 12583039.f));
+    const uint64_t f = f2_fma(f2_add(t, f2_pack(-12583039.f, -12583039.f)), f2_pack(-1.f, -1.f), x);
+    auto c2 = [](float c) { return f2_pack(c, c); };
+    uint64_t q;
+    if (DEG == 3) {
+        q = f2_fma(c2(0.0551716685f), f, c2(0.242611125f));
+        q = f2_fma(q, f, c2(0.693260968f));
+        q = f2_fma(q, f, c2(0.999928057f));
+    } else {
+        q = f2_fma(c2(0.00132764725f), f, c2(0.00967554096f));
+        q = f2_fma(q, f, c2(0.0555071309f));
+        q = f2_fma(q, f, c2(0.240221202f));
+        q = f2_fma(q, f, c2(0.693146944f));
+        q = f2_fma(q, f, c2(1.00000012f));
+    }
+    float t0, t1;
+    f2_unpack(t, t0, t1);
+    f2_unpack(f2_mul(q, f2_pack(__uint_as_float(__float_as_uint(t0) << 23), __uint_as_float(__float_as_uint(t1) << 23))), p0, p1);
 }
 
 // ------------------------------------------------------------------------------------------------ attention, few rows
@@ -189,12 +223,12 @@ __global__ void __launch_bounds__(R_WARPS * 32) k_kv4_attn_rows(const Kv4Args a)
                         mx = fmaxf(mx, __shfl_xor_sync(D1_FULL_MASK, mx, 1));
                         mx = fmaxf(mx, __shfl_xor_sync(D1_FULL_MASK, mx, 2));
                         const float mn = fmaxf(m[mt][hf], mx);
-                        const float alpha = m[mt][hf] == mn ? 1.f : ex2f(m[mt][hf] - mn);
+                        const float alpha = m[mt][hf] == mn ? 1.f : ex2(m[mt][hf] - mn);
                         m[mt][hf] = mn;
                         float sum = 0.f;
 #pragma unroll
                         for (int n = 0; n < 8; n++) {
-                            const float p0 = ex2f(sc[mt][n][2 * hf] - mn), p1 = ex2f(sc[mt][n][2 * hf + 1] - mn);
+                            const float p0 = ex2(sc[mt][n][2 * hf] - mn), p1 = ex2(sc[mt][n][2 * hf + 1] - mn);
                             sum += p0 + p1;
                             pa[mt][n][hf] = pack_h2(p0, p1);
                         }
@@ -278,7 +312,7 @@ __global__ void __launch_bounds__(R_WARPS * 32) k_kv4_attn_rows(const Kv4Args a)
                 for (int w = 0; w < R_WARPS; w++) M = fmaxf(M, sM[w * NR + row]);
                 float L = 0.f, x0 = 0.f, x1 = 0.f, x2 = 0.f, x3 = 0.f;
                 for (int w = 0; w < R_WARPS && w < tiles; w++) {  // warps beyond the tiles hold nothing
-                    const float f = ex2f(sM[w * NR + row] - M);
+                    const float f = ex2(sM[w * NR + row] - M);
                     const float4 v = *reinterpret_cast<const float4*>(sO + (w * NR + row) * R_OLD + d);
                     L += f * sL[w * NR + row];
                     x0 += f * v.x;
@@ -294,6 +328,507 @@ __global__ void __launch_bounds__(R_WARPS * 32) k_kv4_attn_rows(const Kv4Args a)
             }
             __syncthreads();
         }
+    }
+}
+
+// ------------------------------------------------------------------------------------------------ attention, many rows
+// tcgen05 form. Persistent CTAs (one per SM) loop over units of two 128-row query tiles that share their keys: the same
+// rows of two heads of one kv head where the group is even (a sequence of 24 rows then fills both tiles), two successive
+// blocks of rows of one head where it is odd. Keys come in tiles of 128, first the cached ones, then the own ones; the
+// last tile of either kind is filled up with zeros and masked.
+// Warps:
+//   0-3, 4-7   softmax of tiles 0 and 1: thread = query row = TMEM lane. S is copied to registers and released at once,
+//              P goes to TMEM as fp16, O is rescaled only when a row's maximum grows by more than 2^8
+//   8, 10, 11  loaders. A cached tile: every thread fetches 16-byte pieces of codes and their parameters into registers
+//              while the tile before it is stored, then expands them to fp16 (exact) into the swizzled layout that the
+//              MMAs read. Own rows: whole tiles by TMA, partial ones through registers.
+//   9          TMEM, and the MMAs from one thread: S = Q K^T (both in shared memory), O += P V (P in TMEM)
+// TMEM (512 columns), tile w at 256 w: S in 128 columns, P in 64, O in 64.
+constexpr int TQ = 128, TKV = 128, T_QSLOTS = 2, T_STAGES = 4, T_LOADERS = 3, T_THREADS = 384;
+constexpr int T_QT_BYTES = TQ * 128, T_KV_BYTES = TKV * 128, T_O_BYTES = TQ * 128;
+constexpr uint32_t T_TMEM_COLS = 512, T_WG_COLS = 256, T_P_COL = TKV, T_O_COL = TKV + TKV / 2;
+constexpr float kLazyRescale = 8.f;
+enum : int {
+    B_QFULL = 0,
+    B_QEMPTY = B_QFULL + T_QSLOTS,
+    B_KVFULL = B_QEMPTY + T_QSLOTS,
+    B_KVEMPTY = B_KVFULL + T_STAGES,
+    B_SFULL = B_KVEMPTY + T_STAGES,  // [w]: S of the tile's next keys is in TMEM
+    B_SFREE = B_SFULL + 2,           // [w]: it is in registers (4 warps)
+    B_PFULL = B_SFREE + 2,           // [w]: P is in TMEM (4 warps)
+    B_ODONE = B_PFULL + 2,           // [w]: P V has completed
+    B_OFREE = B_ODONE + 2,           // [w]: O has been read (4 warps)
+    B_OSTAGED = B_OFREE + 2,         // [w]: the output tile is in shared memory (4 warps)
+    B_OREAD = B_OSTAGED + 2,         // [w]: its last bulk store has read it
+    B_DRAIN = B_OREAD + 2,
+    T_NBARS = B_DRAIN + 1
+};
+constexpr int T_SMEM = T_QSLOTS * 2 * T_QT_BYTES + T_STAGES * 2 * T_KV_BYTES + 2 * T_O_BYTES + T_NBARS * 8 + 16;
+static_assert(T_SMEM <= 232448 && T_O_COL + 64 <= T_WG_COLS, "shared memory and TMEM of the tcgen05 attention");
+
+// The units of a CTA, walked alike by every role: u -> (sequence, block of rows, head or pair of heads), heads fastest.
+// A sequence longer than max_q comes round again with its later blocks.
+struct Walk {
+    D1Kv4Seq s;
+    int u, nb, hu, block, h, n_units;
+    bool pair, at_unit;
+
+    __device__ Walk(const Kv4Args& a) : u(blockIdx.x), nb(a.n_blocks), block(0), h(0), at_unit(false) {
+        pair = a.group % 2 == 0;
+        hu = pair ? a.heads / 2 : a.heads;
+        n_units = a.n_seqs * nb * hu;
+    }
+    __device__ int rows_per_block() const { return pair ? TQ : 2 * TQ; }
+    __device__ bool next(const Kv4Args& a) {
+        while (true) {
+            if (at_unit) {
+                block += nb;
+            } else {
+                if (u >= n_units) return false;
+                const int sq = u / (nb * hu), rest = u % (nb * hu);
+                block = rest / hu;
+                h = rest % hu * (pair ? 2 : 1);
+                s = a.seqs[sq];
+                at_unit = true;
+                if (!kv4_seq_ok(s) || !rows_ok(s.q_start, s.q_len, a.q_rows) || !rows_ok(s.kv_start, s.kv_len, a.kv_rows)) {
+                    if ((threadIdx.x & 31) == 0) atomicExch(a.err, kErrTable);
+                    s.q_len = 0;
+                }
+            }
+            if ((long long)block * rows_per_block() < s.q_len) return true;
+            u += gridDim.x;
+            at_unit = false;
+        }
+    }
+    __device__ int ext_tiles() const { return (s.ext_len + TKV - 1) / TKV; }
+    __device__ int tiles() const { return ext_tiles() + (s.kv_len + TKV - 1) / TKV; }
+    __device__ int valid(int j) const {  // keys of tile j, at least 1; 128 or more: all
+        const int e = ext_tiles();
+        return j < e ? s.ext_len - j * TKV : s.kv_len - (j - e) * TKV;
+    }
+    __device__ int row0(int w) const { return block * rows_per_block() + (pair ? 0 : w * TQ); }  // of the sequence
+    __device__ int head(int w) const { return h + (pair ? w : 0); }
+    __device__ int tiles_of_rows() const { return pair || s.q_len > row0(1) ? 2 : 1; }
+};
+
+// The pieces of a cached tile that one loader thread moves: 16 bytes (32 codes) each, K in pieces 0-255, V in 256-511.
+constexpr int T_PIECES = (4 * TKV + 32 * T_LOADERS - 1) / (32 * T_LOADERS);
+
+__global__ void __launch_bounds__(T_THREADS, 1)
+    k_kv4_attn_tc(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
+                  const __grid_constant__ CUtensorMap tmV, const __grid_constant__ CUtensorMap tmO, const Kv4Args a) {
+    constexpr uint32_t IDESC_S = idesc_f16_f32(TQ, TKV);
+    constexpr uint32_t IDESC_O = idesc_f16_f32(TQ, 64) | (1u << 16);  // B (= V) MN-major
+    extern __shared__ __align__(1024) uint8_t t_smem[];
+    uint8_t* sQ = t_smem;                                   // slot q: tile 0 at q * 2 * T_QT_BYTES, tile 1 behind it
+    uint8_t* sKV = sQ + T_QSLOTS * 2 * T_QT_BYTES;          // stage s: K at s * 2 * T_KV_BYTES, V behind it
+    uint8_t* sO = sKV + T_STAGES * 2 * T_KV_BYTES;          // output tile of w at w * T_O_BYTES
+    uint64_t* bars = reinterpret_cast<uint64_t*>(sO + 2 * T_O_BYTES);
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + T_NBARS);
+    volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+    auto bar = [&](int i) { return smem_u32(bars + i); };
+    if (smem_u32(t_smem) & 1023) {  // never expected: dynamic shared memory starts at the window's base
+        pdl_wait();
+        if (threadIdx.x == 0) atomicExch(a.err, kErrDrain);
+        return;
+    }
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < T_QSLOTS; i++) {
+            mbar_init(bar(B_QFULL + i), 1);
+            mbar_init(bar(B_QEMPTY + i), 1);
+        }
+        for (int i = 0; i < T_STAGES; i++) {
+            mbar_init(bar(B_KVFULL + i), 32 * T_LOADERS);
+            mbar_init(bar(B_KVEMPTY + i), 1);
+        }
+        for (int w = 0; w < 2; w++) {
+            mbar_init(bar(B_SFULL + w), 1);
+            mbar_init(bar(B_SFREE + w), 4);
+            mbar_init(bar(B_PFULL + w), 4);
+            mbar_init(bar(B_ODONE + w), 1);
+            mbar_init(bar(B_OFREE + w), 4);
+            mbar_init(bar(B_OSTAGED + w), 4);
+            mbar_init(bar(B_OREAD + w), 1);
+        }
+        mbar_init(bar(B_DRAIN), 1);
+        *abort_flag = 0;
+        fence_mbar_init();
+    }
+    if (warp == 9) {
+        tmem_alloc(smem_u32(tmem_slot), T_TMEM_COLS);
+        tmem_relinquish();
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = *tmem_slot;
+    pdl_entry();  // barriers and TMEM are set up; global memory is touched only after this
+    Walk un(a);
+
+    if (warp == 8 || warp >= 10) {
+        // ------------------------------------------------------------------ loaders
+        const int lt = (warp == 8 ? 0 : warp - 9) * 32 + lane;
+        const bool issuer = warp == 8 && lane == 0;
+        int qi = 0, ki = 0;
+        bool ok = true;
+        while (ok && un.next(a)) {
+            const int g = un.h / a.group, nt = un.tiles(), e_tiles = un.ext_tiles();
+            if (nt == 0) continue;
+            const D1Kv4Seq& s = un.s;
+            const uint8_t* k4 = s.k4 + (size_t)g * s.ext_cap * 32;
+            const uint8_t* v4 = s.v4 + (size_t)g * s.ext_cap * 32;
+            const uint16_t* kp = reinterpret_cast<const uint16_t*>(s.kp) + (size_t)g * s.ext_cap;
+            const uint16_t* vp = reinterpret_cast<const uint16_t*>(s.vp) + (size_t)g * s.ext_cap;
+            uint4 piece[T_PIECES];
+            uint32_t par[T_PIECES];
+            auto fetch = [&](int j) {
+                const int n = un.valid(j);
+#pragma unroll
+                for (int i = 0; i < T_PIECES; i++) {
+                    const int c = lt + i * 32 * T_LOADERS, r = (c & 255) >> 1;
+                    piece[i] = make_uint4(0, 0, 0, 0);
+                    par[i] = 0;  // step 0: zeros
+                    if (c < 4 * TKV && r < n) {
+                        const size_t key = (size_t)j * TKV + r;
+                        piece[i] = __ldg(reinterpret_cast<const uint4*>((c < 256 ? k4 : v4) + key * 32) + (c & 1));
+                        par[i] = __ldg((c < 256 ? kp : vp) + key);
+                    }
+                }
+            };
+            if (e_tiles > 0) fetch(0);
+            const int qs = qi % T_QSLOTS;
+            if (warp == 8) {
+                if (!(ok = __all_sync(D1_FULL_MASK, mbar_wait(bar(B_QEMPTY + qs), ((qi / T_QSLOTS) & 1) ^ 1, abort_flag))))
+                    break;
+                // a whole tile inside the sequence comes by TMA; one that the sequence ends in row by row, with zeros
+                // behind the end, so that no load reads a row outside a sequence
+                const uint32_t dq = smem_u32(sQ + qs * 2 * T_QT_BYTES);
+                const int nq = un.tiles_of_rows();
+                bool partial = false;
+                for (int w = 0; w < nq; w++) {
+                    const int rows = s.q_len - un.row0(w);
+                    if (rows >= TQ) continue;
+                    partial = true;
+                    for (int c = lane; c < TQ * 8; c += 32) {
+                        const int r = c >> 3, ch = c & 7;
+                        const __half* src = r < rows ? a.Q + (size_t)(s.q_start + un.row0(w) + r) * a.ldq + un.head(w) * 64 + ch * 8
+                                                     : a.Q;
+                        cp_async16z(dq + w * T_QT_BYTES + r * 128 + ((ch ^ (r & 7)) << 4), src, r < rows ? 16 : 0);
+                    }
+                }
+                if (partial) {
+                    asm volatile("cp.async.wait_all;" ::: "memory");
+                    fence_async_smem_cta();
+                    __syncwarp();
+                }
+                if (issuer) {
+                    uint32_t bytes = 0;
+                    for (int w = 0; w < nq; w++)
+                        if (s.q_len - un.row0(w) >= TQ) bytes += T_QT_BYTES;
+                    mbar_arrive_expect_tx(bar(B_QFULL + qs), bytes);
+                    for (int w = 0; w < nq; w++)
+                        if (s.q_len - un.row0(w) >= TQ)
+                            tma_load_2d(dq + w * T_QT_BYTES, &tmQ, un.head(w) * 64, s.q_start + un.row0(w), bar(B_QFULL + qs));
+                }
+            }
+            qi++;
+            for (int j = 0; j < nt; j++) {
+                const int st = ki % T_STAGES;
+                if (!(ok = __all_sync(D1_FULL_MASK, mbar_wait(bar(B_KVEMPTY + st), ((ki / T_STAGES) & 1) ^ 1, abort_flag))))
+                    break;
+                uint8_t* dK = sKV + st * 2 * T_KV_BYTES;
+                const int n = un.valid(j);
+                if (j < e_tiles) {
+#pragma unroll
+                    for (int i = 0; i < T_PIECES; i++) {
+                        const int c = lt + i * 32 * T_LOADERS, r = (c & 255) >> 1;
+                        if (c < 4 * TKV) {
+                            uint8_t* row = dK + (c >> 8) * T_KV_BYTES + r * 128;
+                            const uint32_t p2 = par[i] * 0x00010001u, step = kv4_step2(p2);
+                            uint32_t z0, z1;
+                            kv4_zero(p2, z0, z1);
+                            const uint32_t word[4] = {piece[i].x, piece[i].y, piece[i].z, piece[i].w};
+#pragma unroll
+                            for (int q = 0; q < 4; q++) {
+                                uint32_t v[4];
+                                kv4_expand(word[q], z0, z1, v);
+                                *reinterpret_cast<uint4*>(row + ((((c & 1) * 4 + q) ^ (r & 7)) << 4)) =
+                                    make_uint4(h2_mul(v[0], step), h2_mul(v[1], step), h2_mul(v[2], step), h2_mul(v[3], step));
+                            }
+                        }
+                    }
+                    if (j + 1 < e_tiles) fetch(j + 1);
+                    fence_async_smem_cta();
+                    mbar_arrive(bar(B_KVFULL + st));
+                } else {
+                    const int row0 = s.kv_start + (j - e_tiles) * TKV;
+                    if (n >= TKV) {
+                        if (issuer) {
+                            mbar_arrive_expect_tx(bar(B_KVFULL + st), 2 * T_KV_BYTES);
+                            tma_load_2d(smem_u32(dK), &tmK, g * 64, row0, bar(B_KVFULL + st));
+                            tma_load_2d(smem_u32(dK + T_KV_BYTES), &tmV, g * 64, row0, bar(B_KVFULL + st));
+                        } else {
+                            mbar_arrive(bar(B_KVFULL + st));
+                        }
+                    } else {
+                        for (int c = lt; c < TKV * 8; c += 32 * T_LOADERS) {
+                            const int r = c >> 3, ch = c & 7;
+                            uint4 kx = make_uint4(0, 0, 0, 0), vx = kx;
+                            if (r < n) {
+                                const size_t at = (size_t)(row0 + r) * a.ldkv + g * 64 + ch * 8;
+                                kx = __ldg(reinterpret_cast<const uint4*>(a.K + at));
+                                vx = __ldg(reinterpret_cast<const uint4*>(a.V + at));
+                            }
+                            uint8_t* to = dK + r * 128 + ((ch ^ (r & 7)) << 4);
+                            *reinterpret_cast<uint4*>(to) = kx;
+                            *reinterpret_cast<uint4*>(to + T_KV_BYTES) = vx;
+                        }
+                        fence_async_smem_cta();
+                        mbar_arrive(bar(B_KVFULL + st));
+                    }
+                }
+                ki++;
+            }
+        }
+        asm volatile("cp.async.wait_all;" ::: "memory");  // nothing in flight when the CTA exits
+        if (!ok && lane == 0) record_err(a.err, abort_flag, kErrWaitEmpty);
+        if (issuer) {
+            // TMA copies still in flight (only after an abort) land before the CTA exits
+            for (int i = ki > T_STAGES ? ki - T_STAGES : 0; i < ki; i++)
+                if (!mbar_wait_timed2(bar(B_KVFULL + i % T_STAGES), (i / T_STAGES) & 1)) break;
+            for (int i = qi > T_QSLOTS ? qi - T_QSLOTS : 0; i < qi; i++)
+                if (!mbar_wait_timed2(bar(B_QFULL + i % T_QSLOTS), (i / T_QSLOTS) & 1)) break;
+        }
+    } else if (warp == 9) {
+        // ------------------------------------------------------------------ MMA issuer
+        if (lane == 0) {
+            int cnt[2] = {0, 0}, units[2] = {0, 0};  // key tiles and units of each query tile so far
+            int qi = 0, ki = 0;
+            bool ok = true;
+            while (ok && un.next(a)) {
+                const int nt = un.tiles(), nw = un.tiles_of_rows();
+                if (nt == 0) continue;
+                const int qs = qi % T_QSLOTS;
+                if (!(ok = mbar_wait(bar(B_QFULL + qs), (qi / T_QSLOTS) & 1, abort_flag))) break;
+                tc_fence_after();
+                const uint32_t q_addr = smem_u32(sQ + qs * 2 * T_QT_BYTES);
+                auto k_addr = [&](int j) { return smem_u32(sKV + ((ki + j) % T_STAGES) * 2 * T_KV_BYTES); };
+                auto kv_ready = [&](int j) {
+                    return mbar_wait(bar(B_KVFULL + (ki + j) % T_STAGES), ((ki + j) / T_STAGES) & 1, abort_flag);
+                };
+                auto issue_s = [&](int w, int j) -> bool {
+                    const int c = cnt[w] + j;
+                    if (c > 0 && !mbar_wait(bar(B_SFREE + w), (c - 1) & 1, abort_flag)) return false;
+                    tc_fence_after();
+                    const uint32_t ka = k_addr(j);
+#pragma unroll
+                    for (int k = 0; k < 4; k++)
+                        tc_mma_f16(tmem + w * T_WG_COLS, smem_desc_k128(q_addr + w * T_QT_BYTES + k * 32),
+                                   smem_desc_k128(ka + k * 32), IDESC_S, k != 0);
+                    tc_commit(bar(B_SFULL + w));
+                    return true;
+                };
+                if (!(ok = kv_ready(0))) break;
+                for (int w = 0; w < nw && ok; w++) ok = issue_s(w, 0);
+                for (int j = 0; j < nt && ok; j++) {
+                    if (j + 1 < nt) {  // S(j + 1) computes while the softmax works on tile j
+                        if (!(ok = kv_ready(j + 1))) break;
+                        for (int w = 0; w < nw && ok; w++) ok = issue_s(w, j + 1);
+                        if (!ok) break;
+                    }
+                    const uint32_t v_addr = k_addr(j) + T_KV_BYTES;
+                    for (int w = 0; w < nw && ok; w++) {
+                        const int c = cnt[w] + j;
+                        ok = mbar_wait(bar(B_PFULL + w), c & 1, abort_flag);
+                        // the first P V of a unit overwrites O: the unit before must have been read
+                        if (ok && j == 0 && units[w] > 0) ok = mbar_wait(bar(B_OFREE + w), (units[w] - 1) & 1, abort_flag);
+                        if (!ok) break;
+                        tc_fence_after();
+#pragma unroll
+                        for (int k = 0; k < TKV / 16; k++)
+                            tc_mma_f16_ts(tmem + w * T_WG_COLS + T_O_COL, tmem + w * T_WG_COLS + T_P_COL + k * 8,
+                                          smem_desc_k128(v_addr + k * 2048), IDESC_O, (j | k) != 0);
+                        tc_commit(bar(B_ODONE + w));
+                    }
+                    if (!ok) break;
+                    tc_commit(bar(B_KVEMPTY + (ki + j) % T_STAGES));
+                }
+                if (!ok) break;
+                tc_commit(bar(B_QEMPTY + qs));
+                ki += nt;
+                qi++;
+                for (int w = 0; w < nw; w++) {
+                    cnt[w] += nt;
+                    units[w]++;
+                }
+            }
+            if (!ok) record_err(a.err, abort_flag, kErrWaitFull);
+            tc_commit(bar(B_DRAIN));  // every issued MMA has completed before TMEM is released
+            if (!mbar_wait_timed2(bar(B_DRAIN), 0)) record_err(a.err, abort_flag, kErrDrain);
+        }
+        __syncwarp();
+    } else {
+        // ------------------------------------------------------------------ softmax
+        const int w = warp >> 2, row = (warp & 3) * 32 + lane;
+        const uint32_t lane_off = (uint32_t)((warp & 3) * 32) << 16;
+        const uint32_t tS = tmem + w * T_WG_COLS + lane_off, tP = tS + T_P_COL, tO = tS + T_O_COL;
+        uint8_t* stile = sO + w * T_O_BYTES;
+        int cnt = 0, nst = 0;  // key tiles so far; output tiles staged so far
+        bool ok = true;
+        while (ok && un.next(a)) {
+            if (w == 1 && un.tiles_of_rows() == 1) continue;
+            const int nt = un.tiles(), q0 = un.row0(w), q = q0 + row, h = un.head(w);
+            const size_t grow = (size_t)(un.s.q_start + q);
+            if (nt == 0) {  // no keys: zeros
+                if (q < un.s.q_len) {
+                    for (int i = 0; i < 8; i++)
+                        *reinterpret_cast<uint4*>(a.O + grow * a.ldo + h * 64 + i * 8) = make_uint4(0, 0, 0, 0);
+                    if (a.lse) a.lse[(size_t)h * a.lse_ld + grow] = -INFINITY;
+                }
+                continue;
+            }
+            float m = -INFINITY, l = 0.f;
+            for (int j = 0; j < nt; j++) {
+                const int c = cnt + j;
+                if (!(ok = __all_sync(D1_FULL_MASK, mbar_wait(bar(B_SFULL + w), c & 1, abort_flag)))) break;
+                tc_fence_after();
+                uint32_t sr[TKV];
+#pragma unroll
+                for (int c32 = 0; c32 < TKV / 32; c32++)
+                    tmem_ld32(tS + c32 * 32, *reinterpret_cast<uint32_t(*)[32]>(sr + c32 * 32));
+                tc_wait_ld();
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(bar(B_SFREE + w));
+                const int n = un.valid(j);
+                if (n < TKV) {
+#pragma unroll
+                    for (int i = 0; i < TKV; i++)
+                        if (i >= n) sr[i] = __float_as_uint(-INFINITY);
+                }
+                // maximum of the raw scores (the scale is positive) in eight chains, scaled once
+                float mx8[8];
+#pragma unroll
+                for (int e = 0; e < 8; e++) mx8[e] = fmaxf(__uint_as_float(sr[2 * e]), __uint_as_float(sr[2 * e + 1]));
+#pragma unroll
+                for (int i = 16; i < TKV; i += 16) {
+#pragma unroll
+                    for (int e = 0; e < 8; e++)
+                        mx8[e] = fmax3(mx8[e], __uint_as_float(sr[i + 2 * e]), __uint_as_float(sr[i + 2 * e + 1]));
+                }
+                const float mx = fmaxf(fmax3(mx8[0], mx8[1], mx8[2]), fmax3(mx8[3], mx8[4], fmax3(mx8[5], mx8[6], mx8[7]))) *
+                                 a.scale_log2;
+                float m_use = m, alpha = 1.f;
+                if (j == 0) {
+                    m_use = mx;
+                } else if (mx > m + kLazyRescale) {
+                    m_use = mx;
+                    alpha = ex2(m - mx);
+                }
+                if (j > 0 && __any_sync(D1_FULL_MASK, alpha < 1.f)) {  // rare: O must hold P V up to the tile before
+                    if (!(ok = __all_sync(D1_FULL_MASK, mbar_wait(bar(B_ODONE + w), (c - 1) & 1, abort_flag)))) break;
+                    tc_fence_after();
+#pragma unroll 1
+                    for (int o8 = 0; o8 < 8; o8++) {
+                        uint32_t o[8];
+                        tmem_ld8(tO + o8 * 8, o);
+                        tc_wait_ld();
+#pragma unroll
+                        for (int i = 0; i < 8; i++) o[i] = __float_as_uint(__uint_as_float(o[i]) * alpha);
+                        tmem_st8(tO + o8 * 8, o);
+                    }
+                }
+                // P = 2^(s * scale - m), two scores at a time, an eighth of them on the FMA pipe; the row's sum in fp32
+                const uint64_t sc2 = f2_pack(a.scale_log2, a.scale_log2), nm2 = f2_pack(-m_use, -m_use);
+                uint64_t rs2[4];
+#pragma unroll
+                for (int e = 0; e < 4; e++) rs2[e] = f2_pack(0.f, 0.f);
+                uint32_t pr[TKV / 2];
+#pragma unroll
+                for (int i = 0; i < TKV / 2; i++) {
+                    float x0, x1, p0, p1;
+                    f2_unpack(f2_fma(f2_pack(__uint_as_float(sr[2 * i]), __uint_as_float(sr[2 * i + 1])), sc2, nm2), x0, x1);
+                    if (i % 8 == 7) {
+                        ex2_fma2<3>(x0, x1, p0, p1);
+                    } else {
+                        p0 = ex2(x0);
+                        p1 = ex2(x1);
+                    }
+                    rs2[i & 3] = f2_add(rs2[i & 3], f2_pack(p0, p1));
+                    pr[i] = pack_h2(p0, p1);
+                }
+                if (c > 0) {  // P V of the tile before has read the P columns
+                    if (!(ok = __all_sync(D1_FULL_MASK, mbar_wait(bar(B_ODONE + w), (c - 1) & 1, abort_flag)))) break;
+                    tc_fence_after();
+                }
+#pragma unroll
+                for (int c32 = 0; c32 < TKV / 64; c32++)
+                    tmem_st32(tP + c32 * 32, *reinterpret_cast<uint32_t(*)[32]>(pr + c32 * 32));
+                tc_wait_st();
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(bar(B_PFULL + w));
+                float rs[8];
+#pragma unroll
+                for (int e = 0; e < 4; e++) f2_unpack(rs2[e], rs[2 * e], rs[2 * e + 1]);
+                l = l * alpha + (((rs[0] + rs[1]) + (rs[2] + rs[3])) + ((rs[4] + rs[5]) + (rs[6] + rs[7])));
+                m = m_use;
+            }
+            if (!ok) break;
+            cnt += nt;
+            if (!(ok = __all_sync(D1_FULL_MASK, mbar_wait(bar(B_ODONE + w), (cnt - 1) & 1, abort_flag)))) break;
+            tc_fence_after();
+            const float il = 1.f / l;
+            uint32_t o[64];
+            tmem_ld32(tO, *reinterpret_cast<uint32_t(*)[32]>(o));
+            tmem_ld32(tO + 32, *reinterpret_cast<uint32_t(*)[32]>(o + 32));
+            tc_wait_ld();
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(bar(B_OFREE + w));
+            uint32_t oh[32];
+#pragma unroll
+            for (int i = 0; i < 32; i++) oh[i] = pack_h2(__uint_as_float(o[2 * i]) * il, __uint_as_float(o[2 * i + 1]) * il);
+            if (a.lse && q < un.s.q_len) a.lse[(size_t)h * a.lse_ld + grow] = (m + log2f(l)) * kLn2;
+            if (q0 + TQ <= un.s.q_len) {
+                // a whole tile: staged, then one bulk store; the store before must have read the buffer
+                if (nst > 0) {
+                    if (row == 0) {
+                        o_store_read_done();
+                        mbar_arrive(bar(B_OREAD + w));
+                    }
+                    if (!(ok = __all_sync(D1_FULL_MASK, mbar_wait(bar(B_OREAD + w), (nst - 1) & 1, abort_flag)))) break;
+                }
+#pragma unroll
+                for (int i = 0; i < 8; i++)
+                    *reinterpret_cast<uint4*>(stile + row * 128 + ((i ^ (row & 7)) << 4)) =
+                        make_uint4(oh[4 * i], oh[4 * i + 1], oh[4 * i + 2], oh[4 * i + 3]);
+                fence_async_smem_cta();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(bar(B_OSTAGED + w));
+                bool staged = true;
+                if (row == 0) {
+                    staged = mbar_wait(bar(B_OSTAGED + w), nst & 1, abort_flag);
+                    if (staged) o_tile_store(&tmO, smem_u32(stile), h * 64, un.s.q_start + q0);
+                }
+                nst++;
+                if (!(ok = __all_sync(D1_FULL_MASK, staged))) break;
+            } else if (q < un.s.q_len) {
+#pragma unroll
+                for (int i = 0; i < 8; i++)
+                    *reinterpret_cast<uint4*>(a.O + grow * a.ldo + h * 64 + i * 8) =
+                        make_uint4(oh[4 * i], oh[4 * i + 1], oh[4 * i + 2], oh[4 * i + 3]);
+            }
+        }
+        if (row == 0) o_store_done();  // no store still reads this CTA's shared memory when it exits
+        if (!ok && lane == 0) record_err(a.err, abort_flag, kErrWaitAccFull);
+    }
+    tc_fence_before();
+    __syncthreads();
+    if (warp == 9) {
+        tc_fence_after();
+        tmem_dealloc(tmem, T_TMEM_COLS);
     }
 }
 
@@ -390,8 +925,8 @@ __global__ void __launch_bounds__(256) k_kv4_mass_rows(const Kv4Args a) {
                             mma16816(c, ka[mt][1], x0.z, x0.w);
                             mma16816(c, ka[mt][2], x1.x, x1.y);
                             mma16816(c, ka[mt][3], x1.z, x1.w);
-                            sum[mt][0] += ex2f(c[0] * st[mt][0] - l0) + ex2f(c[1] * st[mt][0] - l1);
-                            sum[mt][1] += ex2f(c[2] * st[mt][1] - l0) + ex2f(c[3] * st[mt][1] - l1);
+                            sum[mt][0] += ex2(c[0] * st[mt][0] - l0) + ex2(c[1] * st[mt][0] - l1);
+                            sum[mt][1] += ex2(c[2] * st[mt][1] - l0) + ex2(c[3] * st[mt][1] - l1);
                         }
                     }
                 }
@@ -434,6 +969,33 @@ int launch_rows(const Kv4Args& a, int max_q, int kv_heads, cudaStream_t st) {
     return (int)cudaGetLastError();
 }
 
+int launch_tc(Kv4Args& a, int max_q, cudaStream_t st) {
+    static unsigned long long done = 0;
+    static int sms[64] = {};
+    int dev = 0;
+    cudaGetDevice(&dev);
+    if (!smem_opt_in(k_kv4_attn_tc, T_SMEM, &done)) return -1;
+    if (!sms[dev & 63] && cudaDeviceGetAttribute(&sms[dev & 63], cudaDevAttrMultiProcessorCount, dev) != cudaSuccess)
+        return -1;
+    const bool pair = a.group % 2 == 0;
+    const int per = pair ? TQ : 2 * TQ;
+    a.n_blocks = max_q > 0 ? (max_q - 1) / per + 1 : 1;
+    const long long units = (long long)a.n_seqs * a.n_blocks * (pair ? a.heads / 2 : a.heads);
+    if (units > 0x7fffffffLL - 4096) return -1;
+    const int kv_cols = a.heads / a.group * 64;
+    CUtensorMap tq, tk, tv, to;
+    if (!attn_tmap(&tq, a.Q, a.heads * 64, a.q_rows, a.ldq, TQ) || !attn_tmap(&to, a.O, a.heads * 64, a.q_rows, a.ldo, TQ))
+        return -1;
+    if (a.kv_rows > 0) {
+        if (!attn_tmap(&tk, a.K, kv_cols, a.kv_rows, a.ldkv, TKV) || !attn_tmap(&tv, a.V, kv_cols, a.kv_rows, a.ldkv, TKV))
+            return -1;
+    } else {
+        tk = tv = tq;  // no own rows: never read
+    }
+    launch_pdl(k_kv4_attn_tc, (int)(units < sms[dev & 63] ? units : sms[dev & 63]), T_THREADS, T_SMEM, st, tq, tk, tv, to, a);
+    return (int)cudaGetLastError();
+}
+
 }  // namespace
 
 extern "C" int d1_flash_attn_kv4(const d1_half* Q, int ldq, const d1_half* K, const d1_half* V, int ldkv, d1_half* O,
@@ -462,12 +1024,14 @@ extern "C" int d1_flash_attn_kv4(const d1_half* Q, int ldq, const d1_half* K, co
     a.ldo = ldo;
     a.lse_ld = lse_ld;
     a.n_seqs = n_seqs;
+    a.heads = heads;
     a.group = group;
     a.q_rows = q_rows;
     a.kv_rows = kv_rows;
     a.scale_log2 = scale * kLog2e;
     if (!a.err) return -1;
     const int kv_heads = heads / group;
+    if ((long long)max_q * group > 64) return launch_tc(a, max_q, st);
     return (long long)max_q * group <= 16 ? launch_rows<1>(a, max_q, kv_heads, st) : launch_rows<2>(a, max_q, kv_heads, st);
 }
 

@@ -358,13 +358,14 @@ def test_attend_sharp_and_shared(pkg, gpu_lib, max_q):
 
 
 @gpu
+@pytest.mark.parametrize("at", [0, 15, 50, 78, 99])
 @pytest.mark.parametrize("max_q", HINTS)
-def test_attend_nan_stays_in_its_rows(pkg, gpu_lib, max_q):
+def test_attend_nan_stays_in_its_rows(pkg, gpu_lib, max_q, at):
     """A NaN key makes its sequence's rows NaN, a NaN query row only itself, as in fp16; other sequences keep theirs."""
     rng = np.random.default_rng(4)
     kvh, group = 2, 2
     c = Caches(rng, [100, 100], kvh)
-    c.dev["kp"][0, 1, 50] = 0x7E00
+    c.dev["kp"][0, 1, at] = 0x7E00
     x, starts = poisoned_rows(rng, [4, 4], (kvh * group + 2 * kvh) * 64)
     x[starts[1] + 2, :64] = np.nan
     seqs = [dict(q_start=s, q_len=4, kv_start=s, kv_len=0) for s in starts]
