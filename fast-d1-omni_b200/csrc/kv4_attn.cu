@@ -19,7 +19,7 @@ struct Kv4Args {
     const D1Kv4Seq* seqs;
     int* err;
     int ldq, ldkv, ldo, lse_ld, n_seqs, heads, group, q_rows, kv_rows, accumulate;
-    int n_blocks;  // tcgen05 form: blocks of rows per sequence, by max_q
+    int n_blocks;  // tcgen05 forms: blocks of rows per sequence (attention), tiles of keys per cache (mass)
     float scale_log2;
 };
 
@@ -36,11 +36,11 @@ __device__ __forceinline__ uint64_t f2_mul(uint64_t a, uint64_t b) {
 
 // 2^x of two numbers without the SFU: x = n + f, n whole by adding and taking away 1.5 * 2^23 (the sum's low bits, with
 // 127 added, are 2^n's exponent), |f| <= 1/2, 2^f by a polynomial fitted here for the smallest relative error: 7.5e-5 of
-// degree 3 (below P's rounding to fp16), 2.1e-7 of degree 5 evaluated in fp32. x below -126 counts as -126; NaN stays.
+// degree 3 (below P's rounding to fp16), 2.1e-7 of degree 5 evaluated in fp32. x below -126.5 gives 0; NaN stays.
 template <int DEG>
 __device__ __forceinline__ void ex2_fma2(float x0, float x1, float& p0, float& p1) {
     static_assert(DEG == 3 || DEG == 5, "fitted degrees");
-    const uint64_t x = f2_pack(fmax_nan(x0, -126.f), fmax_nan(x1, -126.f));
+    const uint64_t x = f2_pack(fmax_nan(x0, -127.f), fmax_nan(x1, -127.f));
     const uint64_t t = f2_add(x, f2_pack(12583039.f, 12583039.f));
     const uint64_t f = f2_fma(f2_add(t, f2_pack(-12583039.f, -12583039.f)), f2_pack(-1.f, -1.f), x);
     auto c2 = [](float c) { return f2_pack(c, c); };
@@ -946,6 +946,340 @@ __global__ void __launch_bounds__(256) k_kv4_mass_rows(const Kv4Args a) {
     }
 }
 
+// ------------------------------------------------------------------------------------------------ mass, many rows
+// tcgen05 form: S^T = K Q^T, so that a key is a TMEM lane and its sum over the query rows stays in one thread. Persistent
+// CTAs loop over units of 128 keys of one (cache, kv head): the keys are expanded once into shared memory, then tiles of
+// up to 256 query columns (a block of rows of every head of the kv head) pass by. The bound is the exponentials: 1 per
+// key and column, some of them on the FMA pipe.
+// Warps:
+//   0-3, 4-7   take the tiles in turn: S from TMEM (256 columns each), exp2(s * scale - lse), summed in fp32. At the
+//              unit's end the second warpgroup passes its sums to the first through shared memory
+//   8, 10, 11  loaders: the keys' codes, expanded; query tiles by TMA where a block is whole, otherwise row by row with
+//              zeros behind the end; the columns' -lse (behind the end and for rows without keys: -inf, which adds 0)
+//   9          TMEM, and the MMAs from one thread
+constexpr int MQ = 256, MK = 128, M_STAGES = 4, M_LOADERS = 3, M_THREADS = 384;
+constexpr int M_Q_BYTES = MQ * 128, M_K_BYTES = MK * 128;
+enum : int {
+    MB_KFULL = 0,                    // [2] the unit's keys
+    MB_KEMPTY = MB_KFULL + 2,        // [2]
+    MB_QFULL = MB_KEMPTY + 2,        // [stage]
+    MB_QEMPTY = MB_QFULL + M_STAGES, // [stage]: read by the MMA (1) and the lse by its 4 warps
+    MB_SFULL = MB_QEMPTY + M_STAGES, // [w]
+    MB_SFREE = MB_SFULL + 2,         // [w] (4 warps)
+    MB_SUM = MB_SFREE + 2,           // [2] the second warpgroup's sums are in shared memory (4 warps)
+    MB_SUMFREE = MB_SUM + 2,         // [2] (4 warps)
+    MB_DRAIN = MB_SUMFREE + 2,
+    M_NBARS = MB_DRAIN + 1
+};
+constexpr int M_SMEM = 2 * M_K_BYTES + M_STAGES * (M_Q_BYTES + MQ * 4) + 2 * MK * 4 + M_NBARS * 8 + 16;
+static_assert(M_SMEM <= 232448, "shared memory of the tcgen05 mass kernel");
+
+// The units of a CTA and, within each, its query tiles, walked alike by every warp (all lanes together). The sequences
+// that share a mass array belong to the first of them.
+struct MassWalk {
+    D1Kv4Seq s;       // the unit's first sequence
+    int u, sq, g, kt, max_kt, kv_heads;
+    int peer, q_start, q_len, row0;  // the tile: rows row0 .. row0 + rows() - 1 of sequence `peer`, every head of g
+    int block;        // rows of a whole tile
+    bool at_unit;
+
+    __device__ MassWalk(const Kv4Args& a) : u(blockIdx.x), at_unit(false) {
+        max_kt = a.n_blocks;
+        kv_heads = a.heads / a.group;
+        block = MQ / a.group;
+    }
+    // The next sequence at or after j with this mass array, or n_seqs.
+    __device__ int find(const Kv4Args& a, int j, const float* mass, int end) const {
+        const int lane = threadIdx.x & 31;
+        for (; j < end; j += 32) {
+            const uint32_t v = __ballot_sync(D1_FULL_MASK, j + lane < end && a.seqs[min(j + lane, end - 1)].mass == mass);
+            if (v) return j + __ffs(v) - 1;
+        }
+        return end;
+    }
+    __device__ bool next_unit(const Kv4Args& a) {
+        while (true) {
+            if (at_unit) {
+                kt += max_kt;  // a cache longer than max_len comes round again
+            } else {
+                if (u >= a.n_seqs * kv_heads * max_kt) return false;
+                kt = u % max_kt;
+                g = u / max_kt % kv_heads;
+                sq = u / max_kt / kv_heads;
+                s = a.seqs[sq];
+                at_unit = true;
+                if (!s.mass) {
+                    s.ext_len = 0;
+                } else if (!kv4_seq_ok(s)) {
+                    if ((threadIdx.x & 31) == 0) atomicExch(a.err, kErrTable);
+                    s.ext_len = 0;
+                } else if (find(a, 0, s.mass, sq) < sq) {
+                    s.ext_len = 0;  // another sequence's
+                }
+            }
+            if ((long long)kt * MK < s.ext_len) {
+                peer = sq - 1;
+                q_len = row0 = 0;
+                return true;
+            }
+            u += gridDim.x;
+            at_unit = false;
+        }
+    }
+    __device__ bool next_tile(const Kv4Args& a) {
+        row0 += block;
+        while (row0 >= q_len) {
+            peer = find(a, peer + 1, s.mass, a.n_seqs);
+            if (peer >= a.n_seqs) return false;
+            const D1Kv4Seq& p = a.seqs[peer];
+            q_start = p.q_start;
+            q_len = p.q_len;
+            row0 = 0;
+            if (p.k4 != s.k4 || p.ext_len != s.ext_len || p.ext_cap != s.ext_cap || !rows_ok(q_start, q_len, a.q_rows)) {
+                if ((threadIdx.x & 31) == 0) atomicExch(a.err, kErrTable);
+                q_len = 0;
+            } else if (q_len > 0) {
+                return true;
+            }
+        }
+        return true;
+    }
+    __device__ int rows() const { return min(block, q_len - row0); }
+};
+
+__global__ void __launch_bounds__(M_THREADS, 1) k_kv4_mass_tc(const __grid_constant__ CUtensorMap tmQ, const Kv4Args a) {
+    extern __shared__ __align__(1024) uint8_t m_smem[];
+    uint8_t* sK = m_smem;                                                          // [2][128 keys]
+    uint8_t* sQ = sK + 2 * M_K_BYTES;                                              // [stage][256 columns]
+    float* sL = reinterpret_cast<float*>(sQ + M_STAGES * M_Q_BYTES);               // [stage][256]: -lse in log2
+    float* sSum = sL + M_STAGES * MQ;                                              // [2][128]
+    uint64_t* bars = reinterpret_cast<uint64_t*>(sSum + 2 * MK);
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + M_NBARS);
+    volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+    auto bar = [&](int i) { return smem_u32(bars + i); };
+    if (smem_u32(m_smem) & 1023) {  // never expected: dynamic shared memory starts at the window's base
+        pdl_wait();
+        if (threadIdx.x == 0) atomicExch(a.err, kErrDrain);
+        return;
+    }
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < 2; i++) {
+            mbar_init(bar(MB_KFULL + i), 32 * M_LOADERS);
+            mbar_init(bar(MB_KEMPTY + i), 1);
+            mbar_init(bar(MB_SFULL + i), 1);
+            mbar_init(bar(MB_SFREE + i), 4);
+            mbar_init(bar(MB_SUM + i), 4);
+            mbar_init(bar(MB_SUMFREE + i), 4);
+        }
+        for (int i = 0; i < M_STAGES; i++) {
+            mbar_init(bar(MB_QFULL + i), 32 * M_LOADERS);
+            mbar_init(bar(MB_QEMPTY + i), 5);
+        }
+        mbar_init(bar(MB_DRAIN), 1);
+        *abort_flag = 0;
+        fence_mbar_init();
+    }
+    if (warp == 9) {
+        tmem_alloc(smem_u32(tmem_slot), T_TMEM_COLS);
+        tmem_relinquish();
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = *tmem_slot;
+    pdl_entry();  // barriers and TMEM are set up; global memory is touched only after this
+    MassWalk wk(a);
+    int nu = 0, ti = 0;  // units and tiles so far
+    bool ok = true;
+    auto wait = [&](int b, uint32_t parity) {
+        return __all_sync(D1_FULL_MASK, mbar_wait(bar(b), parity, abort_flag)) != 0;
+    };
+
+    if (warp == 8 || warp >= 10) {
+        // ------------------------------------------------------------------ loaders
+        const int lt = (warp == 8 ? 0 : warp - 9) * 32 + lane;
+        const bool issuer = warp == 8 && lane == 0;
+        for (; ok && wk.next_unit(a); nu++) {
+            const uint8_t* k4 = wk.s.k4 + (size_t)wk.g * wk.s.ext_cap * 32;
+            const uint16_t* kp = reinterpret_cast<const uint16_t*>(wk.s.kp) + (size_t)wk.g * wk.s.ext_cap;
+            if (!(ok = wait(MB_KEMPTY + (nu & 1), ((nu >> 1) & 1) ^ 1))) break;
+            uint8_t* dK = sK + (nu & 1) * M_K_BYTES;
+            for (int c = lt; c < 2 * MK; c += 32 * M_LOADERS) {
+                const int r = c >> 1, key = wk.kt * MK + r;
+                uint4 piece = make_uint4(0, 0, 0, 0);
+                uint32_t par = 0;
+                if (key < wk.s.ext_len) {
+                    piece = __ldg(reinterpret_cast<const uint4*>(k4 + (size_t)key * 32) + (c & 1));
+                    par = __ldg(kp + key);
+                }
+                const uint32_t p2 = par * 0x00010001u, step = kv4_step2(p2);
+                uint32_t z0, z1;
+                kv4_zero(p2, z0, z1);
+                const uint32_t word[4] = {piece.x, piece.y, piece.z, piece.w};
+#pragma unroll
+                for (int q = 0; q < 4; q++) {
+                    uint32_t v[4];
+                    kv4_expand(word[q], z0, z1, v);
+                    *reinterpret_cast<uint4*>(dK + r * 128 + ((((c & 1) * 4 + q) ^ (r & 7)) << 4)) =
+                        make_uint4(h2_mul(v[0], step), h2_mul(v[1], step), h2_mul(v[2], step), h2_mul(v[3], step));
+                }
+            }
+            fence_async_smem_cta();
+            mbar_arrive(bar(MB_KFULL + (nu & 1)));
+            for (; wk.next_tile(a); ti++) {
+                const int st = ti % M_STAGES, n = wk.rows(), cols = n * a.group, pad = (cols + 31) & ~31;
+                if (!(ok = wait(MB_QEMPTY + st, ((ti / M_STAGES) & 1) ^ 1))) break;
+                uint8_t* dQ = sQ + st * M_Q_BYTES;
+                float* dL = sL + st * MQ;
+                const int row = wk.q_start + wk.row0, h0 = wk.g * a.group;
+                const bool whole = cols == MQ && n % 8 == 0;  // heads at whole swizzle atoms
+                for (int c = lt; c < pad; c += 32 * M_LOADERS) {
+                    float v = -INFINITY;
+                    if (c < cols) {
+                        const int hh = c / n;
+                        const float l = __ldg(a.lse + (size_t)(h0 + hh) * a.lse_ld + row + (c - hh * n));
+                        if (l != -INFINITY) v = -l * kLog2e;
+                    }
+                    dL[c] = v;
+                }
+                if (!whole) {
+                    for (int i = lt; i < pad * 8; i += 32 * M_LOADERS) {
+                        const int c = i >> 3, ch = i & 7;
+                        uint4 x = make_uint4(0, 0, 0, 0);
+                        if (c < cols) {
+                            const int hh = c / n;
+                            x = __ldg(reinterpret_cast<const uint4*>(a.Q + (size_t)(row + (c - hh * n)) * a.ldq + (h0 + hh) * 64) + ch);
+                        }
+                        *reinterpret_cast<uint4*>(dQ + c * 128 + ((ch ^ (c & 7)) << 4)) = x;
+                    }
+                    fence_async_smem_cta();
+                }
+                if (whole && issuer) {
+                    mbar_arrive_expect_tx(bar(MB_QFULL + st), M_Q_BYTES);
+                    for (int hh = 0; hh < a.group; hh++)
+                        tma_load_2d(smem_u32(dQ) + hh * n * 128, &tmQ, (h0 + hh) * 64, row, bar(MB_QFULL + st));
+                } else {
+                    mbar_arrive(bar(MB_QFULL + st));
+                }
+            }
+        }
+        if (!ok && lane == 0) record_err(a.err, abort_flag, kErrWaitEmpty);
+        if (issuer)  // TMA copies still in flight (only after an abort) land before the CTA exits
+            for (int i = ti > M_STAGES ? ti - M_STAGES : 0; i < ti; i++)
+                if (!mbar_wait_timed2(bar(MB_QFULL + i % M_STAGES), (i / M_STAGES) & 1)) break;
+    } else if (warp == 9) {
+        // ------------------------------------------------------------------ MMA issuer (lane 0)
+        for (; ok && wk.next_unit(a); nu++) {
+            if (!(ok = wait(MB_KFULL + (nu & 1), (nu >> 1) & 1))) break;
+            const uint32_t k_addr = smem_u32(sK + (nu & 1) * M_K_BYTES);
+            for (; wk.next_tile(a); ti++) {
+                const int st = ti % M_STAGES, w = ti & 1, pad = (wk.rows() * a.group + 31) & ~31;
+                if (!(ok = wait(MB_QFULL + st, (ti / M_STAGES) & 1))) break;
+                if (ti > 1 && !(ok = wait(MB_SFREE + w, ((ti >> 1) - 1) & 1))) break;
+                tc_fence_after();
+                if (lane == 0) {
+                    const uint32_t q_addr = smem_u32(sQ + st * M_Q_BYTES), idesc = idesc_f16_f32(MK, pad);
+#pragma unroll
+                    for (int k = 0; k < 4; k++)
+                        tc_mma_f16(tmem + w * MQ, smem_desc_k128(k_addr + k * 32), smem_desc_k128(q_addr + k * 32), idesc, k != 0);
+                    tc_commit(bar(MB_SFULL + w));
+                    tc_commit(bar(MB_QEMPTY + st));
+                }
+                __syncwarp();
+            }
+            if (!ok) break;
+            if (lane == 0) tc_commit(bar(MB_KEMPTY + (nu & 1)));
+            __syncwarp();
+        }
+        if (lane == 0) {
+            if (!ok) record_err(a.err, abort_flag, kErrWaitFull);
+            tc_commit(bar(MB_DRAIN));  // every issued MMA has completed before TMEM is released
+            if (!mbar_wait_timed2(bar(MB_DRAIN), 0)) record_err(a.err, abort_flag, kErrDrain);
+        }
+        __syncwarp();
+    } else {
+        // ------------------------------------------------------------------ exponentials and sums
+        const int w = warp >> 2, row = (warp & 3) * 32 + lane;
+        const uint32_t tS = tmem + w * MQ + ((uint32_t)((warp & 3) * 32) << 16);
+        const uint64_t sc2 = f2_pack(a.scale_log2, a.scale_log2);
+        for (; ok && wk.next_unit(a); nu++) {
+            uint64_t sum[4];
+#pragma unroll
+            for (int e = 0; e < 4; e++) sum[e] = f2_pack(0.f, 0.f);
+            bool any = false;
+            for (; wk.next_tile(a); ti++) {
+                any = true;
+                if ((ti & 1) != w) continue;
+                const int st = ti % M_STAGES, pad = (wk.rows() * a.group + 31) & ~31;
+                if (!(ok = wait(MB_QFULL + st, (ti / M_STAGES) & 1))) break;  // the lse
+                if (!(ok = wait(MB_SFULL + w, (ti >> 1) & 1))) break;
+                tc_fence_after();
+                const float4* l4 = reinterpret_cast<const float4*>(sL + st * MQ);
+                for (int c0 = 0; c0 < pad; c0 += 32) {
+                    uint32_t sr[32];
+                    tmem_ld32(tS + c0, sr);
+                    tc_wait_ld();
+#pragma unroll
+                    for (int i = 0; i < 8; i++) {
+                        const float4 l = l4[(c0 >> 2) + i];
+                        float x[4], p[4];
+                        f2_unpack(f2_fma(f2_pack(__uint_as_float(sr[4 * i]), __uint_as_float(sr[4 * i + 1])), sc2,
+                                         f2_pack(l.x, l.y)), x[0], x[1]);
+                        f2_unpack(f2_fma(f2_pack(__uint_as_float(sr[4 * i + 2]), __uint_as_float(sr[4 * i + 3])), sc2,
+                                         f2_pack(l.z, l.w)), x[2], x[3]);
+                        p[0] = ex2(x[0]);
+                        p[1] = ex2(x[1]);
+                        if (i % 4 != 0) {
+                            ex2_fma2<5>(x[2], x[3], p[2], p[3]);
+                        } else {
+                            p[2] = ex2(x[2]);
+                            p[3] = ex2(x[3]);
+                        }
+                        sum[(2 * i) & 3] = f2_add(sum[(2 * i) & 3], f2_pack(p[0], p[1]));
+                        sum[(2 * i + 1) & 3] = f2_add(sum[(2 * i + 1) & 3], f2_pack(p[2], p[3]));
+                    }
+                }
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) {
+                    mbar_arrive(bar(MB_SFREE + w));
+                    mbar_arrive(bar(MB_QEMPTY + st));
+                }
+            }
+            if (!ok) break;
+            float v[8];
+#pragma unroll
+            for (int e = 0; e < 4; e++) f2_unpack(sum[e], v[2 * e], v[2 * e + 1]);
+            const float mine = ((v[0] + v[1]) + (v[2] + v[3])) + ((v[4] + v[5]) + (v[6] + v[7]));
+            const int slot = nu & 1;
+            if (w == 1) {
+                if (!(ok = wait(MB_SUMFREE + slot, ((nu >> 1) & 1) ^ 1))) break;
+                sSum[slot * MK + row] = mine;
+                __syncwarp();
+                if (lane == 0) mbar_arrive(bar(MB_SUM + slot));
+            } else {
+                if (!(ok = wait(MB_SUM + slot, (nu >> 1) & 1))) break;
+                const float both = mine + sSum[slot * MK + row];
+                __syncwarp();
+                if (lane == 0) mbar_arrive(bar(MB_SUMFREE + slot));
+                const long long key = (long long)wk.kt * MK + row;
+                if (any && key < wk.s.ext_len) {
+                    float* m = wk.s.mass + (size_t)wk.g * wk.s.ext_cap + key;
+                    *m = a.accumulate ? *m + both : both;
+                }
+            }
+        }
+        if (!ok && lane == 0) record_err(a.err, abort_flag, kErrWaitAccFull);
+    }
+    tc_fence_before();
+    __syncthreads();
+    if (warp == 9) {
+        tc_fence_after();
+        tmem_dealloc(tmem, T_TMEM_COLS);
+    }
+}
+
 // The shared-memory opt-in is per function and device: set on the first launch on each device (`done`: its bits).
 template <typename F>
 bool smem_opt_in(F* kernel, int bytes, unsigned long long* done) {
@@ -956,6 +1290,15 @@ bool smem_opt_in(F* kernel, int bytes, unsigned long long* done) {
     if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) != cudaSuccess) return false;
     __atomic_fetch_or(done, bit, __ATOMIC_RELEASE);
     return true;
+}
+
+int sm_count() {
+    static int sms[64] = {};
+    int dev = 0;
+    cudaGetDevice(&dev);
+    if (!sms[dev & 63] && cudaDeviceGetAttribute(&sms[dev & 63], cudaDevAttrMultiProcessorCount, dev) != cudaSuccess)
+        return 0;
+    return sms[dev & 63];
 }
 
 template <int MT>
@@ -971,12 +1314,9 @@ int launch_rows(const Kv4Args& a, int max_q, int kv_heads, cudaStream_t st) {
 
 int launch_tc(Kv4Args& a, int max_q, cudaStream_t st) {
     static unsigned long long done = 0;
-    static int sms[64] = {};
-    int dev = 0;
-    cudaGetDevice(&dev);
     if (!smem_opt_in(k_kv4_attn_tc, T_SMEM, &done)) return -1;
-    if (!sms[dev & 63] && cudaDeviceGetAttribute(&sms[dev & 63], cudaDevAttrMultiProcessorCount, dev) != cudaSuccess)
-        return -1;
+    const int sms = sm_count();
+    if (!sms) return -1;
     const bool pair = a.group % 2 == 0;
     const int per = pair ? TQ : 2 * TQ;
     a.n_blocks = max_q > 0 ? (max_q - 1) / per + 1 : 1;
@@ -992,7 +1332,22 @@ int launch_tc(Kv4Args& a, int max_q, cudaStream_t st) {
     } else {
         tk = tv = tq;  // no own rows: never read
     }
-    launch_pdl(k_kv4_attn_tc, (int)(units < sms[dev & 63] ? units : sms[dev & 63]), T_THREADS, T_SMEM, st, tq, tk, tv, to, a);
+    launch_pdl(k_kv4_attn_tc, (int)(units < sms ? units : sms), T_THREADS, T_SMEM, st, tq, tk, tv, to, a);
+    return (int)cudaGetLastError();
+}
+
+int launch_mass_tc(Kv4Args& a, int max_len, cudaStream_t st) {
+    static unsigned long long done = 0;
+    if (!smem_opt_in(k_kv4_mass_tc, M_SMEM, &done)) return -1;
+    const int sms = sm_count();
+    if (!sms) return -1;
+    a.n_blocks = max_len > 0 ? (max_len - 1) / MK + 1 : 1;
+    const long long units = (long long)a.n_seqs * a.n_blocks * (a.heads / a.group);
+    if (units > 0x7fffffffLL - 4096) return -1;
+    CUtensorMap tq;
+    // whole tiles: a block of 256 / group rows of each head
+    if (!attn_tmap(&tq, a.Q, a.heads * 64, a.q_rows, a.ldq, MQ / a.group)) return -1;
+    launch_pdl(k_kv4_mass_tc, (int)(units < sms ? units : sms), M_THREADS, M_SMEM, st, tq, a);
     return (int)cudaGetLastError();
 }
 
@@ -1051,11 +1406,13 @@ extern "C" int d1_kv4_mass(const d1_half* Q, int ldq, const float* lse, int lse_
     a.ldq = ldq;
     a.lse_ld = lse_ld;
     a.n_seqs = n_seqs;
+    a.heads = heads;
     a.group = group;
     a.q_rows = q_rows;
     a.accumulate = accumulate;
     a.scale_log2 = scale * kLog2e;
     if (!a.err) return -1;
+    if ((long long)max_q * group > 64 && group <= MQ && q_rows > 0) return launch_mass_tc(a, max_len, st);
     int x = (max_len + M_KEYS - 1) / M_KEYS;
     x = x < 1 ? 1 : x > 65536 ? 65536 : x;
     launch_pdl(k_kv4_mass_rows, dim3(x, heads / group, n_seqs < 65535 ? n_seqs : 65535), 256, 0, st, a);
