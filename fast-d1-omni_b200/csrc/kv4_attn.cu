@@ -952,26 +952,29 @@ __global__ void __launch_bounds__(256) k_kv4_mass_rows(const Kv4Args a) {
 // up to 256 query columns (a block of rows of every head of the kv head) pass by. The bound is the exponentials: 1 per
 // key and column, some of them on the FMA pipe.
 // Warps:
-//   0-3, 4-7   take the tiles in turn: S from TMEM (256 columns each), exp2(s * scale - lse), summed in fp32. At the
-//              unit's end the second warpgroup passes its sums to the first through shared memory
-//   8, 10, 11  loaders: the keys' codes, expanded; query tiles by TMA where a block is whole, otherwise row by row with
+//   0-15       four warpgroups share every tile (two of its eight 32-column pieces each): S from TMEM, where the next
+//              tile's S is computed meanwhile, exp2(s * scale - lse), summed in fp32; one pair of exponentials in eight on
+//              the FMA pipe. At the unit's end three pass their sums to the first through shared memory. (Two documents of
+//              2048 rows over 8192 keys: 91 us; 98 with two warpgroups and the next piece's load on its way, 97 with
+//              both pieces loaded at once, 93 without the FMA pipe, 94 and 99 with a quarter and three eighths there)
+//   16, 18, 19 loaders: the keys' codes, expanded; query tiles by TMA where a block is whole, otherwise row by row with
 //              zeros behind the end; the columns' -lse (behind the end and for rows without keys: -inf, which adds 0)
-//   9          TMEM, and the MMAs from one thread
-constexpr int MQ = 256, MK = 128, M_STAGES = 4, M_LOADERS = 3, M_THREADS = 384;
+//   17         TMEM, and the MMAs from one thread
+constexpr int MQ = 256, MK = 128, M_STAGES = 4, M_LOADERS = 3, M_WGS = 4, M_THREADS = 128 * M_WGS + 128;
 constexpr int M_Q_BYTES = MQ * 128, M_K_BYTES = MK * 128;
 enum : int {
     MB_KFULL = 0,                    // [2] the unit's keys
     MB_KEMPTY = MB_KFULL + 2,        // [2]
     MB_QFULL = MB_KEMPTY + 2,        // [stage]
-    MB_QEMPTY = MB_QFULL + M_STAGES, // [stage]: read by the MMA (1) and the lse by its 4 warps
-    MB_SFULL = MB_QEMPTY + M_STAGES, // [w]
-    MB_SFREE = MB_SFULL + 2,         // [w] (4 warps)
-    MB_SUM = MB_SFREE + 2,           // [2] the second warpgroup's sums are in shared memory (4 warps)
+    MB_QEMPTY = MB_QFULL + M_STAGES, // [stage]: read by the MMA (1), and its lse by 16 warps
+    MB_SFULL = MB_QEMPTY + M_STAGES, // [buffer] S of a tile is in TMEM
+    MB_SFREE = MB_SFULL + 2,         // [buffer] (16 warps)
+    MB_SUM = MB_SFREE + 2,           // [2] the other warpgroups' sums are in shared memory (12 warps)
     MB_SUMFREE = MB_SUM + 2,         // [2] (4 warps)
     MB_DRAIN = MB_SUMFREE + 2,
     M_NBARS = MB_DRAIN + 1
 };
-constexpr int M_SMEM = 2 * M_K_BYTES + M_STAGES * (M_Q_BYTES + MQ * 4) + 2 * MK * 4 + M_NBARS * 8 + 16;
+constexpr int M_SMEM = 2 * M_K_BYTES + M_STAGES * (M_Q_BYTES + MQ * 4) + 2 * (M_WGS - 1) * MK * 4 + M_NBARS * 8 + 16;
 static_assert(M_SMEM <= 232448, "shared memory of the tcgen05 mass kernel");
 
 // The units of a CTA and, within each, its query tiles, walked alike by every warp (all lanes together). The sequences
@@ -1052,8 +1055,8 @@ __global__ void __launch_bounds__(M_THREADS, 1) k_kv4_mass_tc(const __grid_const
     uint8_t* sK = m_smem;                                                          // [2][128 keys]
     uint8_t* sQ = sK + 2 * M_K_BYTES;                                              // [stage][256 columns]
     float* sL = reinterpret_cast<float*>(sQ + M_STAGES * M_Q_BYTES);               // [stage][256]: -lse in log2
-    float* sSum = sL + M_STAGES * MQ;                                              // [2][128]
-    uint64_t* bars = reinterpret_cast<uint64_t*>(sSum + 2 * MK);
+    float* sSum = sL + M_STAGES * MQ;                                              // [2][warpgroup - 1][128]
+    uint64_t* bars = reinterpret_cast<uint64_t*>(sSum + 2 * (M_WGS - 1) * MK);
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + M_NBARS);
     volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
     auto bar = [&](int i) { return smem_u32(bars + i); };
@@ -1062,25 +1065,26 @@ __global__ void __launch_bounds__(M_THREADS, 1) k_kv4_mass_tc(const __grid_const
         if (threadIdx.x == 0) atomicExch(a.err, kErrDrain);
         return;
     }
+    constexpr int M_WARP = 4 * M_WGS + 1;  // the MMA warp
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     if (threadIdx.x == 0) {
         for (int i = 0; i < 2; i++) {
             mbar_init(bar(MB_KFULL + i), 32 * M_LOADERS);
             mbar_init(bar(MB_KEMPTY + i), 1);
             mbar_init(bar(MB_SFULL + i), 1);
-            mbar_init(bar(MB_SFREE + i), 4);
-            mbar_init(bar(MB_SUM + i), 4);
+            mbar_init(bar(MB_SFREE + i), 4 * M_WGS);
+            mbar_init(bar(MB_SUM + i), 4 * (M_WGS - 1));
             mbar_init(bar(MB_SUMFREE + i), 4);
         }
         for (int i = 0; i < M_STAGES; i++) {
-            mbar_init(bar(MB_QFULL + i), 32 * M_LOADERS);
-            mbar_init(bar(MB_QEMPTY + i), 5);
+            mbar_init(bar(MB_QFULL + i), 32);
+            mbar_init(bar(MB_QEMPTY + i), 1 + 4 * M_WGS);
         }
         mbar_init(bar(MB_DRAIN), 1);
         *abort_flag = 0;
         fence_mbar_init();
     }
-    if (warp == 9) {
+    if (warp == M_WARP) {
         tmem_alloc(smem_u32(tmem_slot), T_TMEM_COLS);
         tmem_relinquish();
     }
@@ -1096,27 +1100,35 @@ __global__ void __launch_bounds__(M_THREADS, 1) k_kv4_mass_tc(const __grid_const
         return __all_sync(D1_FULL_MASK, mbar_wait(bar(b), parity, abort_flag)) != 0;
     };
 
-    if (warp == 8 || warp >= 10) {
+    if (warp == M_WARP - 1 || warp > M_WARP) {
         // ------------------------------------------------------------------ loaders
-        const int lt = (warp == 8 ? 0 : warp - 9) * 32 + lane;
-        const bool issuer = warp == 8 && lane == 0;
+        const int lw = warp < M_WARP ? 0 : warp - M_WARP, lt = lw * 32 + lane;
         for (; ok && wk.next_unit(a); nu++) {
             const uint8_t* k4 = wk.s.k4 + (size_t)wk.g * wk.s.ext_cap * 32;
             const uint16_t* kp = reinterpret_cast<const uint16_t*>(wk.s.kp) + (size_t)wk.g * wk.s.ext_cap;
+            constexpr int PIECES = (2 * MK + 32 * M_LOADERS - 1) / (32 * M_LOADERS);
+            uint4 piece[PIECES];
+            uint32_t par[PIECES];
+#pragma unroll
+            for (int i = 0; i < PIECES; i++) {
+                const int c = lt + i * 32 * M_LOADERS, key = wk.kt * MK + (c >> 1);
+                piece[i] = make_uint4(0, 0, 0, 0);
+                par[i] = 0;  // step 0: zeros
+                if (c < 2 * MK && key < wk.s.ext_len) {
+                    piece[i] = __ldg(reinterpret_cast<const uint4*>(k4 + (size_t)key * 32) + (c & 1));
+                    par[i] = __ldg(kp + key);
+                }
+            }
             if (!(ok = wait(MB_KEMPTY + (nu & 1), ((nu >> 1) & 1) ^ 1))) break;
             uint8_t* dK = sK + (nu & 1) * M_K_BYTES;
-            for (int c = lt; c < 2 * MK; c += 32 * M_LOADERS) {
-                const int r = c >> 1, key = wk.kt * MK + r;
-                uint4 piece = make_uint4(0, 0, 0, 0);
-                uint32_t par = 0;
-                if (key < wk.s.ext_len) {
-                    piece = __ldg(reinterpret_cast<const uint4*>(k4 + (size_t)key * 32) + (c & 1));
-                    par = __ldg(kp + key);
-                }
-                const uint32_t p2 = par * 0x00010001u, step = kv4_step2(p2);
+#pragma unroll
+            for (int i = 0; i < PIECES; i++) {
+                const int c = lt + i * 32 * M_LOADERS, r = c >> 1;
+                if (c >= 2 * MK) continue;
+                const uint32_t p2 = par[i] * 0x00010001u, step = kv4_step2(p2);
                 uint32_t z0, z1;
                 kv4_zero(p2, z0, z1);
-                const uint32_t word[4] = {piece.x, piece.y, piece.z, piece.w};
+                const uint32_t word[4] = {piece[i].x, piece[i].y, piece[i].z, piece[i].w};
 #pragma unroll
                 for (int q = 0; q < 4; q++) {
                     uint32_t v[4];
@@ -1128,47 +1140,48 @@ __global__ void __launch_bounds__(M_THREADS, 1) k_kv4_mass_tc(const __grid_const
             fence_async_smem_cta();
             mbar_arrive(bar(MB_KFULL + (nu & 1)));
             for (; wk.next_tile(a); ti++) {
+                if (ti % M_LOADERS != lw) continue;  // the warps take the tiles in turn: their latencies overlap
                 const int st = ti % M_STAGES, n = wk.rows(), cols = n * a.group, pad = (cols + 31) & ~31;
-                if (!(ok = wait(MB_QEMPTY + st, ((ti / M_STAGES) & 1) ^ 1))) break;
-                uint8_t* dQ = sQ + st * M_Q_BYTES;
-                float* dL = sL + st * MQ;
+                const int inv = (65536 + n - 1) / n;  // c / n = c * inv >> 16 for c < 256: off by less than 1 / n
                 const int row = wk.q_start + wk.row0, h0 = wk.g * a.group;
+                float l[MQ / 32];
+#pragma unroll
+                for (int i = 0; i < MQ / 32; i++) {
+                    const int c = lane + 32 * i, hh = c * inv >> 16;
+                    l[i] = -INFINITY;
+                    if (c < cols) l[i] = __ldg(a.lse + (size_t)(h0 + hh) * a.lse_ld + row + (c - hh * n));
+                }
+                if (!(ok = wait(MB_QEMPTY + st, ((ti / M_STAGES) & 1) ^ 1))) break;
+                const uint32_t dQ = smem_u32(sQ + st * M_Q_BYTES);
                 const bool whole = cols == MQ && n % 8 == 0;  // heads at whole swizzle atoms
-                for (int c = lt; c < pad; c += 32 * M_LOADERS) {
-                    float v = -INFINITY;
-                    if (c < cols) {
-                        const int hh = c / n;
-                        const float l = __ldg(a.lse + (size_t)(h0 + hh) * a.lse_ld + row + (c - hh * n));
-                        if (l != -INFINITY) v = -l * kLog2e;
-                    }
-                    dL[c] = v;
-                }
                 if (!whole) {
-                    for (int i = lt; i < pad * 8; i += 32 * M_LOADERS) {
-                        const int c = i >> 3, ch = i & 7;
-                        uint4 x = make_uint4(0, 0, 0, 0);
-                        if (c < cols) {
-                            const int hh = c / n;
-                            x = __ldg(reinterpret_cast<const uint4*>(a.Q + (size_t)(row + (c - hh * n)) * a.ldq + (h0 + hh) * 64) + ch);
-                        }
-                        *reinterpret_cast<uint4*>(dQ + c * 128 + ((ch ^ (c & 7)) << 4)) = x;
+                    for (int i = lane; i < pad * 8; i += 32) {
+                        const int c = i >> 3, ch = i & 7, hh = c * inv >> 16;
+                        const __half* src =
+                            c < cols ? a.Q + (size_t)(row + (c - hh * n)) * a.ldq + (h0 + hh) * 64 + ch * 8 : a.Q;
+                        cp_async16z(dQ + c * 128 + ((ch ^ (c & 7)) << 4), src, c < cols ? 16 : 0);
                     }
-                    fence_async_smem_cta();
-                }
-                if (whole && issuer) {
+                } else if (lane == 0) {
                     mbar_arrive_expect_tx(bar(MB_QFULL + st), M_Q_BYTES);
                     for (int hh = 0; hh < a.group; hh++)
-                        tma_load_2d(smem_u32(dQ) + hh * n * 128, &tmQ, (h0 + hh) * 64, row, bar(MB_QFULL + st));
-                } else {
-                    mbar_arrive(bar(MB_QFULL + st));
+                        tma_load_2d(dQ + hh * n * 128, &tmQ, (h0 + hh) * 64, row, bar(MB_QFULL + st));
                 }
+#pragma unroll
+                for (int i = 0; i < MQ / 32; i++)
+                    if (32 * i < pad) sL[st * MQ + lane + 32 * i] = l[i] == -INFINITY ? -INFINITY : -l[i] * kLog2e;
+                if (!whole) {
+                    asm volatile("cp.async.wait_all;" ::: "memory");
+                    fence_async_smem_cta();
+                }
+                if (!whole || lane > 0) mbar_arrive(bar(MB_QFULL + st));
             }
         }
+        asm volatile("cp.async.wait_all;" ::: "memory");  // nothing in flight when the CTA exits
         if (!ok && lane == 0) record_err(a.err, abort_flag, kErrWaitEmpty);
-        if (issuer)  // TMA copies still in flight (only after an abort) land before the CTA exits
+        if (lane == 0)  // TMA copies still in flight (only after an abort) land before the CTA exits
             for (int i = ti > M_STAGES ? ti - M_STAGES : 0; i < ti; i++)
                 if (!mbar_wait_timed2(bar(MB_QFULL + i % M_STAGES), (i / M_STAGES) & 1)) break;
-    } else if (warp == 9) {
+    } else if (warp == M_WARP) {
         // ------------------------------------------------------------------ MMA issuer (lane 0)
         for (; ok && wk.next_unit(a); nu++) {
             if (!(ok = wait(MB_KFULL + (nu & 1), (nu >> 1) & 1))) break;
@@ -1200,8 +1213,8 @@ __global__ void __launch_bounds__(M_THREADS, 1) k_kv4_mass_tc(const __grid_const
         __syncwarp();
     } else {
         // ------------------------------------------------------------------ exponentials and sums
-        const int w = warp >> 2, row = (warp & 3) * 32 + lane;
-        const uint32_t tS = tmem + w * MQ + ((uint32_t)((warp & 3) * 32) << 16);
+        const int wg = warp >> 2, row = (warp & 3) * 32 + lane;
+        const uint32_t tS = tmem + 32 * wg + ((uint32_t)((warp & 3) * 32) << 16);
         const uint64_t sc2 = f2_pack(a.scale_log2, a.scale_log2);
         for (; ok && wk.next_unit(a); nu++) {
             uint64_t sum[4];
@@ -1210,27 +1223,26 @@ __global__ void __launch_bounds__(M_THREADS, 1) k_kv4_mass_tc(const __grid_const
             bool any = false;
             for (; wk.next_tile(a); ti++) {
                 any = true;
-                if ((ti & 1) != w) continue;
-                const int st = ti % M_STAGES, pad = (wk.rows() * a.group + 31) & ~31;
+                const int st = ti % M_STAGES, b = ti & 1, pad = (wk.rows() * a.group + 31) & ~31;
                 if (!(ok = wait(MB_QFULL + st, (ti / M_STAGES) & 1))) break;  // the lse
-                if (!(ok = wait(MB_SFULL + w, (ti >> 1) & 1))) break;
+                if (!(ok = wait(MB_SFULL + b, (ti >> 1) & 1))) break;
                 tc_fence_after();
-                const float4* l4 = reinterpret_cast<const float4*>(sL + st * MQ);
-                for (int c0 = 0; c0 < pad; c0 += 32) {
-                    uint32_t sr[32];
-                    tmem_ld32(tS + c0, sr);
+                for (int c0 = 32 * wg; c0 < pad; c0 += 32 * M_WGS) {
+                    const float4* l4 = reinterpret_cast<const float4*>(sL + st * MQ + c0);
+                    uint32_t y[32];
+                    tmem_ld32(tS + b * MQ + (c0 - 32 * wg), y);
                     tc_wait_ld();
 #pragma unroll
                     for (int i = 0; i < 8; i++) {
-                        const float4 l = l4[(c0 >> 2) + i];
+                        const float4 l = l4[i];
                         float x[4], p[4];
-                        f2_unpack(f2_fma(f2_pack(__uint_as_float(sr[4 * i]), __uint_as_float(sr[4 * i + 1])), sc2,
+                        f2_unpack(f2_fma(f2_pack(__uint_as_float(y[4 * i]), __uint_as_float(y[4 * i + 1])), sc2,
                                          f2_pack(l.x, l.y)), x[0], x[1]);
-                        f2_unpack(f2_fma(f2_pack(__uint_as_float(sr[4 * i + 2]), __uint_as_float(sr[4 * i + 3])), sc2,
+                        f2_unpack(f2_fma(f2_pack(__uint_as_float(y[4 * i + 2]), __uint_as_float(y[4 * i + 3])), sc2,
                                          f2_pack(l.z, l.w)), x[2], x[3]);
                         p[0] = ex2(x[0]);
                         p[1] = ex2(x[1]);
-                        if (i % 4 != 0) {
+                        if (i % 4 == 3) {
                             ex2_fma2<5>(x[2], x[3], p[2], p[3]);
                         } else {
                             p[2] = ex2(x[2]);
@@ -1243,7 +1255,7 @@ __global__ void __launch_bounds__(M_THREADS, 1) k_kv4_mass_tc(const __grid_const
                 tc_fence_before();
                 __syncwarp();
                 if (lane == 0) {
-                    mbar_arrive(bar(MB_SFREE + w));
+                    mbar_arrive(bar(MB_SFREE + b));
                     mbar_arrive(bar(MB_QEMPTY + st));
                 }
             }
@@ -1253,20 +1265,21 @@ __global__ void __launch_bounds__(M_THREADS, 1) k_kv4_mass_tc(const __grid_const
             for (int e = 0; e < 4; e++) f2_unpack(sum[e], v[2 * e], v[2 * e + 1]);
             const float mine = ((v[0] + v[1]) + (v[2] + v[3])) + ((v[4] + v[5]) + (v[6] + v[7]));
             const int slot = nu & 1;
-            if (w == 1) {
+            if (wg > 0) {
                 if (!(ok = wait(MB_SUMFREE + slot, ((nu >> 1) & 1) ^ 1))) break;
-                sSum[slot * MK + row] = mine;
+                sSum[(slot * (M_WGS - 1) + wg - 1) * MK + row] = mine;
                 __syncwarp();
                 if (lane == 0) mbar_arrive(bar(MB_SUM + slot));
             } else {
                 if (!(ok = wait(MB_SUM + slot, (nu >> 1) & 1))) break;
-                const float both = mine + sSum[slot * MK + row];
+                const float* other = sSum + slot * (M_WGS - 1) * MK + row;
+                const float all = (mine + other[0]) + (other[MK] + other[2 * MK]);
                 __syncwarp();
                 if (lane == 0) mbar_arrive(bar(MB_SUMFREE + slot));
                 const long long key = (long long)wk.kt * MK + row;
                 if (any && key < wk.s.ext_len) {
                     float* m = wk.s.mass + (size_t)wk.g * wk.s.ext_cap + key;
-                    *m = a.accumulate ? *m + both : both;
+                    *m = a.accumulate ? *m + all : all;
                 }
             }
         }
@@ -1274,7 +1287,7 @@ __global__ void __launch_bounds__(M_THREADS, 1) k_kv4_mass_tc(const __grid_const
     }
     tc_fence_before();
     __syncthreads();
-    if (warp == 9) {
+    if (warp == M_WARP) {
         tc_fence_after();
         tmem_dealloc(tmem, T_TMEM_COLS);
     }
