@@ -155,177 +155,201 @@ __global__ void __launch_bounds__(256) k_kv4_load(const D1Kv4Seq* __restrict__ s
 }
 
 // ------------------------------------------------------------------------------------------------ evict
-// One CTA per (part of the destination, kv head, item). Every part finds the head's threshold for itself (the masses are
-// small beside the rows that move), so that the parts need not wait for each other; then each copies its slice of the
-// destination's rows. The threshold is found 8 bits at a time from histograms with a column per lane: no two lanes of a
-// warp count in the same place, however alike the masses are.
-constexpr int E_THREADS = 512, E_WARPS = E_THREADS / 32, E_KEYS = 16384, E_LIST = 4096;
-constexpr int E_SMEM = (E_KEYS + 256 * 32) * 4;
-static_assert(E_LIST <= 256 * 32 && E_KEYS / E_THREADS * E_WARPS == E_THREADS, "the list replaces the histogram");
+// One CTA per (part of the destination, kv head, item). Every part finds the head's threshold (the mass of the last key to
+// be kept) for itself, so that the parts need not wait for each other, and then moves its slice of the destination's rows.
+// The keys are held in registers, a run of up to 32 to a thread. The threshold is found 11, 11 and 10 bits at a time from
+// histograms in shared memory. What bounds it: few heads, the latency of a dozen dependent steps; many, HBM, which fetches
+// about twice the bytes of a scattered choice of rows (runs of 32 and of 2 bytes).
+// Tried and slower (192 heads of 8192 to 16384 keys, 4096 kept): the threshold 2 bits at a time by counting keys above
+// three candidates, 109 us; 8 bits at a time, by one CTA 90 us, by a cluster that adds its histograms up through
+// distributed shared memory 91 to 121 us.
+constexpr int E_THREADS = 512, E_WARPS = E_THREADS / 32, E_PER = 32, E_KEYS = E_THREADS * E_PER, E_PER_SM = 2;
+constexpr int E_BINS = 2048, E_SMEM = E_BINS * 4 + E_KEYS * 2;
+static_assert(E_WARPS == 16 && E_BINS == 4 * E_THREADS && E_KEYS <= 65535, "scans of 16 warps, 4 bins a thread, 16-bit counts");
 
-// A mass as an unsigned number of the same order: NaN as -inf, -0 as +0.
+// A mass as an unsigned number of the same order, above 0: NaN as -inf, -0 as +0.
 __device__ __forceinline__ uint32_t mass_key(float m) {
     const uint32_t b = m != m ? 0xff800000u : __float_as_uint(m + 0.f);
     return b & 0x80000000u ? ~b : b | 0x80000000u;
 }
 
-__global__ void __launch_bounds__(E_THREADS, 2) k_kv4_evict(const D1Kv4Evict* __restrict__ items, int n_items) {
+// Sum of v over the threads before this one, and over all of them; buf: a word per warp. Ends with every thread having
+// read buf only after the next barrier.
+__device__ __forceinline__ uint32_t cta_scan(uint32_t v, uint32_t* buf, uint32_t& all) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    uint32_t upto = v;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const uint32_t x = __shfl_up_sync(D1_FULL_MASK, upto, o);
+        if (lane >= o) upto += x;
+    }
+    if (lane == 31) buf[warp] = upto;
+    __syncthreads();
+    const uint32_t w = lane < E_WARPS ? buf[lane] : 0;
+    all = __reduce_add_sync(D1_FULL_MASK, w);
+    return upto - v + __reduce_add_sync(D1_FULL_MASK, lane < warp ? w : 0);
+}
+
+__global__ void __launch_bounds__(E_THREADS, E_PER_SM) k_kv4_evict(const D1Kv4Evict* __restrict__ items, int n_items) {
     extern __shared__ __align__(16) uint32_t e_smem[];
-    uint32_t* keys = e_smem;              // [E_KEYS]: the head's keys, or a stretch of them
-    uint32_t* hist = e_smem + E_KEYS;     // [256][32]
-    int* list = reinterpret_cast<int*>(hist);
-    __shared__ uint32_t bins[256], cnt[E_THREADS], wsum[E_WARPS], found[2];
+    uint32_t* hist = e_smem;                                       // [E_BINS]
+    uint16_t* list = reinterpret_cast<uint16_t*>(hist + E_BINS);   // [E_KEYS]: kept keys of the stretch, of the part's slice
+    __shared__ uint32_t buf[3][E_WARPS], found[3];
     pdl_entry();
-    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = blockIdx.y;
+    const int tid = threadIdx.x, g = blockIdx.y;
     for (int item = blockIdx.z; item < n_items; item += gridDim.z) {
-        const D1Kv4Evict it = items[item];
-        const int keep = min(it.keep, it.len), recent = min(it.recent, keep);
-        if (it.keep < 0 || it.recent < 0 || !kv4_cache_ok(it.len, it.cap, it.k4, it.v4, it.kp, it.vp) ||
-            (it.len > 0 && !it.mass) ||
-            !kv4_cache_ok(keep, it.dst_cap, it.dst_k4, it.dst_v4, it.dst_kp, it.dst_vp)) {
+        const D1Kv4Evict* it = items + item;
+        const int len = it->len, cap = it->cap, dst_cap = it->dst_cap;
+        const int keep = min(it->keep, len), recent = min(it->recent, keep);
+        if (it->keep < 0 || it->recent < 0 || !kv4_cache_ok(len, cap, it->k4, it->v4, it->kp, it->vp) ||
+            (len > 0 && !it->mass) || !kv4_cache_ok(keep, dst_cap, it->dst_k4, it->dst_v4, it->dst_kp, it->dst_vp)) {
             if (tid == 0) table_error();
             continue;
         }
-        const int per = (keep + gridDim.x - 1) / gridDim.x;
-        const int p0 = (int)min((long long)keep, (long long)blockIdx.x * per), p1 = min(keep, p0 + per);
+        const int slice = (keep + gridDim.x - 1) / gridDim.x;
+        const int p0 = (int)min((long long)keep, (long long)blockIdx.x * slice), p1 = min(keep, p0 + slice);
         if (p0 >= p1) continue;
-        const int nc = it.len - recent, want = keep - recent;  // keys to choose from, and how many
-        const bool choose = p0 < want;                         // (a slice of recent rows alone needs no threshold)
-        const float* m = it.mass + (size_t)g * it.cap;
-        const bool resident = nc <= E_KEYS;
-        auto stretch = [&](int base) {  // keys base .. into shared memory; zeros, below every key, behind the last
-            __syncthreads();
-            const int n = min(nc - base, E_KEYS), up = (n + E_THREADS - 1) / E_THREADS * E_THREADS;
-            for (int i = tid; i < up; i += E_THREADS) keys[i] = i < n ? mass_key(__ldg(m + base + i)) : 0;
-            __syncthreads();
-            return n;
+        const int nc = len - recent, want = keep - recent;  // keys to choose from, and how many
+        const size_t src0 = (size_t)g * cap, dst0 = (size_t)g * dst_cap;
+        const float* m = it->mass + src0;
+        // moves n rows base + list[i] -> to + i, and the recent ones at positions q0 .. q0 + more - 1. Four threads to a
+        // row, each with 16 bytes of K or V and one of the row's parameters, mass and index
+        auto move = [&](int n, int base, int to, int q0, int more) {
+            constexpr int UN = 4, ROWS = E_THREADS / 4;
+            const int part = tid & 3;
+            const uint4* from = reinterpret_cast<const uint4*>(part & 2 ? it->v4 : it->k4) + src0 * 2 + (part & 1);
+            uint4* dst = reinterpret_cast<uint4*>(part & 2 ? it->dst_v4 : it->dst_k4) + dst0 * 2 + (part & 1);
+            const uint16_t* par = reinterpret_cast<const uint16_t*>(part & 1 ? it->vp : it->kp) + src0;
+            uint16_t* dst_par = reinterpret_cast<uint16_t*>(part & 1 ? it->dst_vp : it->dst_kp) + dst0;
+            float* dst_mass = part == 2 ? it->dst_mass : nullptr;
+            int* kept = part == 3 ? it->kept : nullptr;
+            for (int r = tid >> 2; r < n + more; r += ROWS * UN) {
+                uint4 x[UN];
+                uint32_t y[UN];
+#pragma unroll
+                for (int i = 0; i < UN; i++) {
+                    const int q = r + i * ROWS;
+                    if (q >= n + more) continue;
+                    const int src = q < n ? base + list[q] : nc + (q0 - want) + q - n;
+                    x[i] = __ldg(from + (size_t)src * 2);
+                    y[i] = part < 2 ? __ldg(par + src) : part == 2 ? __float_as_uint(__ldg(m + src)) : (uint32_t)src;
+                }
+#pragma unroll
+                for (int i = 0; i < UN; i++) {
+                    const int q = r + i * ROWS;
+                    if (q >= n + more) continue;
+                    const size_t at = q < n ? to + q : q0 + q - n;
+                    dst[at * 2] = x[i];
+                    if (part < 2) dst_par[at] = (uint16_t)y[i];
+                    if (dst_mass) dst_mass[dst0 + at] = __uint_as_float(y[i]);
+                    if (kept) kept[dst0 + at] = (int)y[i];
+                }
+            }
         };
-        uint32_t t = 0, mask = 0, need = want;  // the threshold's known bits, and how many keys of those that share them
-        if (choose) {
-            if (resident) stretch(0);
+        const int q0 = max(p0, want);  // the slice's recent rows
+        int more = max(0, p1 - q0);
+        if (p0 < want) {
+            const bool resident = nc <= E_KEYS, wide = ((uintptr_t)m & 15) == 0;
+            const int run = resident ? ((nc + E_THREADS - 1) / E_THREADS + 3) & ~3 : E_PER;  // keys of a thread
+            uint32_t key[E_PER];  // keys base + tid * run + j; 0, below every key, behind the last
+            auto fetch = [&](int base) {
+                const int i0 = base + tid * run;
+#pragma unroll
+                for (int j = 0; j < E_PER; j += 4) {
+                    float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+                    if (j < run && wide && i0 + j + 3 < nc) {
+                        x = __ldg(reinterpret_cast<const float4*>(m + i0 + j));
+                    } else if (j < run) {
+                        if (i0 + j < nc) x.x = __ldg(m + i0 + j);
+                        if (i0 + j + 1 < nc) x.y = __ldg(m + i0 + j + 1);
+                        if (i0 + j + 2 < nc) x.z = __ldg(m + i0 + j + 2);
+                        if (i0 + j + 3 < nc) x.w = __ldg(m + i0 + j + 3);
+                    }
+                    key[j] = __float_as_uint(x.x);
+                    key[j + 1] = __float_as_uint(x.y);
+                    key[j + 2] = __float_as_uint(x.z);
+                    key[j + 3] = __float_as_uint(x.w);
+                }
+#pragma unroll
+                for (int j = 0; j < E_PER; j++)
+                    key[j] = j < run && i0 + j < nc ? mass_key(__uint_as_float(key[j])) : 0;
+            };
+            if (resident) fetch(0);
+            uint32_t t = 0, mask = 0, need = want;  // the threshold's known bits; how many of the keys sharing them are kept
+            bool exact = false;                     // all of them are
 #pragma unroll 1
-            for (int shift = 24; shift >= 0; shift -= 8) {
-                for (int i = tid; i < 256 * 32; i += E_THREADS) hist[i] = 0;
+            for (int d = 0; d < 3 && !exact; d++) {
+                const int shift = d == 0 ? 21 : d == 1 ? 10 : 0;
+                const uint32_t field = d == 2 ? 1023u : 2047u;
+                reinterpret_cast<uint4*>(hist)[tid] = make_uint4(0, 0, 0, 0);
                 __syncthreads();
                 for (int base = 0; base < nc; base += E_KEYS) {
-                    const int n = resident ? nc : stretch(base);
-                    for (int i = tid; i < n; i += E_THREADS) {
-                        const uint32_t k = keys[i];
-                        if ((k & mask) == t) atomicAdd(hist + ((k >> shift) & 255) * 32 + lane, 1u);
+                    if (!resident) fetch(base);
+#pragma unroll
+                    for (int j = 0; j < E_PER; j++) {
+                        if (j % 8 == 0 && j >= run) break;
+                        if (key[j] != 0 && (key[j] & mask) == t) atomicAdd(hist + ((key[j] >> shift) & field), 1u);
                     }
                 }
                 __syncthreads();
-                for (int b = warp; b < 256; b += E_WARPS) {
-                    const uint32_t v = __reduce_add_sync(D1_FULL_MASK, hist[b * 32 + lane]);
-                    if (lane == 0) bins[b] = v;
-                }
-                __syncthreads();
-                if (warp == 0) {  // the largest bin with at least `need` keys in it and above it
-                    uint32_t v[8], own = 0;
+                // the largest bin with `need` keys or more in it and above it: four bins a thread, from the top
+                const uint4 h = reinterpret_cast<const uint4*>(hist)[E_THREADS - 1 - tid];
+                const uint32_t v[4] = {h.w, h.z, h.y, h.x};
+                uint32_t all, before = cta_scan((h.x + h.y) + (h.z + h.w), buf[d], all);
 #pragma unroll
-                    for (int i = 0; i < 8; i++) own += v[i] = bins[255 - (lane * 8 + i)];
-                    uint32_t upto = own;
-#pragma unroll
-                    for (int o = 1; o < 32; o <<= 1) {
-                        const uint32_t x = __shfl_up_sync(D1_FULL_MASK, upto, o);
-                        if (lane >= o) upto += x;
+                for (int i = 0; i < 4; i++) {
+                    if (before < need && need <= before + v[i]) {
+                        found[0] = E_BINS - 1 - (tid * 4 + i);
+                        found[1] = need - before;
+                        found[2] = v[i];
                     }
-                    uint32_t before = upto - own;
-                    if (before < need && need <= upto) {
-#pragma unroll
-                        for (int i = 0; i < 8; i++) {
-                            if (before < need && need <= before + v[i]) {
-                                found[0] = 255 - (lane * 8 + i);
-                                found[1] = need - before;
-                                break;
-                            }
-                            before += v[i];
-                        }
-                    }
+                    before += v[i];
                 }
                 __syncthreads();
                 t |= found[0] << shift;
+                mask |= field << shift;
                 need = found[1];
-                mask |= 255u << shift;
+                exact = need == found[2];
             }
-        }
-        // of the keys equal to t, the first `need` are kept. Positions: keys above t and kept equal ones before
-        const size_t src0 = (size_t)g * it.cap, dst0 = (size_t)g * it.dst_cap;
-        for (int s0 = p0; s0 < p1; s0 += E_LIST) {
-            const int s1 = min(p1, s0 + E_LIST);
-            if (s0 < want) {
-                uint32_t above0 = 0, equal0 = 0;
-                for (int base = 0; base < nc; base += E_KEYS) {
-                    const int n = resident ? nc : stretch(base);
-                    // the counts of 32 successive keys (above t in the upper half, equal in the lower), summed up
-                    const int groups = (n + 31) / 32;
-                    for (int q = warp; q < groups; q += E_WARPS) {
-                        const uint32_t k = q * 32 + lane < n ? keys[q * 32 + lane] : 0;
-                        const uint32_t a = __ballot_sync(D1_FULL_MASK, k > t);
-                        const uint32_t e = __ballot_sync(D1_FULL_MASK, k == t && q * 32 + lane < n);
-                        if (lane == 0) cnt[q] = (uint32_t)__popc(a) << 16 | __popc(e);
-                    }
-                    __syncthreads();
-                    const uint32_t own = tid < groups ? cnt[tid] : 0;
-                    uint32_t upto = own;
+            if (exact) {  // every key with t's known bits is above a threshold just below them
+                t = t > 0 ? t - 1 : 0;
+                need = 0;
+            }
+            // the keys above t are kept, and the first `need` of those equal to it
+            uint32_t above0 = 0, equal0 = 0;
+            for (int base = 0; base < nc; base += E_KEYS) {
+                if (!resident) fetch(base);
+                uint32_t mine = 0;  // keys above t in the upper half, equal to it in the lower
 #pragma unroll
-                    for (int o = 1; o < 32; o <<= 1) {
-                        const uint32_t x = __shfl_up_sync(D1_FULL_MASK, upto, o);
-                        if (lane >= o) upto += x;
-                    }
-                    if (lane == 31) wsum[warp] = upto;
-                    __syncthreads();
-                    uint32_t add = 0, all = 0;
-                    for (int w = 0; w < E_WARPS; w++) {
-                        add += w < warp ? wsum[w] : 0;
-                        all += wsum[w];
-                    }
-                    cnt[tid] = upto - own + add;
-                    __syncthreads();
-                    for (int q = warp; q < groups; q += E_WARPS) {
-                        const int i = q * 32 + lane;
-                        const uint32_t k = i < n ? keys[i] : 0;
-                        const bool is_a = k > t, is_e = k == t && i < n;
-                        const uint32_t a = __ballot_sync(D1_FULL_MASK, is_a), e = __ballot_sync(D1_FULL_MASK, is_e);
-                        const uint32_t lower = (1u << lane) - 1, c = cnt[q];
-                        const uint32_t na = above0 + (c >> 16) + __popc(a & lower);
-                        const uint32_t ne = equal0 + (c & 0xffffu) + __popc(e & lower);
-                        const int pos = (int)(na + min(ne, need));
-                        if ((is_a || (is_e && ne < need)) && pos >= s0 && pos < s1) list[pos - s0] = base + i;
-                    }
-                    above0 += all >> 16;
-                    equal0 += all & 0xffffu;
-                    __syncthreads();
+                for (int j = 0; j < E_PER; j++) {
+                    if (j % 8 == 0 && j >= run) break;
+                    mine += (key[j] > t ? 0x10000u : 0u) + (key[j] == t && key[j] != 0 ? 1u : 0u);
                 }
-            }
-            auto source = [&](int pos) { return pos < want ? list[pos - s0] : nc + pos - want; };
-            const uint4 *k4 = reinterpret_cast<const uint4*>(it.k4), *v4 = reinterpret_cast<const uint4*>(it.v4);
-            uint4 *dk4 = reinterpret_cast<uint4*>(it.dst_k4), *dv4 = reinterpret_cast<uint4*>(it.dst_v4);
-            // a row is 4 pieces of 16 bytes: K, V and their halves
-            const int half = tid & 1;
-            const uint4* from = (tid & 2 ? v4 : k4) + src0 * 2 + half;
-            uint4* to = (tid & 2 ? dv4 : dk4) + dst0 * 2 + half;
-            constexpr int UN = 4, ROWS = E_THREADS / 4;
-            for (int r = s0 + (tid >> 2); r < s1; r += ROWS * UN) {
-                uint4 x[UN];
+                __syncthreads();  // buf[0] and the list have been read
+                uint32_t all;
+                const uint32_t ahead = cta_scan(mine, buf[0], all);
+                uint32_t na = above0 + (ahead >> 16), ne = equal0 + (ahead & 0xffffu);
+                const int to = (int)(above0 + min(equal0, need));  // position of this stretch's first kept key
+                const int first = max(to, p0);
 #pragma unroll
-                for (int i = 0; i < UN; i++)
-                    if (r + i * ROWS < s1) x[i] = __ldg(from + (size_t)source(r + i * ROWS) * 2);
-#pragma unroll
-                for (int i = 0; i < UN; i++)
-                    if (r + i * ROWS < s1) to[(size_t)(r + i * ROWS) * 2] = x[i];
+                for (int j = 0; j < E_PER; j++) {
+                    if (j % 8 == 0 && j >= run) break;
+                    const bool is_a = key[j] > t, is_e = key[j] == t && key[j] != 0;
+                    const int pos = (int)(na + min(ne, need));
+                    if ((is_a || (is_e && ne < need)) && pos >= first && pos < p1) list[pos - first] = (uint16_t)(tid * run + j);
+                    na += is_a;
+                    ne += is_e;
+                }
+                above0 += all >> 16;
+                equal0 += all & 0xffffu;
+                __syncthreads();
+                const bool last = base + E_KEYS >= nc;
+                move(max(0, min(p1, (int)(above0 + min(equal0, need))) - first), base, first, q0, last ? more : 0);
+                if (last) more = 0;
             }
-            for (int pos = s0 + tid; pos < s1; pos += E_THREADS) {
-                const int i = source(pos);
-                const d1_half a = it.kp[src0 + i], b = it.vp[src0 + i];
-                const float w = m[i];
-                it.dst_kp[dst0 + pos] = a;
-                it.dst_vp[dst0 + pos] = b;
-                if (it.dst_mass) it.dst_mass[dst0 + pos] = w;
-                if (it.kept) it.kept[dst0 + pos] = i;
-            }
-            __syncthreads();
+            __syncthreads();  // the list and the histogram have been read
         }
+        if (more > 0) move(0, 0, 0, q0, more);
     }
 }
 
@@ -368,10 +392,10 @@ extern "C" int d1_kv4_evict(const D1Kv4Evict* items, int n_items, int max_len, i
         if (cudaFuncSetAttribute(k_kv4_evict, cudaFuncAttributeMaxDynamicSharedMemorySize, E_SMEM) != cudaSuccess) return -1;
         __atomic_fetch_or(&done, bit, __ATOMIC_RELEASE);
     }
-    // two CTAs fit an SM: enough parts to occupy them all, of no less than 128 rows were every key kept
+    // parts to occupy the GPU, at most 8 (each finds the threshold again), of no less than 64 rows were every key kept
     const int z = n_items < kMaxGridZ ? n_items : kMaxGridZ;
-    const long long heads = (long long)kv_heads * z;
-    long long parts = (2 * 148 + heads - 1) / heads, most = (max_len + 127) / 128;
+    const long long heads = (long long)kv_heads * z, most = max_len > 448 ? 8 : (max_len + 63) / 64;
+    long long parts = E_PER_SM * 148 / heads;
     parts = parts > most ? most : parts;
     launch_pdl(k_kv4_evict, dim3(parts < 1 ? 1 : (unsigned)parts, kv_heads, z), E_THREADS, E_SMEM, st, items, n_items);
     return (int)cudaGetLastError();
