@@ -1,5 +1,6 @@
 // Key/value caches held in 4 bits (format: include/d1kernels.h, D1Kv4Seq): rows into a cache and back, and eviction by
 // accumulated attention weight. The attention over such caches is in kv4_attn.cu.
+#include "attn_tc.cuh"
 #include "kv4.cuh"
 
 using namespace d1;
@@ -30,52 +31,52 @@ __device__ __forceinline__ bool append_ok(const D1Kv4Seq& s) {
 }
 
 // One vector's word of codes (this lane's 8 elements) and parameter. round(x / step) without a division per element:
-// t = x * (1 / step) is within 2^-19 of the quotient q, |q| < 15.6. As x has 11 significant bits and step 7, q either is
-// k + 1/2 exactly or at least 2^-13 away from it; t rounded to a multiple of 2^-14 (by adding and taking away 768) is
-// therefore k + 1/2 in the first case and on q's side of it in the second, and rounds as q does.
+// t = x * (1 / step) is within 2^-18 of the quotient q, |q| < 15.6. As x has 11 significant bits and step 7, q either is
+// k + 1/2 exactly or at least 2^-13 away from it; 768 + t, whose last place is 2^-14, is therefore 768 + k + 1/2 in the
+// first case and on q's side of it in the second, and rounds as q does. (hi - lo) / 15 is rounded correctly, since whole
+// multiples of 15 are common: one step of correction after the product with 1 / 15.
 __device__ __forceinline__ void quantise8(const uint4& raw, uint32_t& word, uint32_t& par) {
     const __half2* x2 = reinterpret_cast<const __half2*>(&raw);
-    __half2 mn = __float2half2_rn(0.f), mx = mn, bad = mn;  // the range, with zero in it
+    __half2 mn = __float2half2_rn(0.f), mx = mn;  // the range, with zero in it; NaN stays
 #pragma unroll
     for (int i = 0; i < 4; i++) {
-        mn = __hmin2(mn, x2[i]);
-        mx = __hmax2(mx, x2[i]);
-        bad = __hfma2(x2[i], __float2half2_rn(0.f), bad);  // NaN after a NaN or an infinity
+        mn = __hmin2_nan(mn, x2[i]);
+        mx = __hmax2_nan(mx, x2[i]);
     }
+    __half2 ends = __halves2half2(__hneg(__hmin_nan(__low2half(mn), __high2half(mn))),
+                                  __hmax_nan(__low2half(mx), __high2half(mx)));  // (-lo, hi)
 #pragma unroll
-    for (int o = 1; o < 8; o <<= 1) {
-        mn = __hmin2(mn, __shfl_xor_sync(D1_FULL_MASK, mn, o));
-        mx = __hmax2(mx, __shfl_xor_sync(D1_FULL_MASK, mx, o));
-        bad = __hadd2(bad, __shfl_xor_sync(D1_FULL_MASK, bad, o));
-    }
-    const float lo = __half2float(__hmin(__low2half(mn), __high2half(mn)));
-    const float hi = __half2float(__hmax(__low2half(mx), __high2half(mx)));
+    for (int o = 1; o < 8; o <<= 1) ends = __hmax2_nan(ends, __shfl_xor_sync(D1_FULL_MASK, ends, o));
+    const float nlo = __low2float(ends), hi = __high2float(ends), range = hi + nlo;
+    constexpr float kFifteenth = 1.f / 15.f;
+    float want = range * kFifteenth;
+    want = fmaf(fmaf(-15.f, want, range), kFifteenth, want);
     // 7 significant bits upwards: carry into the mantissa's upper 6 bits; below 2^-14 a multiple of 2^-20
-    const float want = __fdiv_rn(hi - lo, 15.f);
     const float step = want >= 6.103515625e-5f ? __uint_as_float((__float_as_uint(want) + 0x1ffffu) & ~0x1ffffu)
                                                : ceilf(want * 1048576.f) * 9.5367431640625e-7f;
-    const float div = step > 0.f ? step : 1.f, inv = __fdiv_rn(1.f, div);
-    const int zero = min(__float2int_rn(__fdiv_rn(-lo, div)), 15);
+    float inv;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(inv) : "f"(step > 0.f ? step : 1.f));
+    constexpr int kBias = 0x4b400000 + 768;  // 768 + t + 1.5 * 2^23 has round(t) + 768 in the low bits
+    const int zero = min(__float_as_int(fmaf(nlo, inv, 768.f) + 12582912.f) - kBias, 15);
     int top = 15;  // |code - zero| * step stays within fp16; only a range above 65504 comes near
-    if (step > 4096.f) top = min(15, __float2int_rd(__fdiv_rn(65504.f, div)));
-    constexpr int kBias = 0x4b400000;  // 1.5 * 2^23: its sum with t is round(t) in the low bits
+    if (step > 4096.f) top = min(15, __float2int_rd(__fdiv_rn(65504.f, step)));
     const int least = kBias + max(-top, -zero), most = kBias + min(top, 15 - zero);
+    const uint64_t inv2 = f2_pack(inv, inv);
     uint32_t w = 0;
 #pragma unroll
     for (int i = 0; i < 4; i++) {
         const float2 f = __half22float2(x2[i]);
-#pragma unroll
-        for (int h = 0; h < 2; h++) {
-            const float t = ((h ? f.y : f.x) * inv + 768.f) - 768.f;
-            const int q = max(least, min(most, __float_as_int(t + 12582912.f)));
-            w += (uint32_t)q << (16 * h + 4 * i);  // the biases go out of all eight places together
-        }
+        float a, b;
+        f2_unpack(f2_add(f2_fma(f2_pack(f.x, f.y), inv2, f2_pack(768.f, 768.f)), f2_pack(12582912.f, 12582912.f)), a, b);
+        // the biases go out of all eight places together
+        w += (uint32_t)max(least, min(most, __float_as_int(a))) << (4 * i);
+        w += (uint32_t)max(least, min(most, __float_as_int(b))) << (16 + 4 * i);
     }
     word = w + (uint32_t)(zero - kBias) * 0x11111111u;
     par = (uint32_t)__half_as_ushort(__float2half_rn(step)) | (uint32_t)zero;
-    if (__hisnan(__low2half(bad)) || __hisnan(__high2half(bad))) {
+    if (!(range <= 131008.f)) {  // NaN or an infinity among them: a NaN step
         word = 0;
-        par = 0x7e00u;  // a NaN step
+        par = 0x7e00u;
     }
 }
 
