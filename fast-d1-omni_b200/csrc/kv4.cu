@@ -22,9 +22,11 @@ __device__ __forceinline__ void table_error() { atomicExch(&g_kv4_err, kErrTable
 
 // ------------------------------------------------------------------------------------------------ append, load
 // Bound by HBM. 8 lanes per vector of 64 dimensions (8 elements, one word of codes a lane), 4 consecutive rows of one kv
-// head per warp, so that a warp's codes are one 128-byte run of the cache. CTA: 128 rows of (K or V, kv head), four to a
-// thread, whose loads go out together.
-constexpr int A_STEP = 32, A_PER = 4, A_ROWS = A_STEP * A_PER;
+// head per warp, so that a warp's codes are one 128-byte run of the cache. A CTA takes 32 rows of (K or V, kv head) for
+// each of PER to a thread, whose loads go out together. Append: 8 where that still occupies every SM twice, otherwise 2
+// (32 x 4096 rows, 8 kv heads: 78 us with 8, 85 with 4, 91 with 2, and 53 at the copy rate; one prefix of 1025 rows: 3.8,
+// 2.9 and 2.5 us). Load: 4 (56, 57 and 66 us with 4, 8 and 2, and 53 at the copy rate).
+constexpr int A_STEP = 32;
 
 __device__ __forceinline__ bool append_ok(const D1Kv4Seq& s) {
     return s.kv_start >= 0 && s.kv_len >= 0 && kv4_seq_ok(s) && (long long)s.ext_len + s.kv_len <= s.ext_cap;
@@ -80,6 +82,7 @@ __device__ __forceinline__ void quantise8(const uint4& raw, uint32_t& word, uint
     }
 }
 
+template <int PER>
 __global__ void __launch_bounds__(256) k_kv4_append(const __half* __restrict__ K, const __half* __restrict__ V,
                                                     int ldkv, const D1Kv4Seq* __restrict__ seqs, int n_seqs) {
     pdl_entry();
@@ -95,15 +98,15 @@ __global__ void __launch_bounds__(256) k_kv4_append(const __half* __restrict__ K
         const size_t at = (size_t)g * s.ext_cap + s.ext_len;
         uint32_t* codes = reinterpret_cast<uint32_t*>(is_v ? s.v4 : s.k4) + at * 8 + sub;
         uint16_t* pars = reinterpret_cast<uint16_t*>(is_v ? s.vp : s.kp) + at;
-        for (int r0 = blockIdx.x * A_ROWS; r0 < s.kv_len; r0 += gridDim.x * A_ROWS) {
-            uint4 raw[A_PER];
+        for (int r0 = blockIdx.x * (A_STEP * PER); r0 < s.kv_len; r0 += gridDim.x * (A_STEP * PER)) {
+            uint4 raw[PER];
 #pragma unroll
-            for (int i = 0; i < A_PER; i++) {
+            for (int i = 0; i < PER; i++) {
                 const int r = r0 + i * A_STEP + row;
                 raw[i] = r < s.kv_len ? __ldcs(reinterpret_cast<const uint4*>(src + (size_t)r * ldkv)) : make_uint4(0, 0, 0, 0);
             }
 #pragma unroll
-            for (int i = 0; i < A_PER; i++) {
+            for (int i = 0; i < PER; i++) {
                 if (r0 + i * A_STEP >= s.kv_len) break;
                 const int r = r0 + i * A_STEP + row;
                 uint32_t word, par;
@@ -117,6 +120,7 @@ __global__ void __launch_bounds__(256) k_kv4_append(const __half* __restrict__ K
     }
 }
 
+template <int PER>
 __global__ void __launch_bounds__(256) k_kv4_load(const D1Kv4Seq* __restrict__ seqs, int n_seqs, __half* __restrict__ K,
                                                   __half* __restrict__ V, int ldkv) {
     pdl_entry();
@@ -132,16 +136,16 @@ __global__ void __launch_bounds__(256) k_kv4_load(const D1Kv4Seq* __restrict__ s
         const size_t at = (size_t)g * s.ext_cap + s.ext_len;
         const uint32_t* codes = reinterpret_cast<const uint32_t*>(is_v ? s.v4 : s.k4) + at * 8 + sub;
         const uint16_t* pars = reinterpret_cast<const uint16_t*>(is_v ? s.vp : s.kp) + at;
-        for (int r0 = blockIdx.x * A_ROWS; r0 < s.kv_len; r0 += gridDim.x * A_ROWS) {
-            uint32_t word[A_PER], par[A_PER];
+        for (int r0 = blockIdx.x * (A_STEP * PER); r0 < s.kv_len; r0 += gridDim.x * (A_STEP * PER)) {
+            uint32_t word[PER], par[PER];
 #pragma unroll
-            for (int i = 0; i < A_PER; i++) {
+            for (int i = 0; i < PER; i++) {
                 const int r = min(r0 + i * A_STEP + row, s.kv_len - 1);
                 word[i] = codes[(size_t)r * 8];
                 par[i] = pars[r];
             }
 #pragma unroll
-            for (int i = 0; i < A_PER; i++) {
+            for (int i = 0; i < PER; i++) {
                 const int r = r0 + i * A_STEP + row;
                 const uint32_t p2 = par[i] * 0x00010001u, st = kv4_step2(p2);
                 uint32_t z0, z1, v[4];
@@ -358,9 +362,8 @@ bool bad_rows(const void* K, const void* V, int ldkv, int kv_heads) {
     return !K || !V || (((uintptr_t)K | (uintptr_t)V) & 15) || ldkv % 8 || ldkv < kv_heads * 64;
 }
 
-dim3 row_grid(int max_rows, int kv_heads, int n_seqs) {
-    int x = (max_rows + A_ROWS - 1) / A_ROWS;
-    x = x < 1 ? 1 : x > 4096 ? 4096 : x;
+dim3 row_grid(int max_rows, int per, int kv_heads, int n_seqs) {
+    const int rows = A_STEP * per, x = max_rows <= rows ? 1 : max_rows > 4096 * rows ? 4096 : (max_rows - 1) / rows + 1;
     return dim3(x, kv_heads * 2, n_seqs < kMaxGridZ ? n_seqs : kMaxGridZ);
 }
 
@@ -370,7 +373,11 @@ extern "C" int d1_kv4_append(const d1_half* K, const d1_half* V, int ldkv, const
                              int max_rows, int kv_heads, cudaStream_t st) {
     if (n_seqs <= 0) return n_seqs == 0 ? 0 : -1;
     if (!seqs || max_rows < 0 || kv_heads <= 0 || kv_heads > 4096 || bad_rows(K, V, ldkv, kv_heads)) return -1;
-    launch_pdl(k_kv4_append, row_grid(max_rows, kv_heads, n_seqs), 256, 0, st, K, V, ldkv, seqs, n_seqs);
+    const dim3 g8 = row_grid(max_rows, 8, kv_heads, n_seqs);
+    if ((long long)g8.x * g8.y * g8.z >= 2 * 148)
+        launch_pdl(k_kv4_append<8>, g8, 256, 0, st, K, V, ldkv, seqs, n_seqs);
+    else
+        launch_pdl(k_kv4_append<2>, row_grid(max_rows, 2, kv_heads, n_seqs), 256, 0, st, K, V, ldkv, seqs, n_seqs);
     return (int)cudaGetLastError();
 }
 
@@ -378,7 +385,7 @@ extern "C" int d1_kv4_load(const D1Kv4Seq* seqs, int n_seqs, int max_rows, int k
                            int ldkv, cudaStream_t st) {
     if (n_seqs <= 0) return n_seqs == 0 ? 0 : -1;
     if (!seqs || max_rows < 0 || kv_heads <= 0 || kv_heads > 4096 || bad_rows(K, V, ldkv, kv_heads)) return -1;
-    launch_pdl(k_kv4_load, row_grid(max_rows, kv_heads, n_seqs), 256, 0, st, seqs, n_seqs, K, V, ldkv);
+    launch_pdl(k_kv4_load<4>, row_grid(max_rows, 4, kv_heads, n_seqs), 256, 0, st, seqs, n_seqs, K, V, ldkv);
     return (int)cudaGetLastError();
 }
 
