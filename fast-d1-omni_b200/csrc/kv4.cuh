@@ -46,9 +46,9 @@ __device__ __forceinline__ uint32_t lop3(uint32_t a, uint32_t b, uint32_t c) {
 // The zero points of two parameters (one in each half) as the fp16 pairs that the expansion subtracts: 1024 + zero for
 // codes at bits 0-3 of a half, 64 + zero for codes at bits 4-7.
 __device__ __forceinline__ void kv4_zero(uint32_t par2, uint32_t& z0, uint32_t& z1) {
-    const uint32_t z = par2 & 0x000f000fu;
-    z0 = z | 0x64006400u;
-    z1 = (z << 4) | 0x54005400u;
+    constexpr int kAndOr = (0xf0 & 0xcc) | 0xaa;
+    z0 = lop3<kAndOr>(par2, 0x000f000fu, 0x64006400u);
+    z1 = lop3<kAndOr>(par2 << 4, 0x00f000f0u, 0x54005400u);
 }
 __device__ __forceinline__ uint32_t kv4_step2(uint32_t par2) { return par2 & 0xfff0fff0u; }
 __device__ __forceinline__ float kv4_step(uint32_t par) { return __half2float(__ushort_as_half(par & 0xfff0u)); }

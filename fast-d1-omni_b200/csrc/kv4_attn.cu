@@ -9,6 +9,7 @@ using namespace d1;
 namespace {
 
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
+constexpr float kLazyRescale = 8.f;  // log2: how far scores may exceed the reference of a running softmax
 
 struct Kv4Args {
     const __half* Q;
@@ -18,7 +19,7 @@ struct Kv4Args {
     float* lse;
     const D1Kv4Seq* seqs;
     int* err;
-    int ldq, ldkv, ldo, lse_ld, n_seqs, heads, group, q_rows, kv_rows, accumulate;
+    int ldq, ldkv, ldo, lse_ld, n_seqs, heads, group, q_rows, kv_rows, accumulate, ranks;
     int n_blocks;  // tcgen05 forms: blocks of rows per sequence (attention), tiles of keys per cache (mass)
     float scale_log2;
 };
@@ -63,32 +64,60 @@ __device__ __forceinline__ void ex2_fma2(float x0, float x1, float& p0, float& p
 
 // ------------------------------------------------------------------------------------------------ attention, few rows
 // The query rows of a kv head's group are packed: packed row p is row p / group of the sequence, head p % group of the
-// group. A CTA takes 16 * MT packed rows of one (sequence, kv head); its warps take tiles of 64 keys in turn, each with
-// its own running maximum, sum and output, which they join at the end through shared memory.
+// group. A cluster of 1 to 8 CTAs takes 8 * NT packed rows of one (sequence, kv head); the CTAs share out its tiles of 64
+// keys, and the warps of a CTA take theirs in turn, each with its own running maximum, sum and output. They are joined
+// through shared memory, and the CTAs of a cluster through distributed shared memory, always in the same order.
 //
-// The codes go from global memory to the registers of the MMAs (m16n8k16) directly. An MMA's k index may run over the
-// dimensions in any order as long as both operands use the same: for S = Q K^T lane (r, t) = (lane / 4, lane % 4) holds
-// dimensions 16t .. 16t+15 of key r of each 8 keys: 8 bytes of codes, and 32 bytes of a query row. The MMA sees the whole
-// numbers code - zero; a key's step multiplies its column of S afterwards, in fp32, with the softmax scale. For O = P V
-// lane (r, t) holds word r (dimensions 8r .. 8r+7) of keys 2t, 2t+1, 2t+8, 2t+9 of each 16 keys; byte permutes bring two
-// keys' codes of one dimension together, and the values are (code - zero) * step, exact in fp16. n index r of the j-th MMA
-// is dimension 8r + j, so that a lane ends with dimensions 16t .. 16t+15 of its rows.
-constexpr int R_KEYS = 64, R_WARPS = 8, R_OLD = 68;  // padded row of the joining buffer (floats)
+// Everything is transposed, S^T = K Q^T and O^T = V^T P^T on m16n8k16, so that 8 rows fill an MMA's n. The codes go from
+// global memory to the registers of the A operands directly. An MMA's k index may run over the dimensions in any order as
+// long as both operands use the same: for S^T lane (r, t) = (lane / 4, lane % 4) holds dimensions 16t .. 16t+15 of keys r
+// and r + 8 of each 16: 8 bytes of codes, and 32 bytes of a query row. The MMA sees the codes as they are, for a code at
+// bits 0-3 or 4-7 of a half is the fp16 number code * 2^-24 or code * 2^-20; in fp32, a key's step and the softmax scale
+// multiply the sums, and zero times the query row's sum is taken away. For O^T lane (r, t) holds word r (dimensions
+// 8r .. 8r+7) of keys 2t, 2t+1, 2t+8, 2t+9 of each 16; byte permutes bring two keys' codes of one dimension together, and
+// the values are (code - zero) * step, exact in fp16. Row r of the j-th m tile is dimension 8r + 2j, row r + 8 dimension
+// 8r + 2j + 1, so that a lane ends with dimensions 8r .. 8r+7 of packed rows 2t and 2t + 1. P^T turns from the result's
+// layout into the B operand's by movmatrix.
+// Bound: the issue slots (about 750 instructions a tile, half of them for the expansion of codes).
+constexpr int R_KEYS = 64, R_WARPS = 4, R_CLUSTER = 8, R_LD = 68;  // padded row of the joining buffers (floats)
 
-template <int MT>
+template <int NT>
 constexpr int rows_smem() {
-    return R_WARPS * 16 * MT * (R_OLD + 2) * 4;
+    return (R_WARPS + 1) * 8 * NT * (R_LD + 2) * 4;
 }
 
-template <int MT>
-__global__ void __launch_bounds__(R_WARPS * 32) k_kv4_attn_rows(const Kv4Args a) {
+__device__ __forceinline__ uint32_t movmatrix_trans(uint32_t x) {
+    uint32_t y;
+    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+    return y;
+}
+__device__ __forceinline__ float ld_cluster_f32(uint32_t addr) {
+    float v;
+    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
+    return v;
+}
+__device__ __forceinline__ float4 ld_cluster_f32x4(uint32_t addr) {
+    float4 v;
+    asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+                 : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
+                 : "r"(addr)
+                 : "memory");
+    return v;
+}
+
+template <int NT>
+__global__ void __launch_bounds__(R_WARPS * 32, NT == 1 ? 4 : 2) k_kv4_attn_rows(const Kv4Args a) {
     extern __shared__ __align__(16) float r_smem[];
-    constexpr int NR = 16 * MT;
-    float* sO = r_smem;                           // [warp][NR][R_OLD]
-    float* sM = sO + R_WARPS * NR * R_OLD;        // [warp][NR]
-    float* sL = sM + R_WARPS * NR;                // [warp][NR]
+    constexpr int NR = 8 * NT;
+    float* sO = r_smem;                               // [warp][NR][R_LD]
+    float* cO = sO + R_WARPS * NR * R_LD;             // [NR][R_LD]: the CTA's sum, read by the cluster
+    float* sM = cO + NR * R_LD;                       // [warp][NR]
+    float* cM = sM + R_WARPS * NR;                    // [NR]
+    float* sL = cM + NR;                              // [warp][NR]
+    float* cL = sL + R_WARPS * NR;                    // [NR]
     pdl_entry();
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, r = lane >> 2, t = lane & 3, g = blockIdx.y;
+    const int rank = (int)cluster_ctarank(), ranks = a.ranks;
     for (int sq = blockIdx.z; sq < a.n_seqs; sq += gridDim.z) {
         const D1Kv4Seq s = a.seqs[sq];
         if (!kv4_seq_ok(s) || !rows_ok(s.q_start, s.q_len, a.q_rows) || !rows_ok(s.kv_start, s.kv_len, a.kv_rows)) {
@@ -97,155 +126,219 @@ __global__ void __launch_bounds__(R_WARPS * 32) k_kv4_attn_rows(const Kv4Args a)
         }
         const long long n_rows = (long long)s.q_len * a.group;
         const int ext_tiles = (s.ext_len + R_KEYS - 1) / R_KEYS, tiles = ext_tiles + (s.kv_len + R_KEYS - 1) / R_KEYS;
-        const uint8_t* k4 = s.k4 + (size_t)g * s.ext_cap * 32;
-        const uint8_t* v4 = s.v4 + (size_t)g * s.ext_cap * 32;
+        // this CTA's tiles
+        const int per = (tiles + ranks - 1) / ranks, tile0 = min(tiles, rank * per), tile1 = min(tiles, tile0 + per);
+        const uint8_t* k4 = s.k4 + (size_t)g * s.ext_cap * 32 + 8 * t;
+        const uint8_t* v4 = s.v4 + (size_t)g * s.ext_cap * 32 + 4 * r;
         const uint16_t* kp = reinterpret_cast<const uint16_t*>(s.kp) + (size_t)g * s.ext_cap;
         const uint16_t* vp = reinterpret_cast<const uint16_t*>(s.vp) + (size_t)g * s.ext_cap;
-        for (long long base = (long long)blockIdx.x * NR; base < n_rows; base += (long long)gridDim.x * NR) {
-            // ---- the query rows, as A operands
-            uint32_t qa[MT][4][4];
+        for (long long base = (long long)(blockIdx.x / ranks) * NR; base < n_rows; base += (long long)(gridDim.x / ranks) * NR) {
+            // ---- the query rows, as B operands: [n tile][k step][2]
+            uint32_t qb[NT][4][2];
 #pragma unroll
-            for (int mt = 0; mt < MT; mt++) {
-#pragma unroll
-                for (int hf = 0; hf < 2; hf++) {
-                    const long long p = base + mt * 16 + hf * 8 + r;
-                    uint4 x0 = make_uint4(0, 0, 0, 0), x1 = x0;
-                    if (p < n_rows) {
-                        const int row = (int)(p / a.group), h = g * a.group + (int)(p % a.group);
-                        const uint4* src =
-                            reinterpret_cast<const uint4*>(a.Q + (size_t)(s.q_start + row) * a.ldq + h * 64 + 16 * t);
-                        x0 = __ldg(src);
-                        x1 = __ldg(src + 1);
-                    }
-                    const uint32_t w[8] = {x0.x, x0.y, x0.z, x0.w, x1.x, x1.y, x1.z, x1.w};
-#pragma unroll
-                    for (int ks = 0; ks < 4; ks++) {
-                        qa[mt][ks][hf] = w[2 * ks];
-                        qa[mt][ks][2 + hf] = w[2 * ks + 1];
-                    }
+            for (int nt = 0; nt < NT; nt++) {
+                const long long p = base + nt * 8 + r;
+                uint4 x0 = make_uint4(0, 0, 0, 0), x1 = x0;
+                if (p < n_rows) {
+                    const int row = (int)(p / a.group), h = g * a.group + (int)(p % a.group);
+                    const uint4* src =
+                        reinterpret_cast<const uint4*>(a.Q + (size_t)(s.q_start + row) * a.ldq + h * 64 + 16 * t);
+                    x0 = __ldg(src);
+                    x1 = __ldg(src + 1);
                 }
+                const uint32_t w[8] = {x0.x, x0.y, x0.z, x0.w, x1.x, x1.y, x1.z, x1.w};
+#pragma unroll
+                for (int i = 0; i < 8; i++) qb[nt][i >> 1][i & 1] = w[i];
             }
-            float o[MT][8][4], m[MT][2], l[MT][2];
+            float o[NT][4][4], m[NT][2], l[NT][2];  // rows 2t and 2t + 1 of each n tile
+            float qs[NT][2];                        // sums of the query rows, for the zeros
 #pragma unroll
-            for (int mt = 0; mt < MT; mt++) {
+            for (int nt = 0; nt < NT; nt++) {
+                float sum = 0.f;
 #pragma unroll
-                for (int j = 0; j < 8; j++)
+                for (int i = 0; i < 8; i++) {
+                    const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&qb[nt][i >> 1][i & 1]));
+                    sum += f.x + f.y;
+                }
+                sum += __shfl_xor_sync(D1_FULL_MASK, sum, 1);
+                sum += __shfl_xor_sync(D1_FULL_MASK, sum, 2);
+                qs[nt][0] = __shfl_sync(D1_FULL_MASK, sum, 8 * t);
+                qs[nt][1] = __shfl_sync(D1_FULL_MASK, sum, 8 * t + 4);
 #pragma unroll
-                    for (int c = 0; c < 4; c++) o[mt][j][c] = 0.f;
-                m[mt][0] = m[mt][1] = -INFINITY;
-                l[mt][0] = l[mt][1] = 0.f;
+                for (int j = 0; j < 4; j++)
+#pragma unroll
+                    for (int c = 0; c < 4; c++) o[nt][j][c] = 0.f;
+                m[nt][0] = m[nt][1] = 0.f;
+                l[nt][0] = l[nt][1] = 0.f;
             }
-            for (int tile = warp; tile < tiles; tile += R_WARPS) {
+            bool started = false;  // this warp has had a tile
+            uint2 kw[8];       // cached: this lane's codes of keys 8i + r
+            uint32_t pk = 0;   // K parameters of keys 2 lane, 2 lane + 1
+            auto fetch_k = [&](int tile) {
+                const int key0 = tile * R_KEYS, last = min(s.ext_len - key0, R_KEYS) - 1;
+                const uint8_t* src = k4 + (size_t)key0 * 32;
+                if (last == R_KEYS - 1) {
+#pragma unroll
+                    for (int i = 0; i < 8; i++) kw[i] = __ldg(reinterpret_cast<const uint2*>(src + r * 32 + i * 256));
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 8; i++) kw[i] = __ldg(reinterpret_cast<const uint2*>(src + min(8 * i + r, last) * 32));
+                }
+                // whole pairs are inside the cache's arrays: ext_cap is a multiple of 8
+                pk = __ldg(reinterpret_cast<const uint32_t*>(kp + key0 + (min(2 * lane, last) & ~1)));
+            };
+            int tile = tile0 + warp;
+            if (tile < tile1 && tile < ext_tiles) fetch_k(tile);
+            for (; tile < tile1; tile += R_WARPS) {
                 const bool ext = tile < ext_tiles;
                 const int key0 = (ext ? tile : tile - ext_tiles) * R_KEYS;
                 const int left = (ext ? s.ext_len : s.kv_len) - key0;  // keys of this tile: min(left, 64), at least 1
                 const int last = min(left, R_KEYS) - 1;
-                float sc[MT][8][4];
+                float sc[NT][4][4];  // keys 16i + r (0, 1) and 16i + 8 + r (2, 3), rows 2t and 2t + 1
                 uint32_t vw[4][4];   // cached: the words of V
                 uint32_t pv = 0;     // cached: V parameters of keys 2 lane, 2 lane + 1
                 if (ext) {
-                    uint2 kw[8];
+                    const uint8_t* src = v4 + (size_t)key0 * 32;
+                    if (last == R_KEYS - 1) {
 #pragma unroll
-                    for (int n = 0; n < 8; n++)
-                        kw[n] = __ldg(reinterpret_cast<const uint2*>(k4 + (size_t)(key0 + min(8 * n + r, last)) * 32) + t);
+                        for (int i = 0; i < 16; i++)
+                            vw[i >> 2][i & 3] = __ldg(reinterpret_cast<const uint32_t*>(
+                                src + t * 64 + ((i >> 2) * 16 + (i & 1) + (i & 2) * 4) * 32));
+                    } else {
 #pragma unroll
-                    for (int ks = 0; ks < 4; ks++)
-#pragma unroll
-                        for (int i = 0; i < 4; i++)
-                            vw[ks][i] = __ldg(reinterpret_cast<const uint32_t*>(
-                                                  v4 + (size_t)(key0 + min(16 * ks + 2 * t + (i & 1) + (i >> 1) * 8, last)) * 32) +
-                                              r);
-                    // whole pairs are inside the cache's arrays: ext_cap is a multiple of 8
-                    const int pk = key0 + (min(2 * lane, last) & ~1);
-                    const uint32_t pkw = __ldg(reinterpret_cast<const uint32_t*>(kp + pk));
-                    pv = __ldg(reinterpret_cast<const uint32_t*>(vp + pk));
+                        for (int i = 0; i < 16; i++)
+                            vw[i >> 2][i & 3] = __ldg(reinterpret_cast<const uint32_t*>(
+                                src + min((i >> 2) * 16 + 2 * t + (i & 1) + (i & 2) * 4, last) * 32));
+                    }
+                    pv = __ldg(reinterpret_cast<const uint32_t*>(vp + key0 + (min(2 * lane, last) & ~1)));
                     // rows behind the cached ones hold anything: step 0 there, so that 0 * V is 0
                     if (2 * lane + 1 > last) pv = 2 * lane > last ? 0 : pv & 0xffffu;
 #pragma unroll
-                    for (int n = 0; n < 8; n++) {
-                        const uint32_t both = __shfl_sync(D1_FULL_MASK, pkw, 4 * n + (r >> 1));
-                        const uint32_t par = __byte_perm(both, 0, r & 1 ? 0x3232 : 0x1010);
-                        uint32_t z0, z1, b0[4], b1[4];
-                        kv4_zero(par, z0, z1);
-                        kv4_expand(kw[n].x, z0, z1, b0);
-                        kv4_expand(kw[n].y, z0, z1, b1);
-                        const uint32_t pc = __shfl_sync(D1_FULL_MASK, pkw, 4 * n + t);
-                        const float st0 = kv4_step(pc & 0xffffu) * a.scale_log2, st1 = kv4_step(pc >> 16) * a.scale_log2;
+                    for (int i = 0; i < 4; i++) {
+                        // even and odd places of a half, whose codes count 2^-24 and 2^-20, in MMAs of their own
+                        uint32_t ke[2][4], ko[2][4];
+                        float st[2], zs[2];
 #pragma unroll
-                        for (int mt = 0; mt < MT; mt++) {
-                            float c[4] = {0.f, 0.f, 0.f, 0.f};
-                            mma16816(c, qa[mt][0], b0[0], b0[1]);
-                            mma16816(c, qa[mt][1], b0[2], b0[3]);
-                            mma16816(c, qa[mt][2], b1[0], b1[1]);
-                            mma16816(c, qa[mt][3], b1[2], b1[3]);
-                            sc[mt][n][0] = c[0] * st0;
-                            sc[mt][n][1] = c[1] * st1;
-                            sc[mt][n][2] = c[2] * st0;
-                            sc[mt][n][3] = c[3] * st1;
+                        for (int hf = 0; hf < 2; hf++) {
+                            const int n = 2 * i + hf;
+                            const uint32_t both = __shfl_sync(D1_FULL_MASK, pk, 4 * n + (r >> 1));
+                            const uint32_t par = both >> (16 * (r & 1));
+                            ke[0][hf] = kw[n].x & 0x000f000fu;
+                            ko[0][hf] = kw[n].x & 0x00f000f0u;
+                            ke[0][2 + hf] = (kw[n].x >> 8) & 0x000f000fu;
+                            ko[0][2 + hf] = (kw[n].x >> 8) & 0x00f000f0u;
+                            ke[1][hf] = kw[n].y & 0x000f000fu;
+                            ko[1][hf] = kw[n].y & 0x00f000f0u;
+                            ke[1][2 + hf] = (kw[n].y >> 8) & 0x000f000fu;
+                            ko[1][2 + hf] = (kw[n].y >> 8) & 0x00f000f0u;
+                            st[hf] = kv4_step(par & 0xffffu) * a.scale_log2;
+                            zs[hf] = st[hf] * (8388608.f - __uint_as_float(0x4b000000u | (par & 15u)));  // -zero * st
+                        }
+#pragma unroll
+                        for (int nt = 0; nt < NT; nt++) {
+                            float ce[4], co[4];
+                            mma16816_first(ce, ke[0], qb[nt][0][0], qb[nt][1][0]);
+                            mma16816_first(co, ko[0], qb[nt][0][1], qb[nt][1][1]);
+                            mma16816(ce, ke[1], qb[nt][2][0], qb[nt][3][0]);
+                            mma16816(co, ko[1], qb[nt][2][1], qb[nt][3][1]);
+                            const uint64_t qs2 = f2_pack(qs[nt][0], qs[nt][1]), m2 = f2_pack(-m[nt][0], -m[nt][1]);
+#pragma unroll
+                            for (int hf = 0; hf < 2; hf++) {
+                                const float se = st[hf] * 16777216.f, so = st[hf] * 1048576.f;
+                                uint64_t x = f2_fma(f2_pack(zs[hf], zs[hf]), qs2, m2);
+                                x = f2_fma(f2_pack(co[2 * hf], co[2 * hf + 1]), f2_pack(so, so), x);
+                                x = f2_fma(f2_pack(ce[2 * hf], ce[2 * hf + 1]), f2_pack(se, se), x);
+                                f2_unpack(x, sc[nt][i][2 * hf], sc[nt][i][2 * hf + 1]);
+                            }
                         }
                     }
+                    if (tile + R_WARPS < tile1 && tile + R_WARPS < ext_tiles) fetch_k(tile + R_WARPS);
                 } else {
                     const __half* kr = a.K + (size_t)(s.kv_start + key0) * a.ldkv + g * 64 + 16 * t;
 #pragma unroll
-                    for (int n = 0; n < 8; n++) {
-                        const uint4* src = reinterpret_cast<const uint4*>(kr + (size_t)min(8 * n + r, last) * a.ldkv);
-                        const uint4 x0 = __ldg(src), x1 = __ldg(src + 1);
+                    for (int i = 0; i < 4; i++) {
+                        uint32_t ka[4][4];
 #pragma unroll
-                        for (int mt = 0; mt < MT; mt++) {
-                            float c[4] = {0.f, 0.f, 0.f, 0.f};
-                            mma16816(c, qa[mt][0], x0.x, x0.y);
-                            mma16816(c, qa[mt][1], x0.z, x0.w);
-                            mma16816(c, qa[mt][2], x1.x, x1.y);
-                            mma16816(c, qa[mt][3], x1.z, x1.w);
+                        for (int hf = 0; hf < 2; hf++) {
+                            const uint4* src =
+                                reinterpret_cast<const uint4*>(kr + (size_t)min(16 * i + 8 * hf + r, last) * a.ldkv);
+                            const uint4 x0 = __ldg(src), x1 = __ldg(src + 1);
+                            const uint32_t w[8] = {x0.x, x0.y, x0.z, x0.w, x1.x, x1.y, x1.z, x1.w};
 #pragma unroll
-                            for (int i = 0; i < 4; i++) sc[mt][n][i] = c[i] * a.scale_log2;
+                            for (int q = 0; q < 8; q++) ka[q >> 1][(q & 1) * 2 + hf] = w[q];
+                        }
+#pragma unroll
+                        for (int nt = 0; nt < NT; nt++) {
+                            float c[4];
+                            mma16816_first(c, ka[0], qb[nt][0][0], qb[nt][0][1]);
+#pragma unroll
+                            for (int ks = 1; ks < 4; ks++) mma16816(c, ka[ks], qb[nt][ks][0], qb[nt][ks][1]);
+#pragma unroll
+                            for (int q = 0; q < 4; q++) sc[nt][i][q] = c[q] * a.scale_log2 - m[nt][q & 1];
                         }
                     }
                 }
                 if (left < R_KEYS) {
 #pragma unroll
-                    for (int mt = 0; mt < MT; mt++)
+                    for (int nt = 0; nt < NT; nt++)
 #pragma unroll
-                        for (int n = 0; n < 8; n++)
+                        for (int i = 0; i < 4; i++)
 #pragma unroll
-                            for (int i = 0; i < 4; i++)
-                                if (8 * n + 2 * t + (i & 1) >= left) sc[mt][n][i] = -INFINITY;
+                            for (int q = 0; q < 4; q++)
+                                if (16 * i + 8 * (q >> 1) + r >= left) sc[nt][i][q] = -INFINITY;
                 }
-                // ---- running softmax, in the exp2 domain
-                uint32_t pa[MT][8][2];
+                // ---- running softmax, in the exp2 domain. The scores are taken against the reference m as it was before
+                // this tile; only where one exceeds it by more than 2^8 (and in the first tile) does m move, and what was
+                // summed so far is rescaled: P stays below 2^8, well inside fp16. P^T as B operands: keys 16i + 2t,
+                // 16i + 2t + 1 and 8 above
+                uint32_t pb[NT][4][2];
 #pragma unroll
-                for (int mt = 0; mt < MT; mt++)
+                for (int nt = 0; nt < NT; nt++) {
+                    float over[2];
 #pragma unroll
-                    for (int hf = 0; hf < 2; hf++) {
-                        float mx = -INFINITY;
+                    for (int q = 0; q < 2; q++) {
+                        over[q] = fmaxf(sc[nt][0][q], sc[nt][0][q + 2]);
 #pragma unroll
-                        for (int n = 0; n < 8; n++) mx = fmaxf(mx, fmaxf(sc[mt][n][2 * hf], sc[mt][n][2 * hf + 1]));
-                        mx = fmaxf(mx, __shfl_xor_sync(D1_FULL_MASK, mx, 1));
-                        mx = fmaxf(mx, __shfl_xor_sync(D1_FULL_MASK, mx, 2));
-                        const float mn = fmaxf(m[mt][hf], mx);
-                        const float alpha = m[mt][hf] == mn ? 1.f : ex2(m[mt][hf] - mn);
-                        m[mt][hf] = mn;
-                        float sum = 0.f;
+                        for (int i = 1; i < 4; i++) over[q] = fmax3(over[q], sc[nt][i][q], sc[nt][i][q + 2]);
+                    }
+                    if (!started || __any_sync(D1_FULL_MASK, fmaxf(over[0], over[1]) > kLazyRescale)) {
 #pragma unroll
-                        for (int n = 0; n < 8; n++) {
-                            const float p0 = ex2(sc[mt][n][2 * hf] - mn), p1 = ex2(sc[mt][n][2 * hf + 1] - mn);
-                            sum += p0 + p1;
-                            pa[mt][n][hf] = pack_h2(p0, p1);
-                        }
-                        l[mt][hf] = l[mt][hf] * alpha + sum;
+                        for (int q = 0; q < 2; q++) {
+                            float up = over[q];
+                            up = fmaxf(up, __shfl_xor_sync(D1_FULL_MASK, up, 4));
+                            up = fmaxf(up, __shfl_xor_sync(D1_FULL_MASK, up, 8));
+                            up = fmaxf(up, __shfl_xor_sync(D1_FULL_MASK, up, 16));
+                            if (started) up = fmaxf(up, 0.f);
+                            const float alpha = started ? ex2(-up) : 0.f;
+                            m[nt][q] += up;
+                            l[nt][q] *= alpha;
 #pragma unroll
-                        for (int j = 0; j < 8; j++) {
-                            o[mt][j][2 * hf] *= alpha;
-                            o[mt][j][2 * hf + 1] *= alpha;
+                            for (int i = 0; i < 4; i++) {
+                                o[nt][i][q] *= alpha;
+                                o[nt][i][q + 2] *= alpha;
+                                sc[nt][i][q] -= up;
+                                sc[nt][i][q + 2] -= up;
+                            }
                         }
                     }
-                // ---- O += P V
+#pragma unroll
+                    for (int i = 0; i < 4; i++)
+#pragma unroll
+                        for (int hf = 0; hf < 2; hf++) {
+                            const float p0 = ex2(sc[nt][i][2 * hf]), p1 = ex2(sc[nt][i][2 * hf + 1]);
+                            l[nt][0] += p0;
+                            l[nt][1] += p1;
+                            pb[nt][i][hf] = movmatrix_trans(pack_h2(p0, p1));
+                        }
+                }
+                started = true;
+                // ---- O^T += V^T P^T
 #pragma unroll
                 for (int ks = 0; ks < 4; ks++) {
-                    uint32_t b[2][8];  // [keys 2t, 2t+1 | 2t+8, 2t+9][j]
-                    if (ext) {
+                    uint32_t va[4][4];  // [m tile][dimensions 8r + 2j, 8r + 2j + 1 of keys 2t, 2t+1; of 2t+8, 2t+9]
 #pragma unroll
-                        for (int i = 0; i < 2; i++) {
+                    for (int i = 0; i < 2; i++) {
+                        if (ext) {
                             const uint32_t par = __shfl_sync(D1_FULL_MASK, pv, 8 * ks + 4 * i + t);
                             const uint32_t st = kv4_step2(par);
                             uint32_t z0, z1, ev[4], od[4];
@@ -254,79 +347,122 @@ __global__ void __launch_bounds__(R_WARPS * 32) k_kv4_attn_rows(const Kv4Args a)
                             kv4_expand(__byte_perm(vw[ks][2 * i], vw[ks][2 * i + 1], 0x7632), z0, z1, od);
 #pragma unroll
                             for (int j = 0; j < 4; j++) {
-                                b[i][2 * j] = h2_mul(ev[j], st);
-                                b[i][2 * j + 1] = h2_mul(od[j], st);
+                                va[j][2 * i] = h2_mul(ev[j], st);
+                                va[j][2 * i + 1] = h2_mul(od[j], st);
                             }
-                        }
-                    } else {
-                        const __half* vr = a.V + (size_t)(s.kv_start + key0) * a.ldkv + g * 64 + 8 * r;
-#pragma unroll
-                        for (int i = 0; i < 2; i++) {
+                        } else {
+                            const __half* vr = a.V + (size_t)(s.kv_start + key0) * a.ldkv + g * 64 + 8 * r;
                             const int k = 16 * ks + 8 * i + 2 * t;
                             const uint4 x = __ldg(reinterpret_cast<const uint4*>(vr + (size_t)min(k, last) * a.ldkv));
                             const uint4 y = __ldg(reinterpret_cast<const uint4*>(vr + (size_t)min(k + 1, last) * a.ldkv));
                             const uint32_t xs[4] = {x.x, x.y, x.z, x.w}, ys[4] = {y.x, y.y, y.z, y.w};
 #pragma unroll
                             for (int j = 0; j < 4; j++) {
-                                b[i][2 * j] = __byte_perm(xs[j], ys[j], 0x5410);
-                                b[i][2 * j + 1] = __byte_perm(xs[j], ys[j], 0x7632);
+                                va[j][2 * i] = __byte_perm(xs[j], ys[j], 0x5410);
+                                va[j][2 * i + 1] = __byte_perm(xs[j], ys[j], 0x7632);
                             }
                         }
                     }
 #pragma unroll
-                    for (int mt = 0; mt < MT; mt++) {
-                        const uint32_t pr[4] = {pa[mt][2 * ks][0], pa[mt][2 * ks][1], pa[mt][2 * ks + 1][0],
-                                                pa[mt][2 * ks + 1][1]};
+                    for (int nt = 0; nt < NT; nt++)
 #pragma unroll
-                        for (int j = 0; j < 8; j++) mma16816(o[mt][j], pr, b[0][j], b[1][j]);
-                    }
+                        for (int j = 0; j < 4; j++) mma16816(o[nt][j], va[j], pb[nt][ks][0], pb[nt][ks][1]);
                 }
             }
-            // ---- join the warps: weights 2^(m - M), in the warps' order
+            // ---- join the warps, weights 2^(m - M), in their order; a warp without tiles has m = -inf and l = 0
 #pragma unroll
-            for (int mt = 0; mt < MT; mt++)
+            for (int nt = 0; nt < NT; nt++)
 #pragma unroll
-                for (int hf = 0; hf < 2; hf++) {
-                    float sum = l[mt][hf];
-                    sum += __shfl_xor_sync(D1_FULL_MASK, sum, 1);
-                    sum += __shfl_xor_sync(D1_FULL_MASK, sum, 2);
-                    const int row = mt * 16 + hf * 8 + r;
-                    if (t == 0) {
-                        sM[warp * NR + row] = m[mt][hf];
-                        sL[warp * NR + row] = sum;
+                for (int q = 0; q < 2; q++) {
+                    float sum = l[nt][q];
+                    sum += __shfl_xor_sync(D1_FULL_MASK, sum, 4);
+                    sum += __shfl_xor_sync(D1_FULL_MASK, sum, 8);
+                    sum += __shfl_xor_sync(D1_FULL_MASK, sum, 16);
+                    const int row = warp * NR + nt * 8 + 2 * t + q;
+                    if (r == 0) {
+                        sM[row] = started ? m[nt][q] : -INFINITY;
+                        sL[row] = sum;
                     }
-                    float4* dst = reinterpret_cast<float4*>(sO + (warp * NR + row) * R_OLD + 16 * t);
-#pragma unroll
-                    for (int q = 0; q < 4; q++)  // dimensions 16t + 4q .. : j = 4 (q & 1) .., column 2t + q / 2
-                        dst[q] = make_float4(o[mt][4 * (q & 1)][2 * hf + (q >> 1)], o[mt][4 * (q & 1) + 1][2 * hf + (q >> 1)],
-                                             o[mt][4 * (q & 1) + 2][2 * hf + (q >> 1)],
-                                             o[mt][4 * (q & 1) + 3][2 * hf + (q >> 1)]);
+                    float4* dst = reinterpret_cast<float4*>(sO + row * R_LD + 8 * r);
+                    dst[0] = make_float4(o[nt][0][q], o[nt][0][q + 2], o[nt][1][q], o[nt][1][q + 2]);
+                    dst[1] = make_float4(o[nt][2][q], o[nt][2][q + 2], o[nt][3][q], o[nt][3][q + 2]);
                 }
             __syncthreads();
-            for (int i = tid; i < NR * 16; i += R_WARPS * 32) {
-                const int row = i >> 4, d = (i & 15) * 4;
-                const long long p = base + row;
-                if (p >= n_rows) continue;
-                float M = -INFINITY;
-#pragma unroll
-                for (int w = 0; w < R_WARPS; w++) M = fmaxf(M, sM[w * NR + row]);
-                float L = 0.f, x0 = 0.f, x1 = 0.f, x2 = 0.f, x3 = 0.f;
-                for (int w = 0; w < R_WARPS && w < tiles; w++) {  // warps beyond the tiles hold nothing
-                    const float f = ex2(sM[w * NR + row] - M);
-                    const float4 v = *reinterpret_cast<const float4*>(sO + (w * NR + row) * R_OLD + d);
-                    L += f * sL[w * NR + row];
-                    x0 += f * v.x;
-                    x1 += f * v.y;
-                    x2 += f * v.z;
-                    x3 += f * v.w;
-                }
+            auto finish = [&](long long p, int d, float M, float L, const float4& x) {
                 const float il = tiles ? 1.f / L : 0.f;
                 const int q = s.q_start + (int)(p / a.group), h = g * a.group + (int)(p % a.group);
                 *reinterpret_cast<uint2*>(a.O + (size_t)q * a.ldo + h * 64 + d) =
-                    make_uint2(pack_h2(x0 * il, x1 * il), pack_h2(x2 * il, x3 * il));
+                    make_uint2(pack_h2(x.x * il, x.y * il), pack_h2(x.z * il, x.w * il));
                 if (a.lse && d == 0) a.lse[(size_t)h * a.lse_ld + q] = tiles ? (M + log2f(L)) * kLn2 : -INFINITY;
+            };
+            const int warps = min(R_WARPS, tile1 - tile0);  // those with tiles
+            for (int i = tid; i < NR * 16; i += R_WARPS * 32) {
+                const int row = i >> 4, d = (i & 15) * 4;
+                if (base + row >= n_rows) break;
+                float M = -INFINITY, L = 0.f;
+                for (int w = 0; w < warps; w++) M = fmaxf(M, sM[w * NR + row]);
+                float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+                for (int w = 0; w < warps; w++) {
+                    const float f = ex2(sM[w * NR + row] - M);
+                    const float4 v = *reinterpret_cast<const float4*>(sO + (w * NR + row) * R_LD + d);
+                    L += f * sL[w * NR + row];
+                    x.x += f * v.x;
+                    x.y += f * v.y;
+                    x.z += f * v.z;
+                    x.w += f * v.w;
+                }
+                if (ranks == 1) {
+                    finish(base + row, d, M, L, x);
+                    continue;
+                }
+                *reinterpret_cast<float4*>(cO + row * R_LD + d) = x;
+                if (d == 0) {
+                    cM[row] = M;
+                    cL[row] = L;
+                }
             }
-            __syncthreads();
+            if (ranks == 1) {
+                __syncthreads();  // before the next rows
+                continue;
+            }
+            // ---- join the CTAs; each writes its share of the output
+            __syncwarp();
+            cluster_sync();
+            const int parts = tiles == 0 ? 0 : (tiles - 1) / per + 1;  // CTAs with tiles
+            for (int i = rank * R_WARPS * 32 + tid; i < NR * 16; i += ranks * R_WARPS * 32) {
+                const int row = i >> 4, d = (i & 15) * 4;
+                if (base + row >= n_rows) break;
+                float cm[R_CLUSTER], cl[R_CLUSTER];
+                float4 v[R_CLUSTER];
+#pragma unroll
+                for (int c = 0; c < R_CLUSTER; c++) {
+                    cm[c] = -INFINITY;
+                    cl[c] = 0.f;
+                    v[c] = make_float4(0.f, 0.f, 0.f, 0.f);
+                    if (c < parts) {
+                        cm[c] = ld_cluster_f32(mapa_shared(smem_u32(cM + row), c));
+                        cl[c] = ld_cluster_f32(mapa_shared(smem_u32(cL + row), c));
+                        v[c] = ld_cluster_f32x4(mapa_shared(smem_u32(cO + row * R_LD + d), c));
+                    }
+                }
+                float M = -INFINITY, L = 0.f;
+#pragma unroll
+                for (int c = 0; c < R_CLUSTER; c++) M = fmaxf(M, cm[c]);
+                float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+                for (int c = 0; c < R_CLUSTER; c++) {
+                    if (c >= parts) break;
+                    const float f = ex2(cm[c] - M);
+                    L += f * cl[c];
+                    x.x += f * v[c].x;
+                    x.y += f * v[c].y;
+                    x.z += f * v[c].z;
+                    x.w += f * v[c].w;
+                }
+                finish(base + row, d, M, L, x);
+            }
+            __syncwarp();
+            cluster_sync();  // the other CTAs have read this one's sums
         }
     }
 }
@@ -347,7 +483,6 @@ __global__ void __launch_bounds__(R_WARPS * 32) k_kv4_attn_rows(const Kv4Args a)
 constexpr int TQ = 128, TKV = 128, T_QSLOTS = 2, T_STAGES = 4, T_LOADERS = 3, T_THREADS = 384;
 constexpr int T_QT_BYTES = TQ * 128, T_KV_BYTES = TKV * 128, T_O_BYTES = TQ * 128;
 constexpr uint32_t T_TMEM_COLS = 512, T_WG_COLS = 256, T_P_COL = TKV, T_O_COL = TKV + TKV / 2;
-constexpr float kLazyRescale = 8.f;
 enum : int {
     B_QFULL = 0,
     B_QEMPTY = B_QFULL + T_QSLOTS,
@@ -1314,14 +1449,32 @@ int sm_count() {
     return sms[dev & 63];
 }
 
-template <int MT>
-int launch_rows(const Kv4Args& a, int max_q, int kv_heads, cudaStream_t st) {
+template <int NT>
+int launch_rows(Kv4Args& a, int max_q, int max_keys, int kv_heads, cudaStream_t st) {
     static unsigned long long done = 0;
-    if (!smem_opt_in(k_kv4_attn_rows<MT>, rows_smem<MT>(), &done)) return -1;
-    long long x = ((long long)max_q * a.group + 16 * MT - 1) / (16 * MT);
+    if (!smem_opt_in(k_kv4_attn_rows<NT>, rows_smem<NT>(), &done)) return -1;
+    long long x = ((long long)max_q * a.group + 8 * NT - 1) / (8 * NT);
     x = x < 1 ? 1 : x > 65536 ? 65536 : x;
     const int z = a.n_seqs < 65535 ? a.n_seqs : 65535;
-    launch_pdl(k_kv4_attn_rows<MT>, dim3((unsigned)x, kv_heads, z), R_WARPS * 32, rows_smem<MT>(), st, a);
+    // CTAs to a cluster: as many as the keys give every warp a tile and more than a few waves of CTAs are not needed
+    int ranks = R_CLUSTER;
+    const long long tiles = ((long long)max_keys + R_KEYS - 1) / R_KEYS;
+    while (ranks > 1 && ((ranks / 2) * R_WARPS >= tiles || x * kv_heads * z * ranks / 2 >= 148 * 12)) ranks /= 2;
+    a.ranks = ranks;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)x * ranks, kv_heads, z);
+    cfg.blockDim = dim3(R_WARPS * 32);
+    cfg.dynamicSmemBytes = rows_smem<NT>();
+    cfg.stream = st;
+    cudaLaunchAttribute at[2];
+    at[0].id = cudaLaunchAttributeClusterDimension;
+    at[0].val.clusterDim.x = ranks;
+    at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+    at[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[1].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = at;
+    cfg.numAttrs = pdl_enabled() ? 2 : 1;
+    cudaLaunchKernelEx(&cfg, k_kv4_attn_rows<NT>, (const Kv4Args)a);
     return (int)cudaGetLastError();
 }
 
@@ -1400,7 +1553,10 @@ extern "C" int d1_flash_attn_kv4(const d1_half* Q, int ldq, const d1_half* K, co
     if (!a.err) return -1;
     const int kv_heads = heads / group;
     if ((long long)max_q * group > 64) return launch_tc(a, max_q, st);
-    return (long long)max_q * group <= 16 ? launch_rows<1>(a, max_q, kv_heads, st) : launch_rows<2>(a, max_q, kv_heads, st);
+    const long long rows = (long long)max_q * group;
+    return rows <= 8 ? launch_rows<1>(a, max_q, max_keys, kv_heads, st)
+                     : rows <= 16 ? launch_rows<2>(a, max_q, max_keys, kv_heads, st)
+                                  : launch_rows<4>(a, max_q, max_keys, kv_heads, st);
 }
 
 extern "C" int d1_kv4_mass(const d1_half* Q, int ldq, const float* lse, int lse_ld, const D1Kv4Seq* seqs, int n_seqs,
