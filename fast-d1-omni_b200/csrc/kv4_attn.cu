@@ -20,7 +20,7 @@ struct Kv4Args {
     const D1Kv4Seq* seqs;
     int* err;
     int ldq, ldkv, ldo, lse_ld, n_seqs, heads, group, q_rows, kv_rows, accumulate, ranks;
-    int n_blocks;  // tcgen05 forms: blocks of rows per sequence (attention), tiles of keys per cache (mass)
+    int n_blocks;  // tcgen05 form of the mass: tiles of keys per cache
     float scale_log2;
 };
 
@@ -71,14 +71,15 @@ __device__ __forceinline__ void ex2_fma2(float x0, float x1, float& p0, float& p
 // Everything is transposed, S^T = K Q^T and O^T = V^T P^T on m16n8k16, so that 8 rows fill an MMA's n. The codes go from
 // global memory to the registers of the A operands directly. An MMA's k index may run over the dimensions in any order as
 // long as both operands use the same: for S^T lane (r, t) = (lane / 4, lane % 4) holds dimensions 16t .. 16t+15 of keys r
-// and r + 8 of each 16: 8 bytes of codes, and 32 bytes of a query row. The MMA sees the codes as they are, for a code at
-// bits 0-3 or 4-7 of a half is the fp16 number code * 2^-24 or code * 2^-20; in fp32, a key's step and the softmax scale
-// multiply the sums, and zero times the query row's sum is taken away. For O^T lane (r, t) holds word r (dimensions
+// and r + 8 of each 16: 8 bytes of codes, and 32 bytes of a query row. The MMA sees the whole numbers code - zero; a key's
+// step multiplies its scores afterwards, in fp32, with the softmax scale. For O^T lane (r, t) holds word r (dimensions
 // 8r .. 8r+7) of keys 2t, 2t+1, 2t+8, 2t+9 of each 16; byte permutes bring two keys' codes of one dimension together, and
 // the values are (code - zero) * step, exact in fp16. Row r of the j-th m tile is dimension 8r + 2j, row r + 8 dimension
 // 8r + 2j + 1, so that a lane ends with dimensions 8r .. 8r+7 of packed rows 2t and 2t + 1. P^T turns from the result's
 // layout into the B operand's by movmatrix.
-// Bound: the issue slots (about 750 instructions a tile, half of them for the expansion of codes).
+// Bound: the issue slots (about 800 instructions a tile, half of them for the expansion of codes). Tried and dropped: the
+// codes as fp16 subnormals (code * 2^-24 or * 2^-20, no subtraction), with zeros and steps taken care of by the sums: an
+// eighth fewer instructions, but the MMA aligns its fp32 sums to the operands' exponent, and their last 10 bits are lost.
 constexpr int R_KEYS = 64, R_WARPS = 4, R_CLUSTER = 8, R_LD = 68;  // padded row of the joining buffers (floats)
 
 template <int NT>
@@ -151,19 +152,8 @@ __global__ void __launch_bounds__(R_WARPS * 32, NT == 1 ? 4 : 2) k_kv4_attn_rows
                 for (int i = 0; i < 8; i++) qb[nt][i >> 1][i & 1] = w[i];
             }
             float o[NT][4][4], m[NT][2], l[NT][2];  // rows 2t and 2t + 1 of each n tile
-            float qs[NT][2];                        // sums of the query rows, for the zeros
 #pragma unroll
             for (int nt = 0; nt < NT; nt++) {
-                float sum = 0.f;
-#pragma unroll
-                for (int i = 0; i < 8; i++) {
-                    const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&qb[nt][i >> 1][i & 1]));
-                    sum += f.x + f.y;
-                }
-                sum += __shfl_xor_sync(D1_FULL_MASK, sum, 1);
-                sum += __shfl_xor_sync(D1_FULL_MASK, sum, 2);
-                qs[nt][0] = __shfl_sync(D1_FULL_MASK, sum, 8 * t);
-                qs[nt][1] = __shfl_sync(D1_FULL_MASK, sum, 8 * t + 4);
 #pragma unroll
                 for (int j = 0; j < 4; j++)
 #pragma unroll
@@ -215,41 +205,38 @@ __global__ void __launch_bounds__(R_WARPS * 32, NT == 1 ? 4 : 2) k_kv4_attn_rows
                     if (2 * lane + 1 > last) pv = 2 * lane > last ? 0 : pv & 0xffffu;
 #pragma unroll
                     for (int i = 0; i < 4; i++) {
-                        // even and odd places of a half, whose codes count 2^-24 and 2^-20, in MMAs of their own
-                        uint32_t ke[2][4], ko[2][4];
-                        float st[2], zs[2];
+                        uint32_t ka[4][4];
+                        float st[2];
 #pragma unroll
                         for (int hf = 0; hf < 2; hf++) {
                             const int n = 2 * i + hf;
                             const uint32_t both = __shfl_sync(D1_FULL_MASK, pk, 4 * n + (r >> 1));
-                            const uint32_t par = both >> (16 * (r & 1));
-                            ke[0][hf] = kw[n].x & 0x000f000fu;
-                            ko[0][hf] = kw[n].x & 0x00f000f0u;
-                            ke[0][2 + hf] = (kw[n].x >> 8) & 0x000f000fu;
-                            ko[0][2 + hf] = (kw[n].x >> 8) & 0x00f000f0u;
-                            ke[1][hf] = kw[n].y & 0x000f000fu;
-                            ko[1][hf] = kw[n].y & 0x00f000f0u;
-                            ke[1][2 + hf] = (kw[n].y >> 8) & 0x000f000fu;
-                            ko[1][2 + hf] = (kw[n].y >> 8) & 0x00f000f0u;
+                            const uint32_t par = __byte_perm(both, 0, r & 1 ? 0x3232 : 0x1010);
+                            uint32_t z0, z1, x[4], y[4];
+                            kv4_zero(par, z0, z1);
+                            kv4_expand(kw[n].x, z0, z1, x);
+                            kv4_expand(kw[n].y, z0, z1, y);
+                            ka[0][hf] = x[0];
+                            ka[0][2 + hf] = x[1];
+                            ka[1][hf] = x[2];
+                            ka[1][2 + hf] = x[3];
+                            ka[2][hf] = y[0];
+                            ka[2][2 + hf] = y[1];
+                            ka[3][hf] = y[2];
+                            ka[3][2 + hf] = y[3];
                             st[hf] = kv4_step(par & 0xffffu) * a.scale_log2;
-                            zs[hf] = st[hf] * (8388608.f - __uint_as_float(0x4b000000u | (par & 15u)));  // -zero * st
                         }
 #pragma unroll
                         for (int nt = 0; nt < NT; nt++) {
-                            float ce[4], co[4];
-                            mma16816_first(ce, ke[0], qb[nt][0][0], qb[nt][1][0]);
-                            mma16816_first(co, ko[0], qb[nt][0][1], qb[nt][1][1]);
-                            mma16816(ce, ke[1], qb[nt][2][0], qb[nt][3][0]);
-                            mma16816(co, ko[1], qb[nt][2][1], qb[nt][3][1]);
-                            const uint64_t qs2 = f2_pack(qs[nt][0], qs[nt][1]), m2 = f2_pack(-m[nt][0], -m[nt][1]);
+                            float c[4];
+                            mma16816_first(c, ka[0], qb[nt][0][0], qb[nt][0][1]);
 #pragma unroll
-                            for (int hf = 0; hf < 2; hf++) {
-                                const float se = st[hf] * 16777216.f, so = st[hf] * 1048576.f;
-                                uint64_t x = f2_fma(f2_pack(zs[hf], zs[hf]), qs2, m2);
-                                x = f2_fma(f2_pack(co[2 * hf], co[2 * hf + 1]), f2_pack(so, so), x);
-                                x = f2_fma(f2_pack(ce[2 * hf], ce[2 * hf + 1]), f2_pack(se, se), x);
-                                f2_unpack(x, sc[nt][i][2 * hf], sc[nt][i][2 * hf + 1]);
-                            }
+                            for (int ks = 1; ks < 4; ks++) mma16816(c, ka[ks], qb[nt][ks][0], qb[nt][ks][1]);
+                            const uint64_t m2 = f2_pack(-m[nt][0], -m[nt][1]);
+#pragma unroll
+                            for (int hf = 0; hf < 2; hf++)
+                                f2_unpack(f2_fma(f2_pack(c[2 * hf], c[2 * hf + 1]), f2_pack(st[hf], st[hf]), m2),
+                                          sc[nt][i][2 * hf], sc[nt][i][2 * hf + 1]);
                         }
                     }
                     if (tile + R_WARPS < tile1 && tile + R_WARPS < ext_tiles) fetch_k(tile + R_WARPS);
@@ -468,82 +455,136 @@ __global__ void __launch_bounds__(R_WARPS * 32, NT == 1 ? 4 : 2) k_kv4_attn_rows
 }
 
 // ------------------------------------------------------------------------------------------------ attention, many rows
-// tcgen05 form. Persistent CTAs (one per SM) loop over units of two 128-row query tiles that share their keys: the same
-// rows of two heads of one kv head where the group is even (a sequence of 24 rows then fills both tiles), two successive
-// blocks of rows of one head where it is odd. Keys come in tiles of 128, first the cached ones, then the own ones; the
-// last tile of either kind is filled up with zeros and masked.
+// tcgen05 form. Persistent CTAs (one per SM) loop over units. A unit is, by the length of its sequence,
+//   packed  up to 128 packed query rows (row p / group, head p % group) of one kv head; the two softmax warpgroups take
+//           its key tiles in turn and are joined at the end
+//   pair    128 rows of two heads of one kv head (an even group), a warpgroup each
+//   single  256 rows of one head (an odd group), a warpgroup for each 128
+// Keys come in tiles of 128, first the cached ones, then the own ones; the last tile of either kind is filled up with
+// zeros and masked.
 // Warps:
-//   0-3, 4-7   softmax of tiles 0 and 1: thread = query row = TMEM lane. S is copied to registers and released at once,
-//              P goes to TMEM as fp16, O is rescaled only when a row's maximum grows by more than 2^8
+//   0-3, 4-7   softmax: thread = query row = TMEM lane. S is copied to registers and released at once, P goes to TMEM as
+//              fp16, O is rescaled only when a row's maximum grows by more than 2^8. Warps whose rows are all behind the
+//              sequence's end leave the work out.
 //   8, 10, 11  loaders. A cached tile: every thread fetches 16-byte pieces of codes and their parameters into registers
 //              while the tile before it is stored, then expands them to fp16 (exact) into the swizzled layout that the
 //              MMAs read. Own rows: whole tiles by TMA, partial ones through registers.
 //   9          TMEM, and the MMAs from one thread: S = Q K^T (both in shared memory), O += P V (P in TMEM)
-// TMEM (512 columns), tile w at 256 w: S in 128 columns, P in 64, O in 64.
+// TMEM (512 columns), warpgroup w at 256 w: S in 128 columns, P in 64, O in 64. Both warpgroups' columns share the lanes,
+// so that a packed unit is joined by the first reading the second's O.
 constexpr int TQ = 128, TKV = 128, T_QSLOTS = 2, T_STAGES = 4, T_LOADERS = 3, T_THREADS = 384;
 constexpr int T_QT_BYTES = TQ * 128, T_KV_BYTES = TKV * 128, T_O_BYTES = TQ * 128;
+constexpr int T_ENTRIES = 256;  // of the table of units
 constexpr uint32_t T_TMEM_COLS = 512, T_WG_COLS = 256, T_P_COL = TKV, T_O_COL = TKV + TKV / 2;
 enum : int {
     B_QFULL = 0,
     B_QEMPTY = B_QFULL + T_QSLOTS,
     B_KVFULL = B_QEMPTY + T_QSLOTS,
     B_KVEMPTY = B_KVFULL + T_STAGES,
-    B_SFULL = B_KVEMPTY + T_STAGES,  // [w]: S of the tile's next keys is in TMEM
+    B_SFULL = B_KVEMPTY + T_STAGES,  // [w]: S of the warpgroup's next keys is in TMEM
     B_SFREE = B_SFULL + 2,           // [w]: it is in registers (4 warps)
     B_PFULL = B_SFREE + 2,           // [w]: P is in TMEM (4 warps)
     B_ODONE = B_PFULL + 2,           // [w]: P V has completed
-    B_OFREE = B_ODONE + 2,           // [w]: O has been read (4 warps)
+    B_OFREE = B_ODONE + 2,           // [w]: O has been read (4 warps; of a packed unit those of warpgroup 0)
     B_OSTAGED = B_OFREE + 2,         // [w]: the output tile is in shared memory (4 warps)
     B_OREAD = B_OSTAGED + 2,         // [w]: its last bulk store has read it
-    B_DRAIN = B_OREAD + 2,
+    B_JOIN = B_OREAD + 2,            // a packed unit's maxima and sums of warpgroup 1 are in shared memory (4 warps)
+    B_JOINED = B_JOIN + 1,           // and have been read (4 warps)
+    B_DRAIN = B_JOINED + 1,
     T_NBARS = B_DRAIN + 1
 };
-constexpr int T_SMEM = T_QSLOTS * 2 * T_QT_BYTES + T_STAGES * 2 * T_KV_BYTES + 2 * T_O_BYTES + T_NBARS * 8 + 16;
+constexpr int T_SMEM = T_QSLOTS * 2 * T_QT_BYTES + T_STAGES * 2 * T_KV_BYTES + 2 * T_O_BYTES + T_NBARS * 8 + 16 + TQ * 8 +
+                       (T_ENTRIES + 1) * 4;
 static_assert(T_SMEM <= 232448 && T_O_COL + 64 <= T_WG_COLS, "shared memory and TMEM of the tcgen05 attention");
 
-// The units of a CTA, walked alike by every role: u -> (sequence, block of rows, head or pair of heads), heads fastest.
-// A sequence longer than max_q comes round again with its later blocks.
-struct Walk {
-    D1Kv4Seq s;
-    int u, nb, hu, block, h, n_units;
-    bool pair, at_unit;
+enum : int { kPacked, kPair, kSingle };
 
-    __device__ Walk(const Kv4Args& a) : u(blockIdx.x), nb(a.n_blocks), block(0), h(0), at_unit(false) {
-        pair = a.group % 2 == 0;
-        hu = pair ? a.heads / 2 : a.heads;
-        n_units = a.n_seqs * nb * hu;
+__device__ __forceinline__ int unit_mode(const Kv4Args& a, int q_len) {
+    return (long long)q_len * a.group <= TQ ? kPacked : a.group % 2 == 0 ? kPair : kSingle;
+}
+// Units of sequence sq; none of a sequence without rows or with a bad entry (report: tell).
+__device__ __forceinline__ int seq_units(const Kv4Args& a, int sq, bool report) {
+    const D1Kv4Seq s = a.seqs[sq];
+    if (!kv4_seq_ok(s) || !rows_ok(s.q_start, s.q_len, a.q_rows) || !rows_ok(s.kv_start, s.kv_len, a.kv_rows)) {
+        if (report) atomicExch(a.err, kErrTable);
+        return 0;
     }
-    __device__ int rows_per_block() const { return pair ? TQ : 2 * TQ; }
-    __device__ bool next(const Kv4Args& a) {
-        while (true) {
-            if (at_unit) {
-                block += nb;
-            } else {
-                if (u >= n_units) return false;
-                const int sq = u / (nb * hu), rest = u % (nb * hu);
-                block = rest / hu;
-                h = rest % hu * (pair ? 2 : 1);
-                s = a.seqs[sq];
-                at_unit = true;
-                if (!kv4_seq_ok(s) || !rows_ok(s.q_start, s.q_len, a.q_rows) || !rows_ok(s.kv_start, s.kv_len, a.kv_rows)) {
-                    if ((threadIdx.x & 31) == 0) atomicExch(a.err, kErrTable);
-                    s.q_len = 0;
-                }
-            }
-            if ((long long)block * rows_per_block() < s.q_len) return true;
-            u += gridDim.x;
-            at_unit = false;
+    if (s.q_len == 0) return 0;
+    const int mode = unit_mode(a, s.q_len);
+    return mode == kPacked ? a.heads / a.group
+                           : mode == kPair ? ((s.q_len - 1) / TQ + 1) * (a.heads / 2) : ((s.q_len - 1) / (2 * TQ) + 1) * a.heads;
+}
+// The table of units: cum[e] = units of the sequences before the e-th run of `run` sequences. Ends with a barrier.
+__device__ __forceinline__ void build_units(const Kv4Args& a, int* cum, int run) {
+    for (int e = threadIdx.x; e < T_ENTRIES; e += blockDim.x) {
+        int n = 0;
+        for (int i = e * run; i < min(a.n_seqs, (e + 1) * run); i++) n += seq_units(a, i, true);
+        cum[e + 1] = n;
+    }
+    if (threadIdx.x == 0) cum[0] = 0;
+    __syncthreads();
+    if (threadIdx.x < 32) {
+        constexpr int PER = T_ENTRIES / 32;
+        int v[PER], sum = 0;
+#pragma unroll
+        for (int i = 0; i < PER; i++) sum += v[i] = cum[1 + threadIdx.x * PER + i];
+        int upto = sum;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int x = __shfl_up_sync(D1_FULL_MASK, upto, o);
+            if ((int)threadIdx.x >= o) upto += x;
         }
+        upto -= sum;
+#pragma unroll
+        for (int i = 0; i < PER; i++) cum[1 + threadIdx.x * PER + i] = upto += v[i];
     }
-    __device__ int ext_tiles() const { return (s.ext_len + TKV - 1) / TKV; }
-    __device__ int tiles() const { return ext_tiles() + (s.kv_len + TKV - 1) / TKV; }
+    __syncthreads();
+}
+
+struct Unit {
+    int sq, q_start, q_len, kv_start, kv_len, ext_len;
+    int mode, block, h;  // h: first head; of a packed unit the first of its kv head
+
+    // unit u of the table
+    __device__ void find(const Kv4Args& a, const int* cum, int run, int u) {
+        int lo = 0, hi = T_ENTRIES - 1;  // the last entry that begins at or before u
+        while (lo < hi) {
+            const int mid = (lo + hi + 1) / 2;
+            if (cum[mid] <= u) lo = mid;
+            else hi = mid - 1;
+        }
+        int rest = u - cum[lo];
+        sq = lo * run;
+        if (run > 1)
+            for (int n; rest >= (n = seq_units(a, sq, false)); sq++) rest -= n;
+        const D1Kv4Seq& s = a.seqs[sq];
+        q_start = s.q_start;
+        q_len = s.q_len;
+        kv_start = s.kv_start;
+        kv_len = s.kv_len;
+        ext_len = s.ext_len;
+        mode = unit_mode(a, q_len);
+        const int hu = mode == kPacked ? a.heads / a.group : mode == kPair ? a.heads / 2 : a.heads;
+        block = rest / hu;
+        h = rest % hu * (mode == kPacked ? a.group : mode == kPair ? 2 : 1);
+    }
+    __device__ int ext_tiles() const { return (ext_len + TKV - 1) / TKV; }
+    __device__ int tiles() const { return ext_tiles() + (kv_len + TKV - 1) / TKV; }
     __device__ int valid(int j) const {  // keys of tile j, at least 1; 128 or more: all
         const int e = ext_tiles();
-        return j < e ? s.ext_len - j * TKV : s.kv_len - (j - e) * TKV;
+        return j < e ? ext_len - j * TKV : kv_len - (j - e) * TKV;
     }
-    __device__ int row0(int w) const { return block * rows_per_block() + (pair ? 0 : w * TQ); }  // of the sequence
-    __device__ int head(int w) const { return h + (pair ? w : 0); }
-    __device__ int tiles_of_rows() const { return pair || s.q_len > row0(1) ? 2 : 1; }
+    __device__ int q_tiles() const { return mode == kPacked ? 1 : mode == kPair || q_len > row0(1) ? 2 : 1; }
+    __device__ int row0(int w) const {  // of the sequence; not of a packed unit
+        return mode == kPair ? block * TQ : (2 * block + w) * TQ;
+    }
+    __device__ int head(int w) const { return h + (mode == kPair ? w : 0); }
+    __device__ int rows(const Kv4Args& a, int w) const { return mode == kPacked ? q_len * a.group : q_len - row0(w); }
+    // key tiles that warpgroup w takes: all, or of a packed unit every other one, from w
+    __device__ int tiles_of(int w) const {
+        return mode == kPacked ? (tiles() - w + 1) / 2 : w < q_tiles() ? tiles() : 0;
+    }
+    __device__ int tile_of(int w, int i) const { return mode == kPacked ? 2 * i + w : i; }
 };
 
 // The pieces of a cached tile that one loader thread moves: 16 bytes (32 codes) each, K in pieces 0-255, V in 256-511.
@@ -561,6 +602,8 @@ __global__ void __launch_bounds__(T_THREADS, 1)
     uint64_t* bars = reinterpret_cast<uint64_t*>(sO + 2 * T_O_BYTES);
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + T_NBARS);
     volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+    float* join = reinterpret_cast<float*>(tmem_slot + 4);  // [128][2]: maximum and sum of warpgroup 1's rows
+    int* cum = reinterpret_cast<int*>(join + 2 * TQ);       // [T_ENTRIES + 1]
     auto bar = [&](int i) { return smem_u32(bars + i); };
     if (smem_u32(t_smem) & 1023) {  // never expected: dynamic shared memory starts at the window's base
         pdl_wait();
@@ -586,6 +629,8 @@ __global__ void __launch_bounds__(T_THREADS, 1)
             mbar_init(bar(B_OSTAGED + w), 4);
             mbar_init(bar(B_OREAD + w), 1);
         }
+        mbar_init(bar(B_JOIN), 4);
+        mbar_init(bar(B_JOINED), 4);
         mbar_init(bar(B_DRAIN), 1);
         *abort_flag = 0;
         fence_mbar_init();
@@ -599,7 +644,10 @@ __global__ void __launch_bounds__(T_THREADS, 1)
     tc_fence_after();
     const uint32_t tmem = *tmem_slot;
     pdl_entry();  // barriers and TMEM are set up; global memory is touched only after this
-    Walk un(a);
+    const int run = (a.n_seqs + T_ENTRIES - 1) / T_ENTRIES;
+    build_units(a, cum, run);
+    const int n_units = cum[T_ENTRIES];
+    Unit un;
 
     if (warp == 8 || warp >= 10) {
         // ------------------------------------------------------------------ loaders
@@ -607,10 +655,11 @@ __global__ void __launch_bounds__(T_THREADS, 1)
         const bool issuer = warp == 8 && lane == 0;
         int qi = 0, ki = 0;
         bool ok = true;
-        while (ok && un.next(a)) {
+        for (int u = blockIdx.x; ok && u < n_units; u += gridDim.x) {
+            un.find(a, cum, run, u);
             const int g = un.h / a.group, nt = un.tiles(), e_tiles = un.ext_tiles();
             if (nt == 0) continue;
-            const D1Kv4Seq& s = un.s;
+            const D1Kv4Seq& s = a.seqs[un.sq];
             const uint8_t* k4 = s.k4 + (size_t)g * s.ext_cap * 32;
             const uint8_t* v4 = s.v4 + (size_t)g * s.ext_cap * 32;
             const uint16_t* kp = reinterpret_cast<const uint16_t*>(s.kp) + (size_t)g * s.ext_cap;
@@ -639,16 +688,20 @@ __global__ void __launch_bounds__(T_THREADS, 1)
                 // a whole tile inside the sequence comes by TMA; one that the sequence ends in row by row, with zeros
                 // behind the end, so that no load reads a row outside a sequence
                 const uint32_t dq = smem_u32(sQ + qs * 2 * T_QT_BYTES);
-                const int nq = un.tiles_of_rows();
+                const int nq = un.q_tiles();
                 bool partial = false;
                 for (int w = 0; w < nq; w++) {
-                    const int rows = s.q_len - un.row0(w);
-                    if (rows >= TQ) continue;
+                    const int rows = un.rows(a, w);
+                    if (un.mode != kPacked && rows >= TQ) continue;
                     partial = true;
                     for (int c = lane; c < TQ * 8; c += 32) {
                         const int r = c >> 3, ch = c & 7;
-                        const __half* src = r < rows ? a.Q + (size_t)(s.q_start + un.row0(w) + r) * a.ldq + un.head(w) * 64 + ch * 8
-                                                     : a.Q;
+                        const __half* src = a.Q;
+                        if (r < rows) {
+                            const int row = un.mode == kPacked ? r / a.group : un.row0(w) + r;
+                            const int h = un.mode == kPacked ? un.h + r % a.group : un.head(w);
+                            src += (size_t)(un.q_start + row) * a.ldq + h * 64 + ch * 8;
+                        }
                         cp_async16z(dq + w * T_QT_BYTES + r * 128 + ((ch ^ (r & 7)) << 4), src, r < rows ? 16 : 0);
                     }
                 }
@@ -660,11 +713,11 @@ __global__ void __launch_bounds__(T_THREADS, 1)
                 if (issuer) {
                     uint32_t bytes = 0;
                     for (int w = 0; w < nq; w++)
-                        if (s.q_len - un.row0(w) >= TQ) bytes += T_QT_BYTES;
+                        if (un.mode != kPacked && un.rows(a, w) >= TQ) bytes += T_QT_BYTES;
                     mbar_arrive_expect_tx(bar(B_QFULL + qs), bytes);
                     for (int w = 0; w < nq; w++)
-                        if (s.q_len - un.row0(w) >= TQ)
-                            tma_load_2d(dq + w * T_QT_BYTES, &tmQ, un.head(w) * 64, s.q_start + un.row0(w), bar(B_QFULL + qs));
+                        if (un.mode != kPacked && un.rows(a, w) >= TQ)
+                            tma_load_2d(dq + w * T_QT_BYTES, &tmQ, un.head(w) * 64, un.q_start + un.row0(w), bar(B_QFULL + qs));
                 }
             }
             qi++;
@@ -697,7 +750,7 @@ __global__ void __launch_bounds__(T_THREADS, 1)
                     fence_async_smem_cta();
                     mbar_arrive(bar(B_KVFULL + st));
                 } else {
-                    const int row0 = s.kv_start + (j - e_tiles) * TKV;
+                    const int row0 = un.kv_start + (j - e_tiles) * TKV;
                     if (n >= TKV) {
                         if (issuer) {
                             mbar_arrive_expect_tx(bar(B_KVFULL + st), 2 * T_KV_BYTES);
@@ -738,52 +791,50 @@ __global__ void __launch_bounds__(T_THREADS, 1)
     } else if (warp == 9) {
         // ------------------------------------------------------------------ MMA issuer
         if (lane == 0) {
-            int cnt[2] = {0, 0}, units[2] = {0, 0};  // key tiles and units of each query tile so far
+            int cnt[2] = {0, 0}, units[2] = {0, 0};  // key tiles and units of each warpgroup so far
             int qi = 0, ki = 0;
             bool ok = true;
-            while (ok && un.next(a)) {
-                const int nt = un.tiles(), nw = un.tiles_of_rows();
+            for (int u = blockIdx.x; ok && u < n_units; u += gridDim.x) {
+                un.find(a, cum, run, u);
+                const int nt = un.tiles(), nw = un.q_tiles();
+                const bool packed = un.mode == kPacked;
                 if (nt == 0) continue;
                 const int qs = qi % T_QSLOTS;
                 if (!(ok = mbar_wait(bar(B_QFULL + qs), (qi / T_QSLOTS) & 1, abort_flag))) break;
                 tc_fence_after();
                 const uint32_t q_addr = smem_u32(sQ + qs * 2 * T_QT_BYTES);
                 auto k_addr = [&](int j) { return smem_u32(sKV + ((ki + j) % T_STAGES) * 2 * T_KV_BYTES); };
-                auto kv_ready = [&](int j) {
-                    return mbar_wait(bar(B_KVFULL + (ki + j) % T_STAGES), ((ki + j) / T_STAGES) & 1, abort_flag);
-                };
-                auto issue_s = [&](int w, int j) -> bool {
-                    const int c = cnt[w] + j;
-                    if (c > 0 && !mbar_wait(bar(B_SFREE + w), (c - 1) & 1, abort_flag)) return false;
-                    tc_fence_after();
-                    const uint32_t ka = k_addr(j);
+                // S of key tile j, for the warpgroups that take it
+                auto issue_s = [&](int j) -> bool {
+                    if (!mbar_wait(bar(B_KVFULL + (ki + j) % T_STAGES), ((ki + j) / T_STAGES) & 1, abort_flag)) return false;
+                    for (int w = packed ? j & 1 : 0; w < (packed ? (j & 1) + 1 : nw); w++) {
+                        const int c = cnt[w] + (packed ? j >> 1 : j);
+                        if (c > 0 && !mbar_wait(bar(B_SFREE + w), (c - 1) & 1, abort_flag)) return false;
+                        tc_fence_after();
+                        const uint32_t ka = k_addr(j), qa = q_addr + (packed ? 0 : w * T_QT_BYTES);
 #pragma unroll
-                    for (int k = 0; k < 4; k++)
-                        tc_mma_f16(tmem + w * T_WG_COLS, smem_desc_k128(q_addr + w * T_QT_BYTES + k * 32),
-                                   smem_desc_k128(ka + k * 32), IDESC_S, k != 0);
-                    tc_commit(bar(B_SFULL + w));
+                        for (int k = 0; k < 4; k++)
+                            tc_mma_f16(tmem + w * T_WG_COLS, smem_desc_k128(qa + k * 32), smem_desc_k128(ka + k * 32), IDESC_S,
+                                       k != 0);
+                        tc_commit(bar(B_SFULL + w));
+                    }
                     return true;
                 };
-                if (!(ok = kv_ready(0))) break;
-                for (int w = 0; w < nw && ok; w++) ok = issue_s(w, 0);
-                for (int j = 0; j < nt && ok; j++) {
-                    if (j + 1 < nt) {  // S(j + 1) computes while the softmax works on tile j
-                        if (!(ok = kv_ready(j + 1))) break;
-                        for (int w = 0; w < nw && ok; w++) ok = issue_s(w, j + 1);
-                        if (!ok) break;
-                    }
+                const int ahead = packed ? 2 : 1;  // S of the next tile of a warpgroup computes while it works on one
+                for (int j = 0, js = 0; j < nt && ok; j++) {
+                    for (; js < nt && js <= j + ahead && ok; js++) ok = issue_s(js);
                     const uint32_t v_addr = k_addr(j) + T_KV_BYTES;
-                    for (int w = 0; w < nw && ok; w++) {
-                        const int c = cnt[w] + j;
+                    for (int w = packed ? j & 1 : 0; w < (packed ? (j & 1) + 1 : nw) && ok; w++) {
+                        const int i = packed ? j >> 1 : j, c = cnt[w] + i;
                         ok = mbar_wait(bar(B_PFULL + w), c & 1, abort_flag);
                         // the first P V of a unit overwrites O: the unit before must have been read
-                        if (ok && j == 0 && units[w] > 0) ok = mbar_wait(bar(B_OFREE + w), (units[w] - 1) & 1, abort_flag);
+                        if (ok && i == 0 && units[w] > 0) ok = mbar_wait(bar(B_OFREE + w), (units[w] - 1) & 1, abort_flag);
                         if (!ok) break;
                         tc_fence_after();
 #pragma unroll
                         for (int k = 0; k < TKV / 16; k++)
                             tc_mma_f16_ts(tmem + w * T_WG_COLS + T_O_COL, tmem + w * T_WG_COLS + T_P_COL + k * 8,
-                                          smem_desc_k128(v_addr + k * 2048), IDESC_O, (j | k) != 0);
+                                          smem_desc_k128(v_addr + k * 2048), IDESC_O, (i | k) != 0);
                         tc_commit(bar(B_ODONE + w));
                     }
                     if (!ok) break;
@@ -793,9 +844,9 @@ __global__ void __launch_bounds__(T_THREADS, 1)
                 tc_commit(bar(B_QEMPTY + qs));
                 ki += nt;
                 qi++;
-                for (int w = 0; w < nw; w++) {
-                    cnt[w] += nt;
-                    units[w]++;
+                for (int w = 0; w < 2; w++) {
+                    cnt[w] += un.tiles_of(w);
+                    units[w] += un.tiles_of(w) > 0;
                 }
             }
             if (!ok) record_err(a.err, abort_flag, kErrWaitFull);
@@ -809,24 +860,38 @@ __global__ void __launch_bounds__(T_THREADS, 1)
         const uint32_t lane_off = (uint32_t)((warp & 3) * 32) << 16;
         const uint32_t tS = tmem + w * T_WG_COLS + lane_off, tP = tS + T_P_COL, tO = tS + T_O_COL;
         uint8_t* stile = sO + w * T_O_BYTES;
-        int cnt = 0, nst = 0;  // key tiles so far; output tiles staged so far
+        int cnt = 0, nst = 0, njoin = 0;  // key tiles so far; output tiles staged; packed units joined
         bool ok = true;
-        while (ok && un.next(a)) {
-            if (w == 1 && un.tiles_of_rows() == 1) continue;
-            const int nt = un.tiles(), q0 = un.row0(w), q = q0 + row, h = un.head(w);
-            const size_t grow = (size_t)(un.s.q_start + q);
-            if (nt == 0) {  // no keys: zeros
-                if (q < un.s.q_len) {
+        for (int u = blockIdx.x; ok && u < n_units; u += gridDim.x) {
+            un.find(a, cum, run, u);
+            const bool packed = un.mode == kPacked;
+            if (w == 1 && !packed && un.q_tiles() == 1) continue;
+            // this thread's row: of the sequence and the head
+            const int rows = un.rows(a, w), nt = un.tiles_of(w);
+            const bool there = row < rows;
+            const int q = packed ? row / a.group : un.row0(w) + row, h = packed ? un.h + row % a.group : un.head(w);
+            const size_t grow = (size_t)(un.q_start + q);
+            if (un.tiles() == 0) {  // no keys: zeros
+                if (there && !(packed && w == 1)) {
                     for (int i = 0; i < 8; i++)
                         *reinterpret_cast<uint4*>(a.O + grow * a.ldo + h * 64 + i * 8) = make_uint4(0, 0, 0, 0);
                     if (a.lse) a.lse[(size_t)h * a.lse_ld + grow] = -INFINITY;
                 }
                 continue;
             }
+            const bool idle = (warp & 3) * 32 >= rows;  // none of the warp's rows is there
             float m = -INFINITY, l = 0.f;
             for (int j = 0; j < nt; j++) {
                 const int c = cnt + j;
                 if (!(ok = __all_sync(D1_FULL_MASK, mbar_wait(bar(B_SFULL + w), c & 1, abort_flag)))) break;
+                if (idle) {  // in step with the others: their P of the tile before must be complete
+                    if (c > 0 && !(ok = __all_sync(D1_FULL_MASK, mbar_wait(bar(B_PFULL + w), (c - 1) & 1, abort_flag)))) break;
+                    if (lane == 0) {
+                        mbar_arrive(bar(B_SFREE + w));
+                        mbar_arrive(bar(B_PFULL + w));
+                    }
+                    continue;
+                }
                 tc_fence_after();
                 uint32_t sr[TKV];
 #pragma unroll
@@ -836,7 +901,7 @@ __global__ void __launch_bounds__(T_THREADS, 1)
                 tc_fence_before();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(bar(B_SFREE + w));
-                const int n = un.valid(j);
+                const int n = un.valid(un.tile_of(w, j));
                 if (n < TKV) {
 #pragma unroll
                     for (int i = 0; i < TKV; i++)
@@ -912,21 +977,61 @@ __global__ void __launch_bounds__(T_THREADS, 1)
             }
             if (!ok) break;
             cnt += nt;
+            if (packed && w == 1) {  // the rest is warpgroup 0's, which shares the lanes
+                if (njoin > 0 && !(ok = __all_sync(D1_FULL_MASK, mbar_wait(bar(B_JOINED), (njoin - 1) & 1, abort_flag)))) break;
+                if (nt > 0) {
+                    if (!(ok = __all_sync(D1_FULL_MASK, mbar_wait(bar(B_ODONE + 1), (cnt - 1) & 1, abort_flag)))) break;
+                    tc_fence_after();
+                }
+                join[2 * row] = m;
+                join[2 * row + 1] = l;
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(bar(B_JOIN));
+                njoin++;
+                continue;
+            }
             if (!(ok = __all_sync(D1_FULL_MASK, mbar_wait(bar(B_ODONE + w), (cnt - 1) & 1, abort_flag)))) break;
             tc_fence_after();
-            const float il = 1.f / l;
             uint32_t o[64];
             tmem_ld32(tO, *reinterpret_cast<uint32_t(*)[32]>(o));
             tmem_ld32(tO + 32, *reinterpret_cast<uint32_t(*)[32]>(o + 32));
             tc_wait_ld();
+            if (packed) {
+                if (!(ok = __all_sync(D1_FULL_MASK, mbar_wait(bar(B_JOIN), njoin & 1, abort_flag)))) break;
+                tc_fence_after();
+                njoin++;
+                const float m1 = join[2 * row], l1 = join[2 * row + 1];
+                if (un.tiles_of(1) > 0) {
+                    const float both = fmaxf(m, m1), f0 = ex2(m - both), f1 = ex2(m1 - both);
+#pragma unroll
+                    for (int i = 0; i < 8; i++) {
+                        uint32_t o1[8];
+                        tmem_ld8(tO + T_WG_COLS + i * 8, o1);
+                        tc_wait_ld();
+#pragma unroll
+                        for (int k = 0; k < 8; k++)
+                            o[i * 8 + k] = __float_as_uint(__uint_as_float(o[i * 8 + k]) * f0 + __uint_as_float(o1[k]) * f1);
+                    }
+                    l = l * f0 + l1 * f1;
+                    m = both;
+                }
+            }
             tc_fence_before();
             __syncwarp();
-            if (lane == 0) mbar_arrive(bar(B_OFREE + w));
+            if (lane == 0) {
+                mbar_arrive(bar(B_OFREE + w));
+                if (packed) {
+                    if (un.tiles_of(1) > 0) mbar_arrive(bar(B_OFREE + 1));
+                    mbar_arrive(bar(B_JOINED));
+                }
+            }
+            const float il = 1.f / l;
             uint32_t oh[32];
 #pragma unroll
             for (int i = 0; i < 32; i++) oh[i] = pack_h2(__uint_as_float(o[2 * i]) * il, __uint_as_float(o[2 * i + 1]) * il);
-            if (a.lse && q < un.s.q_len) a.lse[(size_t)h * a.lse_ld + grow] = (m + log2f(l)) * kLn2;
-            if (q0 + TQ <= un.s.q_len) {
+            if (a.lse && there) a.lse[(size_t)h * a.lse_ld + grow] = (m + log2f(l)) * kLn2;
+            if (!packed && rows >= TQ) {
                 // a whole tile: staged, then one bulk store; the store before must have read the buffer
                 if (nst > 0) {
                     if (row == 0) {
@@ -945,11 +1050,11 @@ __global__ void __launch_bounds__(T_THREADS, 1)
                 bool staged = true;
                 if (row == 0) {
                     staged = mbar_wait(bar(B_OSTAGED + w), nst & 1, abort_flag);
-                    if (staged) o_tile_store(&tmO, smem_u32(stile), h * 64, un.s.q_start + q0);
+                    if (staged) o_tile_store(&tmO, smem_u32(stile), h * 64, un.q_start + un.row0(w));
                 }
                 nst++;
                 if (!(ok = __all_sync(D1_FULL_MASK, staged))) break;
-            } else if (q < un.s.q_len) {
+            } else if (there) {
 #pragma unroll
                 for (int i = 0; i < 8; i++)
                     *reinterpret_cast<uint4*>(a.O + grow * a.ldo + h * 64 + i * 8) =
@@ -1456,10 +1561,12 @@ int launch_rows(Kv4Args& a, int max_q, int max_keys, int kv_heads, cudaStream_t 
     long long x = ((long long)max_q * a.group + 8 * NT - 1) / (8 * NT);
     x = x < 1 ? 1 : x > 65536 ? 65536 : x;
     const int z = a.n_seqs < 65535 ? a.n_seqs : 65535;
-    // CTAs to a cluster: as many as the keys give every warp a tile and more than a few waves of CTAs are not needed
+    // CTAs to a cluster: as many as are resident at once, and no more than the keys give a tile to every warp (16
+    // sequences of 8 rows, 4096 keys, 2 CTAs to an SM: 24 us with 2, 33 with 1, 31 with 4 and 46 with 8; one token over
+    // 4097 keys: 8.5 us with 8, 11, 17 and 27 with 4, 2 and 1)
     int ranks = R_CLUSTER;
-    const long long tiles = ((long long)max_keys + R_KEYS - 1) / R_KEYS;
-    while (ranks > 1 && ((ranks / 2) * R_WARPS >= tiles || x * kv_heads * z * ranks / 2 >= 148 * 12)) ranks /= 2;
+    const long long tiles = ((long long)max_keys + R_KEYS - 1) / R_KEYS, slots = 148 * (NT == 1 ? 4 : 2);
+    while (ranks > 1 && ((ranks / 2) * R_WARPS >= tiles || x * kv_heads * z * ranks > slots)) ranks /= 2;
     a.ranks = ranks;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)x * ranks, kv_heads, z);
@@ -1483,11 +1590,10 @@ int launch_tc(Kv4Args& a, int max_q, cudaStream_t st) {
     if (!smem_opt_in(k_kv4_attn_tc, T_SMEM, &done)) return -1;
     const int sms = sm_count();
     if (!sms) return -1;
-    const bool pair = a.group % 2 == 0;
-    const int per = pair ? TQ : 2 * TQ;
-    a.n_blocks = max_q > 0 ? (max_q - 1) / per + 1 : 1;
-    const long long units = (long long)a.n_seqs * a.n_blocks * (pair ? a.heads / 2 : a.heads);
-    if (units > 0x7fffffffLL - 4096) return -1;
+    // no more CTAs than units, were every sequence max_q rows long
+    const long long hu = (long long)max_q * a.group <= TQ ? a.heads / a.group : a.group % 2 == 0 ? a.heads / 2 : a.heads;
+    const int per = a.group % 2 == 0 ? TQ : 2 * TQ;
+    const long long units = a.n_seqs * hu * (max_q > per ? (max_q - 1) / per + 1 : 1);
     const int kv_cols = a.heads / a.group * 64;
     CUtensorMap tq, tk, tv, to;
     if (!attn_tmap(&tq, a.Q, a.heads * 64, a.q_rows, a.ldq, TQ) || !attn_tmap(&to, a.O, a.heads * 64, a.q_rows, a.ldo, TQ))
