@@ -466,15 +466,22 @@ __global__ void __launch_bounds__(R_WARPS * 32, NT == 1 ? 4 : 2) k_kv4_attn_rows
 //   0-3, 4-7   softmax: thread = query row = TMEM lane. S is copied to registers and released at once, P goes to TMEM as
 //              fp16, O is rescaled only when a row's maximum grows by more than 2^8. Warps whose rows are all behind the
 //              sequence's end leave the work out.
-//   8, 10, 11  loaders. A cached tile: every thread fetches 16-byte pieces of codes and their parameters into registers
-//              while the tile before it is stored, then expands them to fp16 (exact) into the swizzled layout that the
-//              MMAs read. Own rows: whole tiles by TMA, partial ones through registers.
-//   9          TMEM, and the MMAs from one thread: S = Q K^T (both in shared memory), O += P V (P in TMEM)
+//   8          fetches the query rows (whole tiles by TMA, partial and packed ones row by row) and, by bulk copies into a
+//              ring of their own, the codes and parameters of the cached tiles
+//   10-13      expand them to fp16 (exact) into the swizzled layout that the MMAs read. Own rows: whole tiles by TMA,
+//              partial ones through registers. (The codes straight to the expanding warps' registers, a tile ahead: 3200
+//              clocks a tile with 4 such warps and nothing else running, all of it latency.)
+//   9, 14      MMA issuers of warpgroups 0 and 1, one thread each: S = Q K^T (both in shared memory), O += P V (P in
+//              TMEM). Warp 9 also keeps the TMEM. (One issuer for both: each warpgroup then waits for the other's P.)
+// The softmax warps take 192 registers, the others 64.
 // TMEM (512 columns), warpgroup w at 256 w: S in 128 columns, P in 64, O in 64. Both warpgroups' columns share the lanes,
 // so that a packed unit is joined by the first reading the second's O.
-constexpr int TQ = 128, TKV = 128, T_QSLOTS = 2, T_STAGES = 4, T_LOADERS = 3, T_THREADS = 384;
-constexpr int T_QT_BYTES = TQ * 128, T_KV_BYTES = TKV * 128, T_O_BYTES = TQ * 128;
+constexpr int TQ = 128, TKV = 128, T_QSLOTS = 2, T_STAGES = 4, T_RAW_STAGES = 3, T_EXPANDERS = 128, T_THREADS = 512;
+constexpr int T_QT_BYTES = TQ * 128, T_KV_BYTES = TKV * 128;
+constexpr int T_RAW_V = TKV * 32, T_RAW_KP = 2 * TKV * 32, T_RAW_VP = T_RAW_KP + TKV * 2, T_RAW_BYTES = T_RAW_VP + TKV * 2;
 constexpr int T_ENTRIES = 256;  // of the table of units
+constexpr int T_SOFTMAX_REGS = 192, T_OTHER_REGS = 64;
+static_assert(T_SOFTMAX_REGS + T_OTHER_REGS <= 2 * 128, "what the launch of 512 threads, 128 registers each, has");
 constexpr uint32_t T_TMEM_COLS = 512, T_WG_COLS = 256, T_P_COL = TKV, T_O_COL = TKV + TKV / 2;
 enum : int {
     B_QFULL = 0,
@@ -486,14 +493,14 @@ enum : int {
     B_PFULL = B_SFREE + 2,           // [w]: P is in TMEM (4 warps)
     B_ODONE = B_PFULL + 2,           // [w]: P V has completed
     B_OFREE = B_ODONE + 2,           // [w]: O has been read (4 warps; of a packed unit those of warpgroup 0)
-    B_OSTAGED = B_OFREE + 2,         // [w]: the output tile is in shared memory (4 warps)
-    B_OREAD = B_OSTAGED + 2,         // [w]: its last bulk store has read it
-    B_JOIN = B_OREAD + 2,            // a packed unit's maxima and sums of warpgroup 1 are in shared memory (4 warps)
+    B_RAWFULL = B_OFREE + 2,         // [raw stage]: a tile's codes and parameters are in shared memory
+    B_RAWEMPTY = B_RAWFULL + T_RAW_STAGES,  // [raw stage] (4 warps)
+    B_JOIN = B_RAWEMPTY + T_RAW_STAGES,  // a packed unit's maxima and sums of warpgroup 1 are in shared memory (4 warps)
     B_JOINED = B_JOIN + 1,           // and have been read (4 warps)
-    B_DRAIN = B_JOINED + 1,
-    T_NBARS = B_DRAIN + 1
+    B_DRAIN = B_JOINED + 1,          // [issuer]
+    T_NBARS = B_DRAIN + 2
 };
-constexpr int T_SMEM = T_QSLOTS * 2 * T_QT_BYTES + T_STAGES * 2 * T_KV_BYTES + 2 * T_O_BYTES + T_NBARS * 8 + 16 + TQ * 8 +
+constexpr int T_SMEM = T_QSLOTS * 2 * T_QT_BYTES + T_STAGES * 2 * T_KV_BYTES + T_RAW_STAGES * T_RAW_BYTES + T_NBARS * 8 + 16 + TQ * 8 +
                        (T_ENTRIES + 1) * 4;
 static_assert(T_SMEM <= 232448 && T_O_COL + 64 <= T_WG_COLS, "shared memory and TMEM of the tcgen05 attention");
 
@@ -587,19 +594,23 @@ struct Unit {
     __device__ int tile_of(int w, int i) const { return mode == kPacked ? 2 * i + w : i; }
 };
 
-// The pieces of a cached tile that one loader thread moves: 16 bytes (32 codes) each, K in pieces 0-255, V in 256-511.
-constexpr int T_PIECES = (4 * TKV + 32 * T_LOADERS - 1) / (32 * T_LOADERS);
+// A run of bytes global -> shared (addresses and size multiples of 16), completing on the mbarrier.
+__device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
+    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst),
+                 "l"(src), "r"(bytes), "r"(bar)
+                 : "memory");
+}
 
 __global__ void __launch_bounds__(T_THREADS, 1)
     k_kv4_attn_tc(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
-                  const __grid_constant__ CUtensorMap tmV, const __grid_constant__ CUtensorMap tmO, const Kv4Args a) {
+                  const __grid_constant__ CUtensorMap tmV, const Kv4Args a) {
     constexpr uint32_t IDESC_S = idesc_f16_f32(TQ, TKV);
     constexpr uint32_t IDESC_O = idesc_f16_f32(TQ, 64) | (1u << 16);  // B (= V) MN-major
     extern __shared__ __align__(1024) uint8_t t_smem[];
     uint8_t* sQ = t_smem;                                   // slot q: tile 0 at q * 2 * T_QT_BYTES, tile 1 behind it
     uint8_t* sKV = sQ + T_QSLOTS * 2 * T_QT_BYTES;          // stage s: K at s * 2 * T_KV_BYTES, V behind it
-    uint8_t* sO = sKV + T_STAGES * 2 * T_KV_BYTES;          // output tile of w at w * T_O_BYTES
-    uint64_t* bars = reinterpret_cast<uint64_t*>(sO + 2 * T_O_BYTES);
+    uint8_t* sRaw = sKV + T_STAGES * 2 * T_KV_BYTES;        // raw stage r at r * T_RAW_BYTES: K, V, parameters of K, of V
+    uint64_t* bars = reinterpret_cast<uint64_t*>(sRaw + T_RAW_STAGES * T_RAW_BYTES);
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + T_NBARS);
     volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
     float* join = reinterpret_cast<float*>(tmem_slot + 4);  // [128][2]: maximum and sum of warpgroup 1's rows
@@ -614,11 +625,11 @@ __global__ void __launch_bounds__(T_THREADS, 1)
     if (threadIdx.x == 0) {
         for (int i = 0; i < T_QSLOTS; i++) {
             mbar_init(bar(B_QFULL + i), 1);
-            mbar_init(bar(B_QEMPTY + i), 1);
+            mbar_init(bar(B_QEMPTY + i), 2);
         }
         for (int i = 0; i < T_STAGES; i++) {
-            mbar_init(bar(B_KVFULL + i), 32 * T_LOADERS);
-            mbar_init(bar(B_KVEMPTY + i), 1);
+            mbar_init(bar(B_KVFULL + i), T_EXPANDERS);
+            mbar_init(bar(B_KVEMPTY + i), 2);
         }
         for (int w = 0; w < 2; w++) {
             mbar_init(bar(B_SFULL + w), 1);
@@ -626,12 +637,14 @@ __global__ void __launch_bounds__(T_THREADS, 1)
             mbar_init(bar(B_PFULL + w), 4);
             mbar_init(bar(B_ODONE + w), 1);
             mbar_init(bar(B_OFREE + w), 4);
-            mbar_init(bar(B_OSTAGED + w), 4);
-            mbar_init(bar(B_OREAD + w), 1);
+            mbar_init(bar(B_DRAIN + w), 1);
+        }
+        for (int i = 0; i < T_RAW_STAGES; i++) {
+            mbar_init(bar(B_RAWFULL + i), 1);
+            mbar_init(bar(B_RAWEMPTY + i), T_EXPANDERS / 32);
         }
         mbar_init(bar(B_JOIN), 4);
         mbar_init(bar(B_JOINED), 4);
-        mbar_init(bar(B_DRAIN), 1);
         *abort_flag = 0;
         fence_mbar_init();
     }
@@ -649,218 +662,247 @@ __global__ void __launch_bounds__(T_THREADS, 1)
     const int n_units = cum[T_ENTRIES];
     Unit un;
 
-    if (warp == 8 || warp >= 10) {
-        // ------------------------------------------------------------------ loaders
-        const int lt = (warp == 8 ? 0 : warp - 9) * 32 + lane;
-        const bool issuer = warp == 8 && lane == 0;
-        int qi = 0, ki = 0;
+    if (warp >= 8) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(T_OTHER_REGS));
+        if (warp == 8) {
+        // ------------------------------------------------------------------ fetching
+        int qi = 0, ri = 0;
         bool ok = true;
         for (int u = blockIdx.x; ok && u < n_units; u += gridDim.x) {
             un.find(a, cum, run, u);
-            const int g = un.h / a.group, nt = un.tiles(), e_tiles = un.ext_tiles();
-            if (nt == 0) continue;
-            const D1Kv4Seq& s = a.seqs[un.sq];
-            const uint8_t* k4 = s.k4 + (size_t)g * s.ext_cap * 32;
-            const uint8_t* v4 = s.v4 + (size_t)g * s.ext_cap * 32;
-            const uint16_t* kp = reinterpret_cast<const uint16_t*>(s.kp) + (size_t)g * s.ext_cap;
-            const uint16_t* vp = reinterpret_cast<const uint16_t*>(s.vp) + (size_t)g * s.ext_cap;
-            uint4 piece[T_PIECES];
-            uint32_t par[T_PIECES];
-            auto fetch = [&](int j) {
-                const int n = un.valid(j);
-#pragma unroll
-                for (int i = 0; i < T_PIECES; i++) {
-                    const int c = lt + i * 32 * T_LOADERS, r = (c & 255) >> 1;
-                    piece[i] = make_uint4(0, 0, 0, 0);
-                    par[i] = 0;  // step 0: zeros
-                    if (c < 4 * TKV && r < n) {
-                        const size_t key = (size_t)j * TKV + r;
-                        piece[i] = __ldg(reinterpret_cast<const uint4*>((c < 256 ? k4 : v4) + key * 32) + (c & 1));
-                        par[i] = __ldg((c < 256 ? kp : vp) + key);
-                    }
-                }
-            };
-            if (e_tiles > 0) fetch(0);
+            const int g = un.h / a.group, e_tiles = un.ext_tiles();
+            if (un.tiles() == 0) continue;
             const int qs = qi % T_QSLOTS;
-            if (warp == 8) {
-                if (!(ok = __all_sync(D1_FULL_MASK, mbar_wait(bar(B_QEMPTY + qs), ((qi / T_QSLOTS) & 1) ^ 1, abort_flag))))
-                    break;
-                // a whole tile inside the sequence comes by TMA; one that the sequence ends in row by row, with zeros
-                // behind the end, so that no load reads a row outside a sequence
-                const uint32_t dq = smem_u32(sQ + qs * 2 * T_QT_BYTES);
-                const int nq = un.q_tiles();
-                bool partial = false;
-                for (int w = 0; w < nq; w++) {
-                    const int rows = un.rows(a, w);
-                    if (un.mode != kPacked && rows >= TQ) continue;
-                    partial = true;
-                    for (int c = lane; c < TQ * 8; c += 32) {
-                        const int r = c >> 3, ch = c & 7;
-                        const __half* src = a.Q;
-                        if (r < rows) {
-                            const int row = un.mode == kPacked ? r / a.group : un.row0(w) + r;
-                            const int h = un.mode == kPacked ? un.h + r % a.group : un.head(w);
-                            src += (size_t)(un.q_start + row) * a.ldq + h * 64 + ch * 8;
-                        }
-                        cp_async16z(dq + w * T_QT_BYTES + r * 128 + ((ch ^ (r & 7)) << 4), src, r < rows ? 16 : 0);
+            if (!(ok = __all_sync(D1_FULL_MASK, mbar_wait(bar(B_QEMPTY + qs), ((qi / T_QSLOTS) & 1) ^ 1, abort_flag)))) break;
+            // a whole tile inside the sequence comes by TMA; one that the sequence ends in row by row, with zeros behind
+            // the end, so that no load reads a row outside a sequence
+            const uint32_t dq = smem_u32(sQ + qs * 2 * T_QT_BYTES);
+            const int nq = un.q_tiles();
+            bool partial = false;
+            for (int w = 0; w < nq; w++) {
+                const int rows = un.rows(a, w);
+                if (un.mode != kPacked && rows >= TQ) continue;
+                partial = true;
+                for (int c = lane; c < TQ * 8; c += 32) {
+                    const int r = c >> 3, ch = c & 7;
+                    const __half* src = a.Q;
+                    if (r < rows) {
+                        const int row = un.mode == kPacked ? r / a.group : un.row0(w) + r;
+                        const int h = un.mode == kPacked ? un.h + r % a.group : un.head(w);
+                        src += (size_t)(un.q_start + row) * a.ldq + h * 64 + ch * 8;
                     }
-                }
-                if (partial) {
-                    asm volatile("cp.async.wait_all;" ::: "memory");
-                    fence_async_smem_cta();
-                    __syncwarp();
-                }
-                if (issuer) {
-                    uint32_t bytes = 0;
-                    for (int w = 0; w < nq; w++)
-                        if (un.mode != kPacked && un.rows(a, w) >= TQ) bytes += T_QT_BYTES;
-                    mbar_arrive_expect_tx(bar(B_QFULL + qs), bytes);
-                    for (int w = 0; w < nq; w++)
-                        if (un.mode != kPacked && un.rows(a, w) >= TQ)
-                            tma_load_2d(dq + w * T_QT_BYTES, &tmQ, un.head(w) * 64, un.q_start + un.row0(w), bar(B_QFULL + qs));
+                    cp_async16z(dq + w * T_QT_BYTES + r * 128 + ((ch ^ (r & 7)) << 4), src, r < rows ? 16 : 0);
                 }
             }
+            if (partial) {
+                asm volatile("cp.async.wait_all;" ::: "memory");
+                fence_async_smem_cta();
+                __syncwarp();
+            }
+            if (lane == 0) {
+                uint32_t bytes = 0;
+                for (int w = 0; w < nq; w++)
+                    if (un.mode != kPacked && un.rows(a, w) >= TQ) bytes += T_QT_BYTES;
+                mbar_arrive_expect_tx(bar(B_QFULL + qs), bytes);
+                for (int w = 0; w < nq; w++)
+                    if (un.mode != kPacked && un.rows(a, w) >= TQ)
+                        tma_load_2d(dq + w * T_QT_BYTES, &tmQ, un.head(w) * 64, un.q_start + un.row0(w), bar(B_QFULL + qs));
+            }
             qi++;
-            for (int j = 0; j < nt; j++) {
-                const int st = ki % T_STAGES;
-                if (!(ok = __all_sync(D1_FULL_MASK, mbar_wait(bar(B_KVEMPTY + st), ((ki / T_STAGES) & 1) ^ 1, abort_flag))))
+            const D1Kv4Seq& s = a.seqs[un.sq];
+            const size_t at = (size_t)g * s.ext_cap;
+            for (int j = 0; j < e_tiles; j++, ri++) {
+                const int rs = ri % T_RAW_STAGES;
+                if (!(ok = __all_sync(D1_FULL_MASK,
+                                      mbar_wait(bar(B_RAWEMPTY + rs), ((ri / T_RAW_STAGES) & 1) ^ 1, abort_flag))))
                     break;
-                uint8_t* dK = sKV + st * 2 * T_KV_BYTES;
-                const int n = un.valid(j);
-                if (j < e_tiles) {
-#pragma unroll
-                    for (int i = 0; i < T_PIECES; i++) {
-                        const int c = lt + i * 32 * T_LOADERS, r = (c & 255) >> 1;
-                        if (c < 4 * TKV) {
-                            uint8_t* row = dK + (c >> 8) * T_KV_BYTES + r * 128;
-                            const uint32_t p2 = par[i] * 0x00010001u, step = kv4_step2(p2);
-                            uint32_t z0, z1;
-                            kv4_zero(p2, z0, z1);
-                            const uint32_t word[4] = {piece[i].x, piece[i].y, piece[i].z, piece[i].w};
-#pragma unroll
-                            for (int q = 0; q < 4; q++) {
-                                uint32_t v[4];
-                                kv4_expand(word[q], z0, z1, v);
-                                *reinterpret_cast<uint4*>(row + ((((c & 1) * 4 + q) ^ (r & 7)) << 4)) =
-                                    make_uint4(h2_mul(v[0], step), h2_mul(v[1], step), h2_mul(v[2], step), h2_mul(v[3], step));
-                            }
-                        }
-                    }
-                    if (j + 1 < e_tiles) fetch(j + 1);
-                    fence_async_smem_cta();
-                    mbar_arrive(bar(B_KVFULL + st));
-                } else {
-                    const int row0 = un.kv_start + (j - e_tiles) * TKV;
-                    if (n >= TKV) {
-                        if (issuer) {
-                            mbar_arrive_expect_tx(bar(B_KVFULL + st), 2 * T_KV_BYTES);
-                            tma_load_2d(smem_u32(dK), &tmK, g * 64, row0, bar(B_KVFULL + st));
-                            tma_load_2d(smem_u32(dK + T_KV_BYTES), &tmV, g * 64, row0, bar(B_KVFULL + st));
-                        } else {
-                            mbar_arrive(bar(B_KVFULL + st));
-                        }
-                    } else {
-                        for (int c = lt; c < TKV * 8; c += 32 * T_LOADERS) {
-                            const int r = c >> 3, ch = c & 7;
-                            uint4 kx = make_uint4(0, 0, 0, 0), vx = kx;
-                            if (r < n) {
-                                const size_t at = (size_t)(row0 + r) * a.ldkv + g * 64 + ch * 8;
-                                kx = __ldg(reinterpret_cast<const uint4*>(a.K + at));
-                                vx = __ldg(reinterpret_cast<const uint4*>(a.V + at));
-                            }
-                            uint8_t* to = dK + r * 128 + ((ch ^ (r & 7)) << 4);
-                            *reinterpret_cast<uint4*>(to) = kx;
-                            *reinterpret_cast<uint4*>(to + T_KV_BYTES) = vx;
-                        }
-                        fence_async_smem_cta();
-                        mbar_arrive(bar(B_KVFULL + st));
-                    }
+                if (lane == 0) {
+                    // whole 16-byte runs: up to 8 parameters, which the arrays hold (ext_cap is a multiple of 8)
+                    const int n = min(un.valid(j), TKV);
+                    const uint32_t codes = n * 32, pars = ((n + 7) & ~7) * 2;
+                    const uint32_t dst = smem_u32(sRaw + rs * T_RAW_BYTES), full = bar(B_RAWFULL + rs);
+                    const size_t key = at + (size_t)j * TKV;
+                    mbar_arrive_expect_tx(full, 2 * (codes + pars));
+                    bulk_load(dst, s.k4 + key * 32, codes, full);
+                    bulk_load(dst + T_RAW_V, s.v4 + key * 32, codes, full);
+                    bulk_load(dst + T_RAW_KP, s.kp + key, pars, full);
+                    bulk_load(dst + T_RAW_VP, s.vp + key, pars, full);
                 }
-                ki++;
+                __syncwarp();
             }
         }
         asm volatile("cp.async.wait_all;" ::: "memory");  // nothing in flight when the CTA exits
         if (!ok && lane == 0) record_err(a.err, abort_flag, kErrWaitEmpty);
-        if (issuer) {
-            // TMA copies still in flight (only after an abort) land before the CTA exits
-            for (int i = ki > T_STAGES ? ki - T_STAGES : 0; i < ki; i++)
-                if (!mbar_wait_timed2(bar(B_KVFULL + i % T_STAGES), (i / T_STAGES) & 1)) break;
+        if (lane == 0) {
+            // copies still in flight (only after an abort) land before the CTA exits
+            for (int i = ri > T_RAW_STAGES ? ri - T_RAW_STAGES : 0; i < ri; i++)
+                if (!mbar_wait_timed2(bar(B_RAWFULL + i % T_RAW_STAGES), (i / T_RAW_STAGES) & 1)) break;
             for (int i = qi > T_QSLOTS ? qi - T_QSLOTS : 0; i < qi; i++)
                 if (!mbar_wait_timed2(bar(B_QFULL + i % T_QSLOTS), (i / T_QSLOTS) & 1)) break;
         }
-    } else if (warp == 9) {
-        // ------------------------------------------------------------------ MMA issuer
+        __syncwarp();
+    } else if (warp >= 10 && warp < 14) {
+        // ------------------------------------------------------------------ expanding
+        const int lt = (warp - 10) * 32 + lane;
+        int ri = 0, ki = 0;
+        bool ok = true;
+        for (int u = blockIdx.x; ok && u < n_units; u += gridDim.x) {
+            un.find(a, cum, run, u);
+            const int g = un.h / a.group, nt = un.tiles(), e_tiles = un.ext_tiles();
+            for (int j = 0; j < nt; j++, ki++) {
+                const int st = ki % T_STAGES, n = un.valid(j);
+                uint8_t* dK = sKV + st * 2 * T_KV_BYTES;
+                if (j < e_tiles) {
+                    // the thread's 16-byte pieces: of K, then of V, those of keys lt / 2 and 64 more, half lt % 2
+                    const int rs = ri % T_RAW_STAGES;
+                    const uint8_t* raw = sRaw + rs * T_RAW_BYTES;
+                    if (!(ok = __all_sync(D1_FULL_MASK, mbar_wait(bar(B_RAWFULL + rs), (ri / T_RAW_STAGES) & 1, abort_flag))))
+                        break;
+                    uint4 piece[4];
+                    uint32_t par[4];
+#pragma unroll
+                    for (int i = 0; i < 4; i++) {
+                        const int r = (lt >> 1) + (i & 1) * 64;
+                        piece[i] = *reinterpret_cast<const uint4*>(raw + (i >> 1) * T_RAW_V + r * 32 + (lt & 1) * 16);
+                        par[i] = *reinterpret_cast<const uint16_t*>(raw + T_RAW_KP + (i >> 1) * (TKV * 2) + r * 2);
+                        if (r >= n) {  // behind the cached keys: zeros
+                            piece[i] = make_uint4(0, 0, 0, 0);
+                            par[i] = 0;
+                        }
+                    }
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(bar(B_RAWEMPTY + rs));
+                    ri++;
+                    if (!(ok = __all_sync(D1_FULL_MASK, mbar_wait(bar(B_KVEMPTY + st), ((ki / T_STAGES) & 1) ^ 1, abort_flag))))
+                        break;
+#pragma unroll
+                    for (int i = 0; i < 4; i++) {
+                        const int r = (lt >> 1) + (i & 1) * 64;
+                        uint8_t* row = dK + (i >> 1) * T_KV_BYTES + r * 128;
+                        const uint32_t p2 = par[i] * 0x00010001u, step = kv4_step2(p2);
+                        uint32_t z0, z1;
+                        kv4_zero(p2, z0, z1);
+                        const uint32_t word[4] = {piece[i].x, piece[i].y, piece[i].z, piece[i].w};
+#pragma unroll
+                        for (int q = 0; q < 4; q++) {
+                            uint32_t x[4];
+                            kv4_expand(word[q], z0, z1, x);
+                            *reinterpret_cast<uint4*>(row + ((((lt & 1) * 4 + q) ^ (r & 7)) << 4)) =
+                                make_uint4(h2_mul(x[0], step), h2_mul(x[1], step), h2_mul(x[2], step), h2_mul(x[3], step));
+                        }
+                    }
+                    fence_async_smem_cta();
+                    mbar_arrive(bar(B_KVFULL + st));
+                    continue;
+                }
+                if (!(ok = __all_sync(D1_FULL_MASK, mbar_wait(bar(B_KVEMPTY + st), ((ki / T_STAGES) & 1) ^ 1, abort_flag))))
+                    break;
+                const int row0 = un.kv_start + (j - e_tiles) * TKV;
+                if (n >= TKV) {
+                    if (lt == 0) {
+                        mbar_arrive_expect_tx(bar(B_KVFULL + st), 2 * T_KV_BYTES);
+                        tma_load_2d(smem_u32(dK), &tmK, g * 64, row0, bar(B_KVFULL + st));
+                        tma_load_2d(smem_u32(dK + T_KV_BYTES), &tmV, g * 64, row0, bar(B_KVFULL + st));
+                    } else {
+                        mbar_arrive(bar(B_KVFULL + st));
+                    }
+                } else {
+                    for (int c = lt; c < TKV * 8; c += T_EXPANDERS) {
+                        const int r = c >> 3, ch = c & 7;
+                        uint4 kx = make_uint4(0, 0, 0, 0), vx = kx;
+                        if (r < n) {
+                            const size_t at = (size_t)(row0 + r) * a.ldkv + g * 64 + ch * 8;
+                            kx = __ldg(reinterpret_cast<const uint4*>(a.K + at));
+                            vx = __ldg(reinterpret_cast<const uint4*>(a.V + at));
+                        }
+                        uint8_t* to = dK + r * 128 + ((ch ^ (r & 7)) << 4);
+                        *reinterpret_cast<uint4*>(to) = kx;
+                        *reinterpret_cast<uint4*>(to + T_KV_BYTES) = vx;
+                    }
+                    fence_async_smem_cta();
+                    mbar_arrive(bar(B_KVFULL + st));
+                }
+            }
+        }
+        if (!ok && lane == 0) record_err(a.err, abort_flag, kErrWaitEmpty);
+        if (lt == 0)  // copies still in flight (only after an abort) land before the CTA exits
+            for (int i = ki > T_STAGES ? ki - T_STAGES : 0; i < ki; i++)
+                if (!mbar_wait_timed2(bar(B_KVFULL + i % T_STAGES), (i / T_STAGES) & 1)) break;
+        __syncwarp();
+    } else if (warp == 9 || warp == 14) {
+        // ------------------------------------------------------------------ MMA issuer of warpgroup w
+        const int w = warp == 9 ? 0 : 1;
         if (lane == 0) {
-            int cnt[2] = {0, 0}, units[2] = {0, 0};  // key tiles and units of each warpgroup so far
+            const uint32_t tS = tmem + w * T_WG_COLS, tP = tS + T_P_COL, tO = tS + T_O_COL;
+            int cnt = 0, units = 0;  // key tiles and units of the warpgroup so far
             int qi = 0, ki = 0;
             bool ok = true;
             for (int u = blockIdx.x; ok && u < n_units; u += gridDim.x) {
                 un.find(a, cum, run, u);
-                const int nt = un.tiles(), nw = un.q_tiles();
-                const bool packed = un.mode == kPacked;
+                const int nt = un.tiles(), mine = un.tiles_of(w);
                 if (nt == 0) continue;
+                const int step = un.mode == kPacked ? 2 : 1, first = un.mode == kPacked ? w : 0;  // its key tiles
                 const int qs = qi % T_QSLOTS;
                 if (!(ok = mbar_wait(bar(B_QFULL + qs), (qi / T_QSLOTS) & 1, abort_flag))) break;
-                tc_fence_after();
-                const uint32_t q_addr = smem_u32(sQ + qs * 2 * T_QT_BYTES);
-                auto k_addr = [&](int j) { return smem_u32(sKV + ((ki + j) % T_STAGES) * 2 * T_KV_BYTES); };
-                // S of key tile j, for the warpgroups that take it
-                auto issue_s = [&](int j) -> bool {
-                    if (!mbar_wait(bar(B_KVFULL + (ki + j) % T_STAGES), ((ki + j) / T_STAGES) & 1, abort_flag)) return false;
-                    for (int w = packed ? j & 1 : 0; w < (packed ? (j & 1) + 1 : nw); w++) {
-                        const int c = cnt[w] + (packed ? j >> 1 : j);
-                        if (c > 0 && !mbar_wait(bar(B_SFREE + w), (c - 1) & 1, abort_flag)) return false;
-                        tc_fence_after();
-                        const uint32_t ka = k_addr(j), qa = q_addr + (packed ? 0 : w * T_QT_BYTES);
-#pragma unroll
-                        for (int k = 0; k < 4; k++)
-                            tc_mma_f16(tmem + w * T_WG_COLS, smem_desc_k128(qa + k * 32), smem_desc_k128(ka + k * 32), IDESC_S,
-                                       k != 0);
-                        tc_commit(bar(B_SFULL + w));
-                    }
+                const uint64_t dq = smem_desc_k128(smem_u32(sQ + qs * 2 * T_QT_BYTES) + (un.mode == kPacked ? 0 : w * T_QT_BYTES));
+                auto kv_addr = [&](int j) { return smem_u32(sKV + ((ki + j) % T_STAGES) * 2 * T_KV_BYTES); };
+                auto kv_ready = [&](int j) {
+                    return mbar_wait(bar(B_KVFULL + (ki + j) % T_STAGES), ((ki + j) / T_STAGES) & 1, abort_flag);
+                };
+                auto pass = [&](int j) {  // a tile of the other warpgroup's
+                    if (!kv_ready(j)) return false;
+                    mbar_arrive(bar(B_KVEMPTY + (ki + j) % T_STAGES));
                     return true;
                 };
-                const int ahead = packed ? 2 : 1;  // S of the next tile of a warpgroup computes while it works on one
-                for (int j = 0, js = 0; j < nt && ok; j++) {
-                    for (; js < nt && js <= j + ahead && ok; js++) ok = issue_s(js);
-                    const uint32_t v_addr = k_addr(j) + T_KV_BYTES;
-                    for (int w = packed ? j & 1 : 0; w < (packed ? (j & 1) + 1 : nw) && ok; w++) {
-                        const int i = packed ? j >> 1 : j, c = cnt[w] + i;
-                        ok = mbar_wait(bar(B_PFULL + w), c & 1, abort_flag);
-                        // the first P V of a unit overwrites O: the unit before must have been read
-                        if (ok && i == 0 && units[w] > 0) ok = mbar_wait(bar(B_OFREE + w), (units[w] - 1) & 1, abort_flag);
-                        if (!ok) break;
-                        tc_fence_after();
+                // S of its i-th tile, once the softmax has read the one before
+                auto issue_s = [&](int i) {
+                    const int c = cnt + i;
+                    if (!kv_ready(first + i * step)) return false;
+                    if (c > 0 && !mbar_wait(bar(B_SFREE + w), (c - 1) & 1, abort_flag)) return false;
+                    tc_fence_after();
+                    const uint64_t dk = smem_desc_k128(kv_addr(first + i * step));
 #pragma unroll
-                        for (int k = 0; k < TKV / 16; k++)
-                            tc_mma_f16_ts(tmem + w * T_WG_COLS + T_O_COL, tmem + w * T_WG_COLS + T_P_COL + k * 8,
-                                          smem_desc_k128(v_addr + k * 2048), IDESC_O, (i | k) != 0);
-                        tc_commit(bar(B_ODONE + w));
-                    }
-                    if (!ok) break;
+                    for (int k = 0; k < 4; k++) tc_mma_f16(tS, dq + 2 * k, dk + 2 * k, IDESC_S, k != 0);
+                    tc_commit(bar(B_SFULL + w));
+                    return true;
+                };
+                for (int j = 0; j < (mine > 0 ? first : nt) && ok; j++) ok = pass(j);
+                if (ok && mine > 0) ok = issue_s(0);
+                for (int i = 0; i < mine && ok; i++) {
+                    const int j = first + i * step, c = cnt + i;
+                    if (step == 2 && j + 1 < nt && !(ok = pass(j + 1))) break;
+                    if (i + 1 < mine && !(ok = issue_s(i + 1))) break;  // computes while the softmax works on tile i
+                    if (!(ok = mbar_wait(bar(B_PFULL + w), c & 1, abort_flag))) break;
+                    // the first P V of a unit overwrites O: the unit before must have been read
+                    if (i == 0 && units > 0 && !(ok = mbar_wait(bar(B_OFREE + w), (units - 1) & 1, abort_flag))) break;
+                    tc_fence_after();
+                    const uint64_t dv = smem_desc_k128(kv_addr(j) + T_KV_BYTES);
+#pragma unroll
+                    for (int k = 0; k < TKV / 16; k++)
+                        tc_mma_f16_ts(tO, tP + k * 8, dv + k * (2048 >> 4), IDESC_O, (i | k) != 0);
+                    tc_commit(bar(B_ODONE + w));
                     tc_commit(bar(B_KVEMPTY + (ki + j) % T_STAGES));
                 }
                 if (!ok) break;
                 tc_commit(bar(B_QEMPTY + qs));
                 ki += nt;
                 qi++;
-                for (int w = 0; w < 2; w++) {
-                    cnt[w] += un.tiles_of(w);
-                    units[w] += un.tiles_of(w) > 0;
-                }
+                cnt += mine;
+                units += mine > 0;
             }
             if (!ok) record_err(a.err, abort_flag, kErrWaitFull);
-            tc_commit(bar(B_DRAIN));  // every issued MMA has completed before TMEM is released
-            if (!mbar_wait_timed2(bar(B_DRAIN), 0)) record_err(a.err, abort_flag, kErrDrain);
+            tc_commit(bar(B_DRAIN + w));  // every issued MMA has completed before TMEM is released
+            if (!mbar_wait_timed2(bar(B_DRAIN + w), 0)) record_err(a.err, abort_flag, kErrDrain);
         }
         __syncwarp();
+    }
     } else {
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(T_SOFTMAX_REGS));
         // ------------------------------------------------------------------ softmax
         const int w = warp >> 2, row = (warp & 3) * 32 + lane;
         const uint32_t lane_off = (uint32_t)((warp & 3) * 32) << 16;
         const uint32_t tS = tmem + w * T_WG_COLS + lane_off, tP = tS + T_P_COL, tO = tS + T_O_COL;
-        uint8_t* stile = sO + w * T_O_BYTES;
-        int cnt = 0, nst = 0, njoin = 0;  // key tiles so far; output tiles staged; packed units joined
+        int cnt = 0, njoin = 0;  // key tiles and packed units joined so far
         bool ok = true;
         for (int u = blockIdx.x; ok && u < n_units; u += gridDim.x) {
             un.find(a, cum, run, u);
@@ -1031,37 +1073,13 @@ __global__ void __launch_bounds__(T_THREADS, 1)
 #pragma unroll
             for (int i = 0; i < 32; i++) oh[i] = pack_h2(__uint_as_float(o[2 * i]) * il, __uint_as_float(o[2 * i + 1]) * il);
             if (a.lse && there) a.lse[(size_t)h * a.lse_ld + grow] = (m + log2f(l)) * kLn2;
-            if (!packed && rows >= TQ) {
-                // a whole tile: staged, then one bulk store; the store before must have read the buffer
-                if (nst > 0) {
-                    if (row == 0) {
-                        o_store_read_done();
-                        mbar_arrive(bar(B_OREAD + w));
-                    }
-                    if (!(ok = __all_sync(D1_FULL_MASK, mbar_wait(bar(B_OREAD + w), (nst - 1) & 1, abort_flag)))) break;
-                }
-#pragma unroll
-                for (int i = 0; i < 8; i++)
-                    *reinterpret_cast<uint4*>(stile + row * 128 + ((i ^ (row & 7)) << 4)) =
-                        make_uint4(oh[4 * i], oh[4 * i + 1], oh[4 * i + 2], oh[4 * i + 3]);
-                fence_async_smem_cta();
-                __syncwarp();
-                if (lane == 0) mbar_arrive(bar(B_OSTAGED + w));
-                bool staged = true;
-                if (row == 0) {
-                    staged = mbar_wait(bar(B_OSTAGED + w), nst & 1, abort_flag);
-                    if (staged) o_tile_store(&tmO, smem_u32(stile), h * 64, un.q_start + un.row0(w));
-                }
-                nst++;
-                if (!(ok = __all_sync(D1_FULL_MASK, staged))) break;
-            } else if (there) {
+            if (there) {
 #pragma unroll
                 for (int i = 0; i < 8; i++)
                     *reinterpret_cast<uint4*>(a.O + grow * a.ldo + h * 64 + i * 8) =
                         make_uint4(oh[4 * i], oh[4 * i + 1], oh[4 * i + 2], oh[4 * i + 3]);
             }
         }
-        if (row == 0) o_store_done();  // no store still reads this CTA's shared memory when it exits
         if (!ok && lane == 0) record_err(a.err, abort_flag, kErrWaitAccFull);
     }
     tc_fence_before();
@@ -1595,16 +1613,15 @@ int launch_tc(Kv4Args& a, int max_q, cudaStream_t st) {
     const int per = a.group % 2 == 0 ? TQ : 2 * TQ;
     const long long units = a.n_seqs * hu * (max_q > per ? (max_q - 1) / per + 1 : 1);
     const int kv_cols = a.heads / a.group * 64;
-    CUtensorMap tq, tk, tv, to;
-    if (!attn_tmap(&tq, a.Q, a.heads * 64, a.q_rows, a.ldq, TQ) || !attn_tmap(&to, a.O, a.heads * 64, a.q_rows, a.ldo, TQ))
-        return -1;
+    CUtensorMap tq, tk, tv;
+    if (!attn_tmap(&tq, a.Q, a.heads * 64, a.q_rows, a.ldq, TQ)) return -1;
     if (a.kv_rows > 0) {
         if (!attn_tmap(&tk, a.K, kv_cols, a.kv_rows, a.ldkv, TKV) || !attn_tmap(&tv, a.V, kv_cols, a.kv_rows, a.ldkv, TKV))
             return -1;
     } else {
         tk = tv = tq;  // no own rows: never read
     }
-    launch_pdl(k_kv4_attn_tc, (int)(units < sms ? units : sms), T_THREADS, T_SMEM, st, tq, tk, tv, to, a);
+    launch_pdl(k_kv4_attn_tc, (int)(units < sms ? units : sms), T_THREADS, T_SMEM, st, tq, tk, tv, a);
     return (int)cudaGetLastError();
 }
 
