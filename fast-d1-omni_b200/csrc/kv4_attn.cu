@@ -469,8 +469,8 @@ __global__ void __launch_bounds__(R_WARPS * 32, NT == 1 ? 4 : 2) k_kv4_attn_rows
 //   8          fetches the query rows (whole tiles by TMA, partial and packed ones row by row) and, by bulk copies into a
 //              ring of their own, the codes and parameters of the cached tiles
 //   10-13      expand them to fp16 (exact) into the swizzled layout that the MMAs read. Own rows: whole tiles by TMA,
-//              partial ones through registers. (The codes straight to the expanding warps' registers, a tile ahead: 3200
-//              clocks a tile with 4 such warps and nothing else running, all of it latency.)
+//              partial ones through registers. (A tile takes the four warps 1700 clocks, most of it latency; 3200 with the
+//              codes loaded straight into their registers, a tile ahead; 2200 with two warps to a tile, in turn.)
 //   9, 14      MMA issuers of warpgroups 0 and 1, one thread each: S = Q K^T (both in shared memory), O += P V (P in
 //              TMEM). Warp 9 also keeps the TMEM. (One issuer for both: each warpgroup then waits for the other's P.)
 // The softmax warps take 192 registers, the others 64.
@@ -594,6 +594,26 @@ struct Unit {
     __device__ int tile_of(int w, int i) const { return mode == kPacked ? 2 * i + w : i; }
 };
 
+// Whether the phase of `parity` has completed, at once; and after half a microsecond's wait at most.
+__device__ __forceinline__ bool mbar_test(uint32_t bar, uint32_t parity) {
+    uint32_t ok;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tmbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(ok)
+        : "r"(bar), "r"(parity)
+        : "memory");
+    return ok != 0;
+}
+__device__ __forceinline__ bool mbar_try_wait_brief(uint32_t bar, uint32_t parity) {
+    uint32_t ok;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, 500;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(ok)
+        : "r"(bar), "r"(parity)
+        : "memory");
+    return ok != 0;
+}
+
 // A run of bytes global -> shared (addresses and size multiples of 16), completing on the mbarrier.
 __device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
     asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst),
@@ -683,15 +703,24 @@ __global__ void __launch_bounds__(T_THREADS, 1)
                 const int rows = un.rows(a, w);
                 if (un.mode != kPacked && rows >= TQ) continue;
                 partial = true;
-                for (int c = lane; c < TQ * 8; c += 32) {
-                    const int r = c >> 3, ch = c & 7;
-                    const __half* src = a.Q;
-                    if (r < rows) {
-                        const int row = un.mode == kPacked ? r / a.group : un.row0(w) + r;
-                        const int h = un.mode == kPacked ? un.h + r % a.group : un.head(w);
-                        src += (size_t)(un.q_start + row) * a.ldq + h * 64 + ch * 8;
+                // rows lane / 8 and every fourth from there, 16 bytes a lane; of a packed unit, the row and head counted on
+                const int ch = lane & 7, group = un.mode == kPacked ? a.group : 1;
+                int row = un.mode == kPacked ? (lane >> 3) / group : un.row0(w) + (lane >> 3);
+                int h = un.mode == kPacked ? (lane >> 3) % group : 0;
+                const __half* src = a.Q + (size_t)un.q_start * a.ldq + un.head(w) * 64 + ch * 8;
+#pragma unroll 4
+                for (int r = lane >> 3; r < TQ; r += 4) {
+                    cp_async16z(dq + w * T_QT_BYTES + r * 128 + ((ch ^ (r & 7)) << 4),
+                                r < rows ? src + (size_t)row * a.ldq + h * 64 : a.Q, r < rows ? 16 : 0);
+                    if (un.mode == kPacked) {
+                        h += 4;
+                        while (h >= group) {
+                            h -= group;
+                            row++;
+                        }
+                    } else {
+                        row += 4;
                     }
-                    cp_async16z(dq + w * T_QT_BYTES + r * 128 + ((ch ^ (r & 7)) << 4), src, r < rows ? 16 : 0);
                 }
             }
             if (partial) {
@@ -849,11 +878,6 @@ __global__ void __launch_bounds__(T_THREADS, 1)
                 auto kv_ready = [&](int j) {
                     return mbar_wait(bar(B_KVFULL + (ki + j) % T_STAGES), ((ki + j) / T_STAGES) & 1, abort_flag);
                 };
-                auto pass = [&](int j) {  // a tile of the other warpgroup's
-                    if (!kv_ready(j)) return false;
-                    mbar_arrive(bar(B_KVEMPTY + (ki + j) % T_STAGES));
-                    return true;
-                };
                 // S of its i-th tile, once the softmax has read the one before
                 auto issue_s = [&](int i) {
                     const int c = cnt + i;
@@ -866,13 +890,26 @@ __global__ void __launch_bounds__(T_THREADS, 1)
                     tc_commit(bar(B_SFULL + w));
                     return true;
                 };
-                for (int j = 0; j < (mine > 0 ? first : nt) && ok; j++) ok = pass(j);
-                if (ok && mine > 0) ok = issue_s(0);
+                const bool both = un.mode != kPacked && un.q_tiles() == 2;  // the other issuer's MMAs read the tiles, too
+                if (mine > 0) ok = issue_s(0);
                 for (int i = 0; i < mine && ok; i++) {
                     const int j = first + i * step, c = cnt + i;
-                    if (step == 2 && j + 1 < nt && !(ok = pass(j + 1))) break;
-                    if (i + 1 < mine && !(ok = issue_s(i + 1))) break;  // computes while the softmax works on tile i
-                    if (!(ok = mbar_wait(bar(B_PFULL + w), c & 1, abort_flag))) break;
+                    // the next S computes while the softmax works on tile i; where its keys are late, P V goes first (it
+                    // frees a stage that they may be waiting for)
+                    bool s_next = i + 1 == mine;
+                    const uint64_t t0 = globaltimer_ns();
+                    while (true) {
+                        if (!s_next && mbar_test(bar(B_KVFULL + (ki + j + step) % T_STAGES), ((ki + j + step) / T_STAGES) & 1)) {
+                            if (!(ok = issue_s(i + 1))) break;
+                            s_next = true;
+                        }
+                        if (mbar_try_wait_brief(bar(B_PFULL + w), c & 1)) break;
+                        if (*abort_flag || globaltimer_ns() - t0 > kWaitLimitNs) {
+                            ok = false;
+                            break;
+                        }
+                    }
+                    if (!ok) break;
                     // the first P V of a unit overwrites O: the unit before must have been read
                     if (i == 0 && units > 0 && !(ok = mbar_wait(bar(B_OFREE + w), (units - 1) & 1, abort_flag))) break;
                     tc_fence_after();
@@ -882,6 +919,8 @@ __global__ void __launch_bounds__(T_THREADS, 1)
                         tc_mma_f16_ts(tO, tP + k * 8, dv + k * (2048 >> 4), IDESC_O, (i | k) != 0);
                     tc_commit(bar(B_ODONE + w));
                     tc_commit(bar(B_KVEMPTY + (ki + j) % T_STAGES));
+                    if (!both) tc_commit(bar(B_KVEMPTY + (ki + j) % T_STAGES));
+                    if (!s_next && !(ok = issue_s(i + 1))) break;
                 }
                 if (!ok) break;
                 tc_commit(bar(B_QEMPTY + qs));
