@@ -738,8 +738,9 @@ __global__ void __launch_bounds__(T_THREADS, 1)
                         tma_load_2d(dq + w * T_QT_BYTES, &tmQ, un.head(w) * 64, un.q_start + un.row0(w), bar(B_QFULL + qs));
             }
             qi++;
-            const D1Kv4Seq& s = a.seqs[un.sq];
-            const size_t at = (size_t)g * s.ext_cap;
+            const size_t at = (size_t)g * a.seqs[un.sq].ext_cap;
+            const uint8_t *k4 = a.seqs[un.sq].k4 + at * 32, *v4 = a.seqs[un.sq].v4 + at * 32;
+            const d1_half *kp = a.seqs[un.sq].kp + at, *vp = a.seqs[un.sq].vp + at;
             for (int j = 0; j < e_tiles; j++, ri++) {
                 const int rs = ri % T_RAW_STAGES;
                 if (!(ok = __all_sync(D1_FULL_MASK,
@@ -750,12 +751,12 @@ __global__ void __launch_bounds__(T_THREADS, 1)
                     const int n = min(un.valid(j), TKV);
                     const uint32_t codes = n * 32, pars = ((n + 7) & ~7) * 2;
                     const uint32_t dst = smem_u32(sRaw + rs * T_RAW_BYTES), full = bar(B_RAWFULL + rs);
-                    const size_t key = at + (size_t)j * TKV;
+                    const size_t key = (size_t)j * TKV;
                     mbar_arrive_expect_tx(full, 2 * (codes + pars));
-                    bulk_load(dst, s.k4 + key * 32, codes, full);
-                    bulk_load(dst + T_RAW_V, s.v4 + key * 32, codes, full);
-                    bulk_load(dst + T_RAW_KP, s.kp + key, pars, full);
-                    bulk_load(dst + T_RAW_VP, s.vp + key, pars, full);
+                    bulk_load(dst, k4 + key * 32, codes, full);
+                    bulk_load(dst + T_RAW_V, v4 + key * 32, codes, full);
+                    bulk_load(dst + T_RAW_KP, kp + key, pars, full);
+                    bulk_load(dst + T_RAW_VP, vp + key, pars, full);
                 }
                 __syncwarp();
             }
@@ -836,18 +837,15 @@ __global__ void __launch_bounds__(T_THREADS, 1)
                         mbar_arrive(bar(B_KVFULL + st));
                     }
                 } else {
-                    for (int c = lt; c < TKV * 8; c += T_EXPANDERS) {
-                        const int r = c >> 3, ch = c & 7;
-                        uint4 kx = make_uint4(0, 0, 0, 0), vx = kx;
-                        if (r < n) {
-                            const size_t at = (size_t)(row0 + r) * a.ldkv + g * 64 + ch * 8;
-                            kx = __ldg(reinterpret_cast<const uint4*>(a.K + at));
-                            vx = __ldg(reinterpret_cast<const uint4*>(a.V + at));
-                        }
-                        uint8_t* to = dK + r * 128 + ((ch ^ (r & 7)) << 4);
-                        *reinterpret_cast<uint4*>(to) = kx;
-                        *reinterpret_cast<uint4*>(to + T_KV_BYTES) = vx;
+                    const int ch = lt & 7;
+                    const size_t at = (size_t)row0 * a.ldkv + g * 64 + ch * 8;
+                    for (int r = lt >> 3; r < TKV; r += T_EXPANDERS / 8) {  // zeros behind the end
+                        const uint32_t to = smem_u32(dK) + r * 128 + ((ch ^ (r & 7)) << 4);
+                        const size_t off = r < n ? at + (size_t)r * a.ldkv : 0;
+                        cp_async16z(to, a.K + off, r < n ? 16 : 0);
+                        cp_async16z(to + T_KV_BYTES, a.V + off, r < n ? 16 : 0);
                     }
+                    asm volatile("cp.async.wait_all;" ::: "memory");
                     fence_async_smem_cta();
                     mbar_arrive(bar(B_KVFULL + st));
                 }
