@@ -466,10 +466,10 @@ __global__ void __launch_bounds__(R_WARPS * 32, NT == 1 ? 4 : 2) k_kv4_attn_rows
 //   0-3, 4-7   softmax: thread = query row = TMEM lane. S is copied to registers and released at once, P goes to TMEM as
 //              fp16, O is rescaled only when a row's maximum grows by more than 2^8. Warps whose rows are all behind the
 //              sequence's end leave the work out.
-//   8          fetches the query rows (whole tiles by TMA, partial and packed ones row by row) and, by bulk copies into a
-//              ring of their own, the codes and parameters of the cached tiles
-//   10-13      expand them to fp16 (exact) into the swizzled layout that the MMAs read. Own rows: whole tiles by TMA,
-//              partial ones through registers. (A tile takes the four warps 1700 clocks, most of it latency; 3200 with the
+//   8          fetches the query rows by TMA (packed ones from a view of [row][head][64]) and, by bulk copies into a ring
+//              of their own, the codes and parameters of the cached tiles, from one thread
+//   10-13      expand them to fp16 (exact) into the swizzled layout that the MMAs read. Own rows come by
+//              TMA. (A tile takes the four warps 1700 clocks, most of it latency; 3200 with the
 //              codes loaded straight into their registers, a tile ahead; 2200 with two warps to a tile, in turn.)
 //   9, 14      MMA issuers of warpgroups 0 and 1, one thread each: S = Q K^T (both in shared memory), O += P V (P in
 //              TMEM). Warp 9 also keeps the TMEM. (One issuer for both: each warpgroup then waits for the other's P.)
@@ -495,13 +495,14 @@ enum : int {
     B_OFREE = B_ODONE + 2,           // [w]: O has been read (4 warps; of a packed unit those of warpgroup 0)
     B_RAWFULL = B_OFREE + 2,         // [raw stage]: a tile's codes and parameters are in shared memory
     B_RAWEMPTY = B_RAWFULL + T_RAW_STAGES,  // [raw stage] (4 warps)
-    B_JOIN = B_RAWEMPTY + T_RAW_STAGES,  // a packed unit's maxima and sums of warpgroup 1 are in shared memory (4 warps)
+    B_OWN = B_RAWEMPTY + T_RAW_STAGES,  // a partial tile of own rows has landed
+    B_JOIN = B_OWN + 1,              // a packed unit's maxima and sums of warpgroup 1 are in shared memory (4 warps)
     B_JOINED = B_JOIN + 1,           // and have been read (4 warps)
     B_DRAIN = B_JOINED + 1,          // [issuer]
     T_NBARS = B_DRAIN + 2
 };
 constexpr int T_SMEM = T_QSLOTS * 2 * T_QT_BYTES + T_STAGES * 2 * T_KV_BYTES + T_RAW_STAGES * T_RAW_BYTES + T_NBARS * 8 + 16 + TQ * 8 +
-                       (T_ENTRIES + 1) * 4;
+                       (T_ENTRIES * 6 + 1) * 4;
 static_assert(T_SMEM <= 232448 && T_O_COL + 64 <= T_WG_COLS, "shared memory and TMEM of the tcgen05 attention");
 
 enum : int { kPacked, kPair, kSingle };
@@ -521,12 +522,22 @@ __device__ __forceinline__ int seq_units(const Kv4Args& a, int sq, bool report) 
     return mode == kPacked ? a.heads / a.group
                            : mode == kPair ? ((s.q_len - 1) / TQ + 1) * (a.heads / 2) : ((s.q_len - 1) / (2 * TQ) + 1) * a.heads;
 }
-// The table of units: cum[e] = units of the sequences before the e-th run of `run` sequences. Ends with a barrier.
+// The table of units: cum[e] = units of the sequences before the e-th run of `run` sequences, and behind it, for runs of
+// one, what a unit needs of its sequence, five words each. Ends with a barrier.
 __device__ __forceinline__ void build_units(const Kv4Args& a, int* cum, int run) {
     for (int e = threadIdx.x; e < T_ENTRIES; e += blockDim.x) {
         int n = 0;
         for (int i = e * run; i < min(a.n_seqs, (e + 1) * run); i++) n += seq_units(a, i, true);
         cum[e + 1] = n;
+        if (run == 1 && e < a.n_seqs) {
+            const D1Kv4Seq& s = a.seqs[e];
+            int* info = cum + T_ENTRIES + 1 + e;
+            info[0] = s.q_start;
+            info[T_ENTRIES] = s.q_len;
+            info[2 * T_ENTRIES] = s.kv_start;
+            info[3 * T_ENTRIES] = s.kv_len;
+            info[4 * T_ENTRIES] = s.ext_len;
+        }
     }
     if (threadIdx.x == 0) cum[0] = 0;
     __syncthreads();
@@ -564,12 +575,21 @@ struct Unit {
         sq = lo * run;
         if (run > 1)
             for (int n; rest >= (n = seq_units(a, sq, false)); sq++) rest -= n;
-        const D1Kv4Seq& s = a.seqs[sq];
-        q_start = s.q_start;
-        q_len = s.q_len;
-        kv_start = s.kv_start;
-        kv_len = s.kv_len;
-        ext_len = s.ext_len;
+        if (run == 1) {
+            const int* info = cum + T_ENTRIES + 1 + sq;
+            q_start = info[0];
+            q_len = info[T_ENTRIES];
+            kv_start = info[2 * T_ENTRIES];
+            kv_len = info[3 * T_ENTRIES];
+            ext_len = info[4 * T_ENTRIES];
+        } else {
+            const D1Kv4Seq& s = a.seqs[sq];
+            q_start = s.q_start;
+            q_len = s.q_len;
+            kv_start = s.kv_start;
+            kv_len = s.kv_len;
+            ext_len = s.ext_len;
+        }
         mode = unit_mode(a, q_len);
         const int hu = mode == kPacked ? a.heads / a.group : mode == kPair ? a.heads / 2 : a.heads;
         block = rest / hu;
@@ -614,6 +634,14 @@ __device__ __forceinline__ bool mbar_try_wait_brief(uint32_t bar, uint32_t parit
     return ok != 0;
 }
 
+__device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap* map, int x, int y, int z, uint32_t bar) {
+    asm volatile(
+        "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(
+            dst),
+        "l"((uint64_t)map), "r"(x), "r"(y), "r"(z), "r"(bar)
+        : "memory");
+}
+
 // A run of bytes global -> shared (addresses and size multiples of 16), completing on the mbarrier.
 __device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
     asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst),
@@ -622,8 +650,8 @@ __device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_
 }
 
 __global__ void __launch_bounds__(T_THREADS, 1)
-    k_kv4_attn_tc(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
-                  const __grid_constant__ CUtensorMap tmV, const Kv4Args a) {
+    k_kv4_attn_tc(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmQp,
+                  const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV, const Kv4Args a) {
     constexpr uint32_t IDESC_S = idesc_f16_f32(TQ, TKV);
     constexpr uint32_t IDESC_O = idesc_f16_f32(TQ, 64) | (1u << 16);  // B (= V) MN-major
     extern __shared__ __align__(1024) uint8_t t_smem[];
@@ -663,6 +691,7 @@ __global__ void __launch_bounds__(T_THREADS, 1)
             mbar_init(bar(B_RAWFULL + i), 1);
             mbar_init(bar(B_RAWEMPTY + i), T_EXPANDERS / 32);
         }
+        mbar_init(bar(B_OWN), 1);
         mbar_init(bar(B_JOIN), 4);
         mbar_init(bar(B_JOINED), 4);
         *abort_flag = 0;
@@ -685,85 +714,49 @@ __global__ void __launch_bounds__(T_THREADS, 1)
     if (warp >= 8) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(T_OTHER_REGS));
         if (warp == 8) {
-        // ------------------------------------------------------------------ fetching
-        int qi = 0, ri = 0;
-        bool ok = true;
-        for (int u = blockIdx.x; ok && u < n_units; u += gridDim.x) {
-            un.find(a, cum, run, u);
-            const int g = un.h / a.group, e_tiles = un.ext_tiles();
-            if (un.tiles() == 0) continue;
-            const int qs = qi % T_QSLOTS;
-            if (!(ok = __all_sync(D1_FULL_MASK, mbar_wait(bar(B_QEMPTY + qs), ((qi / T_QSLOTS) & 1) ^ 1, abort_flag)))) break;
-            // a whole tile inside the sequence comes by TMA; one that the sequence ends in row by row, with zeros behind
-            // the end, so that no load reads a row outside a sequence
-            const uint32_t dq = smem_u32(sQ + qs * 2 * T_QT_BYTES);
-            const int nq = un.q_tiles();
-            bool partial = false;
-            for (int w = 0; w < nq; w++) {
-                const int rows = un.rows(a, w);
-                if (un.mode != kPacked && rows >= TQ) continue;
-                partial = true;
-                // rows lane / 8 and every fourth from there, 16 bytes a lane; of a packed unit, the row and head counted on
-                const int ch = lane & 7, group = un.mode == kPacked ? a.group : 1;
-                int row = un.mode == kPacked ? (lane >> 3) / group : un.row0(w) + (lane >> 3);
-                int h = un.mode == kPacked ? (lane >> 3) % group : 0;
-                const __half* src = a.Q + (size_t)un.q_start * a.ldq + un.head(w) * 64 + ch * 8;
-#pragma unroll 4
-                for (int r = lane >> 3; r < TQ; r += 4) {
-                    cp_async16z(dq + w * T_QT_BYTES + r * 128 + ((ch ^ (r & 7)) << 4),
-                                r < rows ? src + (size_t)row * a.ldq + h * 64 : a.Q, r < rows ? 16 : 0);
-                    if (un.mode == kPacked) {
-                        h += 4;
-                        while (h >= group) {
-                            h -= group;
-                            row++;
-                        }
-                    } else {
-                        row += 4;
-                    }
+        // ------------------------------------------------------------------ fetching (one thread)
+        if (lane == 0) {
+            int qi = 0, ri = 0;
+            bool ok = true;
+            for (int u = blockIdx.x; ok && u < n_units; u += gridDim.x) {
+                un.find(a, cum, run, u);
+                const int g = un.h / a.group, e_tiles = un.ext_tiles();
+                if (un.tiles() == 0) continue;
+                const int qs = qi % T_QSLOTS;
+                if (!(ok = mbar_wait(bar(B_QEMPTY + qs), ((qi / T_QSLOTS) & 1) ^ 1, abort_flag))) break;
+                // whole tiles always: rows behind the sequence's end are other sequences', or zeros behind the buffer's;
+                // the lanes that they fall to are not used
+                const uint32_t dq = smem_u32(sQ + qs * 2 * T_QT_BYTES), full = bar(B_QFULL + qs);
+                const int row = un.q_start + (un.mode == kPacked ? 0 : un.row0(0));
+                if (un.mode == kPacked) {
+                    mbar_arrive_expect_tx(full, TQ / a.group * a.group * 128);
+                    tma_load_3d(dq, &tmQp, 0, un.h, row, full);
+                } else {
+                    const int nq = un.q_tiles();
+                    mbar_arrive_expect_tx(full, nq * T_QT_BYTES);
+                    tma_load_2d(dq, &tmQ, un.head(0) * 64, row, full);
+                    if (nq == 2) tma_load_2d(dq + T_QT_BYTES, &tmQ, un.head(1) * 64, un.q_start + un.row0(1), full);
                 }
-            }
-            if (partial) {
-                asm volatile("cp.async.wait_all;" ::: "memory");
-                fence_async_smem_cta();
-                __syncwarp();
-            }
-            if (lane == 0) {
-                uint32_t bytes = 0;
-                for (int w = 0; w < nq; w++)
-                    if (un.mode != kPacked && un.rows(a, w) >= TQ) bytes += T_QT_BYTES;
-                mbar_arrive_expect_tx(bar(B_QFULL + qs), bytes);
-                for (int w = 0; w < nq; w++)
-                    if (un.mode != kPacked && un.rows(a, w) >= TQ)
-                        tma_load_2d(dq + w * T_QT_BYTES, &tmQ, un.head(w) * 64, un.q_start + un.row0(w), bar(B_QFULL + qs));
-            }
-            qi++;
-            const size_t at = (size_t)g * a.seqs[un.sq].ext_cap;
-            const uint8_t *k4 = a.seqs[un.sq].k4 + at * 32, *v4 = a.seqs[un.sq].v4 + at * 32;
-            const d1_half *kp = a.seqs[un.sq].kp + at, *vp = a.seqs[un.sq].vp + at;
-            for (int j = 0; j < e_tiles; j++, ri++) {
-                const int rs = ri % T_RAW_STAGES;
-                if (!(ok = __all_sync(D1_FULL_MASK,
-                                      mbar_wait(bar(B_RAWEMPTY + rs), ((ri / T_RAW_STAGES) & 1) ^ 1, abort_flag))))
-                    break;
-                if (lane == 0) {
+                qi++;
+                const size_t at = (size_t)g * a.seqs[un.sq].ext_cap;
+                const uint8_t *k4 = a.seqs[un.sq].k4 + at * 32, *v4 = a.seqs[un.sq].v4 + at * 32;
+                const d1_half *kp = a.seqs[un.sq].kp + at, *vp = a.seqs[un.sq].vp + at;
+                for (int j = 0; j < e_tiles; j++, ri++) {
+                    const int rs = ri % T_RAW_STAGES;
+                    if (!(ok = mbar_wait(bar(B_RAWEMPTY + rs), ((ri / T_RAW_STAGES) & 1) ^ 1, abort_flag))) break;
                     // whole 16-byte runs: up to 8 parameters, which the arrays hold (ext_cap is a multiple of 8)
                     const int n = min(un.valid(j), TKV);
                     const uint32_t codes = n * 32, pars = ((n + 7) & ~7) * 2;
-                    const uint32_t dst = smem_u32(sRaw + rs * T_RAW_BYTES), full = bar(B_RAWFULL + rs);
+                    const uint32_t dst = smem_u32(sRaw + rs * T_RAW_BYTES), landed = bar(B_RAWFULL + rs);
                     const size_t key = (size_t)j * TKV;
-                    mbar_arrive_expect_tx(full, 2 * (codes + pars));
-                    bulk_load(dst, k4 + key * 32, codes, full);
-                    bulk_load(dst + T_RAW_V, v4 + key * 32, codes, full);
-                    bulk_load(dst + T_RAW_KP, kp + key, pars, full);
-                    bulk_load(dst + T_RAW_VP, vp + key, pars, full);
+                    mbar_arrive_expect_tx(landed, 2 * (codes + pars));
+                    bulk_load(dst, k4 + key * 32, codes, landed);
+                    bulk_load(dst + T_RAW_V, v4 + key * 32, codes, landed);
+                    bulk_load(dst + T_RAW_KP, kp + key, pars, landed);
+                    bulk_load(dst + T_RAW_VP, vp + key, pars, landed);
                 }
-                __syncwarp();
             }
-        }
-        asm volatile("cp.async.wait_all;" ::: "memory");  // nothing in flight when the CTA exits
-        if (!ok && lane == 0) record_err(a.err, abort_flag, kErrWaitEmpty);
-        if (lane == 0) {
+            if (!ok) record_err(a.err, abort_flag, kErrWaitEmpty);
             // copies still in flight (only after an abort) land before the CTA exits
             for (int i = ri > T_RAW_STAGES ? ri - T_RAW_STAGES : 0; i < ri; i++)
                 if (!mbar_wait_timed2(bar(B_RAWFULL + i % T_RAW_STAGES), (i / T_RAW_STAGES) & 1)) break;
@@ -774,7 +767,7 @@ __global__ void __launch_bounds__(T_THREADS, 1)
     } else if (warp >= 10 && warp < 14) {
         // ------------------------------------------------------------------ expanding
         const int lt = (warp - 10) * 32 + lane;
-        int ri = 0, ki = 0;
+        int ri = 0, ki = 0, oi = 0;  // cached tiles, tiles, and partial tiles of own rows so far
         bool ok = true;
         for (int u = blockIdx.x; ok && u < n_units; u += gridDim.x) {
             un.find(a, cum, run, u);
@@ -827,32 +820,30 @@ __global__ void __launch_bounds__(T_THREADS, 1)
                 }
                 if (!(ok = __all_sync(D1_FULL_MASK, mbar_wait(bar(B_KVEMPTY + st), ((ki / T_STAGES) & 1) ^ 1, abort_flag))))
                     break;
+                // own rows: a whole tile by TMA. Rows behind the sequence's end are others', or zeros behind the buffer's:
+                // their scores are masked, and their values, which P = 0 multiplies, are overwritten with zeros
                 const int row0 = un.kv_start + (j - e_tiles) * TKV;
-                if (n >= TKV) {
-                    if (lt == 0) {
-                        mbar_arrive_expect_tx(bar(B_KVFULL + st), 2 * T_KV_BYTES);
-                        tma_load_2d(smem_u32(dK), &tmK, g * 64, row0, bar(B_KVFULL + st));
-                        tma_load_2d(smem_u32(dK + T_KV_BYTES), &tmV, g * 64, row0, bar(B_KVFULL + st));
-                    } else {
-                        mbar_arrive(bar(B_KVFULL + st));
-                    }
-                } else {
-                    const int ch = lt & 7;
-                    const size_t at = (size_t)row0 * a.ldkv + g * 64 + ch * 8;
-                    for (int r = lt >> 3; r < TKV; r += T_EXPANDERS / 8) {  // zeros behind the end
-                        const uint32_t to = smem_u32(dK) + r * 128 + ((ch ^ (r & 7)) << 4);
-                        const size_t off = r < n ? at + (size_t)r * a.ldkv : 0;
-                        cp_async16z(to, a.K + off, r < n ? 16 : 0);
-                        cp_async16z(to + T_KV_BYTES, a.V + off, r < n ? 16 : 0);
-                    }
-                    asm volatile("cp.async.wait_all;" ::: "memory");
-                    fence_async_smem_cta();
-                    mbar_arrive(bar(B_KVFULL + st));
+                const uint32_t landed = bar(n >= TKV ? B_KVFULL + st : B_OWN);
+                if (lt == 0) {
+                    mbar_arrive_expect_tx(landed, 2 * T_KV_BYTES);
+                    tma_load_2d(smem_u32(dK), &tmK, g * 64, row0, landed);
+                    tma_load_2d(smem_u32(dK + T_KV_BYTES), &tmV, g * 64, row0, landed);
                 }
+                if (n >= TKV) {
+                    if (lt != 0) mbar_arrive(landed);
+                    continue;
+                }
+                if (!(ok = __all_sync(D1_FULL_MASK, mbar_wait(landed, oi & 1, abort_flag)))) break;
+                oi++;
+                for (int c = n * 8 + lt; c < TKV * 8; c += T_EXPANDERS)
+                    *reinterpret_cast<uint4*>(dK + T_KV_BYTES + c * 16) = make_uint4(0, 0, 0, 0);
+                fence_async_smem_cta();
+                mbar_arrive(bar(B_KVFULL + st));
             }
         }
         if (!ok && lane == 0) record_err(a.err, abort_flag, kErrWaitEmpty);
-        if (lt == 0)  // copies still in flight (only after an abort) land before the CTA exits
+        if (lt == 0 && !ok) mbar_wait_timed2(bar(B_OWN), oi & 1);  // copies still in flight land before the CTA exits
+        if (lt == 0)
             for (int i = ki > T_STAGES ? ki - T_STAGES : 0; i < ki; i++)
                 if (!mbar_wait_timed2(bar(B_KVFULL + i % T_STAGES), (i / T_STAGES) & 1)) break;
         __syncwarp();
@@ -1083,15 +1074,13 @@ __global__ void __launch_bounds__(T_THREADS, 1)
                 const float m1 = join[2 * row], l1 = join[2 * row + 1];
                 if (un.tiles_of(1) > 0) {
                     const float both = fmaxf(m, m1), f0 = ex2(m - both), f1 = ex2(m1 - both);
+                    uint32_t o1[64];
+                    tmem_ld32(tO + T_WG_COLS, *reinterpret_cast<uint32_t(*)[32]>(o1));
+                    tmem_ld32(tO + T_WG_COLS + 32, *reinterpret_cast<uint32_t(*)[32]>(o1 + 32));
+                    tc_wait_ld();
 #pragma unroll
-                    for (int i = 0; i < 8; i++) {
-                        uint32_t o1[8];
-                        tmem_ld8(tO + T_WG_COLS + i * 8, o1);
-                        tc_wait_ld();
-#pragma unroll
-                        for (int k = 0; k < 8; k++)
-                            o[i * 8 + k] = __float_as_uint(__uint_as_float(o[i * 8 + k]) * f0 + __uint_as_float(o1[k]) * f1);
-                    }
+                    for (int i = 0; i < 64; i++)
+                        o[i] = __float_as_uint(__uint_as_float(o[i]) * f0 + __uint_as_float(o1[i]) * f1);
                     l = l * f0 + l1 * f1;
                     m = both;
                 }
@@ -1252,8 +1241,8 @@ __global__ void __launch_bounds__(256) k_kv4_mass_rows(const Kv4Args a) {
 //              the FMA pipe. At the unit's end three pass their sums to the first through shared memory. (Two documents of
 //              2048 rows over 8192 keys: 91 us; 98 with two warpgroups and the next piece's load on its way, 97 with
 //              both pieces loaded at once, 93 without the FMA pipe, 94 and 99 with a quarter and three eighths there)
-//   16, 18, 19 loaders: the keys' codes, expanded; query tiles by TMA where a block is whole, otherwise row by row with
-//              zeros behind the end; the columns' -lse (behind the end and for rows without keys: -inf, which adds 0)
+//   16, 18, 19 loaders: the keys' codes, expanded; query tiles by TMA from a view of [row][head][64], always whole; the
+//              columns' -lse (behind the end and for rows without keys: -inf, which adds 0 whatever the score)
 //   17         TMEM, and the MMAs from one thread
 constexpr int MQ = 256, MK = 128, M_STAGES = 4, M_LOADERS = 3, M_WGS = 4, M_THREADS = 128 * M_WGS + 128;
 constexpr int M_Q_BYTES = MQ * 128, M_K_BYTES = MK * 128;
@@ -1345,7 +1334,7 @@ struct MassWalk {
     __device__ int rows() const { return min(block, q_len - row0); }
 };
 
-__global__ void __launch_bounds__(M_THREADS, 1) k_kv4_mass_tc(const __grid_constant__ CUtensorMap tmQ, const Kv4Args a) {
+__global__ void __launch_bounds__(M_THREADS, 1) k_kv4_mass_tc(const __grid_constant__ CUtensorMap tmQp, const Kv4Args a) {
     extern __shared__ __align__(1024) uint8_t m_smem[];
     uint8_t* sK = m_smem;                                                          // [2][128 keys]
     uint8_t* sQ = sK + 2 * M_K_BYTES;                                              // [stage][256 columns]
@@ -1398,6 +1387,7 @@ __global__ void __launch_bounds__(M_THREADS, 1) k_kv4_mass_tc(const __grid_const
     if (warp == M_WARP - 1 || warp > M_WARP) {
         // ------------------------------------------------------------------ loaders
         const int lw = warp < M_WARP ? 0 : warp - M_WARP, lt = lw * 32 + lane;
+        const int inv = (65536 + a.group - 1) / a.group;  // c / group = c * inv >> 16 for c < 256: off by less than 1 / group
         for (; ok && wk.next_unit(a); nu++) {
             const uint8_t* k4 = wk.s.k4 + (size_t)wk.g * wk.s.ext_cap * 32;
             const uint16_t* kp = reinterpret_cast<const uint16_t*>(wk.s.kp) + (size_t)wk.g * wk.s.ext_cap;
@@ -1436,42 +1426,27 @@ __global__ void __launch_bounds__(M_THREADS, 1) k_kv4_mass_tc(const __grid_const
             mbar_arrive(bar(MB_KFULL + (nu & 1)));
             for (; wk.next_tile(a); ti++) {
                 if (ti % M_LOADERS != lw) continue;  // the warps take the tiles in turn: their latencies overlap
-                const int st = ti % M_STAGES, n = wk.rows(), cols = n * a.group, pad = (cols + 31) & ~31;
-                const int inv = (65536 + n - 1) / n;  // c / n = c * inv >> 16 for c < 256: off by less than 1 / n
+                const int st = ti % M_STAGES, cols = wk.rows() * a.group, pad = (cols + 31) & ~31;
                 const int row = wk.q_start + wk.row0, h0 = wk.g * a.group;
                 float l[MQ / 32];
 #pragma unroll
                 for (int i = 0; i < MQ / 32; i++) {
-                    const int c = lane + 32 * i, hh = c * inv >> 16;
+                    const int c = lane + 32 * i, r = c * inv >> 16;
                     l[i] = -INFINITY;
-                    if (c < cols) l[i] = __ldg(a.lse + (size_t)(h0 + hh) * a.lse_ld + row + (c - hh * n));
+                    if (c < cols) l[i] = __ldg(a.lse + (size_t)(h0 + c - r * a.group) * a.lse_ld + row + r);
                 }
                 if (!(ok = wait(MB_QEMPTY + st, ((ti / M_STAGES) & 1) ^ 1))) break;
-                const uint32_t dQ = smem_u32(sQ + st * M_Q_BYTES);
-                const bool whole = cols == MQ && n % 8 == 0;  // heads at whole swizzle atoms
-                if (!whole) {
-                    for (int i = lane; i < pad * 8; i += 32) {
-                        const int c = i >> 3, ch = i & 7, hh = c * inv >> 16;
-                        const __half* src =
-                            c < cols ? a.Q + (size_t)(row + (c - hh * n)) * a.ldq + (h0 + hh) * 64 + ch * 8 : a.Q;
-                        cp_async16z(dQ + c * 128 + ((ch ^ (c & 7)) << 4), src, c < cols ? 16 : 0);
-                    }
-                } else if (lane == 0) {
-                    mbar_arrive_expect_tx(bar(MB_QFULL + st), M_Q_BYTES);
-                    for (int hh = 0; hh < a.group; hh++)
-                        tma_load_2d(dQ + hh * n * 128, &tmQ, (h0 + hh) * 64, row, bar(MB_QFULL + st));
-                }
 #pragma unroll
                 for (int i = 0; i < MQ / 32; i++)
                     if (32 * i < pad) sL[st * MQ + lane + 32 * i] = l[i] == -INFINITY ? -INFINITY : -l[i] * kLog2e;
-                if (!whole) {
-                    asm volatile("cp.async.wait_all;" ::: "memory");
-                    fence_async_smem_cta();
+                if (lane == 0) {
+                    mbar_arrive_expect_tx(bar(MB_QFULL + st), wk.block * a.group * 128);
+                    tma_load_3d(smem_u32(sQ + st * M_Q_BYTES), &tmQp, 0, h0, row, bar(MB_QFULL + st));
+                } else {
+                    mbar_arrive(bar(MB_QFULL + st));
                 }
-                if (!whole || lane > 0) mbar_arrive(bar(MB_QFULL + st));
             }
         }
-        asm volatile("cp.async.wait_all;" ::: "memory");  // nothing in flight when the CTA exits
         if (!ok && lane == 0) record_err(a.err, abort_flag, kErrWaitEmpty);
         if (lane == 0)  // TMA copies still in flight (only after an abort) land before the CTA exits
             for (int i = ti > M_STAGES ? ti - M_STAGES : 0; i < ti; i++)
@@ -1522,11 +1497,17 @@ __global__ void __launch_bounds__(M_THREADS, 1) k_kv4_mass_tc(const __grid_const
                 if (!(ok = wait(MB_QFULL + st, (ti / M_STAGES) & 1))) break;  // the lse
                 if (!(ok = wait(MB_SFULL + b, (ti >> 1) & 1))) break;
                 tc_fence_after();
+                const int cols = wk.rows() * a.group;
                 for (int c0 = 32 * wg; c0 < pad; c0 += 32 * M_WGS) {
                     const float4* l4 = reinterpret_cast<const float4*>(sL + st * MQ + c0);
                     uint32_t y[32];
                     tmem_ld32(tS + b * MQ + (c0 - 32 * wg), y);
                     tc_wait_ld();
+                    if (c0 + 32 > cols) {  // columns of other sequences' rows, or of none: whatever they hold, a score of 0
+#pragma unroll
+                        for (int i = 0; i < 32; i++)
+                            if (c0 + i >= cols) y[i] = 0;
+                    }
 #pragma unroll
                     for (int i = 0; i < 8; i++) {
                         const float4 l = l4[i];
@@ -1640,6 +1621,20 @@ int launch_rows(Kv4Args& a, int max_q, int max_keys, int kv_heads, cudaStream_t 
     return (int)cudaGetLastError();
 }
 
+// Q as [row][head][64], in boxes of the group's heads of `most` / group rows: the packed rows of a tile in their order, in
+// the 128-byte swizzle; rows behind the buffer read as zeros.
+bool packed_tmap(CUtensorMap* m, const Kv4Args& a, int most) {
+    EncodeTiledFn enc = encode_fn();
+    if (!enc) return false;
+    cuuint64_t dims[3] = {64, (cuuint64_t)a.heads, (cuuint64_t)a.q_rows};
+    cuuint64_t strides[2] = {128, (cuuint64_t)a.ldq * 2};
+    cuuint32_t box[3] = {64, (cuuint32_t)a.group, (cuuint32_t)(most / a.group)};
+    cuuint32_t estr[3] = {1, 1, 1};
+    return enc(m, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3, const_cast<__half*>(a.Q), dims, strides, box, estr,
+               CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+               CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
 int launch_tc(Kv4Args& a, int max_q, cudaStream_t st) {
     static unsigned long long done = 0;
     if (!smem_opt_in(k_kv4_attn_tc, T_SMEM, &done)) return -1;
@@ -1650,15 +1645,19 @@ int launch_tc(Kv4Args& a, int max_q, cudaStream_t st) {
     const int per = a.group % 2 == 0 ? TQ : 2 * TQ;
     const long long units = a.n_seqs * hu * (max_q > per ? (max_q - 1) / per + 1 : 1);
     const int kv_cols = a.heads / a.group * 64;
-    CUtensorMap tq, tk, tv;
+    CUtensorMap tq, tqp, tk, tv;
     if (!attn_tmap(&tq, a.Q, a.heads * 64, a.q_rows, a.ldq, TQ)) return -1;
+    if (a.group > TQ)
+        tqp = tq;  // no packed units: never read
+    else if (!packed_tmap(&tqp, a, TQ))
+        return -1;
     if (a.kv_rows > 0) {
         if (!attn_tmap(&tk, a.K, kv_cols, a.kv_rows, a.ldkv, TKV) || !attn_tmap(&tv, a.V, kv_cols, a.kv_rows, a.ldkv, TKV))
             return -1;
     } else {
         tk = tv = tq;  // no own rows: never read
     }
-    launch_pdl(k_kv4_attn_tc, (int)(units < sms ? units : sms), T_THREADS, T_SMEM, st, tq, tk, tv, a);
+    launch_pdl(k_kv4_attn_tc, (int)(units < sms ? units : sms), T_THREADS, T_SMEM, st, tq, tqp, tk, tv, a);
     return (int)cudaGetLastError();
 }
 
@@ -1671,8 +1670,7 @@ int launch_mass_tc(Kv4Args& a, int max_len, cudaStream_t st) {
     const long long units = (long long)a.n_seqs * a.n_blocks * (a.heads / a.group);
     if (units > 0x7fffffffLL - 4096) return -1;
     CUtensorMap tq;
-    // whole tiles: a block of 256 / group rows of each head
-    if (!attn_tmap(&tq, a.Q, a.heads * 64, a.q_rows, a.ldq, MQ / a.group)) return -1;
+    if (!packed_tmap(&tq, a, MQ)) return -1;
     launch_pdl(k_kv4_mass_tc, (int)(units < sms ? units : sms), M_THREADS, M_SMEM, st, tq, a);
     return (int)cudaGetLastError();
 }
