@@ -562,17 +562,14 @@ __device__ __forceinline__ void build_units(const Kv4Args& a, int* cum, int run)
 struct Unit {
     int sq, q_start, q_len, kv_start, kv_len, ext_len;
     int mode, block, h;  // h: first head; of a packed unit the first of its kv head
+    int entry = 0;       // of the table
 
-    // unit u of the table
+    // unit u of the table, at or behind the one found before (a CTA's units ascend). Little code, and no loop of fixed
+    // length: it runs once a unit, mostly from outside the instruction cache, in every role
     __device__ void find(const Kv4Args& a, const int* cum, int run, int u) {
-        int lo = 0, hi = T_ENTRIES - 1;  // the last entry that begins at or before u
-        while (lo < hi) {
-            const int mid = (lo + hi + 1) / 2;
-            if (cum[mid] <= u) lo = mid;
-            else hi = mid - 1;
-        }
-        int rest = u - cum[lo];
-        sq = lo * run;
+        while (cum[entry + 1] <= u) entry++;
+        int rest = u - cum[entry];
+        sq = entry * run;
         if (run > 1)
             for (int n; rest >= (n = seq_units(a, sq, false)); sq++) rest -= n;
         if (run == 1) {
@@ -591,9 +588,13 @@ struct Unit {
             ext_len = s.ext_len;
         }
         mode = unit_mode(a, q_len);
-        const int hu = mode == kPacked ? a.heads / a.group : mode == kPair ? a.heads / 2 : a.heads;
-        block = rest / hu;
-        h = rest % hu * (mode == kPacked ? a.group : mode == kPair ? 2 : 1);
+        block = 0;
+        if (mode != kPacked) {
+            const int hu = mode == kPair ? a.heads / 2 : a.heads;
+            block = rest / hu;
+            rest -= block * hu;
+        }
+        h = rest * (mode == kPacked ? a.group : mode == kPair ? 2 : 1);
     }
     __device__ int ext_tiles() const { return (ext_len + TKV - 1) / TKV; }
     __device__ int tiles() const { return ext_tiles() + (kv_len + TKV - 1) / TKV; }
