@@ -559,10 +559,12 @@ __device__ __forceinline__ void build_units(const Kv4Args& a, int* cum, int run)
     __syncthreads();
 }
 
+template <bool SPLIT>
 struct Unit {
     int sq, q_start, q_len, kv_start, kv_len, ext_len;
     int mode, block, h;  // h: first head; of a packed unit the first of its kv head
     int entry = 0;       // of the table
+    int t0, t1;          // SPLIT: its key tiles
 
     // unit u of the table, at or behind the one found before (a CTA's units ascend). Little code, and no loop of fixed
     // length: it runs once a unit, mostly from outside the instruction cache, in every role
@@ -595,11 +597,21 @@ struct Unit {
             rest -= block * hu;
         }
         h = rest * (mode == kPacked ? a.group : mode == kPair ? 2 : 1);
+        t0 = 0;
+        t1 = all_tiles();
     }
-    __device__ int ext_tiles() const { return (ext_len + TKV - 1) / TKV; }
-    __device__ int tiles() const { return ext_tiles() + (kv_len + TKV - 1) / TKV; }
-    __device__ int valid(int j) const {  // keys of tile j, at least 1; 128 or more: all
-        const int e = ext_tiles();
+    __device__ void part(int rank, int ranks) {  // the rank's share of the key tiles
+        const int per = (all_tiles() + ranks - 1) / ranks;
+        t0 = min(all_tiles(), rank * per);
+        t1 = min(all_tiles(), t0 + per);
+    }
+    __device__ int all_ext_tiles() const { return (ext_len + TKV - 1) / TKV; }
+    __device__ int all_tiles() const { return all_ext_tiles() + (kv_len + TKV - 1) / TKV; }
+    __device__ int first() const { return SPLIT ? t0 : 0; }
+    __device__ int ext_tiles() const { return SPLIT ? max(0, min(t1, all_ext_tiles()) - t0) : all_ext_tiles(); }
+    __device__ int tiles() const { return SPLIT ? t1 - t0 : all_tiles(); }
+    __device__ int valid(int i) const {  // keys of its tile i, at least 1; 128 or more: all
+        const int e = all_ext_tiles(), j = first() + i;
         return j < e ? ext_len - j * TKV : kv_len - (j - e) * TKV;
     }
     __device__ int q_tiles() const { return mode == kPacked ? 1 : mode == kPair || q_len > row0(1) ? 2 : 1; }
@@ -650,6 +662,7 @@ __device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_
                  : "memory");
 }
 
+template <bool SPLIT>
 __global__ void __launch_bounds__(T_THREADS, 1)
     k_kv4_attn_tc(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmQp,
                   const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV, const Kv4Args a) {
@@ -710,21 +723,33 @@ __global__ void __launch_bounds__(T_THREADS, 1)
     const int run = (a.n_seqs + T_ENTRIES - 1) / T_ENTRIES;
     build_units(a, cum, run);
     const int n_units = cum[T_ENTRIES];
-    Unit un;
+    Unit<SPLIT> un;
+    // SPLIT: the CTAs of a cluster share out the key tiles of the cluster's first unit. Should there be more units than
+    // clusters (max_q was too small), the first CTA goes on alone. Every warp passes the three barriers behind the first unit.
+    const int ranks = SPLIT ? a.ranks : 1, rank = SPLIT ? (int)cluster_ctarank() : 0;
+    const int u0 = blockIdx.x / ranks, u_step = gridDim.x / ranks;
+    auto find_unit = [&](int u) {
+        un.find(a, cum, run, u);
+        if (SPLIT && u == u0) un.part(rank, ranks);
+    };
+    auto pass_barriers = [&]() {
+        __syncwarp();
+        for (int i = 0; i < 3; i++) cluster_sync();
+    };
 
     if (warp >= 8) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(T_OTHER_REGS));
         if (warp == 8) {
         // ------------------------------------------------------------------ fetching (one thread)
-        if (lane == 0) {
+        if (SPLIT || lane == 0) {
             int qi = 0, ri = 0;
             bool ok = true;
-            for (int u = blockIdx.x; ok && u < n_units; u += gridDim.x) {
-                un.find(a, cum, run, u);
+            auto unit = [&](int u) {
+                find_unit(u);
                 const int g = un.h / a.group, e_tiles = un.ext_tiles();
-                if (un.tiles() == 0) continue;
+                if (un.tiles() == 0) return;
                 const int qs = qi % T_QSLOTS;
-                if (!(ok = mbar_wait(bar(B_QEMPTY + qs), ((qi / T_QSLOTS) & 1) ^ 1, abort_flag))) break;
+                if (!(ok = mbar_wait(bar(B_QEMPTY + qs), ((qi / T_QSLOTS) & 1) ^ 1, abort_flag))) return;
                 // whole tiles always: rows behind the sequence's end are other sequences', or zeros behind the buffer's;
                 // the lanes that they fall to are not used
                 const uint32_t dq = smem_u32(sQ + qs * 2 * T_QT_BYTES), full = bar(B_QFULL + qs);
@@ -744,19 +769,27 @@ __global__ void __launch_bounds__(T_THREADS, 1)
                 const d1_half *kp = a.seqs[un.sq].kp + at, *vp = a.seqs[un.sq].vp + at;
                 for (int j = 0; j < e_tiles; j++, ri++) {
                     const int rs = ri % T_RAW_STAGES;
-                    if (!(ok = mbar_wait(bar(B_RAWEMPTY + rs), ((ri / T_RAW_STAGES) & 1) ^ 1, abort_flag))) break;
+                    if (!(ok = mbar_wait(bar(B_RAWEMPTY + rs), ((ri / T_RAW_STAGES) & 1) ^ 1, abort_flag))) return;
                     // whole 16-byte runs: up to 8 parameters, which the arrays hold (ext_cap is a multiple of 8)
                     const int n = min(un.valid(j), TKV);
                     const uint32_t codes = n * 32, pars = ((n + 7) & ~7) * 2;
                     const uint32_t dst = smem_u32(sRaw + rs * T_RAW_BYTES), landed = bar(B_RAWFULL + rs);
-                    const size_t key = (size_t)j * TKV;
+                    const size_t key = (size_t)(un.first() + j) * TKV;
                     mbar_arrive_expect_tx(landed, 2 * (codes + pars));
                     bulk_load(dst, k4 + key * 32, codes, landed);
                     bulk_load(dst + T_RAW_V, v4 + key * 32, codes, landed);
                     bulk_load(dst + T_RAW_KP, kp + key, pars, landed);
                     bulk_load(dst + T_RAW_VP, vp + key, pars, landed);
                 }
+            };
+            for (int u = u0; ok && u < n_units; u += u_step) {
+                if (lane == 0) unit(u);
+                if (SPLIT && u == u0) {
+                    pass_barriers();
+                    if (rank > 0) break;
+                }
             }
+        if (lane == 0) {
             if (!ok) record_err(a.err, abort_flag, kErrWaitEmpty);
             // copies still in flight (only after an abort) land before the CTA exits
             for (int i = ri > T_RAW_STAGES ? ri - T_RAW_STAGES : 0; i < ri; i++)
@@ -764,14 +797,15 @@ __global__ void __launch_bounds__(T_THREADS, 1)
             for (int i = qi > T_QSLOTS ? qi - T_QSLOTS : 0; i < qi; i++)
                 if (!mbar_wait_timed2(bar(B_QFULL + i % T_QSLOTS), (i / T_QSLOTS) & 1)) break;
         }
+        }
         __syncwarp();
     } else if (warp >= 10 && warp < 14) {
         // ------------------------------------------------------------------ expanding
         const int lt = (warp - 10) * 32 + lane;
         int ri = 0, ki = 0, oi = 0;  // cached tiles, tiles, and partial tiles of own rows so far
         bool ok = true;
-        for (int u = blockIdx.x; ok && u < n_units; u += gridDim.x) {
-            un.find(a, cum, run, u);
+        auto unit = [&](int u) {
+            find_unit(u);
             const int g = un.h / a.group, nt = un.tiles(), e_tiles = un.ext_tiles();
             for (int j = 0; j < nt; j++, ki++) {
                 const int st = ki % T_STAGES, n = un.valid(j);
@@ -781,7 +815,7 @@ __global__ void __launch_bounds__(T_THREADS, 1)
                     const int rs = ri % T_RAW_STAGES;
                     const uint8_t* raw = sRaw + rs * T_RAW_BYTES;
                     if (!(ok = __all_sync(D1_FULL_MASK, mbar_wait(bar(B_RAWFULL + rs), (ri / T_RAW_STAGES) & 1, abort_flag))))
-                        break;
+                        return;
                     uint4 piece[4];
                     uint32_t par[4];
 #pragma unroll
@@ -798,7 +832,7 @@ __global__ void __launch_bounds__(T_THREADS, 1)
                     if (lane == 0) mbar_arrive(bar(B_RAWEMPTY + rs));
                     ri++;
                     if (!(ok = __all_sync(D1_FULL_MASK, mbar_wait(bar(B_KVEMPTY + st), ((ki / T_STAGES) & 1) ^ 1, abort_flag))))
-                        break;
+                        return;
 #pragma unroll
                     for (int i = 0; i < 4; i++) {
                         const int r = (lt >> 1) + (i & 1) * 64;
@@ -820,10 +854,10 @@ __global__ void __launch_bounds__(T_THREADS, 1)
                     continue;
                 }
                 if (!(ok = __all_sync(D1_FULL_MASK, mbar_wait(bar(B_KVEMPTY + st), ((ki / T_STAGES) & 1) ^ 1, abort_flag))))
-                    break;
+                    return;
                 // own rows: a whole tile by TMA. Rows behind the sequence's end are others', or zeros behind the buffer's:
                 // their scores are masked, and their values, which P = 0 multiplies, are overwritten with zeros
-                const int row0 = un.kv_start + (j - e_tiles) * TKV;
+                const int row0 = un.kv_start + (un.first() + j - un.all_ext_tiles()) * TKV;
                 const uint32_t landed = bar(n >= TKV ? B_KVFULL + st : B_OWN);
                 if (lt == 0) {
                     mbar_arrive_expect_tx(landed, 2 * T_KV_BYTES);
@@ -834,12 +868,19 @@ __global__ void __launch_bounds__(T_THREADS, 1)
                     if (lt != 0) mbar_arrive(landed);
                     continue;
                 }
-                if (!(ok = __all_sync(D1_FULL_MASK, mbar_wait(landed, oi & 1, abort_flag)))) break;
+                if (!(ok = __all_sync(D1_FULL_MASK, mbar_wait(landed, oi & 1, abort_flag)))) return;
                 oi++;
                 for (int c = n * 8 + lt; c < TKV * 8; c += T_EXPANDERS)
                     *reinterpret_cast<uint4*>(dK + T_KV_BYTES + c * 16) = make_uint4(0, 0, 0, 0);
                 fence_async_smem_cta();
                 mbar_arrive(bar(B_KVFULL + st));
+            }
+        };
+        for (int u = u0; ok && u < n_units; u += u_step) {
+            unit(u);
+            if (SPLIT && u == u0) {
+                pass_barriers();
+                if (rank > 0) break;
             }
         }
         if (!ok && lane == 0) record_err(a.err, abort_flag, kErrWaitEmpty);
@@ -851,18 +892,18 @@ __global__ void __launch_bounds__(T_THREADS, 1)
     } else if (warp == 9 || warp == 14) {
         // ------------------------------------------------------------------ MMA issuer of warpgroup w
         const int w = warp == 9 ? 0 : 1;
-        if (lane == 0) {
+        if (SPLIT || lane == 0) {
             const uint32_t tS = tmem + w * T_WG_COLS, tP = tS + T_P_COL, tO = tS + T_O_COL;
             int cnt = 0, units = 0;  // key tiles and units of the warpgroup so far
             int qi = 0, ki = 0;
             bool ok = true;
-            for (int u = blockIdx.x; ok && u < n_units; u += gridDim.x) {
-                un.find(a, cum, run, u);
+            auto unit = [&](int u) {
+                find_unit(u);
                 const int nt = un.tiles(), mine = un.tiles_of(w);
-                if (nt == 0) continue;
+                if (nt == 0) return;
                 const int step = un.mode == kPacked ? 2 : 1, first = un.mode == kPacked ? w : 0;  // its key tiles
                 const int qs = qi % T_QSLOTS;
-                if (!(ok = mbar_wait(bar(B_QFULL + qs), (qi / T_QSLOTS) & 1, abort_flag))) break;
+                if (!(ok = mbar_wait(bar(B_QFULL + qs), (qi / T_QSLOTS) & 1, abort_flag))) return;
                 const uint64_t dq = smem_desc_k128(smem_u32(sQ + qs * 2 * T_QT_BYTES) + (un.mode == kPacked ? 0 : w * T_QT_BYTES));
                 auto kv_addr = [&](int j) { return smem_u32(sKV + ((ki + j) % T_STAGES) * 2 * T_KV_BYTES); };
                 auto kv_ready = [&](int j) {
@@ -912,18 +953,29 @@ __global__ void __launch_bounds__(T_THREADS, 1)
                     if (!both) tc_commit(bar(B_KVEMPTY + (ki + j) % T_STAGES));
                     if (!s_next && !(ok = issue_s(i + 1))) break;
                 }
-                if (!ok) break;
+                if (!ok) return;
                 tc_commit(bar(B_QEMPTY + qs));
                 ki += nt;
                 qi++;
                 cnt += mine;
                 units += mine > 0;
+            };
+            for (int u = u0; ok && u < n_units; u += u_step) {
+                if (lane == 0) unit(u);
+                if (SPLIT && u == u0) {
+                    pass_barriers();
+                    if (rank > 0) break;
+                }
             }
+        if (lane == 0) {
             if (!ok) record_err(a.err, abort_flag, kErrWaitFull);
             tc_commit(bar(B_DRAIN + w));  // every issued MMA has completed before TMEM is released
             if (!mbar_wait_timed2(bar(B_DRAIN + w), 0)) record_err(a.err, abort_flag, kErrDrain);
         }
+        }
         __syncwarp();
+    } else if (SPLIT) {  // the warp without a role
+        if (u0 < n_units) pass_barriers();
     }
     } else {
         asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(T_SOFTMAX_REGS));
@@ -931,22 +983,28 @@ __global__ void __launch_bounds__(T_THREADS, 1)
         const int w = warp >> 2, row = (warp & 3) * 32 + lane;
         const uint32_t lane_off = (uint32_t)((warp & 3) * 32) << 16;
         const uint32_t tS = tmem + w * T_WG_COLS + lane_off, tP = tS + T_P_COL, tO = tS + T_O_COL;
+        // SPLIT: sums [w][row][R_LD], and maxima and weights [w][row][2], where the key tiles were
+        float *part_o = reinterpret_cast<float*>(sKV), *part_ml = part_o + 2 * TQ * R_LD;
         int cnt = 0, njoin = 0;  // key tiles and packed units joined so far
         bool ok = true;
-        for (int u = blockIdx.x; ok && u < n_units; u += gridDim.x) {
-            un.find(a, cum, run, u);
-            const bool packed = un.mode == kPacked;
-            if (w == 1 && !packed && un.q_tiles() == 1) continue;
+        for (int u = u0; ok && u < n_units; u += u_step) {
+            find_unit(u);
+            const bool packed = un.mode == kPacked, split = SPLIT && u == u0;
+            if (!SPLIT && w == 1 && !packed && un.q_tiles() == 1) continue;
             // this thread's row: of the sequence and the head
             const int rows = un.rows(a, w), nt = un.tiles_of(w);
             const bool there = row < rows;
             const int q = packed ? row / a.group : un.row0(w) + row, h = packed ? un.h + row % a.group : un.head(w);
             const size_t grow = (size_t)(un.q_start + q);
-            if (un.tiles() == 0) {  // no keys: zeros
-                if (there && !(packed && w == 1)) {
+            if (un.all_tiles() == 0) {  // no keys: zeros
+                if (there && rank == 0 && !(packed && w == 1)) {
                     for (int i = 0; i < 8; i++)
                         *reinterpret_cast<uint4*>(a.O + grow * a.ldo + h * 64 + i * 8) = make_uint4(0, 0, 0, 0);
                     if (a.lse) a.lse[(size_t)h * a.lse_ld + grow] = -INFINITY;
+                }
+                if (split) {
+                    pass_barriers();
+                    if (rank > 0) break;
                 }
                 continue;
             }
@@ -1046,30 +1104,38 @@ __global__ void __launch_bounds__(T_THREADS, 1)
                 l = l * alpha + (((rs[0] + rs[1]) + (rs[2] + rs[3])) + ((rs[4] + rs[5]) + (rs[6] + rs[7])));
                 m = m_use;
             }
-            if (!ok) break;
+            if (!SPLIT && !ok) break;
             cnt += nt;
-            if (packed && w == 1) {  // the rest is warpgroup 0's, which shares the lanes
-                if (njoin > 0 && !(ok = __all_sync(D1_FULL_MASK, mbar_wait(bar(B_JOINED), (njoin - 1) & 1, abort_flag)))) break;
-                if (nt > 0) {
-                    if (!(ok = __all_sync(D1_FULL_MASK, mbar_wait(bar(B_ODONE + 1), (cnt - 1) & 1, abort_flag)))) break;
-                    tc_fence_after();
-                }
+            if (ok && packed && w == 1 && un.tiles() > 0) {  // the rest is warpgroup 0's, which shares the lanes
+                if (njoin > 0) ok = __all_sync(D1_FULL_MASK, mbar_wait(bar(B_JOINED), (njoin - 1) & 1, abort_flag));
+                if (ok && nt > 0) ok = __all_sync(D1_FULL_MASK, mbar_wait(bar(B_ODONE + 1), (cnt - 1) & 1, abort_flag));
+                if (!SPLIT && !ok) break;
+                tc_fence_after();
                 join[2 * row] = m;
                 join[2 * row + 1] = l;
                 tc_fence_before();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(bar(B_JOIN));
                 njoin++;
-                continue;
+                if (!split) continue;
             }
-            if (!(ok = __all_sync(D1_FULL_MASK, mbar_wait(bar(B_ODONE + w), (cnt - 1) & 1, abort_flag)))) break;
+            const bool mine = nt > 0 && !(packed && w == 1);  // this warpgroup finishes the unit's rows, or some of them
+            if (!SPLIT || (ok && mine)) ok = __all_sync(D1_FULL_MASK, mbar_wait(bar(B_ODONE + w), (cnt - 1) & 1, abort_flag));
+            if (!SPLIT && !ok) break;
             tc_fence_after();
+            if (split) {
+                __syncwarp();
+                cluster_sync();  // both warpgroups have done with the key tiles: their shared memory is free
+            }
+            if (SPLIT && !split && !mine) continue;
+            if (!SPLIT || (ok && mine)) {
             uint32_t o[64];
             tmem_ld32(tO, *reinterpret_cast<uint32_t(*)[32]>(o));
             tmem_ld32(tO + 32, *reinterpret_cast<uint32_t(*)[32]>(o + 32));
             tc_wait_ld();
             if (packed) {
-                if (!(ok = __all_sync(D1_FULL_MASK, mbar_wait(bar(B_JOIN), njoin & 1, abort_flag)))) break;
+                ok = __all_sync(D1_FULL_MASK, mbar_wait(bar(B_JOIN), njoin & 1, abort_flag));
+                if (!SPLIT && !ok) break;
                 tc_fence_after();
                 njoin++;
                 const float m1 = join[2 * row], l1 = join[2 * row + 1];
@@ -1095,6 +1161,18 @@ __global__ void __launch_bounds__(T_THREADS, 1)
                     mbar_arrive(bar(B_JOINED));
                 }
             }
+            if (split) {  // unscaled sums, for the cluster
+                if (there) {
+                    float* dst = part_o + (w * TQ + row) * R_LD;
+#pragma unroll
+                    for (int i = 0; i < 16; i++)
+                        *reinterpret_cast<float4*>(dst + 4 * i) =
+                            make_float4(__uint_as_float(o[4 * i]), __uint_as_float(o[4 * i + 1]), __uint_as_float(o[4 * i + 2]),
+                                        __uint_as_float(o[4 * i + 3]));
+                    part_ml[2 * (w * TQ + row)] = m;
+                    part_ml[2 * (w * TQ + row) + 1] = l;
+                }
+            } else {
             const float il = 1.f / l;
             uint32_t oh[32];
 #pragma unroll
@@ -1105,6 +1183,57 @@ __global__ void __launch_bounds__(T_THREADS, 1)
                 for (int i = 0; i < 8; i++)
                     *reinterpret_cast<uint4*>(a.O + grow * a.ldo + h * 64 + i * 8) =
                         make_uint4(oh[4 * i], oh[4 * i + 1], oh[4 * i + 2], oh[4 * i + 3]);
+            }
+            }
+            }
+            if (split) {
+                fence_async_smem_cta();  // (the next unit's copies come to the same place)
+                __syncwarp();
+                cluster_sync();  // the sums of every CTA are in its shared memory
+                // join them, in their order: each CTA writes its share of the rows
+                const int per = (un.all_tiles() + ranks - 1) / ranks, parts = (un.all_tiles() - 1) / per + 1, share = TQ / ranks;
+                if (!(packed ? w == 1 : w >= un.q_tiles())) {
+                    for (int i = row; i < share * 16; i += TQ) {
+                        const int r = rank * share + (i >> 4), d = (i & 15) * 4;
+                        if (r >= rows) break;
+                        float pm[R_CLUSTER], pl[R_CLUSTER];
+                        float4 v[R_CLUSTER];
+#pragma unroll
+                        for (int c = 0; c < R_CLUSTER; c++) {
+                            pm[c] = -INFINITY;
+                            pl[c] = 0.f;
+                            v[c] = make_float4(0.f, 0.f, 0.f, 0.f);
+                            if (c < parts) {
+                                pm[c] = ld_cluster_f32(mapa_shared(smem_u32(part_ml + 2 * (w * TQ + r)), c));
+                                pl[c] = ld_cluster_f32(mapa_shared(smem_u32(part_ml + 2 * (w * TQ + r) + 1), c));
+                                v[c] = ld_cluster_f32x4(mapa_shared(smem_u32(part_o + (w * TQ + r) * R_LD + d), c));
+                            }
+                        }
+                        float M = -INFINITY, L = 0.f;
+#pragma unroll
+                        for (int c = 0; c < R_CLUSTER; c++) M = fmaxf(M, pm[c]);
+                        float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+                        for (int c = 0; c < R_CLUSTER; c++) {
+                            if (c >= parts) break;
+                            const float f = ex2(pm[c] - M);
+                            L += f * pl[c];
+                            x.x += f * v[c].x;
+                            x.y += f * v[c].y;
+                            x.z += f * v[c].z;
+                            x.w += f * v[c].w;
+                        }
+                        const float il = 1.f / L;
+                        const int qr = un.q_start + (packed ? r / a.group : un.row0(w) + r);
+                        const int hr = packed ? un.h + r % a.group : un.head(w);
+                        *reinterpret_cast<uint2*>(a.O + (size_t)qr * a.ldo + hr * 64 + d) =
+                            make_uint2(pack_h2(x.x * il, x.y * il), pack_h2(x.z * il, x.w * il));
+                        if (a.lse && d == 0) a.lse[(size_t)hr * a.lse_ld + qr] = (M + log2f(L)) * kLn2;
+                    }
+                }
+                __syncwarp();
+                cluster_sync();  // the other CTAs have read this one's sums
+                if (rank > 0) break;
             }
         }
         if (!ok && lane == 0) record_err(a.err, abort_flag, kErrWaitAccFull);
@@ -1591,6 +1720,26 @@ int sm_count() {
     return sms[dev & 63];
 }
 
+// kernel<<<...>>>(args...) in clusters of `ranks` CTAs along x, with programmatic stream serialization.
+template <typename... KP, typename... A>
+int launch_clusters(void (*kernel)(KP...), dim3 grid, int block, size_t smem, int ranks, cudaStream_t st, const A&... args) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = grid;
+    cfg.blockDim = dim3(block);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = st;
+    cudaLaunchAttribute at[2];
+    at[0].id = cudaLaunchAttributeClusterDimension;
+    at[0].val.clusterDim.x = ranks;
+    at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+    at[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[1].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = at;
+    cfg.numAttrs = pdl_enabled() ? 2 : 1;
+    cudaLaunchKernelEx(&cfg, kernel, args...);
+    return (int)cudaGetLastError();
+}
+
 template <int NT>
 int launch_rows(Kv4Args& a, int max_q, int max_keys, int kv_heads, cudaStream_t st) {
     static unsigned long long done = 0;
@@ -1605,21 +1754,8 @@ int launch_rows(Kv4Args& a, int max_q, int max_keys, int kv_heads, cudaStream_t 
     const long long tiles = ((long long)max_keys + R_KEYS - 1) / R_KEYS, slots = 148 * (NT == 1 ? 4 : 2);
     while (ranks > 1 && ((ranks / 2) * R_WARPS >= tiles || x * kv_heads * z * ranks > slots)) ranks /= 2;
     a.ranks = ranks;
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)x * ranks, kv_heads, z);
-    cfg.blockDim = dim3(R_WARPS * 32);
-    cfg.dynamicSmemBytes = rows_smem<NT>();
-    cfg.stream = st;
-    cudaLaunchAttribute at[2];
-    at[0].id = cudaLaunchAttributeClusterDimension;
-    at[0].val.clusterDim.x = ranks;
-    at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
-    at[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    at[1].val.programmaticStreamSerializationAllowed = 1;
-    cfg.attrs = at;
-    cfg.numAttrs = pdl_enabled() ? 2 : 1;
-    cudaLaunchKernelEx(&cfg, k_kv4_attn_rows<NT>, (const Kv4Args)a);
-    return (int)cudaGetLastError();
+    return launch_clusters(k_kv4_attn_rows<NT>, dim3((unsigned)x * ranks, kv_heads, z), R_WARPS * 32, rows_smem<NT>(), ranks, st,
+                           (const Kv4Args)a);
 }
 
 // Q as [row][head][64], in boxes of the group's heads of `most` / group rows: the packed rows of a tile in their order, in
@@ -1636,9 +1772,9 @@ bool packed_tmap(CUtensorMap* m, const Kv4Args& a, int most) {
                CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-int launch_tc(Kv4Args& a, int max_q, cudaStream_t st) {
-    static unsigned long long done = 0;
-    if (!smem_opt_in(k_kv4_attn_tc, T_SMEM, &done)) return -1;
+int launch_tc(Kv4Args& a, int max_q, int max_keys, cudaStream_t st) {
+    static unsigned long long done = 0, done_split = 0;
+    if (!smem_opt_in(k_kv4_attn_tc<false>, T_SMEM, &done) || !smem_opt_in(k_kv4_attn_tc<true>, T_SMEM, &done_split)) return -1;
     const int sms = sm_count();
     if (!sms) return -1;
     // no more CTAs than units, were every sequence max_q rows long
@@ -1658,8 +1794,16 @@ int launch_tc(Kv4Args& a, int max_q, cudaStream_t st) {
     } else {
         tk = tv = tq;  // no own rows: never read
     }
-    launch_pdl(k_kv4_attn_tc, (int)(units < sms ? units : sms), T_THREADS, T_SMEM, st, tq, tqp, tk, tv, a);
-    return (int)cudaGetLastError();
+    // few units: a cluster of CTAs to each, as many as the GPU has room for at once, with two key tiles or more for each
+    int ranks = R_CLUSTER;
+    while (ranks > 1 && (units * ranks > sms || (long long)(ranks - 1) * 2 * TKV >= max_keys)) ranks /= 2;
+    a.ranks = ranks;
+    if (ranks == 1) {
+        launch_pdl(k_kv4_attn_tc<false>, (int)(units < sms ? units : sms), T_THREADS, T_SMEM, st, tq, tqp, tk, tv, a);
+        return (int)cudaGetLastError();
+    }
+    return launch_clusters(k_kv4_attn_tc<true>, dim3((unsigned)units * ranks), T_THREADS, T_SMEM, ranks, st, tq, tqp, tk, tv,
+                           (const Kv4Args)a);
 }
 
 int launch_mass_tc(Kv4Args& a, int max_len, cudaStream_t st) {
@@ -1711,7 +1855,7 @@ extern "C" int d1_flash_attn_kv4(const d1_half* Q, int ldq, const d1_half* K, co
     a.scale_log2 = scale * kLog2e;
     if (!a.err) return -1;
     const int kv_heads = heads / group;
-    if ((long long)max_q * group > 64) return launch_tc(a, max_q, st);
+    if ((long long)max_q * group > 64) return launch_tc(a, max_q, max_keys, st);
     const long long rows = (long long)max_q * group;
     return rows <= 8 ? launch_rows<1>(a, max_q, max_keys, kv_heads, st)
                      : rows <= 16 ? launch_rows<2>(a, max_q, max_keys, kv_heads, st)

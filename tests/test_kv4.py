@@ -308,8 +308,8 @@ def check_attend(O, L, want, h):
         assert (got[~fin] == l[~fin]).all() and (np.abs(got[fin] - l[fin]) <= tL[fin]).all()
 
 
-# which kernel runs follows from max_q; its results must not
-HINTS = [1, 17, 5000]
+# which kernel runs, and whether a cluster of CTAs shares a unit, follows from max_q; the results must not
+HINTS = [1, 17, 40, 200, 5000]
 CASES = {
     "one": ([1], [1], [0], 8, 2),
     "no keys": ([3, 1, 200], [0, 5, 0], [0, 0, 0], 4, 2),
