@@ -8,12 +8,14 @@ namespace d1 {
 // Error codes of the d1_kv4_* kernels beyond those of the waits.
 enum : int { kErrTable = 6 };  // a table entry that breaks the header's rules; it was skipped
 
+constexpr int kKv4MaxRows = 1 << 30;  // of a cache: row counters that step by a grid's rows stay inside 32 bits
+
 // Device address of the error word on the current device, or NULL.
 int* kv4_err_addr();
 
 __device__ __forceinline__ bool kv4_cache_ok(int len, int cap, const void* k4, const void* v4, const void* kp,
                                              const void* vp) {
-    if (len < 0 || len > cap || (cap & 7)) return false;
+    if (len < 0 || len > cap || cap > kKv4MaxRows || (cap & 7)) return false;
     if (cap == 0) return true;
     if (!k4 || !v4 || !kp || !vp) return false;
     return (((uintptr_t)k4 | (uintptr_t)v4 | (uintptr_t)kp | (uintptr_t)vp) & 15) == 0;

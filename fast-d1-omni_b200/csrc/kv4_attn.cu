@@ -20,7 +20,6 @@ struct Kv4Args {
     const D1Kv4Seq* seqs;
     int* err;
     int ldq, ldkv, ldo, lse_ld, n_seqs, heads, group, q_rows, kv_rows, accumulate, ranks;
-    int n_blocks;  // tcgen05 form of the mass: tiles of keys per cache
     float scale_log2;
 };
 
@@ -740,243 +739,243 @@ __global__ void __launch_bounds__(T_THREADS, 1)
     if (warp >= 8) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(T_OTHER_REGS));
         if (warp == 8) {
-        // ------------------------------------------------------------------ fetching (one thread)
-        if (SPLIT || lane == 0) {
-            int qi = 0, ri = 0;
+            // ------------------------------------------------------------------ fetching (one thread)
+            if (SPLIT || lane == 0) {
+                int qi = 0, ri = 0;
+                bool ok = true;
+                auto unit = [&](int u) {
+                    find_unit(u);
+                    const int g = un.h / a.group, e_tiles = un.ext_tiles();
+                    if (un.tiles() == 0) return;
+                    const int qs = qi % T_QSLOTS;
+                    if (!(ok = mbar_wait(bar(B_QEMPTY + qs), ((qi / T_QSLOTS) & 1) ^ 1, abort_flag))) return;
+                    // whole tiles always: rows behind the sequence's end are other sequences', or zeros behind the buffer's;
+                    // the lanes that they fall to are not used
+                    const uint32_t dq = smem_u32(sQ + qs * 2 * T_QT_BYTES), full = bar(B_QFULL + qs);
+                    const int row = un.q_start + (un.mode == kPacked ? 0 : un.row0(0));
+                    if (un.mode == kPacked) {
+                        mbar_arrive_expect_tx(full, TQ / a.group * a.group * 128);
+                        tma_load_3d(dq, &tmQp, 0, un.h, row, full);
+                    } else {
+                        const int nq = un.q_tiles();
+                        mbar_arrive_expect_tx(full, nq * T_QT_BYTES);
+                        tma_load_2d(dq, &tmQ, un.head(0) * 64, row, full);
+                        if (nq == 2) tma_load_2d(dq + T_QT_BYTES, &tmQ, un.head(1) * 64, un.q_start + un.row0(1), full);
+                    }
+                    qi++;
+                    const size_t at = (size_t)g * a.seqs[un.sq].ext_cap;
+                    const uint8_t *k4 = a.seqs[un.sq].k4 + at * 32, *v4 = a.seqs[un.sq].v4 + at * 32;
+                    const d1_half *kp = a.seqs[un.sq].kp + at, *vp = a.seqs[un.sq].vp + at;
+                    for (int j = 0; j < e_tiles; j++, ri++) {
+                        const int rs = ri % T_RAW_STAGES;
+                        if (!(ok = mbar_wait(bar(B_RAWEMPTY + rs), ((ri / T_RAW_STAGES) & 1) ^ 1, abort_flag))) return;
+                        // whole 16-byte runs: up to 8 parameters, which the arrays hold (ext_cap is a multiple of 8)
+                        const int n = min(un.valid(j), TKV);
+                        const uint32_t codes = n * 32, pars = ((n + 7) & ~7) * 2;
+                        const uint32_t dst = smem_u32(sRaw + rs * T_RAW_BYTES), landed = bar(B_RAWFULL + rs);
+                        const size_t key = (size_t)(un.first() + j) * TKV;
+                        mbar_arrive_expect_tx(landed, 2 * (codes + pars));
+                        bulk_load(dst, k4 + key * 32, codes, landed);
+                        bulk_load(dst + T_RAW_V, v4 + key * 32, codes, landed);
+                        bulk_load(dst + T_RAW_KP, kp + key, pars, landed);
+                        bulk_load(dst + T_RAW_VP, vp + key, pars, landed);
+                    }
+                };
+                for (int u = u0; ok && u < n_units; u += u_step) {
+                    if (lane == 0) unit(u);
+                    if (SPLIT && u == u0) {
+                        pass_barriers();
+                        if (rank > 0) break;
+                    }
+                }
+                if (lane == 0) {
+                    if (!ok) record_err(a.err, abort_flag, kErrWaitEmpty);
+                    // copies still in flight (only after an abort) land before the CTA exits
+                    for (int i = ri > T_RAW_STAGES ? ri - T_RAW_STAGES : 0; i < ri; i++)
+                        if (!mbar_wait_timed2(bar(B_RAWFULL + i % T_RAW_STAGES), (i / T_RAW_STAGES) & 1)) break;
+                    for (int i = qi > T_QSLOTS ? qi - T_QSLOTS : 0; i < qi; i++)
+                        if (!mbar_wait_timed2(bar(B_QFULL + i % T_QSLOTS), (i / T_QSLOTS) & 1)) break;
+                }
+            }
+            __syncwarp();
+        } else if (warp >= 10 && warp < 14) {
+            // ------------------------------------------------------------------ expanding
+            const int lt = (warp - 10) * 32 + lane;
+            int ri = 0, ki = 0, oi = 0;  // cached tiles, tiles, and partial tiles of own rows so far
             bool ok = true;
             auto unit = [&](int u) {
                 find_unit(u);
-                const int g = un.h / a.group, e_tiles = un.ext_tiles();
-                if (un.tiles() == 0) return;
-                const int qs = qi % T_QSLOTS;
-                if (!(ok = mbar_wait(bar(B_QEMPTY + qs), ((qi / T_QSLOTS) & 1) ^ 1, abort_flag))) return;
-                // whole tiles always: rows behind the sequence's end are other sequences', or zeros behind the buffer's;
-                // the lanes that they fall to are not used
-                const uint32_t dq = smem_u32(sQ + qs * 2 * T_QT_BYTES), full = bar(B_QFULL + qs);
-                const int row = un.q_start + (un.mode == kPacked ? 0 : un.row0(0));
-                if (un.mode == kPacked) {
-                    mbar_arrive_expect_tx(full, TQ / a.group * a.group * 128);
-                    tma_load_3d(dq, &tmQp, 0, un.h, row, full);
-                } else {
-                    const int nq = un.q_tiles();
-                    mbar_arrive_expect_tx(full, nq * T_QT_BYTES);
-                    tma_load_2d(dq, &tmQ, un.head(0) * 64, row, full);
-                    if (nq == 2) tma_load_2d(dq + T_QT_BYTES, &tmQ, un.head(1) * 64, un.q_start + un.row0(1), full);
-                }
-                qi++;
-                const size_t at = (size_t)g * a.seqs[un.sq].ext_cap;
-                const uint8_t *k4 = a.seqs[un.sq].k4 + at * 32, *v4 = a.seqs[un.sq].v4 + at * 32;
-                const d1_half *kp = a.seqs[un.sq].kp + at, *vp = a.seqs[un.sq].vp + at;
-                for (int j = 0; j < e_tiles; j++, ri++) {
-                    const int rs = ri % T_RAW_STAGES;
-                    if (!(ok = mbar_wait(bar(B_RAWEMPTY + rs), ((ri / T_RAW_STAGES) & 1) ^ 1, abort_flag))) return;
-                    // whole 16-byte runs: up to 8 parameters, which the arrays hold (ext_cap is a multiple of 8)
-                    const int n = min(un.valid(j), TKV);
-                    const uint32_t codes = n * 32, pars = ((n + 7) & ~7) * 2;
-                    const uint32_t dst = smem_u32(sRaw + rs * T_RAW_BYTES), landed = bar(B_RAWFULL + rs);
-                    const size_t key = (size_t)(un.first() + j) * TKV;
-                    mbar_arrive_expect_tx(landed, 2 * (codes + pars));
-                    bulk_load(dst, k4 + key * 32, codes, landed);
-                    bulk_load(dst + T_RAW_V, v4 + key * 32, codes, landed);
-                    bulk_load(dst + T_RAW_KP, kp + key, pars, landed);
-                    bulk_load(dst + T_RAW_VP, vp + key, pars, landed);
-                }
-            };
-            for (int u = u0; ok && u < n_units; u += u_step) {
-                if (lane == 0) unit(u);
-                if (SPLIT && u == u0) {
-                    pass_barriers();
-                    if (rank > 0) break;
-                }
-            }
-        if (lane == 0) {
-            if (!ok) record_err(a.err, abort_flag, kErrWaitEmpty);
-            // copies still in flight (only after an abort) land before the CTA exits
-            for (int i = ri > T_RAW_STAGES ? ri - T_RAW_STAGES : 0; i < ri; i++)
-                if (!mbar_wait_timed2(bar(B_RAWFULL + i % T_RAW_STAGES), (i / T_RAW_STAGES) & 1)) break;
-            for (int i = qi > T_QSLOTS ? qi - T_QSLOTS : 0; i < qi; i++)
-                if (!mbar_wait_timed2(bar(B_QFULL + i % T_QSLOTS), (i / T_QSLOTS) & 1)) break;
-        }
-        }
-        __syncwarp();
-    } else if (warp >= 10 && warp < 14) {
-        // ------------------------------------------------------------------ expanding
-        const int lt = (warp - 10) * 32 + lane;
-        int ri = 0, ki = 0, oi = 0;  // cached tiles, tiles, and partial tiles of own rows so far
-        bool ok = true;
-        auto unit = [&](int u) {
-            find_unit(u);
-            const int g = un.h / a.group, nt = un.tiles(), e_tiles = un.ext_tiles();
-            for (int j = 0; j < nt; j++, ki++) {
-                const int st = ki % T_STAGES, n = un.valid(j);
-                uint8_t* dK = sKV + st * 2 * T_KV_BYTES;
-                if (j < e_tiles) {
-                    // the thread's 16-byte pieces: of K, then of V, those of keys lt / 2 and 64 more, half lt % 2
-                    const int rs = ri % T_RAW_STAGES;
-                    const uint8_t* raw = sRaw + rs * T_RAW_BYTES;
-                    if (!(ok = __all_sync(D1_FULL_MASK, mbar_wait(bar(B_RAWFULL + rs), (ri / T_RAW_STAGES) & 1, abort_flag))))
-                        return;
-                    uint4 piece[4];
-                    uint32_t par[4];
+                const int g = un.h / a.group, nt = un.tiles(), e_tiles = un.ext_tiles();
+                for (int j = 0; j < nt; j++, ki++) {
+                    const int st = ki % T_STAGES, n = un.valid(j);
+                    uint8_t* dK = sKV + st * 2 * T_KV_BYTES;
+                    if (j < e_tiles) {
+                        // the thread's 16-byte pieces: of K, then of V, those of keys lt / 2 and 64 more, half lt % 2
+                        const int rs = ri % T_RAW_STAGES;
+                        const uint8_t* raw = sRaw + rs * T_RAW_BYTES;
+                        if (!(ok = __all_sync(D1_FULL_MASK, mbar_wait(bar(B_RAWFULL + rs), (ri / T_RAW_STAGES) & 1, abort_flag))))
+                            return;
+                        uint4 piece[4];
+                        uint32_t par[4];
 #pragma unroll
-                    for (int i = 0; i < 4; i++) {
-                        const int r = (lt >> 1) + (i & 1) * 64;
-                        piece[i] = *reinterpret_cast<const uint4*>(raw + (i >> 1) * T_RAW_V + r * 32 + (lt & 1) * 16);
-                        par[i] = *reinterpret_cast<const uint16_t*>(raw + T_RAW_KP + (i >> 1) * (TKV * 2) + r * 2);
-                        if (r >= n) {  // behind the cached keys: zeros
-                            piece[i] = make_uint4(0, 0, 0, 0);
-                            par[i] = 0;
+                        for (int i = 0; i < 4; i++) {
+                            const int r = (lt >> 1) + (i & 1) * 64;
+                            piece[i] = *reinterpret_cast<const uint4*>(raw + (i >> 1) * T_RAW_V + r * 32 + (lt & 1) * 16);
+                            par[i] = *reinterpret_cast<const uint16_t*>(raw + T_RAW_KP + (i >> 1) * (TKV * 2) + r * 2);
+                            if (r >= n) {  // behind the cached keys: zeros
+                                piece[i] = make_uint4(0, 0, 0, 0);
+                                par[i] = 0;
+                            }
                         }
+                        __syncwarp();
+                        if (lane == 0) mbar_arrive(bar(B_RAWEMPTY + rs));
+                        ri++;
+                        if (!(ok = __all_sync(D1_FULL_MASK, mbar_wait(bar(B_KVEMPTY + st), ((ki / T_STAGES) & 1) ^ 1, abort_flag))))
+                            return;
+#pragma unroll
+                        for (int i = 0; i < 4; i++) {
+                            const int r = (lt >> 1) + (i & 1) * 64;
+                            uint8_t* row = dK + (i >> 1) * T_KV_BYTES + r * 128;
+                            const uint32_t p2 = par[i] * 0x00010001u, step = kv4_step2(p2);
+                            uint32_t z0, z1;
+                            kv4_zero(p2, z0, z1);
+                            const uint32_t word[4] = {piece[i].x, piece[i].y, piece[i].z, piece[i].w};
+#pragma unroll
+                            for (int q = 0; q < 4; q++) {
+                                uint32_t x[4];
+                                kv4_expand(word[q], z0, z1, x);
+                                *reinterpret_cast<uint4*>(row + ((((lt & 1) * 4 + q) ^ (r & 7)) << 4)) =
+                                    make_uint4(h2_mul(x[0], step), h2_mul(x[1], step), h2_mul(x[2], step), h2_mul(x[3], step));
+                            }
+                        }
+                        fence_async_smem_cta();
+                        mbar_arrive(bar(B_KVFULL + st));
+                        continue;
                     }
-                    __syncwarp();
-                    if (lane == 0) mbar_arrive(bar(B_RAWEMPTY + rs));
-                    ri++;
                     if (!(ok = __all_sync(D1_FULL_MASK, mbar_wait(bar(B_KVEMPTY + st), ((ki / T_STAGES) & 1) ^ 1, abort_flag))))
                         return;
-#pragma unroll
-                    for (int i = 0; i < 4; i++) {
-                        const int r = (lt >> 1) + (i & 1) * 64;
-                        uint8_t* row = dK + (i >> 1) * T_KV_BYTES + r * 128;
-                        const uint32_t p2 = par[i] * 0x00010001u, step = kv4_step2(p2);
-                        uint32_t z0, z1;
-                        kv4_zero(p2, z0, z1);
-                        const uint32_t word[4] = {piece[i].x, piece[i].y, piece[i].z, piece[i].w};
-#pragma unroll
-                        for (int q = 0; q < 4; q++) {
-                            uint32_t x[4];
-                            kv4_expand(word[q], z0, z1, x);
-                            *reinterpret_cast<uint4*>(row + ((((lt & 1) * 4 + q) ^ (r & 7)) << 4)) =
-                                make_uint4(h2_mul(x[0], step), h2_mul(x[1], step), h2_mul(x[2], step), h2_mul(x[3], step));
-                        }
+                    // own rows: a whole tile by TMA. Rows behind the sequence's end are others', or zeros behind the buffer's:
+                    // their scores are masked, and their values, which P = 0 multiplies, are overwritten with zeros
+                    const int row0 = un.kv_start + (un.first() + j - un.all_ext_tiles()) * TKV;
+                    const uint32_t landed = bar(n >= TKV ? B_KVFULL + st : B_OWN);
+                    if (lt == 0) {
+                        mbar_arrive_expect_tx(landed, 2 * T_KV_BYTES);
+                        tma_load_2d(smem_u32(dK), &tmK, g * 64, row0, landed);
+                        tma_load_2d(smem_u32(dK + T_KV_BYTES), &tmV, g * 64, row0, landed);
                     }
+                    if (n >= TKV) {
+                        if (lt != 0) mbar_arrive(landed);
+                        continue;
+                    }
+                    if (!(ok = __all_sync(D1_FULL_MASK, mbar_wait(landed, oi & 1, abort_flag)))) return;
+                    oi++;
+                    for (int c = n * 8 + lt; c < TKV * 8; c += T_EXPANDERS)
+                        *reinterpret_cast<uint4*>(dK + T_KV_BYTES + c * 16) = make_uint4(0, 0, 0, 0);
                     fence_async_smem_cta();
                     mbar_arrive(bar(B_KVFULL + st));
-                    continue;
                 }
-                if (!(ok = __all_sync(D1_FULL_MASK, mbar_wait(bar(B_KVEMPTY + st), ((ki / T_STAGES) & 1) ^ 1, abort_flag))))
-                    return;
-                // own rows: a whole tile by TMA. Rows behind the sequence's end are others', or zeros behind the buffer's:
-                // their scores are masked, and their values, which P = 0 multiplies, are overwritten with zeros
-                const int row0 = un.kv_start + (un.first() + j - un.all_ext_tiles()) * TKV;
-                const uint32_t landed = bar(n >= TKV ? B_KVFULL + st : B_OWN);
-                if (lt == 0) {
-                    mbar_arrive_expect_tx(landed, 2 * T_KV_BYTES);
-                    tma_load_2d(smem_u32(dK), &tmK, g * 64, row0, landed);
-                    tma_load_2d(smem_u32(dK + T_KV_BYTES), &tmV, g * 64, row0, landed);
-                }
-                if (n >= TKV) {
-                    if (lt != 0) mbar_arrive(landed);
-                    continue;
-                }
-                if (!(ok = __all_sync(D1_FULL_MASK, mbar_wait(landed, oi & 1, abort_flag)))) return;
-                oi++;
-                for (int c = n * 8 + lt; c < TKV * 8; c += T_EXPANDERS)
-                    *reinterpret_cast<uint4*>(dK + T_KV_BYTES + c * 16) = make_uint4(0, 0, 0, 0);
-                fence_async_smem_cta();
-                mbar_arrive(bar(B_KVFULL + st));
-            }
-        };
-        for (int u = u0; ok && u < n_units; u += u_step) {
-            unit(u);
-            if (SPLIT && u == u0) {
-                pass_barriers();
-                if (rank > 0) break;
-            }
-        }
-        if (!ok && lane == 0) record_err(a.err, abort_flag, kErrWaitEmpty);
-        if (lt == 0 && !ok) mbar_wait_timed2(bar(B_OWN), oi & 1);  // copies still in flight land before the CTA exits
-        if (lt == 0)
-            for (int i = ki > T_STAGES ? ki - T_STAGES : 0; i < ki; i++)
-                if (!mbar_wait_timed2(bar(B_KVFULL + i % T_STAGES), (i / T_STAGES) & 1)) break;
-        __syncwarp();
-    } else if (warp == 9 || warp == 14) {
-        // ------------------------------------------------------------------ MMA issuer of warpgroup w
-        const int w = warp == 9 ? 0 : 1;
-        if (SPLIT || lane == 0) {
-            const uint32_t tS = tmem + w * T_WG_COLS, tP = tS + T_P_COL, tO = tS + T_O_COL;
-            int cnt = 0, units = 0;  // key tiles and units of the warpgroup so far
-            int qi = 0, ki = 0;
-            bool ok = true;
-            auto unit = [&](int u) {
-                find_unit(u);
-                const int nt = un.tiles(), mine = un.tiles_of(w);
-                if (nt == 0) return;
-                const int step = un.mode == kPacked ? 2 : 1, first = un.mode == kPacked ? w : 0;  // its key tiles
-                const int qs = qi % T_QSLOTS;
-                if (!(ok = mbar_wait(bar(B_QFULL + qs), (qi / T_QSLOTS) & 1, abort_flag))) return;
-                const uint64_t dq = smem_desc_k128(smem_u32(sQ + qs * 2 * T_QT_BYTES) + (un.mode == kPacked ? 0 : w * T_QT_BYTES));
-                auto kv_addr = [&](int j) { return smem_u32(sKV + ((ki + j) % T_STAGES) * 2 * T_KV_BYTES); };
-                auto kv_ready = [&](int j) {
-                    return mbar_wait(bar(B_KVFULL + (ki + j) % T_STAGES), ((ki + j) / T_STAGES) & 1, abort_flag);
-                };
-                // S of its i-th tile, once the softmax has read the one before
-                auto issue_s = [&](int i) {
-                    const int c = cnt + i;
-                    if (!kv_ready(first + i * step)) return false;
-                    if (c > 0 && !mbar_wait(bar(B_SFREE + w), (c - 1) & 1, abort_flag)) return false;
-                    tc_fence_after();
-                    const uint64_t dk = smem_desc_k128(kv_addr(first + i * step));
-#pragma unroll
-                    for (int k = 0; k < 4; k++) tc_mma_f16(tS, dq + 2 * k, dk + 2 * k, IDESC_S, k != 0);
-                    tc_commit(bar(B_SFULL + w));
-                    return true;
-                };
-                const bool both = un.mode != kPacked && un.q_tiles() == 2;  // the other issuer's MMAs read the tiles, too
-                if (mine > 0) ok = issue_s(0);
-                for (int i = 0; i < mine && ok; i++) {
-                    const int j = first + i * step, c = cnt + i;
-                    // the next S computes while the softmax works on tile i; where its keys are late, P V goes first (it
-                    // frees a stage that they may be waiting for)
-                    bool s_next = i + 1 == mine;
-                    const uint64_t t0 = globaltimer_ns();
-                    while (true) {
-                        if (!s_next && mbar_test(bar(B_KVFULL + (ki + j + step) % T_STAGES), ((ki + j + step) / T_STAGES) & 1)) {
-                            if (!(ok = issue_s(i + 1))) break;
-                            s_next = true;
-                        }
-                        if (mbar_try_wait_brief(bar(B_PFULL + w), c & 1)) break;
-                        if (*abort_flag || globaltimer_ns() - t0 > kWaitLimitNs) {
-                            ok = false;
-                            break;
-                        }
-                    }
-                    if (!ok) break;
-                    // the first P V of a unit overwrites O: the unit before must have been read
-                    if (i == 0 && units > 0 && !(ok = mbar_wait(bar(B_OFREE + w), (units - 1) & 1, abort_flag))) break;
-                    tc_fence_after();
-                    const uint64_t dv = smem_desc_k128(kv_addr(j) + T_KV_BYTES);
-#pragma unroll
-                    for (int k = 0; k < TKV / 16; k++)
-                        tc_mma_f16_ts(tO, tP + k * 8, dv + k * (2048 >> 4), IDESC_O, (i | k) != 0);
-                    tc_commit(bar(B_ODONE + w));
-                    tc_commit(bar(B_KVEMPTY + (ki + j) % T_STAGES));
-                    if (!both) tc_commit(bar(B_KVEMPTY + (ki + j) % T_STAGES));
-                    if (!s_next && !(ok = issue_s(i + 1))) break;
-                }
-                if (!ok) return;
-                tc_commit(bar(B_QEMPTY + qs));
-                ki += nt;
-                qi++;
-                cnt += mine;
-                units += mine > 0;
             };
             for (int u = u0; ok && u < n_units; u += u_step) {
-                if (lane == 0) unit(u);
+                unit(u);
                 if (SPLIT && u == u0) {
                     pass_barriers();
                     if (rank > 0) break;
                 }
             }
-        if (lane == 0) {
-            if (!ok) record_err(a.err, abort_flag, kErrWaitFull);
-            tc_commit(bar(B_DRAIN + w));  // every issued MMA has completed before TMEM is released
-            if (!mbar_wait_timed2(bar(B_DRAIN + w), 0)) record_err(a.err, abort_flag, kErrDrain);
+            if (!ok && lane == 0) record_err(a.err, abort_flag, kErrWaitEmpty);
+            if (lt == 0 && !ok) mbar_wait_timed2(bar(B_OWN), oi & 1);  // copies still in flight land before the CTA exits
+            if (lt == 0)
+                for (int i = ki > T_STAGES ? ki - T_STAGES : 0; i < ki; i++)
+                    if (!mbar_wait_timed2(bar(B_KVFULL + i % T_STAGES), (i / T_STAGES) & 1)) break;
+            __syncwarp();
+        } else if (warp == 9 || warp == 14) {
+            // ------------------------------------------------------------------ MMA issuer of warpgroup w
+            const int w = warp == 9 ? 0 : 1;
+            if (SPLIT || lane == 0) {
+                const uint32_t tS = tmem + w * T_WG_COLS, tP = tS + T_P_COL, tO = tS + T_O_COL;
+                int cnt = 0, units = 0;  // key tiles and units of the warpgroup so far
+                int qi = 0, ki = 0;
+                bool ok = true;
+                auto unit = [&](int u) {
+                    find_unit(u);
+                    const int nt = un.tiles(), mine = un.tiles_of(w);
+                    if (nt == 0) return;
+                    const int step = un.mode == kPacked ? 2 : 1, first = un.mode == kPacked ? w : 0;  // its key tiles
+                    const int qs = qi % T_QSLOTS;
+                    if (!(ok = mbar_wait(bar(B_QFULL + qs), (qi / T_QSLOTS) & 1, abort_flag))) return;
+                    const uint64_t dq = smem_desc_k128(smem_u32(sQ + qs * 2 * T_QT_BYTES) + (un.mode == kPacked ? 0 : w * T_QT_BYTES));
+                    auto kv_addr = [&](int j) { return smem_u32(sKV + ((ki + j) % T_STAGES) * 2 * T_KV_BYTES); };
+                    auto kv_ready = [&](int j) {
+                        return mbar_wait(bar(B_KVFULL + (ki + j) % T_STAGES), ((ki + j) / T_STAGES) & 1, abort_flag);
+                    };
+                    // S of its i-th tile, once the softmax has read the one before
+                    auto issue_s = [&](int i) {
+                        const int c = cnt + i;
+                        if (!kv_ready(first + i * step)) return false;
+                        if (c > 0 && !mbar_wait(bar(B_SFREE + w), (c - 1) & 1, abort_flag)) return false;
+                        tc_fence_after();
+                        const uint64_t dk = smem_desc_k128(kv_addr(first + i * step));
+#pragma unroll
+                        for (int k = 0; k < 4; k++) tc_mma_f16(tS, dq + 2 * k, dk + 2 * k, IDESC_S, k != 0);
+                        tc_commit(bar(B_SFULL + w));
+                        return true;
+                    };
+                    const bool both = un.mode != kPacked && un.q_tiles() == 2;  // the other issuer's MMAs read the tiles, too
+                    if (mine > 0) ok = issue_s(0);
+                    for (int i = 0; i < mine && ok; i++) {
+                        const int j = first + i * step, c = cnt + i;
+                        // the next S computes while the softmax works on tile i; where its keys are late, P V goes first (it
+                        // frees a stage that they may be waiting for)
+                        bool s_next = i + 1 == mine;
+                        const uint64_t t0 = globaltimer_ns();
+                        while (true) {
+                            if (!s_next && mbar_test(bar(B_KVFULL + (ki + j + step) % T_STAGES), ((ki + j + step) / T_STAGES) & 1)) {
+                                if (!(ok = issue_s(i + 1))) break;
+                                s_next = true;
+                            }
+                            if (mbar_try_wait_brief(bar(B_PFULL + w), c & 1)) break;
+                            if (*abort_flag || globaltimer_ns() - t0 > kWaitLimitNs) {
+                                ok = false;
+                                break;
+                            }
+                        }
+                        if (!ok) break;
+                        // the first P V of a unit overwrites O: the unit before must have been read
+                        if (i == 0 && units > 0 && !(ok = mbar_wait(bar(B_OFREE + w), (units - 1) & 1, abort_flag))) break;
+                        tc_fence_after();
+                        const uint64_t dv = smem_desc_k128(kv_addr(j) + T_KV_BYTES);
+#pragma unroll
+                        for (int k = 0; k < TKV / 16; k++)
+                            tc_mma_f16_ts(tO, tP + k * 8, dv + k * (2048 >> 4), IDESC_O, (i | k) != 0);
+                        tc_commit(bar(B_ODONE + w));
+                        tc_commit(bar(B_KVEMPTY + (ki + j) % T_STAGES));
+                        if (!both) tc_commit(bar(B_KVEMPTY + (ki + j) % T_STAGES));
+                        if (!s_next && !(ok = issue_s(i + 1))) break;
+                    }
+                    if (!ok) return;
+                    tc_commit(bar(B_QEMPTY + qs));
+                    ki += nt;
+                    qi++;
+                    cnt += mine;
+                    units += mine > 0;
+                };
+                for (int u = u0; ok && u < n_units; u += u_step) {
+                    if (lane == 0) unit(u);
+                    if (SPLIT && u == u0) {
+                        pass_barriers();
+                        if (rank > 0) break;
+                    }
+                }
+                if (lane == 0) {
+                    if (!ok) record_err(a.err, abort_flag, kErrWaitFull);
+                    tc_commit(bar(B_DRAIN + w));  // every issued MMA has completed before TMEM is released
+                    if (!mbar_wait_timed2(bar(B_DRAIN + w), 0)) record_err(a.err, abort_flag, kErrDrain);
+                }
+            }
+            __syncwarp();
+        } else if (SPLIT) {  // the warp without a role
+            if (u0 < n_units) pass_barriers();
         }
-        }
-        __syncwarp();
-    } else if (SPLIT) {  // the warp without a role
-        if (u0 < n_units) pass_barriers();
-    }
     } else {
         asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(T_SOFTMAX_REGS));
         // ------------------------------------------------------------------ softmax
@@ -1129,62 +1128,62 @@ __global__ void __launch_bounds__(T_THREADS, 1)
             }
             if (SPLIT && !split && !mine) continue;
             if (!SPLIT || (ok && mine)) {
-            uint32_t o[64];
-            tmem_ld32(tO, *reinterpret_cast<uint32_t(*)[32]>(o));
-            tmem_ld32(tO + 32, *reinterpret_cast<uint32_t(*)[32]>(o + 32));
-            tc_wait_ld();
-            if (packed) {
-                ok = __all_sync(D1_FULL_MASK, mbar_wait(bar(B_JOIN), njoin & 1, abort_flag));
-                if (!SPLIT && !ok) break;
-                tc_fence_after();
-                njoin++;
-                const float m1 = join[2 * row], l1 = join[2 * row + 1];
-                if (un.tiles_of(1) > 0) {
-                    const float both = fmaxf(m, m1), f0 = ex2(m - both), f1 = ex2(m1 - both);
-                    uint32_t o1[64];
-                    tmem_ld32(tO + T_WG_COLS, *reinterpret_cast<uint32_t(*)[32]>(o1));
-                    tmem_ld32(tO + T_WG_COLS + 32, *reinterpret_cast<uint32_t(*)[32]>(o1 + 32));
-                    tc_wait_ld();
-#pragma unroll
-                    for (int i = 0; i < 64; i++)
-                        o[i] = __float_as_uint(__uint_as_float(o[i]) * f0 + __uint_as_float(o1[i]) * f1);
-                    l = l * f0 + l1 * f1;
-                    m = both;
-                }
-            }
-            tc_fence_before();
-            __syncwarp();
-            if (lane == 0) {
-                mbar_arrive(bar(B_OFREE + w));
+                uint32_t o[64];
+                tmem_ld32(tO, *reinterpret_cast<uint32_t(*)[32]>(o));
+                tmem_ld32(tO + 32, *reinterpret_cast<uint32_t(*)[32]>(o + 32));
+                tc_wait_ld();
                 if (packed) {
-                    if (un.tiles_of(1) > 0) mbar_arrive(bar(B_OFREE + 1));
-                    mbar_arrive(bar(B_JOINED));
+                    ok = __all_sync(D1_FULL_MASK, mbar_wait(bar(B_JOIN), njoin & 1, abort_flag));
+                    if (!SPLIT && !ok) break;
+                    tc_fence_after();
+                    njoin++;
+                    const float m1 = join[2 * row], l1 = join[2 * row + 1];
+                    if (un.tiles_of(1) > 0) {
+                        const float both = fmaxf(m, m1), f0 = ex2(m - both), f1 = ex2(m1 - both);
+                        uint32_t o1[64];
+                        tmem_ld32(tO + T_WG_COLS, *reinterpret_cast<uint32_t(*)[32]>(o1));
+                        tmem_ld32(tO + T_WG_COLS + 32, *reinterpret_cast<uint32_t(*)[32]>(o1 + 32));
+                        tc_wait_ld();
+#pragma unroll
+                        for (int i = 0; i < 64; i++)
+                            o[i] = __float_as_uint(__uint_as_float(o[i]) * f0 + __uint_as_float(o1[i]) * f1);
+                        l = l * f0 + l1 * f1;
+                        m = both;
+                    }
                 }
-            }
-            if (split) {  // unscaled sums, for the cluster
-                if (there) {
-                    float* dst = part_o + (w * TQ + row) * R_LD;
-#pragma unroll
-                    for (int i = 0; i < 16; i++)
-                        *reinterpret_cast<float4*>(dst + 4 * i) =
-                            make_float4(__uint_as_float(o[4 * i]), __uint_as_float(o[4 * i + 1]), __uint_as_float(o[4 * i + 2]),
-                                        __uint_as_float(o[4 * i + 3]));
-                    part_ml[2 * (w * TQ + row)] = m;
-                    part_ml[2 * (w * TQ + row) + 1] = l;
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) {
+                    mbar_arrive(bar(B_OFREE + w));
+                    if (packed) {
+                        if (un.tiles_of(1) > 0) mbar_arrive(bar(B_OFREE + 1));
+                        mbar_arrive(bar(B_JOINED));
+                    }
                 }
-            } else {
-            const float il = 1.f / l;
-            uint32_t oh[32];
+                if (split) {  // unscaled sums, for the cluster
+                    if (there) {
+                        float* dst = part_o + (w * TQ + row) * R_LD;
 #pragma unroll
-            for (int i = 0; i < 32; i++) oh[i] = pack_h2(__uint_as_float(o[2 * i]) * il, __uint_as_float(o[2 * i + 1]) * il);
-            if (a.lse && there) a.lse[(size_t)h * a.lse_ld + grow] = (m + log2f(l)) * kLn2;
-            if (there) {
+                        for (int i = 0; i < 16; i++)
+                            *reinterpret_cast<float4*>(dst + 4 * i) =
+                                make_float4(__uint_as_float(o[4 * i]), __uint_as_float(o[4 * i + 1]), __uint_as_float(o[4 * i + 2]),
+                                            __uint_as_float(o[4 * i + 3]));
+                        part_ml[2 * (w * TQ + row)] = m;
+                        part_ml[2 * (w * TQ + row) + 1] = l;
+                    }
+                } else {
+                    const float il = 1.f / l;
+                    uint32_t oh[32];
 #pragma unroll
-                for (int i = 0; i < 8; i++)
-                    *reinterpret_cast<uint4*>(a.O + grow * a.ldo + h * 64 + i * 8) =
-                        make_uint4(oh[4 * i], oh[4 * i + 1], oh[4 * i + 2], oh[4 * i + 3]);
-            }
-            }
+                    for (int i = 0; i < 32; i++) oh[i] = pack_h2(__uint_as_float(o[2 * i]) * il, __uint_as_float(o[2 * i + 1]) * il);
+                    if (a.lse && there) a.lse[(size_t)h * a.lse_ld + grow] = (m + log2f(l)) * kLn2;
+                    if (there) {
+#pragma unroll
+                        for (int i = 0; i < 8; i++)
+                            *reinterpret_cast<uint4*>(a.O + grow * a.ldo + h * 64 + i * 8) =
+                                make_uint4(oh[4 * i], oh[4 * i + 1], oh[4 * i + 2], oh[4 * i + 3]);
+                }
+                }
             }
             if (split) {
                 fence_async_smem_cta();  // (the next unit's copies come to the same place)
@@ -1313,7 +1312,7 @@ __global__ void __launch_bounds__(256) k_kv4_mass_rows(const Kv4Args a) {
                 for (int e = 0; e < n_peers; e++) {
                     const D1Kv4Seq& p = a.seqs[peers[e]];
                     const int q_start = p.q_start, q_len = p.q_len;
-                    if (p.k4 != s.k4 || p.ext_len != s.ext_len || p.ext_cap != s.ext_cap ||
+                    if (!kv4_seq_ok(p) || p.k4 != s.k4 || p.ext_len != s.ext_len || p.ext_cap != s.ext_cap ||
                         !rows_ok(q_start, q_len, a.q_rows)) {
                         if (tid == 0) atomicExch(a.err, kErrTable);
                         continue;
@@ -1328,8 +1327,11 @@ __global__ void __launch_bounds__(256) k_kv4_mass_rows(const Kv4Args a) {
                             const uint4* src = reinterpret_cast<const uint4*>(a.Q + (size_t)q * a.ldq + h * 64 + 16 * t);
                             x0 = __ldg(src);
                             x1 = __ldg(src + 1);
-                            const float v = __ldg(a.lse + (size_t)h * a.lse_ld + q) * kLog2e;
-                            lse = v == -INFINITY ? INFINITY : v;
+                            lse = __ldg(a.lse + (size_t)h * a.lse_ld + q) * kLog2e;
+                            if (lse == -INFINITY) {  // adds nothing, whatever the row holds
+                                lse = INFINITY;
+                                x0 = x1 = make_uint4(0, 0, 0, 0);
+                            }
                         }
                         const float l0 = __shfl_sync(D1_FULL_MASK, lse, 8 * t), l1 = __shfl_sync(D1_FULL_MASK, lse, 8 * t + 4);
 #pragma unroll
@@ -1369,10 +1371,13 @@ __global__ void __launch_bounds__(256) k_kv4_mass_rows(const Kv4Args a) {
 //   0-15       four warpgroups share every tile (two of its eight 32-column pieces each): S from TMEM, where the next
 //              tile's S is computed meanwhile, exp2(s * scale - lse), summed in fp32; one pair of exponentials in eight on
 //              the FMA pipe. At the unit's end three pass their sums to the first through shared memory. (Two documents of
-//              2048 rows over 8192 keys: 91 us; 98 with two warpgroups and the next piece's load on its way, 97 with
-//              both pieces loaded at once, 93 without the FMA pipe, 94 and 99 with a quarter and three eighths there)
+//              2048 rows over 8192 keys: 77 us. Compared while it took 91: 98 with two warpgroups and the next piece's
+//              load on its way, 97 with both pieces loaded at once, 93 without the FMA pipe, 94 and 99 with a quarter and
+//              three eighths there)
 //   16, 18, 19 loaders: the keys' codes, expanded; query tiles by TMA from a view of [row][head][64], always whole; the
-//              columns' -lse (behind the end and for rows without keys: -inf, which adds 0 whatever the score)
+//              columns' -lse (behind the end and for rows that add nothing: -inf). Such rows are wiped out in shared
+//              memory, so that a NaN in padding stays there (masking their scores instead cost the exponentials' loop its
+//              schedule: 85 us)
 //   17         TMEM, and the MMAs from one thread
 constexpr int MQ = 256, MK = 128, M_STAGES = 4, M_LOADERS = 3, M_WGS = 4, M_THREADS = 128 * M_WGS + 128;
 constexpr int M_Q_BYTES = MQ * 128, M_K_BYTES = MK * 128;
@@ -1385,79 +1390,109 @@ enum : int {
     MB_SFREE = MB_SFULL + 2,         // [buffer] (16 warps)
     MB_SUM = MB_SFREE + 2,           // [2] the other warpgroups' sums are in shared memory (12 warps)
     MB_SUMFREE = MB_SUM + 2,         // [2] (4 warps)
-    MB_DRAIN = MB_SUMFREE + 2,
+    MB_LANDED = MB_SUMFREE + 2,      // [loader] a query tile with rows to wipe out
+    MB_DRAIN = MB_LANDED + M_LOADERS,
     M_NBARS = MB_DRAIN + 1
 };
-constexpr int M_SMEM = 2 * M_K_BYTES + M_STAGES * (M_Q_BYTES + MQ * 4) + 2 * (M_WGS - 1) * MK * 4 + M_NBARS * 8 + 16;
-static_assert(M_SMEM <= 232448, "shared memory of the tcgen05 mass kernel");
 
-// The units of a CTA and, within each, its query tiles, walked alike by every warp (all lanes together). The sequences
-// that share a mass array belong to the first of them.
-struct MassWalk {
-    D1Kv4Seq s;       // the unit's first sequence
-    int u, sq, g, kt, max_kt, kv_heads;
-    int peer, q_start, q_len, row0;  // the tile: rows row0 .. row0 + rows() - 1 of sequence `peer`, every head of g
-    int block;        // rows of a whole tile
-    bool at_unit;
+// What the roles need of up to M_SEQS sequences, in shared memory: units (key tiles of 128 of the caches that belong to a
+// sequence, for each kv head) before each, query rows, cached keys, and the next sequence of the same mass array. The
+// sequences that share a mass array belong to the first of them, whose cache they must share, too.
+constexpr int M_SEQS = 256;
+struct MassTable {
+    const float* mass[M_SEQS];
+    int cum[M_SEQS + 1], q_start[M_SEQS], q_len[M_SEQS], ext_len[M_SEQS], next[M_SEQS];
+};
 
-    __device__ MassWalk(const Kv4Args& a) : u(blockIdx.x), at_unit(false) {
-        max_kt = a.n_blocks;
-        kv_heads = a.heads / a.group;
-        block = MQ / a.group;
+constexpr int M_SMEM = 2 * M_K_BYTES + M_STAGES * (M_Q_BYTES + MQ * 4) + 2 * (M_WGS - 1) * MK * 4 + (int)sizeof(MassTable) +
+                       M_NBARS * 8 + 16;
+static_assert(M_SMEM <= 232448 && sizeof(MassTable) % 8 == 0, "shared memory of the tcgen05 mass kernel");
+
+// Fills the table; ends with a barrier. Every thread of the CTA takes part.
+__device__ __forceinline__ void build_mass_table(const Kv4Args& a, MassTable& tb, int n) {
+    const int tid = threadIdx.x, kv_heads = a.heads / a.group;
+    for (int i = tid; i < n; i += blockDim.x) {
+        const D1Kv4Seq& s = a.seqs[i];
+        tb.mass[i] = s.mass;
+        tb.q_start[i] = s.q_start;
+        tb.q_len[i] = s.q_len;
+        tb.ext_len[i] = s.ext_len;
     }
-    // The next sequence at or after j with this mass array, or n_seqs.
-    __device__ int find(const Kv4Args& a, int j, const float* mass, int end) const {
-        const int lane = threadIdx.x & 31;
-        for (; j < end; j += 32) {
-            const uint32_t v = __ballot_sync(D1_FULL_MASK, j + lane < end && a.seqs[min(j + lane, end - 1)].mass == mass);
-            if (v) return j + __ffs(v) - 1;
-        }
-        return end;
-    }
-    __device__ bool next_unit(const Kv4Args& a) {
-        while (true) {
-            if (at_unit) {
-                kt += max_kt;  // a cache longer than max_len comes round again
-            } else {
-                if (u >= a.n_seqs * kv_heads * max_kt) return false;
-                kt = u % max_kt;
-                g = u / max_kt % kv_heads;
-                sq = u / max_kt / kv_heads;
-                s = a.seqs[sq];
-                at_unit = true;
-                if (!s.mass) {
-                    s.ext_len = 0;
-                } else if (!kv4_seq_ok(s)) {
-                    if ((threadIdx.x & 31) == 0) atomicExch(a.err, kErrTable);
-                    s.ext_len = 0;
-                } else if (find(a, 0, s.mass, sq) < sq) {
-                    s.ext_len = 0;  // another sequence's
+    __syncthreads();
+    for (int i = tid; i < M_SEQS; i += blockDim.x) {
+        int units = 0;
+        if (i < n && tb.mass[i]) {
+            const D1Kv4Seq s = a.seqs[i];
+            bool owner = true;
+            int first = i, next = n;
+            for (int j = 0; j < i && owner; j++)
+                if (tb.mass[j] == s.mass) {
+                    owner = false;
+                    first = j;
                 }
+            for (int j = n - 1; j > i; j--)
+                if (tb.mass[j] == s.mass) next = j;
+            tb.next[i] = next;
+            const D1Kv4Seq& o = a.seqs[first];
+            const bool bad = !kv4_seq_ok(s);
+            if (bad || !rows_ok(s.q_start, s.q_len, a.q_rows) ||
+                (!owner && (o.k4 != s.k4 || o.ext_len != s.ext_len || o.ext_cap != s.ext_cap))) {
+                atomicExch(a.err, kErrTable);
+                tb.q_len[i] = -1;  // its rows do not count
             }
-            if ((long long)kt * MK < s.ext_len) {
-                peer = sq - 1;
-                q_len = row0 = 0;
-                return true;
-            }
-            u += gridDim.x;
-            at_unit = false;
+            if (owner && !bad) units = (s.ext_len + MK - 1) / MK * kv_heads;
         }
+        tb.cum[i + 1] = units;
     }
-    __device__ bool next_tile(const Kv4Args& a) {
+    if (tid == 0) tb.cum[0] = 0;
+    __syncthreads();
+    if (tid < 32) {
+        constexpr int PER = M_SEQS / 32;
+        int v[PER], sum = 0;
+#pragma unroll
+        for (int i = 0; i < PER; i++) sum += v[i] = tb.cum[1 + tid * PER + i];
+        int upto = sum;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int x = __shfl_up_sync(D1_FULL_MASK, upto, o);
+            if (tid >= o) upto += x;
+        }
+        upto -= sum;
+#pragma unroll
+        for (int i = 0; i < PER; i++) tb.cum[1 + tid * PER + i] = upto += v[i];
+    }
+    __syncthreads();
+}
+
+// The units of a CTA and, within each, its query tiles, walked alike by every role: unit u is a sequence, a tile of its
+// keys and a kv head, the heads fastest.
+struct MassWalk {
+    int sq, g, kt;
+    int peer, q_start, q_len, row0;  // the tile: rows row0 .. row0 + rows() - 1 of sequence `peer`, every head of g
+    int block, kv_heads;             // rows of a whole tile
+    bool any;                        // a sequence counted, be it without rows
+    int entry;
+
+    __device__ MassWalk(const Kv4Args& a) : block(MQ / a.group), kv_heads(a.heads / a.group), entry(0) {}
+    __device__ void find(const MassTable& tb, int u) {  // u at or behind the one before
+        while (tb.cum[entry + 1] <= u) entry++;
+        sq = entry;
+        const int rest = u - tb.cum[entry];
+        kt = rest / kv_heads;
+        g = rest - kt * kv_heads;
+        peer = -1;
+        q_len = row0 = 0;
+        any = false;
+    }
+    __device__ bool next_tile(const MassTable& tb, int n) {
         row0 += block;
         while (row0 >= q_len) {
-            peer = find(a, peer + 1, s.mass, a.n_seqs);
-            if (peer >= a.n_seqs) return false;
-            const D1Kv4Seq& p = a.seqs[peer];
-            q_start = p.q_start;
-            q_len = p.q_len;
+            peer = peer < 0 ? sq : tb.next[peer];
+            if (peer >= n) return false;
+            q_start = tb.q_start[peer];
+            q_len = tb.q_len[peer];
             row0 = 0;
-            if (p.k4 != s.k4 || p.ext_len != s.ext_len || p.ext_cap != s.ext_cap || !rows_ok(q_start, q_len, a.q_rows)) {
-                if ((threadIdx.x & 31) == 0) atomicExch(a.err, kErrTable);
-                q_len = 0;
-            } else if (q_len > 0) {
-                return true;
-            }
+            any |= q_len >= 0;
         }
         return true;
     }
@@ -1470,7 +1505,8 @@ __global__ void __launch_bounds__(M_THREADS, 1) k_kv4_mass_tc(const __grid_const
     uint8_t* sQ = sK + 2 * M_K_BYTES;                                              // [stage][256 columns]
     float* sL = reinterpret_cast<float*>(sQ + M_STAGES * M_Q_BYTES);               // [stage][256]: -lse in log2
     float* sSum = sL + M_STAGES * MQ;                                              // [2][warpgroup - 1][128]
-    uint64_t* bars = reinterpret_cast<uint64_t*>(sSum + 2 * (M_WGS - 1) * MK);
+    MassTable& tb = *reinterpret_cast<MassTable*>(sSum + 2 * (M_WGS - 1) * MK);
+    uint64_t* bars = reinterpret_cast<uint64_t*>(&tb + 1);
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + M_NBARS);
     volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
     auto bar = [&](int i) { return smem_u32(bars + i); };
@@ -1494,6 +1530,7 @@ __global__ void __launch_bounds__(M_THREADS, 1) k_kv4_mass_tc(const __grid_const
             mbar_init(bar(MB_QFULL + i), 32);
             mbar_init(bar(MB_QEMPTY + i), 1 + 4 * M_WGS);
         }
+        for (int i = 0; i < M_LOADERS; i++) mbar_init(bar(MB_LANDED + i), 1);
         mbar_init(bar(MB_DRAIN), 1);
         *abort_flag = 0;
         fence_mbar_init();
@@ -1507,6 +1544,9 @@ __global__ void __launch_bounds__(M_THREADS, 1) k_kv4_mass_tc(const __grid_const
     tc_fence_after();
     const uint32_t tmem = *tmem_slot;
     pdl_entry();  // barriers and TMEM are set up; global memory is touched only after this
+    const int n = a.n_seqs;
+    build_mass_table(a, tb, n);
+    const int n_units = tb.cum[M_SEQS];
     MassWalk wk(a);
     int nu = 0, ti = 0;  // units and tiles so far
     bool ok = true;
@@ -1517,10 +1557,14 @@ __global__ void __launch_bounds__(M_THREADS, 1) k_kv4_mass_tc(const __grid_const
     if (warp == M_WARP - 1 || warp > M_WARP) {
         // ------------------------------------------------------------------ loaders
         const int lw = warp < M_WARP ? 0 : warp - M_WARP, lt = lw * 32 + lane;
+        int wiped = 0;  // tiles with rows wiped out so far
         const int inv = (65536 + a.group - 1) / a.group;  // c / group = c * inv >> 16 for c < 256: off by less than 1 / group
-        for (; ok && wk.next_unit(a); nu++) {
-            const uint8_t* k4 = wk.s.k4 + (size_t)wk.g * wk.s.ext_cap * 32;
-            const uint16_t* kp = reinterpret_cast<const uint16_t*>(wk.s.kp) + (size_t)wk.g * wk.s.ext_cap;
+        for (int u = blockIdx.x; ok && u < n_units; u += gridDim.x, nu++) {
+            wk.find(tb, u);
+            const size_t at = (size_t)wk.g * a.seqs[wk.sq].ext_cap;
+            const uint8_t* k4 = a.seqs[wk.sq].k4 + at * 32;
+            const uint16_t* kp = reinterpret_cast<const uint16_t*>(a.seqs[wk.sq].kp) + at;
+            const int ext_len = tb.ext_len[wk.sq];
             constexpr int PIECES = (2 * MK + 32 * M_LOADERS - 1) / (32 * M_LOADERS);
             uint4 piece[PIECES];
             uint32_t par[PIECES];
@@ -1529,7 +1573,7 @@ __global__ void __launch_bounds__(M_THREADS, 1) k_kv4_mass_tc(const __grid_const
                 const int c = lt + i * 32 * M_LOADERS, key = wk.kt * MK + (c >> 1);
                 piece[i] = make_uint4(0, 0, 0, 0);
                 par[i] = 0;  // step 0: zeros
-                if (c < 2 * MK && key < wk.s.ext_len) {
+                if (c < 2 * MK && key < ext_len) {
                     piece[i] = __ldg(reinterpret_cast<const uint4*>(k4 + (size_t)key * 32) + (c & 1));
                     par[i] = __ldg(kp + key);
                 }
@@ -1554,7 +1598,7 @@ __global__ void __launch_bounds__(M_THREADS, 1) k_kv4_mass_tc(const __grid_const
             }
             fence_async_smem_cta();
             mbar_arrive(bar(MB_KFULL + (nu & 1)));
-            for (; wk.next_tile(a); ti++) {
+            for (; wk.next_tile(tb, n); ti++) {
                 if (ti % M_LOADERS != lw) continue;  // the warps take the tiles in turn: their latencies overlap
                 const int st = ti % M_STAGES, cols = wk.rows() * a.group, pad = (cols + 31) & ~31;
                 const int row = wk.q_start + wk.row0, h0 = wk.g * a.group;
@@ -1565,28 +1609,45 @@ __global__ void __launch_bounds__(M_THREADS, 1) k_kv4_mass_tc(const __grid_const
                     l[i] = -INFINITY;
                     if (c < cols) l[i] = __ldg(a.lse + (size_t)(h0 + c - r * a.group) * a.lse_ld + row + r);
                 }
+                bool wipe = false;  // rows that add nothing, whatever they hold: zeros in their place
+#pragma unroll
+                for (int i = 0; i < MQ / 32; i++) wipe |= lane + 32 * i < cols && l[i] == -INFINITY;
+                wipe = __any_sync(D1_FULL_MASK, wipe);
                 if (!(ok = wait(MB_QEMPTY + st, ((ti / M_STAGES) & 1) ^ 1))) break;
 #pragma unroll
                 for (int i = 0; i < MQ / 32; i++)
                     if (32 * i < pad) sL[st * MQ + lane + 32 * i] = l[i] == -INFINITY ? -INFINITY : -l[i] * kLog2e;
+                const uint32_t full = bar(MB_QFULL + st), landed = wipe ? bar(MB_LANDED + lw) : full;
                 if (lane == 0) {
-                    mbar_arrive_expect_tx(bar(MB_QFULL + st), wk.block * a.group * 128);
-                    tma_load_3d(smem_u32(sQ + st * M_Q_BYTES), &tmQp, 0, h0, row, bar(MB_QFULL + st));
-                } else {
-                    mbar_arrive(bar(MB_QFULL + st));
+                    mbar_arrive_expect_tx(landed, wk.block * a.group * 128);
+                    tma_load_3d(smem_u32(sQ + st * M_Q_BYTES), &tmQp, 0, h0, row, landed);
                 }
+                if (wipe) {
+                    if (!(ok = wait(MB_LANDED + lw, wiped & 1))) break;
+                    wiped++;
+#pragma unroll
+                    for (int i = 0; i < MQ / 32; i++)
+                        if (lane + 32 * i < cols && l[i] == -INFINITY)
+                            for (int q = 0; q < 8; q++)
+                                *reinterpret_cast<uint4*>(sQ + st * M_Q_BYTES + (lane + 32 * i) * 128 + q * 16) =
+                                    make_uint4(0, 0, 0, 0);
+                    fence_async_smem_cta();
+                }
+                if (wipe || lane != 0) mbar_arrive(full);
             }
         }
         if (!ok && lane == 0) record_err(a.err, abort_flag, kErrWaitEmpty);
+        if (lane == 0 && !ok) mbar_wait_timed2(bar(MB_LANDED + lw), wiped & 1);
         if (lane == 0)  // TMA copies still in flight (only after an abort) land before the CTA exits
             for (int i = ti > M_STAGES ? ti - M_STAGES : 0; i < ti; i++)
                 if (!mbar_wait_timed2(bar(MB_QFULL + i % M_STAGES), (i / M_STAGES) & 1)) break;
     } else if (warp == M_WARP) {
         // ------------------------------------------------------------------ MMA issuer (lane 0)
-        for (; ok && wk.next_unit(a); nu++) {
+        for (int u = blockIdx.x; ok && u < n_units; u += gridDim.x, nu++) {
+            wk.find(tb, u);
             if (!(ok = wait(MB_KFULL + (nu & 1), (nu >> 1) & 1))) break;
             const uint32_t k_addr = smem_u32(sK + (nu & 1) * M_K_BYTES);
-            for (; wk.next_tile(a); ti++) {
+            for (; wk.next_tile(tb, n); ti++) {
                 const int st = ti % M_STAGES, w = ti & 1, pad = (wk.rows() * a.group + 31) & ~31;
                 if (!(ok = wait(MB_QFULL + st, (ti / M_STAGES) & 1))) break;
                 if (ti > 1 && !(ok = wait(MB_SFREE + w, ((ti >> 1) - 1) & 1))) break;
@@ -1616,13 +1677,12 @@ __global__ void __launch_bounds__(M_THREADS, 1) k_kv4_mass_tc(const __grid_const
         const int wg = warp >> 2, row = (warp & 3) * 32 + lane;
         const uint32_t tS = tmem + 32 * wg + ((uint32_t)((warp & 3) * 32) << 16);
         const uint64_t sc2 = f2_pack(a.scale_log2, a.scale_log2);
-        for (; ok && wk.next_unit(a); nu++) {
+        for (int u = blockIdx.x; ok && u < n_units; u += gridDim.x, nu++) {
+            wk.find(tb, u);
             uint64_t sum[4];
 #pragma unroll
             for (int e = 0; e < 4; e++) sum[e] = f2_pack(0.f, 0.f);
-            bool any = false;
-            for (; wk.next_tile(a); ti++) {
-                any = true;
+            for (; wk.next_tile(tb, n); ti++) {
                 const int st = ti % M_STAGES, b = ti & 1, pad = (wk.rows() * a.group + 31) & ~31;
                 if (!(ok = wait(MB_QFULL + st, (ti / M_STAGES) & 1))) break;  // the lse
                 if (!(ok = wait(MB_SFULL + b, (ti >> 1) & 1))) break;
@@ -1683,8 +1743,8 @@ __global__ void __launch_bounds__(M_THREADS, 1) k_kv4_mass_tc(const __grid_const
                 __syncwarp();
                 if (lane == 0) mbar_arrive(bar(MB_SUMFREE + slot));
                 const long long key = (long long)wk.kt * MK + row;
-                if (any && key < wk.s.ext_len) {
-                    float* m = wk.s.mass + (size_t)wk.g * wk.s.ext_cap + key;
+                if (wk.any && key < tb.ext_len[wk.sq]) {
+                    float* m = a.seqs[wk.sq].mass + (size_t)wk.g * a.seqs[wk.sq].ext_cap + key;
                     *m = a.accumulate ? *m + all : all;
                 }
             }
@@ -1811,9 +1871,8 @@ int launch_mass_tc(Kv4Args& a, int max_len, cudaStream_t st) {
     if (!smem_opt_in(k_kv4_mass_tc, M_SMEM, &done)) return -1;
     const int sms = sm_count();
     if (!sms) return -1;
-    a.n_blocks = max_len > 0 ? (max_len - 1) / MK + 1 : 1;
-    const long long units = (long long)a.n_seqs * a.n_blocks * (a.heads / a.group);
-    if (units > 0x7fffffffLL - 4096) return -1;
+    // no more CTAs than units, were every sequence's cache its own and max_len long
+    const long long units = (long long)a.n_seqs * (max_len > 0 ? (max_len - 1) / MK + 1 : 1) * (a.heads / a.group);
     CUtensorMap tq;
     if (!packed_tmap(&tq, a, MQ)) return -1;
     launch_pdl(k_kv4_mass_tc, (int)(units < sms ? units : sms), M_THREADS, M_SMEM, st, tq, a);
@@ -1855,6 +1914,8 @@ extern "C" int d1_flash_attn_kv4(const d1_half* Q, int ldq, const d1_half* K, co
     a.scale_log2 = scale * kLog2e;
     if (!a.err) return -1;
     const int kv_heads = heads / group;
+    // the tcgen05 form above 64 packed rows. 16 sequences over 1200 keys: 66 rows 20 us and 39 on mma.sync, 64 rows 20 and
+    // 21, 32 rows 20 and 17; over 8000 keys: 77 and 198, 75 and 103, 75 and 55
     if ((long long)max_q * group > 64) return launch_tc(a, max_q, max_keys, st);
     const long long rows = (long long)max_q * group;
     return rows <= 8 ? launch_rows<1>(a, max_q, max_keys, kv_heads, st)
@@ -1884,9 +1945,11 @@ extern "C" int d1_kv4_mass(const d1_half* Q, int ldq, const float* lse, int lse_
     a.accumulate = accumulate;
     a.scale_log2 = scale * kLog2e;
     if (!a.err) return -1;
-    if ((long long)max_q * group > 64 && group <= MQ && q_rows > 0) return launch_mass_tc(a, max_len, st);
-    int x = (max_len + M_KEYS - 1) / M_KEYS;
+    // the tcgen05 form above 64 packed rows a sequence, where its table holds the sequences. 16 caches of 1200 keys: 96
+    // rows 18 us and 25 on mma.sync, 64 rows 18 and 19, 48 rows 18 and 16; of 8000 keys: 82 and 84, 80 and 64
+    if ((long long)max_q * group > 64 && group <= MQ && q_rows > 0 && n_seqs <= M_SEQS) return launch_mass_tc(a, max_len, st);
+    long long x = ((long long)max_len + M_KEYS - 1) / M_KEYS;
     x = x < 1 ? 1 : x > 65536 ? 65536 : x;
-    launch_pdl(k_kv4_mass_rows, dim3(x, heads / group, n_seqs < 65535 ? n_seqs : 65535), 256, 0, st, a);
+    launch_pdl(k_kv4_mass_rows, dim3((unsigned)x, heads / group, n_seqs < 65535 ? n_seqs : 65535), 256, 0, st, a);
     return (int)cudaGetLastError();
 }

@@ -346,9 +346,10 @@ int d1_gemm_noalloc_error(void);
  * and stands for (code - zero) * step, which fp16 holds exactly: |x - value| <= step / 2 (step, beside 65504). A vector
  * with a NaN or an infinity reads as NaN in every element.
  *
- * ext_cap must be a multiple of 8 and the four pointers 16-byte aligned; ext_cap = 0 with null pointers is a sequence
- * without a cache. The tables below are read on the device when the kernel runs. An entry that breaks these rules or
- * reaches outside the rows that the call names is skipped, its outputs left as they were, and d1_kv4_error() tells.
+ * ext_cap must be a multiple of 8, at most 2^30, and the four pointers 16-byte aligned; ext_cap = 0 with null pointers
+ * is a sequence without a cache. The tables below are read on the device when the kernel runs. An entry that breaks
+ * these rules or reaches outside the rows that the call names is skipped, its outputs left as they were, and
+ * d1_kv4_error() tells.
  * The launchers keep no state and no workspace: calls on several streams, and captured ones, do not affect each other
  * as long as what they write does not overlap. */
 typedef struct D1Kv4Seq {
@@ -401,19 +402,21 @@ int d1_kv4_load(const D1Kv4Seq* seqs, int n_seqs, int max_rows, int kv_heads, d1
 /* extension — d1_flash_attn over 4-bit caches: for every sequence, row q and head h,
  *   O[q] = softmax(scale * Q[q] K^T) V over the keys [cached | own], kv head h / group, fp32 softmax
  * and, with lse != NULL, lse[h * lse_ld + row] = ln(sum exp(scale * Q[q] K^T)) in fp32. Rows without any key get O = 0
- * and lse = -inf. Bidirectional, as d1_flash_attn. max_q, max_keys: the longest q_len and the longest ext_len + kv_len,
- * by which the kernel and the split over the keys are chosen (results differ only by rounding; lengths beyond them are
- * computed all the same). q_rows / kv_rows: rows of Q and O (lse: q_rows <= lse_ld) and of K and V. Q, K, V, O 16-byte
- * aligned, leading dimensions multiples of 8; K and V may be NULL with kv_rows = 0. scale > 0. */
+ * and lse = -inf. A NaN or an infinity among a row's Q or a sequence's K and V may make every result that it enters
+ * NaN, and none of another sequence. Bidirectional, as d1_flash_attn. max_q, max_keys: the longest q_len and the longest
+ * ext_len + kv_len, by which the kernel and the split over the keys are chosen (results differ only by rounding; lengths
+ * beyond them are computed all the same). q_rows / kv_rows: rows of Q and O (lse: q_rows <= lse_ld) and of K and V. Q,
+ * K, V, O 16-byte aligned, leading dimensions multiples of 8; K and V may be NULL with kv_rows = 0. scale > 0. */
 int d1_flash_attn_kv4(const d1_half* Q, int ldq, const d1_half* K, const d1_half* V, int ldkv, d1_half* O, int ldo,
                       float* lse, int lse_ld, const D1Kv4Seq* seqs, int n_seqs, int max_q, int max_keys, int heads,
                       int group, float scale, int q_rows, int kv_rows, cudaStream_t stream);
 
 /* extension — the attention weight that every cached key received: for every kv head g and key k of a sequence's cache
  *   mass[g][k] (+)= sum over its rows q and the heads h of g of exp(scale * Q[q] . K[k] - lse[h][q])
- * with lse as d1_flash_attn_kv4 gave it (-inf: the row adds nothing). accumulate = 0 overwrites mass[g][0 .. ext_len-1],
- * 1 adds to it. Sequences with the same `mass` must share their cache; their weights are added up in the table's order,
- * always in the same order for the same call. max_q, max_len: the longest q_len and ext_len (see above). */
+ * with lse as d1_flash_attn_kv4 gave it (-inf: the row adds nothing, whatever its Q holds). accumulate = 0 overwrites
+ * mass[g][0 .. ext_len-1], 1 adds to it. Sequences with the same `mass` must share their cache; their weights are added
+ * up in the table's order, always in the same order for the same call. max_q, max_len: the longest q_len and ext_len
+ * (see above). */
 int d1_kv4_mass(const d1_half* Q, int ldq, const float* lse, int lse_ld, const D1Kv4Seq* seqs, int n_seqs, int max_q,
                 int max_len, int heads, int group, float scale, int accumulate, int q_rows, cudaStream_t stream);
 

@@ -321,6 +321,8 @@ CASES = {
     "wide groups": ([2, 40], [300, 777], [2, 40], 2, 8),
     "group of five": ([19, 150], [400, 130], [0, 150], 1, 5),
     "long": ([3, 2], [16384, 5003], [3, 2], 1, 2),
+    "many sequences": ([1 + i % 5 for i in range(300)], [i % 140 for i in range(300)], [i % 3 for i in range(300)], 1, 2),
+    "two runs of units": ([130 if i % 7 == 0 else 1 for i in range(260)], [i % 9 for i in range(260)], [0] * 260, 1, 2),
 }
 
 
@@ -406,6 +408,7 @@ MASSES = {
     "one head each": ([70, 9], [300, 12], [0, 1], 4, 1),
     "wide groups": ([40, 3], [300, 777], [0, 1], 2, 8),
     "many": ([2] * 300, [90], [0] * 300, 1, 2),
+    "as many as a table holds": ([33] * 256, [130, 1, 260], [i % 3 for i in range(256)], 1, 2),
 }
 
 
@@ -437,6 +440,36 @@ def test_mass(pkg, gpu_lib, name, max_q):
     assert call(1) == 0  # adds the same sums, bit for bit
     for i, e in enumerate(ext):
         assert torch.equal(c.mass[i, :, :e], once[i, :, :e] * 2)
+    assert gpu_lib.d1_kv4_error() == 0
+
+
+@gpu
+@pytest.mark.parametrize("max_q", HINTS)
+def test_mass_of_rows_that_add_nothing(pkg, gpu_lib, max_q):
+    """No rows: the sum is 0, and is written. Rows with lse = -inf add nothing, be they NaN (padding): the same bits as
+    without them."""
+    rng = np.random.default_rng(12)
+    kvh, group, q, ext, of = 2, 2, [0, 70, 5, 0, 0, 64], [130, 77, 9], [0, 1, 1, 2, 2, 1]
+    h = kvh * group
+    c = Caches(rng, ext, kvh, 136)
+    x, starts = poisoned_rows(rng, q, h * 64)
+    lse = (2 + rng.standard_normal((h, len(x)))).astype(np.float32)
+    seqs = [dict(q_start=s, q_len=a) for s, a in zip(starts, q)]
+    tab = table(pkg, seqs, c, of, mass=True)
+    pad = [starts[1], starts[1] + 40, starts[1] + 69, starts[2] + 4, starts[5] + 13]
+    lse[:, pad] = -INF
+    got = []
+    for v in (0.5, np.nan, np.inf):
+        x[pad] = v
+        d, l = torch.from_numpy(x).cuda(), torch.from_numpy(lse).cuda()
+        for acc in (0, 1):
+            c.mass.fill_(3)
+            assert gpu_lib.d1_kv4_mass(P(d), d.shape[1], P(l), len(x), P(tab), len(q), max_q, 130, h, group, 0.125, acc,
+                                       len(x), ST()) == 0
+            assert (c.mass[0, :, :130] == 3 * acc).all() and (c.mass[2, :, :9] == 3 * acc).all()
+            assert all((c.mass[i, :, e:] == 3).all() for i, e in enumerate(ext))
+        got.append(c.mass[1].clone())
+    assert not torch.isnan(got[0]).any() and torch.equal(got[0], got[1]) and torch.equal(got[0], got[2])
     assert gpu_lib.d1_kv4_error() == 0
 
 
@@ -500,7 +533,7 @@ def test_bad_entries_are_skipped(pkg, gpu_lib, max_q):
     lse = torch.full((h, rows), 3.0, device="cuda")
     for bad in (dict(ext_len=57), dict(ext_len=-1), dict(ext_cap=52), dict(k4=None), dict(vp=None),
                 dict(v4=c.dev["v4"].data_ptr() + 8), dict(kp=c.dev["kp"].data_ptr() + 2), dict(q_len=rows), dict(q_start=-1),
-                dict(q_len=-1), dict(q_start=2 ** 31 - 1)):
+                dict(q_len=-1), dict(q_start=2 ** 31 - 1), dict(ext_cap=2 ** 30 + 8)):
         for at in (0, 2):
             seqs = [dict(s) for s in good]
             seqs[at].update(bad)
