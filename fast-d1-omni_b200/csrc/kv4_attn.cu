@@ -35,27 +35,18 @@ __device__ __forceinline__ uint64_t f2_mul(uint64_t a, uint64_t b) {
 }
 
 // 2^x of two numbers without the SFU: x = n + f, n whole by adding and taking away 1.5 * 2^23 (the sum's low bits, with
-// 127 added, are 2^n's exponent), |f| <= 1/2, 2^f by a polynomial fitted here for the smallest relative error: 7.5e-5 of
-// degree 3 (below P's rounding to fp16), 2.1e-7 of degree 5 evaluated in fp32. x below -126.5 gives 0; NaN stays.
-template <int DEG>
+// 127 added, are 2^n's exponent), |f| <= 1/2, 2^f by a polynomial of degree 5 fitted here for the smallest relative error,
+// 2.1e-7 evaluated in fp32. x below -126.5 gives 0; NaN stays.
 __device__ __forceinline__ void ex2_fma2(float x0, float x1, float& p0, float& p1) {
-    static_assert(DEG == 3 || DEG == 5, "fitted degrees");
     const uint64_t x = f2_pack(fmax_nan(x0, -127.f), fmax_nan(x1, -127.f));
     const uint64_t t = f2_add(x, f2_pack(12583039.f, 12583039.f));
     const uint64_t f = f2_fma(f2_add(t, f2_pack(-12583039.f, -12583039.f)), f2_pack(-1.f, -1.f), x);
     auto c2 = [](float c) { return f2_pack(c, c); };
-    uint64_t q;
-    if (DEG == 3) {
-        q = f2_fma(c2(0.0551716685f), f, c2(0.242611125f));
-        q = f2_fma(q, f, c2(0.693260968f));
-        q = f2_fma(q, f, c2(0.999928057f));
-    } else {
-        q = f2_fma(c2(0.00132764725f), f, c2(0.00967554096f));
-        q = f2_fma(q, f, c2(0.0555071309f));
-        q = f2_fma(q, f, c2(0.240221202f));
-        q = f2_fma(q, f, c2(0.693146944f));
-        q = f2_fma(q, f, c2(1.00000012f));
-    }
+    uint64_t q = f2_fma(c2(0.00132764725f), f, c2(0.00967554096f));
+    q = f2_fma(q, f, c2(0.0555071309f));
+    q = f2_fma(q, f, c2(0.240221202f));
+    q = f2_fma(q, f, c2(0.693146944f));
+    q = f2_fma(q, f, c2(1.00000012f));
     float t0, t1;
     f2_unpack(t, t0, t1);
     f2_unpack(f2_mul(q, f2_pack(__uint_as_float(__float_as_uint(t0) << 23), __uint_as_float(__float_as_uint(t1) << 23))), p0, p1);
@@ -1067,7 +1058,9 @@ __global__ void __launch_bounds__(T_THREADS, 1)
                         tmem_st8(tO + o8 * 8, o);
                     }
                 }
-                // P = 2^(s * scale - m), two scores at a time, an eighth of them on the FMA pipe; the row's sum in fp32
+                // P = 2^(s * scale - m), two scores at a time, and the row's sum in fp32. (An eighth of the exponentials on the
+                // FMA pipe: documents 258 -> 253 us with a polynomial of degree 3, whose 7.5e-5 showed in the log-sum-exp;
+                // 259 with degree 5.)
                 const uint64_t sc2 = f2_pack(a.scale_log2, a.scale_log2), nm2 = f2_pack(-m_use, -m_use);
                 uint64_t rs2[4];
 #pragma unroll
@@ -1075,14 +1068,9 @@ __global__ void __launch_bounds__(T_THREADS, 1)
                 uint32_t pr[TKV / 2];
 #pragma unroll
                 for (int i = 0; i < TKV / 2; i++) {
-                    float x0, x1, p0, p1;
+                    float x0, x1;
                     f2_unpack(f2_fma(f2_pack(__uint_as_float(sr[2 * i]), __uint_as_float(sr[2 * i + 1])), sc2, nm2), x0, x1);
-                    if (i % 8 == 7) {
-                        ex2_fma2<3>(x0, x1, p0, p1);
-                    } else {
-                        p0 = ex2(x0);
-                        p1 = ex2(x1);
-                    }
+                    const float p0 = ex2(x0), p1 = ex2(x1);
                     rs2[i & 3] = f2_add(rs2[i & 3], f2_pack(p0, p1));
                     pr[i] = pack_h2(p0, p1);
                 }
@@ -1709,7 +1697,7 @@ __global__ void __launch_bounds__(M_THREADS, 1) k_kv4_mass_tc(const __grid_const
                         p[0] = ex2(x[0]);
                         p[1] = ex2(x[1]);
                         if (i % 4 == 3) {
-                            ex2_fma2<5>(x[2], x[3], p[2], p[3]);
+                            ex2_fma2(x[2], x[3], p[2], p[3]);
                         } else {
                             p[2] = ex2(x[2]);
                             p[3] = ex2(x[3]);

@@ -360,6 +360,24 @@ def test_attend_sharp_and_shared(pkg, gpu_lib, max_q):
 
 
 @gpu
+@pytest.mark.parametrize("max_q", HINTS)
+def test_lse_of_few_keys(pkg, gpu_lib, max_q):
+    """Single exponentials are not averaged out: beside the scores' own error (ds) 2^-22 of an exponential, at most 24 rounded
+    additions and rescalings (2^-19.4) and the logarithm's and its factor's roundings, 2^-21 of the result."""
+    rng = np.random.default_rng(13)
+    kvh, group, q, ext = 2, 2, [130, 40, 70, 3, 200], [2, 16, 31, 128, 9]
+    h = kvh * group
+    c = Caches(rng, ext, kvh, 136)
+    x, starts = poisoned_rows(rng, q, (h + 2 * kvh) * 64)
+    seqs = [dict(q_start=s, q_len=a, kv_start=s, kv_len=0) for s, a in zip(starts, q)]
+    _, L = attend(gpu_lib, x, table(pkg, seqs, c, range(5)), 5, kvh, group, 0.125, max_q, 128)
+    _, l, _, tL = plain_attend(x, seqs, c, range(5), kvh, group, 0.125, True)
+    ok = np.isfinite(l)
+    tight = tL - 2.0 ** -13 + 2.0 ** -22 + 2.0 ** -19.4
+    assert (np.abs(L.double().cpu().numpy()[:, :len(x)] - l)[ok] <= tight[ok]).all()
+
+
+@gpu
 @pytest.mark.parametrize("at", [0, 15, 50, 78, 99])
 @pytest.mark.parametrize("max_q", HINTS)
 def test_attend_nan_stays_in_its_rows(pkg, gpu_lib, max_q, at):
