@@ -1800,7 +1800,12 @@ int launch_rows(Kv4Args& a, int max_q, int max_keys, int kv_heads, cudaStream_t 
     // 4097 keys: 8.5 us with 8, 11, 17 and 27 with 4, 2 and 1)
     int ranks = R_CLUSTER;
     const long long tiles = ((long long)max_keys + R_KEYS - 1) / R_KEYS, slots = 148 * (NT == 1 ? 4 : 2);
-    while (ranks > 1 && ((ranks / 2) * R_WARPS >= tiles || x * kv_heads * z * ranks > slots)) ranks /= 2;
+    const long long ctas = x * kv_heads * z;
+    while (ranks > 1 && ((ranks / 2) * R_WARPS >= tiles || ctas * ranks > slots)) ranks /= 2;
+    // where they leave more than a quarter of the room empty and the keys are long, twice as many, the rest of them as room
+    // comes free (10, 20 and 40 tokens over 8192 to 16384 keys: 32, 72 and 123 us, otherwise 40, 82 and 164; but of 16
+    // tiles a CTA 10 x 16 rows over 4096 keys: 31 us, otherwise 28; and of a fuller GPU, 32 tokens over 16384: 103 and 97)
+    if (ranks < R_CLUSTER && ctas * ranks * 4 < slots * 3 && tiles >= 2 * ranks * 24) ranks *= 2;
     a.ranks = ranks;
     return launch_clusters(k_kv4_attn_rows<NT>, dim3((unsigned)x * ranks, kv_heads, z), R_WARPS * 32, rows_smem<NT>(), ranks, st,
                            (const Kv4Args)a);
