@@ -115,7 +115,7 @@ __global__ void __launch_bounds__(R_WARPS * 32, NT == 1 ? 4 : 2) k_kv4_attn_rows
             if (tid == 0) atomicExch(a.err, kErrTable);
             continue;
         }
-        const long long n_rows = (long long)s.q_len * a.group;
+        const uint32_t group = a.group, n_rows = (uint32_t)s.q_len * group;  // (2^31 rows would exceed the memory)
         const int ext_tiles = (s.ext_len + R_KEYS - 1) / R_KEYS, tiles = ext_tiles + (s.kv_len + R_KEYS - 1) / R_KEYS;
         // this CTA's tiles
         const int per = (tiles + ranks - 1) / ranks, tile0 = min(tiles, rank * per), tile1 = min(tiles, tile0 + per);
@@ -123,15 +123,15 @@ __global__ void __launch_bounds__(R_WARPS * 32, NT == 1 ? 4 : 2) k_kv4_attn_rows
         const uint8_t* v4 = s.v4 + (size_t)g * s.ext_cap * 32 + 4 * r;
         const uint16_t* kp = reinterpret_cast<const uint16_t*>(s.kp) + (size_t)g * s.ext_cap;
         const uint16_t* vp = reinterpret_cast<const uint16_t*>(s.vp) + (size_t)g * s.ext_cap;
-        for (long long base = (long long)(blockIdx.x / ranks) * NR; base < n_rows; base += (long long)(gridDim.x / ranks) * NR) {
+        for (uint32_t base = blockIdx.x / ranks * NR; base < n_rows; base += gridDim.x / ranks * NR) {
             // ---- the query rows, as B operands: [n tile][k step][2]
             uint32_t qb[NT][4][2];
 #pragma unroll
             for (int nt = 0; nt < NT; nt++) {
-                const long long p = base + nt * 8 + r;
+                const uint32_t p = base + nt * 8 + r;
                 uint4 x0 = make_uint4(0, 0, 0, 0), x1 = x0;
                 if (p < n_rows) {
-                    const int row = (int)(p / a.group), h = g * a.group + (int)(p % a.group);
+                    const uint32_t row = p / group, h = g * group + p % group;
                     const uint4* src =
                         reinterpret_cast<const uint4*>(a.Q + (size_t)(s.q_start + row) * a.ldq + h * 64 + 16 * t);
                     x0 = __ldg(src);
@@ -365,9 +365,9 @@ __global__ void __launch_bounds__(R_WARPS * 32, NT == 1 ? 4 : 2) k_kv4_attn_rows
                     dst[1] = make_float4(o[nt][2][q], o[nt][2][q + 2], o[nt][3][q], o[nt][3][q + 2]);
                 }
             __syncthreads();
-            auto finish = [&](long long p, int d, float M, float L, const float4& x) {
+            auto finish = [&](uint32_t p, int d, float M, float L, const float4& x) {
                 const float il = tiles ? 1.f / L : 0.f;
-                const int q = s.q_start + (int)(p / a.group), h = g * a.group + (int)(p % a.group);
+                const int q = s.q_start + (int)(p / group), h = g * a.group + (int)(p % group);
                 *reinterpret_cast<uint2*>(a.O + (size_t)q * a.ldo + h * 64 + d) =
                     make_uint2(pack_h2(x.x * il, x.y * il), pack_h2(x.z * il, x.w * il));
                 if (a.lse && d == 0) a.lse[(size_t)h * a.lse_ld + q] = tiles ? (M + log2f(L)) * kLn2 : -INFINITY;
@@ -1306,12 +1306,12 @@ __global__ void __launch_bounds__(256) k_kv4_mass_rows(const Kv4Args a) {
                         continue;
                     }
                     any = true;
-                    const long long n_rows = (long long)q_len * a.group;
-                    for (long long base = 0; base < n_rows; base += 8) {
+                    const uint32_t n_rows = (uint32_t)q_len * (uint32_t)a.group;
+                    int q = q_start + r / a.group, h = g * a.group + r % a.group;  // of packed row base + r
+                    for (uint32_t base = 0; base < n_rows; base += 8) {
                         uint4 x0 = make_uint4(0, 0, 0, 0), x1 = x0;
-                        float lse = INFINITY;  // of packed row base + r, in log2; +inf: adds nothing
+                        float lse = INFINITY;  // in log2; +inf: adds nothing
                         if (base + r < n_rows) {
-                            const int q = q_start + (int)((base + r) / a.group), h = g * a.group + (int)((base + r) % a.group);
                             const uint4* src = reinterpret_cast<const uint4*>(a.Q + (size_t)q * a.ldq + h * 64 + 16 * t);
                             x0 = __ldg(src);
                             x1 = __ldg(src + 1);
@@ -1320,6 +1320,12 @@ __global__ void __launch_bounds__(256) k_kv4_mass_rows(const Kv4Args a) {
                                 lse = INFINITY;
                                 x0 = x1 = make_uint4(0, 0, 0, 0);
                             }
+                        }
+                        q += 8 / a.group;
+                        h += 8 % a.group;
+                        if (h >= (g + 1) * a.group) {
+                            h -= a.group;
+                            q++;
                         }
                         const float l0 = __shfl_sync(D1_FULL_MASK, lse, 8 * t), l1 = __shfl_sync(D1_FULL_MASK, lse, 8 * t + 4);
 #pragma unroll
