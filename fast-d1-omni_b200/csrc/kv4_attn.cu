@@ -1234,14 +1234,16 @@ __global__ void __launch_bounds__(T_THREADS, 1)
 }
 
 // ------------------------------------------------------------------------------------------------ mass, few rows
-// S^T = K Q^T on m16n8k16: a warp holds 64 keys as A operands (whole numbers code - zero, as above) and goes over the
-// packed query rows 8 at a time, adding exp(s - lse) into 8 sums of its keys; four lanes share a key at the end. The
-// sequences that share a mass array are taken by the first of them, in the table's order.
-constexpr int M_KEYS = 64 * 8;  // keys of a CTA of 8 warps
-
-__global__ void __launch_bounds__(256) k_kv4_mass_rows(const Kv4Args a) {
-    __shared__ int peers[256];
-    __shared__ int n_peers;
+// S^T = K Q^T on m16n8k16: a warp holds 16 * MT keys as A operands (whole numbers code - zero, as above) and goes over the
+// packed query rows 8 at a time, adding exp(s - lse) into its keys' sums; four lanes share a key at the end. The sequences
+// that share a mass array are taken by the first of them, in the table's order. What bounds it are latencies: of the table,
+// of the codes (both at once where the table has 256 entries at most), and of 8 rows after 8 rows.
+template <int MT>
+__global__ void __launch_bounds__(256, 2) k_kv4_mass_rows(const Kv4Args a) {
+    constexpr int KEYS = 16 * MT * 8;   // of a CTA of 8 warps
+    constexpr bool AHEAD = MT < 4;      // the next 8 rows on their way meanwhile; of 64 keys the registers do not hold them
+    __shared__ int2 peers[256];         // of 256 sequences: first row and rows
+    __shared__ uint32_t same[8];        // and which are of this mass array
     pdl_entry();
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, r = lane >> 2, t = lane & 3, g = blockIdx.y;
     for (int sq = blockIdx.z; sq < a.n_seqs; sq += gridDim.z) {
@@ -1251,26 +1253,56 @@ __global__ void __launch_bounds__(256) k_kv4_mass_rows(const Kv4Args a) {
             if (tid == 0) atomicExch(a.err, kErrTable);
             continue;
         }
-        int before = 0;
-        for (int i = tid; i < sq; i += 256) before |= a.seqs[i].mass == s.mass;
-        if (__syncthreads_or(before)) continue;
+        int listed = -1;  // which 256 sequences the list holds
+        // lists sequences b0 .. b0 + 255; whether one before sq, which then takes the mass array, is among them
+        auto list = [&](int b0) {
+            if (listed == b0) return false;
+            if (listed >= 0) __syncthreads();  // the list has been read
+            listed = b0;
+            const int j = b0 + tid;
+            bool mine = false, before = false;
+            if (j < a.n_seqs) {
+                const D1Kv4Seq p = a.seqs[j];
+                mine = p.mass == s.mass;
+                before = mine && j < sq;
+                if (mine && (!kv4_seq_ok(p) || p.k4 != s.k4 || p.ext_len != s.ext_len || p.ext_cap != s.ext_cap ||
+                             !rows_ok(p.q_start, p.q_len, a.q_rows))) {
+                    atomicExch(a.err, kErrTable);
+                    mine = false;
+                }
+                peers[tid] = make_int2(p.q_start, p.q_len);
+            }
+            const uint32_t v = __ballot_sync(D1_FULL_MASK, mine);
+            if (lane == 0) same[warp] = v;
+            return __syncthreads_or(before) != 0;
+        };
         const uint16_t* kp = reinterpret_cast<const uint16_t*>(s.kp) + (size_t)g * s.ext_cap;
         const uint8_t* k4 = s.k4 + (size_t)g * s.ext_cap * 32;
-        for (int k0 = blockIdx.x * M_KEYS; k0 < s.ext_len; k0 += gridDim.x * M_KEYS) {
-            const int key0 = k0 + warp * 64;
-            uint32_t ka[4][4][4];
-            float st[4][2], sum[4][2];
+        bool others = false;
+        for (int k0 = blockIdx.x * KEYS; k0 < s.ext_len && !others; k0 += gridDim.x * KEYS) {
+            const int key0 = k0 + warp * (16 * MT);
+            uint2 code[MT][2];
+            uint32_t par[MT][2];
 #pragma unroll
-            for (int mt = 0; mt < 4; mt++)
+            for (int mt = 0; mt < MT; mt++)
 #pragma unroll
                 for (int hf = 0; hf < 2; hf++) {
                     const int key = min(key0 + mt * 16 + hf * 8 + r, s.ext_len - 1);
-                    const uint2 w = __ldg(reinterpret_cast<const uint2*>(k4 + (size_t)key * 32) + t);
-                    const uint32_t par = __ldg(kp + key);
+                    code[mt][hf] = __ldg(reinterpret_cast<const uint2*>(k4 + (size_t)key * 32) + t);
+                    par[mt][hf] = __ldg(kp + key);
+                }
+            others = list(0);
+            if (others) break;
+            uint32_t ka[MT][4][4];
+            float st[MT][2], sum[MT][2];
+#pragma unroll
+            for (int mt = 0; mt < MT; mt++)
+#pragma unroll
+                for (int hf = 0; hf < 2; hf++) {
                     uint32_t z0, z1, x[4], y[4];
-                    kv4_zero(par * 0x00010001u, z0, z1);
-                    kv4_expand(w.x, z0, z1, x);
-                    kv4_expand(w.y, z0, z1, y);
+                    kv4_zero(par[mt][hf] * 0x00010001u, z0, z1);
+                    kv4_expand(code[mt][hf].x, z0, z1, x);
+                    kv4_expand(code[mt][hf].y, z0, z1, y);
                     ka[mt][0][hf] = x[0];
                     ka[mt][0][2 + hf] = x[1];
                     ka[mt][1][hf] = x[2];
@@ -1279,71 +1311,64 @@ __global__ void __launch_bounds__(256) k_kv4_mass_rows(const Kv4Args a) {
                     ka[mt][2][2 + hf] = y[1];
                     ka[mt][3][hf] = y[2];
                     ka[mt][3][2 + hf] = y[3];
-                    st[mt][hf] = kv4_step(par) * a.scale_log2;
+                    st[mt][hf] = kv4_step(par[mt][hf]) * a.scale_log2;
                     sum[mt][hf] = 0.f;
                 }
             bool any = false;
-            for (int b0 = sq; b0 < a.n_seqs; b0 += 256) {  // the sequences of this mass array, in order
-                __syncthreads();
-                if (warp == 0) {
-                    int n = 0;
-                    for (int i = 0; i < 256; i += 32) {
-                        const int j = b0 + i + lane;
-                        const bool same = j < a.n_seqs && a.seqs[j].mass == s.mass;
-                        const uint32_t v = __ballot_sync(D1_FULL_MASK, same);
-                        if (same) peers[n + __popc(v & ((1u << lane) - 1))] = j;
-                        n += __popc(v);
-                    }
-                    if (lane == 0) n_peers = n;
-                }
-                __syncthreads();
-                for (int e = 0; e < n_peers; e++) {
-                    const D1Kv4Seq& p = a.seqs[peers[e]];
-                    const int q_start = p.q_start, q_len = p.q_len;
-                    if (!kv4_seq_ok(p) || p.k4 != s.k4 || p.ext_len != s.ext_len || p.ext_cap != s.ext_cap ||
-                        !rows_ok(q_start, q_len, a.q_rows)) {
-                        if (tid == 0) atomicExch(a.err, kErrTable);
-                        continue;
-                    }
-                    any = true;
-                    const uint32_t n_rows = (uint32_t)q_len * (uint32_t)a.group;
-                    int q = q_start + r / a.group, h = g * a.group + r % a.group;  // of packed row base + r
-                    for (uint32_t base = 0; base < n_rows; base += 8) {
-                        uint4 x0 = make_uint4(0, 0, 0, 0), x1 = x0;
-                        float lse = INFINITY;  // in log2; +inf: adds nothing
-                        if (base + r < n_rows) {
-                            const uint4* src = reinterpret_cast<const uint4*>(a.Q + (size_t)q * a.ldq + h * 64 + 16 * t);
-                            x0 = __ldg(src);
-                            x1 = __ldg(src + 1);
-                            lse = __ldg(a.lse + (size_t)h * a.lse_ld + q) * kLog2e;
-                            if (lse == -INFINITY) {  // adds nothing, whatever the row holds
+            for (int b0 = 0; b0 < a.n_seqs && !others; b0 += 256) {  // the sequences of this mass array, in order
+                others = list(b0);
+                for (int i = 0; i < 8 && !others; i++)
+                    for (uint32_t left = same[i]; left; left &= left - 1) {
+                        const int2 p = peers[32 * i + __ffs(left) - 1];
+                        any = true;
+                        const uint32_t n_rows = (uint32_t)p.y * (uint32_t)a.group;
+                        int q = p.x + r / a.group, h = g * a.group + r % a.group;  // of the packed row fetched next
+                        uint4 n0, n1;
+                        float nl;
+                        auto fetch = [&](uint32_t row) {
+                            n0 = n1 = make_uint4(0, 0, 0, 0);
+                            nl = -INFINITY;
+                            if (row < n_rows) {
+                                const uint4* src = reinterpret_cast<const uint4*>(a.Q + (size_t)q * a.ldq + h * 64 + 16 * t);
+                                n0 = __ldg(src);
+                                n1 = __ldg(src + 1);
+                                nl = __ldg(a.lse + (size_t)h * a.lse_ld + q);
+                            }
+                            q += 8 / a.group;
+                            h += 8 % a.group;
+                            if (h >= (g + 1) * a.group) {
+                                h -= a.group;
+                                q++;
+                            }
+                        };
+                        if (AHEAD) fetch(r);
+                        for (uint32_t base = 0; base < n_rows; base += 8) {
+                            if (!AHEAD) fetch(base + r);
+                            uint4 x0 = n0, x1 = n1;
+                            float lse = nl * kLog2e;  // in log2; +inf: adds nothing
+                            if (lse == -INFINITY) {   // whatever the row holds
                                 lse = INFINITY;
                                 x0 = x1 = make_uint4(0, 0, 0, 0);
                             }
-                        }
-                        q += 8 / a.group;
-                        h += 8 % a.group;
-                        if (h >= (g + 1) * a.group) {
-                            h -= a.group;
-                            q++;
-                        }
-                        const float l0 = __shfl_sync(D1_FULL_MASK, lse, 8 * t), l1 = __shfl_sync(D1_FULL_MASK, lse, 8 * t + 4);
+                            if (AHEAD) fetch(base + 8 + r);
+                            const float l0 = __shfl_sync(D1_FULL_MASK, lse, 8 * t), l1 = __shfl_sync(D1_FULL_MASK, lse, 8 * t + 4);
 #pragma unroll
-                        for (int mt = 0; mt < 4; mt++) {
-                            float c[4] = {0.f, 0.f, 0.f, 0.f};
-                            mma16816(c, ka[mt][0], x0.x, x0.y);
-                            mma16816(c, ka[mt][1], x0.z, x0.w);
-                            mma16816(c, ka[mt][2], x1.x, x1.y);
-                            mma16816(c, ka[mt][3], x1.z, x1.w);
-                            sum[mt][0] += ex2(c[0] * st[mt][0] - l0) + ex2(c[1] * st[mt][0] - l1);
-                            sum[mt][1] += ex2(c[2] * st[mt][1] - l0) + ex2(c[3] * st[mt][1] - l1);
+                            for (int mt = 0; mt < MT; mt++) {
+                                float c[4];
+                                mma16816_first(c, ka[mt][0], x0.x, x0.y);
+                                mma16816(c, ka[mt][1], x0.z, x0.w);
+                                mma16816(c, ka[mt][2], x1.x, x1.y);
+                                mma16816(c, ka[mt][3], x1.z, x1.w);
+                                sum[mt][0] += ex2(c[0] * st[mt][0] - l0) + ex2(c[1] * st[mt][0] - l1);
+                                sum[mt][1] += ex2(c[2] * st[mt][1] - l0) + ex2(c[3] * st[mt][1] - l1);
+                            }
                         }
                     }
-                }
             }
+            if (others) break;
             float* mass = s.mass + (size_t)g * s.ext_cap;
 #pragma unroll
-            for (int mt = 0; mt < 4; mt++)
+            for (int mt = 0; mt < MT; mt++)
 #pragma unroll
                 for (int hf = 0; hf < 2; hf++) {
                     float v = sum[mt][hf];
@@ -1944,11 +1969,21 @@ extern "C" int d1_kv4_mass(const d1_half* Q, int ldq, const float* lse, int lse_
     a.accumulate = accumulate;
     a.scale_log2 = scale * kLog2e;
     if (!a.err) return -1;
-    // the tcgen05 form above 64 packed rows a sequence, where its table holds the sequences. 16 caches of 1200 keys: 96
-    // rows 18 us and 25 on mma.sync, 64 rows 18 and 19, 48 rows 18 and 16; of 8000 keys: 82 and 84, 80 and 64
+    // the tcgen05 form above 64 packed rows a sequence, where its table holds the sequences. 16 sequences, 1200 keys: 66 rows
+    // 20 us and 17 on mma.sync, 17 and 19 where they share 4 caches; 96 rows 19 and 19, 16 and 22; 192 rows 21 and 32, 21
+    // and 38
     if ((long long)max_q * group > 64 && group <= MQ && q_rows > 0 && n_seqs <= M_SEQS) return launch_mass_tc(a, max_len, st);
-    long long x = ((long long)max_len + M_KEYS - 1) / M_KEYS;
-    x = x < 1 ? 1 : x > 65536 ? 65536 : x;
-    launch_pdl(k_kv4_mass_rows, dim3((unsigned)x, heads / group, n_seqs < 65535 ? n_seqs : 65535), 256, 0, st, a);
+    const int z = n_seqs < 65535 ? n_seqs : 65535, kv_heads = heads / group;
+    auto blocks = [&](int keys) {
+        const long long x = ((long long)max_len + keys - 1) / keys;
+        return (unsigned)(x < 1 ? 1 : x > 65536 ? 65536 : x);
+    };
+    // 32 keys to a warp up to about two waves of CTAs, then 64, whose expansion the rows share out better (8 rows, one cache
+    // of 8000 keys: 4.3 us and 5.0 with 64; 16 caches of 1200: 9.7 and 10.2; 16 of 8000: 43 and 33; 24 rows, 16 sequences
+    // on 4 caches of 1200: 14 and 22)
+    if ((long long)blocks(256) * kv_heads * z <= 5 * 148)
+        launch_pdl(k_kv4_mass_rows<2>, dim3(blocks(256), kv_heads, z), 256, 0, st, a);
+    else
+        launch_pdl(k_kv4_mass_rows<4>, dim3(blocks(512), kv_heads, z), 256, 0, st, a);
     return (int)cudaGetLastError();
 }
