@@ -1423,7 +1423,7 @@ struct MassTable {
     int cum[M_SEQS + 1], q_start[M_SEQS], q_len[M_SEQS], ext_len[M_SEQS], next[M_SEQS];
 };
 
-constexpr int M_SMEM = 2 * M_K_BYTES + M_STAGES * (M_Q_BYTES + MQ * 4) + 2 * (M_WGS - 1) * MK * 4 + (int)sizeof(MassTable) +
+constexpr int M_SMEM = 2 * M_K_BYTES + M_STAGES * (M_Q_BYTES + MQ * 4) + (2 * (M_WGS - 1) + 1) * MK * 4 + (int)sizeof(MassTable) +
                        M_NBARS * 8 + 16;
 static_assert(M_SMEM <= 232448 && sizeof(MassTable) % 8 == 0, "shared memory of the tcgen05 mass kernel");
 
@@ -1491,9 +1491,12 @@ struct MassWalk {
     int block, kv_heads;             // rows of a whole tile
     bool any;                        // a sequence counted, be it without rows
     int entry;
+    int rank, ranks;                 // every ranks-th tile, from the rank's
 
     __device__ MassWalk(const Kv4Args& a) : block(MQ / a.group), kv_heads(a.heads / a.group), entry(0) {}
-    __device__ void find(const MassTable& tb, int u) {  // u at or behind the one before
+    __device__ void find(const MassTable& tb, int u, int rank_, int ranks_) {  // u at or behind the one before
+        rank = rank_;
+        ranks = ranks_;
         while (tb.cum[entry + 1] <= u) entry++;
         sq = entry;
         const int rest = u - tb.cum[entry];
@@ -1504,27 +1507,33 @@ struct MassWalk {
         any = false;
     }
     __device__ bool next_tile(const MassTable& tb, int n) {
+        int ahead = peer < 0 ? rank : ranks - 1;  // tiles of the others before it
         row0 += block;
-        while (row0 >= q_len) {
-            peer = peer < 0 ? sq : tb.next[peer];
-            if (peer >= n) return false;
-            q_start = tb.q_start[peer];
-            q_len = tb.q_len[peer];
-            row0 = 0;
-            any |= q_len >= 0;
+        while (true) {
+            while (row0 >= q_len) {
+                peer = peer < 0 ? sq : tb.next[peer];
+                if (peer >= n) return false;
+                q_start = tb.q_start[peer];
+                q_len = tb.q_len[peer];
+                row0 = 0;
+                any |= q_len >= 0;
+            }
+            if (ahead-- == 0) return true;
+            row0 += block;
         }
-        return true;
     }
     __device__ int rows() const { return min(block, q_len - row0); }
 };
 
+template <bool SPLIT>
 __global__ void __launch_bounds__(M_THREADS, 1) k_kv4_mass_tc(const __grid_constant__ CUtensorMap tmQp, const Kv4Args a) {
     extern __shared__ __align__(1024) uint8_t m_smem[];
     uint8_t* sK = m_smem;                                                          // [2][128 keys]
     uint8_t* sQ = sK + 2 * M_K_BYTES;                                              // [stage][256 columns]
     float* sL = reinterpret_cast<float*>(sQ + M_STAGES * M_Q_BYTES);               // [stage][256]: -lse in log2
     float* sSum = sL + M_STAGES * MQ;                                              // [2][warpgroup - 1][128]
-    MassTable& tb = *reinterpret_cast<MassTable*>(sSum + 2 * (M_WGS - 1) * MK);
+    float* sPart = sSum + 2 * (M_WGS - 1) * MK;                                    // [128] SPLIT: the CTA's sums
+    MassTable& tb = *reinterpret_cast<MassTable*>(sPart + MK);
     uint64_t* bars = reinterpret_cast<uint64_t*>(&tb + 1);
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + M_NBARS);
     volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
@@ -1572,14 +1581,44 @@ __global__ void __launch_bounds__(M_THREADS, 1) k_kv4_mass_tc(const __grid_const
     auto wait = [&](int b, uint32_t parity) {
         return __all_sync(D1_FULL_MASK, mbar_wait(bar(b), parity, abort_flag)) != 0;
     };
+    // SPLIT: the CTAs of a cluster share out the query tiles of the cluster's first unit. Should there be more units than
+    // clusters (max_len was too small), the first CTA goes on alone. Every warp passes the two barriers behind that unit.
+    const int ranks = SPLIT ? a.ranks : 1, rank = SPLIT ? (int)cluster_ctarank() : 0;
+    const int u0 = blockIdx.x / ranks, u_step = gridDim.x / ranks;
+    auto find_unit = [&](int u) {
+        const bool split = SPLIT && u == u0;
+        wk.find(tb, u, split ? rank : 0, split ? ranks : 1);
+    };
+    auto each_unit = [&](auto&& unit) {
+        for (int u = u0; ok && u < n_units; u += u_step, nu++) {
+            unit(u);
+            if (SPLIT && u == u0) {
+                __syncwarp();
+                cluster_sync();  // the CTAs' sums are in their shared memory
+                if (rank == 0 && warp < 4 && ok) {
+                    const int row = warp * 32 + lane;
+                    float all = sPart[row];
+                    for (int c = 1; c < ranks; c++) all += ld_cluster_f32(mapa_shared(smem_u32(sPart + row), c));
+                    const long long key = (long long)wk.kt * MK + row;
+                    if (wk.any && key < tb.ext_len[wk.sq]) {
+                        float* m = a.seqs[wk.sq].mass + (size_t)wk.g * a.seqs[wk.sq].ext_cap + key;
+                        *m = a.accumulate ? *m + all : all;
+                    }
+                }
+                __syncwarp();
+                cluster_sync();  // and have been read
+                if (rank > 0) break;
+            }
+        }
+    };
 
     if (warp == M_WARP - 1 || warp > M_WARP) {
         // ------------------------------------------------------------------ loaders
         const int lw = warp < M_WARP ? 0 : warp - M_WARP, lt = lw * 32 + lane;
         int wiped = 0;  // tiles with rows wiped out so far
         const int inv = (65536 + a.group - 1) / a.group;  // c / group = c * inv >> 16 for c < 256: off by less than 1 / group
-        for (int u = blockIdx.x; ok && u < n_units; u += gridDim.x, nu++) {
-            wk.find(tb, u);
+        each_unit([&](int u) {
+            find_unit(u);
             const size_t at = (size_t)wk.g * a.seqs[wk.sq].ext_cap;
             const uint8_t* k4 = a.seqs[wk.sq].k4 + at * 32;
             const uint16_t* kp = reinterpret_cast<const uint16_t*>(a.seqs[wk.sq].kp) + at;
@@ -1597,7 +1636,7 @@ __global__ void __launch_bounds__(M_THREADS, 1) k_kv4_mass_tc(const __grid_const
                     par[i] = __ldg(kp + key);
                 }
             }
-            if (!(ok = wait(MB_KEMPTY + (nu & 1), ((nu >> 1) & 1) ^ 1))) break;
+            if (!(ok = wait(MB_KEMPTY + (nu & 1), ((nu >> 1) & 1) ^ 1))) return;
             uint8_t* dK = sK + (nu & 1) * M_K_BYTES;
 #pragma unroll
             for (int i = 0; i < PIECES; i++) {
@@ -1632,7 +1671,7 @@ __global__ void __launch_bounds__(M_THREADS, 1) k_kv4_mass_tc(const __grid_const
 #pragma unroll
                 for (int i = 0; i < MQ / 32; i++) wipe |= lane + 32 * i < cols && l[i] == -INFINITY;
                 wipe = __any_sync(D1_FULL_MASK, wipe);
-                if (!(ok = wait(MB_QEMPTY + st, ((ti / M_STAGES) & 1) ^ 1))) break;
+                if (!(ok = wait(MB_QEMPTY + st, ((ti / M_STAGES) & 1) ^ 1))) return;
 #pragma unroll
                 for (int i = 0; i < MQ / 32; i++)
                     if (32 * i < pad) sL[st * MQ + lane + 32 * i] = l[i] == -INFINITY ? -INFINITY : -l[i] * kLog2e;
@@ -1642,7 +1681,7 @@ __global__ void __launch_bounds__(M_THREADS, 1) k_kv4_mass_tc(const __grid_const
                     tma_load_3d(smem_u32(sQ + st * M_Q_BYTES), &tmQp, 0, h0, row, landed);
                 }
                 if (wipe) {
-                    if (!(ok = wait(MB_LANDED + lw, wiped & 1))) break;
+                    if (!(ok = wait(MB_LANDED + lw, wiped & 1))) return;
                     wiped++;
 #pragma unroll
                     for (int i = 0; i < MQ / 32; i++)
@@ -1654,7 +1693,7 @@ __global__ void __launch_bounds__(M_THREADS, 1) k_kv4_mass_tc(const __grid_const
                 }
                 if (wipe || lane != 0) mbar_arrive(full);
             }
-        }
+        });
         if (!ok && lane == 0) record_err(a.err, abort_flag, kErrWaitEmpty);
         if (lane == 0 && !ok) mbar_wait_timed2(bar(MB_LANDED + lw), wiped & 1);
         if (lane == 0)  // TMA copies still in flight (only after an abort) land before the CTA exits
@@ -1662,14 +1701,14 @@ __global__ void __launch_bounds__(M_THREADS, 1) k_kv4_mass_tc(const __grid_const
                 if (!mbar_wait_timed2(bar(MB_QFULL + i % M_STAGES), (i / M_STAGES) & 1)) break;
     } else if (warp == M_WARP) {
         // ------------------------------------------------------------------ MMA issuer (lane 0)
-        for (int u = blockIdx.x; ok && u < n_units; u += gridDim.x, nu++) {
-            wk.find(tb, u);
-            if (!(ok = wait(MB_KFULL + (nu & 1), (nu >> 1) & 1))) break;
+        each_unit([&](int u) {
+            find_unit(u);
+            if (!(ok = wait(MB_KFULL + (nu & 1), (nu >> 1) & 1))) return;
             const uint32_t k_addr = smem_u32(sK + (nu & 1) * M_K_BYTES);
             for (; wk.next_tile(tb, n); ti++) {
                 const int st = ti % M_STAGES, w = ti & 1, pad = (wk.rows() * a.group + 31) & ~31;
-                if (!(ok = wait(MB_QFULL + st, (ti / M_STAGES) & 1))) break;
-                if (ti > 1 && !(ok = wait(MB_SFREE + w, ((ti >> 1) - 1) & 1))) break;
+                if (!(ok = wait(MB_QFULL + st, (ti / M_STAGES) & 1))) return;
+                if (ti > 1 && !(ok = wait(MB_SFREE + w, ((ti >> 1) - 1) & 1))) return;
                 tc_fence_after();
                 if (lane == 0) {
                     const uint32_t q_addr = smem_u32(sQ + st * M_Q_BYTES), idesc = idesc_f16_f32(MK, pad);
@@ -1681,10 +1720,9 @@ __global__ void __launch_bounds__(M_THREADS, 1) k_kv4_mass_tc(const __grid_const
                 }
                 __syncwarp();
             }
-            if (!ok) break;
             if (lane == 0) tc_commit(bar(MB_KEMPTY + (nu & 1)));
             __syncwarp();
-        }
+        });
         if (lane == 0) {
             if (!ok) record_err(a.err, abort_flag, kErrWaitFull);
             tc_commit(bar(MB_DRAIN));  // every issued MMA has completed before TMEM is released
@@ -1696,15 +1734,15 @@ __global__ void __launch_bounds__(M_THREADS, 1) k_kv4_mass_tc(const __grid_const
         const int wg = warp >> 2, row = (warp & 3) * 32 + lane;
         const uint32_t tS = tmem + 32 * wg + ((uint32_t)((warp & 3) * 32) << 16);
         const uint64_t sc2 = f2_pack(a.scale_log2, a.scale_log2);
-        for (int u = blockIdx.x; ok && u < n_units; u += gridDim.x, nu++) {
-            wk.find(tb, u);
+        each_unit([&](int u) {
+            find_unit(u);
             uint64_t sum[4];
 #pragma unroll
             for (int e = 0; e < 4; e++) sum[e] = f2_pack(0.f, 0.f);
             for (; wk.next_tile(tb, n); ti++) {
                 const int st = ti % M_STAGES, b = ti & 1, pad = (wk.rows() * a.group + 31) & ~31;
-                if (!(ok = wait(MB_QFULL + st, (ti / M_STAGES) & 1))) break;  // the lse
-                if (!(ok = wait(MB_SFULL + b, (ti >> 1) & 1))) break;
+                if (!(ok = wait(MB_QFULL + st, (ti / M_STAGES) & 1))) return;  // the lse
+                if (!(ok = wait(MB_SFULL + b, (ti >> 1) & 1))) return;
                 tc_fence_after();
                 const int cols = wk.rows() * a.group;
                 for (int c0 = 32 * wg; c0 < pad; c0 += 32 * M_WGS) {
@@ -1744,30 +1782,31 @@ __global__ void __launch_bounds__(M_THREADS, 1) k_kv4_mass_tc(const __grid_const
                     mbar_arrive(bar(MB_QEMPTY + st));
                 }
             }
-            if (!ok) break;
             float v[8];
 #pragma unroll
             for (int e = 0; e < 4; e++) f2_unpack(sum[e], v[2 * e], v[2 * e + 1]);
             const float mine = ((v[0] + v[1]) + (v[2] + v[3])) + ((v[4] + v[5]) + (v[6] + v[7]));
             const int slot = nu & 1;
             if (wg > 0) {
-                if (!(ok = wait(MB_SUMFREE + slot, ((nu >> 1) & 1) ^ 1))) break;
+                if (!(ok = wait(MB_SUMFREE + slot, ((nu >> 1) & 1) ^ 1))) return;
                 sSum[(slot * (M_WGS - 1) + wg - 1) * MK + row] = mine;
                 __syncwarp();
                 if (lane == 0) mbar_arrive(bar(MB_SUM + slot));
             } else {
-                if (!(ok = wait(MB_SUM + slot, (nu >> 1) & 1))) break;
+                if (!(ok = wait(MB_SUM + slot, (nu >> 1) & 1))) return;
                 const float* other = sSum + slot * (M_WGS - 1) * MK + row;
                 const float all = (mine + other[0]) + (other[MK] + other[2 * MK]);
                 __syncwarp();
                 if (lane == 0) mbar_arrive(bar(MB_SUMFREE + slot));
                 const long long key = (long long)wk.kt * MK + row;
-                if (wk.any && key < tb.ext_len[wk.sq]) {
+                if (SPLIT && u == u0) {
+                    sPart[row] = all;
+                } else if (wk.any && key < tb.ext_len[wk.sq]) {
                     float* m = a.seqs[wk.sq].mass + (size_t)wk.g * a.seqs[wk.sq].ext_cap + key;
                     *m = a.accumulate ? *m + all : all;
                 }
             }
-        }
+        });
         if (!ok && lane == 0) record_err(a.err, abort_flag, kErrWaitAccFull);
     }
     tc_fence_before();
@@ -1797,6 +1836,34 @@ int sm_count() {
     if (!sms[dev & 63] && cudaDeviceGetAttribute(&sms[dev & 63], cudaDevAttrMultiProcessorCount, dev) != cudaSuccess)
         return 0;
     return sms[dev & 63];
+}
+
+// How many clusters of `ranks` CTAs (1, 2, 4 or 8) of a kernel the GPU holds at once: the GPCs' sizes decide (of 8 CTAs, one
+// to an SM, fewer than 148 / 8). Found on the first call for a device and kept in `found`, the kernel's own.
+template <typename F>
+int clusters_at_once(F* kernel, int threads, int smem, int ranks, int (*found)[R_CLUSTER + 1]) {
+    int dev = 0;
+    cudaGetDevice(&dev);
+    int& n = found[dev & 63][ranks];
+    if (!n) {
+        cudaLaunchConfig_t cfg = {};
+        cfg.gridDim = dim3(ranks);
+        cfg.blockDim = dim3(threads);
+        cfg.dynamicSmemBytes = smem;
+        cudaLaunchAttribute at[1];
+        at[0].id = cudaLaunchAttributeClusterDimension;
+        at[0].val.clusterDim.x = ranks;
+        at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+        cfg.attrs = at;
+        cfg.numAttrs = 1;
+        int v = 0;
+        if (cudaOccupancyMaxActiveClusters(&v, kernel, &cfg) != cudaSuccess) {
+            cudaGetLastError();
+            return 0;
+        }
+        n = v;
+    }
+    return n;
 }
 
 // kernel<<<...>>>(args...) in clusters of `ranks` CTAs along x, with programmatic stream serialization.
@@ -1879,8 +1946,12 @@ int launch_tc(Kv4Args& a, int max_q, int max_keys, cudaStream_t st) {
         tk = tv = tq;  // no own rows: never read
     }
     // few units: a cluster of CTAs to each, as many as the GPU has room for at once, with two key tiles or more for each
+    // (8 heads, 128 packed rows over 4097 keys: 17 us, and 69 without; two such sequences: 21 us in clusters of 4, and 32 of 8)
     int ranks = R_CLUSTER;
-    while (ranks > 1 && (units * ranks > sms || (long long)(ranks - 1) * 2 * TKV >= max_keys)) ranks /= 2;
+    static int found[64][R_CLUSTER + 1];
+    while (ranks > 1 && ((long long)(ranks - 1) * 2 * TKV >= max_keys ||
+                         units > clusters_at_once(k_kv4_attn_tc<true>, T_THREADS, T_SMEM, ranks, found)))
+        ranks /= 2;
     a.ranks = ranks;
     if (ranks == 1) {
         launch_pdl(k_kv4_attn_tc<false>, (int)(units < sms ? units : sms), T_THREADS, T_SMEM, st, tq, tqp, tk, tv, a);
@@ -1890,17 +1961,28 @@ int launch_tc(Kv4Args& a, int max_q, int max_keys, cudaStream_t st) {
                            (const Kv4Args)a);
 }
 
-int launch_mass_tc(Kv4Args& a, int max_len, cudaStream_t st) {
-    static unsigned long long done = 0;
-    if (!smem_opt_in(k_kv4_mass_tc, M_SMEM, &done)) return -1;
+int launch_mass_tc(Kv4Args& a, int max_q, int max_len, cudaStream_t st) {
+    static unsigned long long done = 0, done_split = 0;
+    if (!smem_opt_in(k_kv4_mass_tc<false>, M_SMEM, &done) || !smem_opt_in(k_kv4_mass_tc<true>, M_SMEM, &done_split)) return -1;
     const int sms = sm_count();
     if (!sms) return -1;
     // no more CTAs than units, were every sequence's cache its own and max_len long
     const long long units = (long long)a.n_seqs * (max_len > 0 ? (max_len - 1) / MK + 1 : 1) * (a.heads / a.group);
     CUtensorMap tq;
     if (!packed_tmap(&tq, a, MQ)) return -1;
-    launch_pdl(k_kv4_mass_tc, (int)(units < sms ? units : sms), M_THREADS, M_SMEM, st, tq, a);
-    return (int)cudaGetLastError();
+    // few units: a cluster of CTAs to each, as many as the GPU has room for at once, with a query tile for each (8 heads, one
+    // sequence of 4000 rows, 500 keys: 18 us, and 42 without; 16 units in clusters of 8, which do not all fit: 17 us, of 4: 10)
+    int ranks = R_CLUSTER;
+    static int found[64][R_CLUSTER + 1];
+    while (ranks > 1 && ((long long)(ranks - 1) * (MQ / a.group) >= max_q ||
+                         units > clusters_at_once(k_kv4_mass_tc<true>, M_THREADS, M_SMEM, ranks, found)))
+        ranks /= 2;
+    a.ranks = ranks;
+    if (ranks == 1) {
+        launch_pdl(k_kv4_mass_tc<false>, (int)(units < sms ? units : sms), M_THREADS, M_SMEM, st, tq, a);
+        return (int)cudaGetLastError();
+    }
+    return launch_clusters(k_kv4_mass_tc<true>, dim3((unsigned)units * ranks), M_THREADS, M_SMEM, ranks, st, tq, (const Kv4Args)a);
 }
 
 }  // namespace
@@ -1972,7 +2054,7 @@ extern "C" int d1_kv4_mass(const d1_half* Q, int ldq, const float* lse, int lse_
     // the tcgen05 form above 64 packed rows a sequence, where its table holds the sequences. 16 sequences, 1200 keys: 66 rows
     // 20 us and 17 on mma.sync, 17 and 19 where they share 4 caches; 96 rows 19 and 19, 16 and 22; 192 rows 21 and 32, 21
     // and 38
-    if ((long long)max_q * group > 64 && group <= MQ && q_rows > 0 && n_seqs <= M_SEQS) return launch_mass_tc(a, max_len, st);
+    if ((long long)max_q * group > 64 && group <= MQ && q_rows > 0 && n_seqs <= M_SEQS) return launch_mass_tc(a, max_q, max_len, st);
     const int z = n_seqs < 65535 ? n_seqs : 65535, kv_heads = heads / group;
     auto blocks = [&](int keys) {
         const long long x = ((long long)max_len + keys - 1) / keys;

@@ -462,6 +462,34 @@ def test_mass(pkg, gpu_lib, name, max_q):
 
 
 @gpu
+@pytest.mark.parametrize("max_len", [0, 1, 300, 40000])
+@pytest.mark.parametrize("max_q", HINTS)
+def test_mass_wrong_hints(pkg, gpu_lib, max_q, max_len):
+    """Rows and keys beyond the lengths given are computed all the same, however the CTAs are grouped."""
+    rng = np.random.default_rng(14)
+    kvh, group, q, ext, of = 2, 2, [300, 1, 700, 90], [700, 131, 1], [0, 1, 0, 2]
+    h = kvh * group
+    c = Caches(rng, ext, kvh, 704)
+    x, starts = poisoned_rows(rng, q, h * 64)
+    lse = (2 + rng.standard_normal((h, len(x)))).astype(np.float32)
+    seqs = [dict(q_start=s, q_len=a) for s, a in zip(starts, q)]
+    tab = table(pkg, seqs, c, of, mass=True)
+    d, l = torch.from_numpy(x).cuda(), torch.from_numpy(lse).cuda()
+    M, T = plain_mass(x, lse, seqs, c, of, kvh, group, 0.125)
+    first = None
+    for _ in range(3):
+        c.mass.fill_(5)
+        assert gpu_lib.d1_kv4_mass(P(d), d.shape[1], P(l), len(x), P(tab), len(q), max_q, max_len, h, group, 0.125, 0, len(x),
+                                   ST()) == 0
+        got = c.mass.double().cpu().numpy()
+        for i, e in enumerate(ext):
+            assert (got[i, :, e:] == 5).all() and (np.abs(got[i, :, :e] - M[i, :, :e]) <= T[i, :, :e]).all()
+        assert first is None or (got == first).all()  # the same call, the same bits
+        first = got
+    assert gpu_lib.d1_kv4_error() == 0
+
+
+@gpu
 @pytest.mark.parametrize("max_q", HINTS)
 def test_mass_of_rows_that_add_nothing(pkg, gpu_lib, max_q):
     """No rows: the sum is 0, and is written. Rows with lse = -inf add nothing, be they NaN (padding): the same bits as
