@@ -610,11 +610,13 @@ struct Unit {
     }
     __device__ int head(int w) const { return h + (mode == kPair ? w : 0); }
     __device__ int rows(const Kv4Args& a, int w) const { return mode == kPacked ? q_len * a.group : q_len - row0(w); }
-    // key tiles that warpgroup w takes: all, or of a packed unit every other one, from w
+    // key tiles that warpgroup w takes: all, or of a packed unit every other one; warpgroup 0, which finishes the unit, has
+    // the fewer where their number is odd, unless there is only one
+    __device__ int first_of(int w) const { return mode != kPacked ? 0 : tiles() > 1 ? 1 - w : w; }
     __device__ int tiles_of(int w) const {
-        return mode == kPacked ? (tiles() - w + 1) / 2 : w < q_tiles() ? tiles() : 0;
+        return mode == kPacked ? (tiles() - first_of(w) + 1) / 2 : w < q_tiles() ? tiles() : 0;
     }
-    __device__ int tile_of(int w, int i) const { return mode == kPacked ? 2 * i + w : i; }
+    __device__ int tile_of(int w, int i) const { return mode == kPacked ? 2 * i + first_of(w) : i; }
 };
 
 // Whether the phase of `parity` has completed, at once; and after half a microsecond's wait at most.
@@ -891,7 +893,7 @@ __global__ void __launch_bounds__(T_THREADS, 1)
                     find_unit(u);
                     const int nt = un.tiles(), mine = un.tiles_of(w);
                     if (nt == 0) return;
-                    const int step = un.mode == kPacked ? 2 : 1, first = un.mode == kPacked ? w : 0;  // its key tiles
+                    const int step = un.mode == kPacked ? 2 : 1, first = un.first_of(w);  // its key tiles
                     const int qs = qi % T_QSLOTS;
                     if (!(ok = mbar_wait(bar(B_QFULL + qs), (qi / T_QSLOTS) & 1, abort_flag))) return;
                     const uint64_t dq = smem_desc_k128(smem_u32(sQ + qs * 2 * T_QT_BYTES) + (un.mode == kPacked ? 0 : w * T_QT_BYTES));
