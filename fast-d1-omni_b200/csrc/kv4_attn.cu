@@ -447,7 +447,7 @@ __global__ void __launch_bounds__(R_WARPS * 32, NT == 1 ? 4 : 2) k_kv4_attn_rows
 // ------------------------------------------------------------------------------------------------ attention, many rows
 // tcgen05 form. Persistent CTAs (one per SM) loop over units. A unit is, by the length of its sequence,
 //   packed  up to 128 packed query rows (row p / group, head p % group) of one kv head; the two softmax warpgroups take
-//           its key tiles in turn and are joined at the end
+//           its key tiles in turn and are joined at the end, each for half of the dimensions
 //   pair    128 rows of two heads of one kv head (an even group), a warpgroup each
 //   single  256 rows of one head (an odd group), a warpgroup for each 128
 // Keys come in tiles of 128, first the cached ones, then the own ones; the last tile of either kind is filled up with
@@ -482,16 +482,15 @@ enum : int {
     B_SFREE = B_SFULL + 2,           // [w]: it is in registers (4 warps)
     B_PFULL = B_SFREE + 2,           // [w]: P is in TMEM (4 warps)
     B_ODONE = B_PFULL + 2,           // [w]: P V has completed
-    B_OFREE = B_ODONE + 2,           // [w]: O has been read (4 warps; of a packed unit those of warpgroup 0)
+    B_OFREE = B_ODONE + 2,           // [w]: O has been read (8 warps of a packed unit, otherwise 4, twice)
     B_RAWFULL = B_OFREE + 2,         // [raw stage]: a tile's codes and parameters are in shared memory
     B_RAWEMPTY = B_RAWFULL + T_RAW_STAGES,  // [raw stage] (4 warps)
     B_OWN = B_RAWEMPTY + T_RAW_STAGES,  // a partial tile of own rows has landed
-    B_JOIN = B_OWN + 1,              // a packed unit's maxima and sums of warpgroup 1 are in shared memory (4 warps)
-    B_JOINED = B_JOIN + 1,           // and have been read (4 warps)
-    B_DRAIN = B_JOINED + 1,          // [issuer]
+    B_JOIN = B_OWN + 1,              // a packed unit's maxima and sums are in shared memory, its O's complete (8 warps)
+    B_DRAIN = B_JOIN + 1,            // [issuer]
     T_NBARS = B_DRAIN + 2
 };
-constexpr int T_SMEM = T_QSLOTS * 2 * T_QT_BYTES + T_STAGES * 2 * T_KV_BYTES + T_RAW_STAGES * T_RAW_BYTES + T_NBARS * 8 + 16 + TQ * 8 +
+constexpr int T_SMEM = T_QSLOTS * 2 * T_QT_BYTES + T_STAGES * 2 * T_KV_BYTES + T_RAW_STAGES * T_RAW_BYTES + T_NBARS * 8 + 16 + TQ * 16 +
                        (T_ENTRIES * 6 + 1) * 4;
 static_assert(T_SMEM <= 232448 && T_O_COL + 64 <= T_WG_COLS, "shared memory and TMEM of the tcgen05 attention");
 
@@ -667,8 +666,8 @@ __global__ void __launch_bounds__(T_THREADS, 1)
     uint64_t* bars = reinterpret_cast<uint64_t*>(sRaw + T_RAW_STAGES * T_RAW_BYTES);
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + T_NBARS);
     volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
-    float* join = reinterpret_cast<float*>(tmem_slot + 4);  // [128][2]: maximum and sum of warpgroup 1's rows
-    int* cum = reinterpret_cast<int*>(join + 2 * TQ);       // [T_ENTRIES + 1]
+    float* join = reinterpret_cast<float*>(tmem_slot + 4);  // [w][128][2]: maximum and sum of a row
+    int* cum = reinterpret_cast<int*>(join + 4 * TQ);       // [T_ENTRIES + 1]
     auto bar = [&](int i) { return smem_u32(bars + i); };
     if (smem_u32(t_smem) & 1023) {  // never expected: dynamic shared memory starts at the window's base
         pdl_wait();
@@ -690,7 +689,7 @@ __global__ void __launch_bounds__(T_THREADS, 1)
             mbar_init(bar(B_SFREE + w), 4);
             mbar_init(bar(B_PFULL + w), 4);
             mbar_init(bar(B_ODONE + w), 1);
-            mbar_init(bar(B_OFREE + w), 4);
+            mbar_init(bar(B_OFREE + w), 8);
             mbar_init(bar(B_DRAIN + w), 1);
         }
         for (int i = 0; i < T_RAW_STAGES; i++) {
@@ -698,8 +697,7 @@ __global__ void __launch_bounds__(T_THREADS, 1)
             mbar_init(bar(B_RAWEMPTY + i), T_EXPANDERS / 32);
         }
         mbar_init(bar(B_OWN), 1);
-        mbar_init(bar(B_JOIN), 4);
-        mbar_init(bar(B_JOINED), 4);
+        mbar_init(bar(B_JOIN), 8);
         *abort_flag = 0;
         fence_mbar_init();
     }
@@ -1095,84 +1093,92 @@ __global__ void __launch_bounds__(T_THREADS, 1)
             }
             if (!SPLIT && !ok) break;
             cnt += nt;
-            if (ok && packed && w == 1 && un.tiles() > 0) {  // the rest is warpgroup 0's, which shares the lanes
-                if (njoin > 0) ok = __all_sync(D1_FULL_MASK, mbar_wait(bar(B_JOINED), (njoin - 1) & 1, abort_flag));
-                if (ok && nt > 0) ok = __all_sync(D1_FULL_MASK, mbar_wait(bar(B_ODONE + 1), (cnt - 1) & 1, abort_flag));
-                if (!SPLIT && !ok) break;
-                tc_fence_after();
-                join[2 * row] = m;
-                join[2 * row + 1] = l;
-                tc_fence_before();
-                __syncwarp();
-                if (lane == 0) mbar_arrive(bar(B_JOIN));
-                njoin++;
-                if (!split) continue;
-            }
-            const bool mine = nt > 0 && !(packed && w == 1);  // this warpgroup finishes the unit's rows, or some of them
-            if (!SPLIT || (ok && mine)) ok = __all_sync(D1_FULL_MASK, mbar_wait(bar(B_ODONE + w), (cnt - 1) & 1, abort_flag));
+            const bool mine = packed ? un.tiles() > 0 : nt > 0;  // this warpgroup finishes rows of the unit
+            if (ok && nt > 0) ok = __all_sync(D1_FULL_MASK, mbar_wait(bar(B_ODONE + w), (cnt - 1) & 1, abort_flag));
             if (!SPLIT && !ok) break;
-            tc_fence_after();
             if (split) {
                 __syncwarp();
                 cluster_sync();  // both warpgroups have done with the key tiles: their shared memory is free
             }
-            if (SPLIT && !split && !mine) continue;
-            if (!SPLIT || (ok && mine)) {
-                uint32_t o[64];
-                tmem_ld32(tO, *reinterpret_cast<uint32_t(*)[32]>(o));
-                tmem_ld32(tO + 32, *reinterpret_cast<uint32_t(*)[32]>(o + 32));
-                tc_wait_ld();
-                if (packed) {
-                    ok = __all_sync(D1_FULL_MASK, mbar_wait(bar(B_JOIN), njoin & 1, abort_flag));
-                    if (!SPLIT && !ok) break;
-                    tc_fence_after();
-                    njoin++;
-                    const float m1 = join[2 * row], l1 = join[2 * row + 1];
-                    if (un.tiles_of(1) > 0) {
-                        const float both = fmaxf(m, m1), f0 = ex2(m - both), f1 = ex2(m1 - both);
-                        uint32_t o1[64];
-                        tmem_ld32(tO + T_WG_COLS, *reinterpret_cast<uint32_t(*)[32]>(o1));
-                        tmem_ld32(tO + T_WG_COLS + 32, *reinterpret_cast<uint32_t(*)[32]>(o1 + 32));
-                        tc_wait_ld();
-#pragma unroll
-                        for (int i = 0; i < 64; i++)
-                            o[i] = __float_as_uint(__uint_as_float(o[i]) * f0 + __uint_as_float(o1[i]) * f1);
-                        l = l * f0 + l1 * f1;
-                        m = both;
-                    }
+            // A packed unit's rows are in both warpgroups: they tell each other their maxima and sums, and each finishes half
+            // of the dimensions. The shared memory is written again only behind a P V of a later unit, which waits for
+            // B_OFREE, or not read (a warpgroup without tiles)
+            float f0 = 1.f, f1 = 0.f;
+            const bool two = packed && un.tiles_of(1) > 0;
+            if (ok && mine && packed) {
+                if (nt > 0) {
+                    join[2 * (w * TQ + row)] = m;
+                    join[2 * (w * TQ + row) + 1] = l;
                 }
                 tc_fence_before();
                 __syncwarp();
-                if (lane == 0) {
-                    mbar_arrive(bar(B_OFREE + w));
-                    if (packed) {
-                        if (un.tiles_of(1) > 0) mbar_arrive(bar(B_OFREE + 1));
-                        mbar_arrive(bar(B_JOINED));
-                    }
+                if (lane == 0) mbar_arrive(bar(B_JOIN));
+                ok = __all_sync(D1_FULL_MASK, mbar_wait(bar(B_JOIN), njoin & 1, abort_flag));
+                njoin++;
+                m = join[2 * row];
+                l = join[2 * row + 1];
+                if (two) {
+                    const float m1 = join[2 * (TQ + row)], l1 = join[2 * (TQ + row) + 1], both = fmaxf(m, m1);
+                    f0 = ex2(m - both);
+                    f1 = ex2(m1 - both);
+                    l = l * f0 + l1 * f1;
+                    m = both;
                 }
-                if (split) {  // unscaled sums, for the cluster
-                    if (there) {
-                        float* dst = part_o + (w * TQ + row) * R_LD;
+            }
+            if (!SPLIT && !ok) break;
+            if (SPLIT && !split && !mine) continue;
+            if (!SPLIT || (ok && mine)) {
+                tc_fence_after();
+                const float il = 1.f / l;
+#pragma unroll 1
+                for (int hd = packed ? w : 0; hd < (packed ? w + 1 : 2); hd++) {  // dimensions 32 hd .. 32 hd + 31
+                    const uint32_t from = (packed ? tO - w * T_WG_COLS : tO) + 32 * hd;
+                    uint32_t o[32];
+                    tmem_ld32(from, o);
+                    if (two) {
+                        uint32_t o1[32];
+                        tmem_ld32(from + T_WG_COLS, o1);
+                        tc_wait_ld();
 #pragma unroll
-                        for (int i = 0; i < 16; i++)
-                            *reinterpret_cast<float4*>(dst + 4 * i) =
-                                make_float4(__uint_as_float(o[4 * i]), __uint_as_float(o[4 * i + 1]), __uint_as_float(o[4 * i + 2]),
-                                            __uint_as_float(o[4 * i + 3]));
-                        part_ml[2 * (w * TQ + row)] = m;
-                        part_ml[2 * (w * TQ + row) + 1] = l;
+                        for (int i = 0; i < 32; i++)
+                            o[i] = __float_as_uint(__uint_as_float(o[i]) * f0 + __uint_as_float(o1[i]) * f1);
+                    } else {
+                        tc_wait_ld();
                     }
-                } else {
-                    const float il = 1.f / l;
-                    uint32_t oh[32];
-#pragma unroll
-                    for (int i = 0; i < 32; i++) oh[i] = pack_h2(__uint_as_float(o[2 * i]) * il, __uint_as_float(o[2 * i + 1]) * il);
-                    if (a.lse && there) a.lse[(size_t)h * a.lse_ld + grow] = (m + log2f(l)) * kLn2;
-                    if (there) {
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0 && (packed || hd == 1)) {  // eight arrivals for either
+                        mbar_arrive(bar(B_OFREE + (packed ? 0 : w)));
+                        if (!packed) mbar_arrive(bar(B_OFREE + w));
+                        if (two) mbar_arrive(bar(B_OFREE + 1));
+                    }
+                    if (!there) continue;
+                    if (split) {  // unscaled sums, for the cluster
+                        float* dst = part_o + ((packed ? 0 : w) * TQ + row) * R_LD + 32 * hd;
 #pragma unroll
                         for (int i = 0; i < 8; i++)
-                            *reinterpret_cast<uint4*>(a.O + grow * a.ldo + h * 64 + i * 8) =
-                                make_uint4(oh[4 * i], oh[4 * i + 1], oh[4 * i + 2], oh[4 * i + 3]);
+                            *reinterpret_cast<float4*>(dst + 4 * i) =
+                                make_float4(__uint_as_float(o[4 * i]), __uint_as_float(o[4 * i + 1]),
+                                            __uint_as_float(o[4 * i + 2]), __uint_as_float(o[4 * i + 3]));
+                    } else {
+                        uint4* dst = reinterpret_cast<uint4*>(a.O + grow * a.ldo + h * 64 + 32 * hd);
+#pragma unroll
+                        for (int i = 0; i < 4; i++) {
+                            uint32_t oh[4];
+#pragma unroll
+                            for (int e = 0; e < 4; e++)
+                                oh[e] = pack_h2(__uint_as_float(o[8 * i + 2 * e]) * il, __uint_as_float(o[8 * i + 2 * e + 1]) * il);
+                            dst[i] = make_uint4(oh[0], oh[1], oh[2], oh[3]);
+                        }
+                    }
                 }
+                if (there && !(packed && w == 1)) {
+                    if (split) {
+                        part_ml[2 * (w * TQ + row)] = m;
+                        part_ml[2 * (w * TQ + row) + 1] = l;
+                    } else if (a.lse) {
+                        a.lse[(size_t)h * a.lse_ld + grow] = (m + log2f(l)) * kLn2;
+                    }
                 }
             }
             if (split) {
@@ -1181,8 +1187,9 @@ __global__ void __launch_bounds__(T_THREADS, 1)
                 cluster_sync();  // the sums of every CTA are in its shared memory
                 // join them, in their order: each CTA writes its share of the rows
                 const int per = (un.all_tiles() + ranks - 1) / ranks, parts = (un.all_tiles() - 1) / per + 1, share = TQ / ranks;
-                if (!(packed ? w == 1 : w >= un.q_tiles())) {
-                    for (int i = row; i < share * 16; i += TQ) {
+                if (packed || w < un.q_tiles()) {
+                    const int wp = packed ? 0 : w, team = packed ? 2 * TQ : TQ;
+                    for (int i = packed ? w * TQ + row : row; i < share * 16; i += team) {
                         const int r = rank * share + (i >> 4), d = (i & 15) * 4;
                         if (r >= rows) break;
                         float pm[R_CLUSTER], pl[R_CLUSTER];
@@ -1193,9 +1200,9 @@ __global__ void __launch_bounds__(T_THREADS, 1)
                             pl[c] = 0.f;
                             v[c] = make_float4(0.f, 0.f, 0.f, 0.f);
                             if (c < parts) {
-                                pm[c] = ld_cluster_f32(mapa_shared(smem_u32(part_ml + 2 * (w * TQ + r)), c));
-                                pl[c] = ld_cluster_f32(mapa_shared(smem_u32(part_ml + 2 * (w * TQ + r) + 1), c));
-                                v[c] = ld_cluster_f32x4(mapa_shared(smem_u32(part_o + (w * TQ + r) * R_LD + d), c));
+                                pm[c] = ld_cluster_f32(mapa_shared(smem_u32(part_ml + 2 * (wp * TQ + r)), c));
+                                pl[c] = ld_cluster_f32(mapa_shared(smem_u32(part_ml + 2 * (wp * TQ + r) + 1), c));
+                                v[c] = ld_cluster_f32x4(mapa_shared(smem_u32(part_o + (wp * TQ + r) * R_LD + d), c));
                             }
                         }
                         float M = -INFINITY, L = 0.f;
