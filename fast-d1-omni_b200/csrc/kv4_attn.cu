@@ -1961,6 +1961,10 @@ int launch_tc(Kv4Args& a, int max_q, int max_keys, cudaStream_t st) {
     while (ranks > 1 && ((long long)(ranks - 1) * 2 * TKV >= max_keys ||
                          units > clusters_at_once(k_kv4_attn_tc<true>, T_THREADS, T_SMEM, ranks, found)))
         ranks /= 2;
+    // the clusters' barriers and joins cost as much as five key tiles (100 packed rows: over 600 keys 11.8 us alone and 14.6
+    // in twos, over 800 13.6 and in fours 13.0, over 1600 19.5, in twos 18.3 and in fours 15.0)
+    const long long key_tiles = ((long long)max_keys + TKV - 1) / TKV;
+    if (key_tiles * (ranks - 1) < 5 * ranks) ranks = 1;
     a.ranks = ranks;
     if (ranks == 1) {
         launch_pdl(k_kv4_attn_tc<false>, (int)(units < sms ? units : sms), T_THREADS, T_SMEM, st, tq, tqp, tk, tv, a);
@@ -1983,7 +1987,7 @@ int launch_mass_tc(Kv4Args& a, int max_q, int max_len, cudaStream_t st) {
     // sequence of 4000 rows, 500 keys: 18 us, and 42 without; 16 units in clusters of 8, which do not all fit: 17 us, of 4: 10)
     int ranks = R_CLUSTER;
     static int found[64][R_CLUSTER + 1];
-    while (ranks > 1 && ((long long)(ranks - 1) * (MQ / a.group) >= max_q ||
+    while (ranks > 1 && ((long long)max(2, ranks - 1) * (MQ / a.group) >= max_q ||  // (two tiles alone: 7.5 us, and 8.0)
                          units > clusters_at_once(k_kv4_mass_tc<true>, M_THREADS, M_SMEM, ranks, found)))
         ranks /= 2;
     a.ranks = ranks;
