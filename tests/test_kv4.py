@@ -359,6 +359,41 @@ def test_attend_sharp_and_shared(pkg, gpu_lib, max_q):
     assert gpu_lib.d1_kv4_error() == 0
 
 
+SHARED_OUT = {
+    "packed": ([30, 1, 0, 50], [1300, 0, 128, 257], [30, 0, 0, 1], 2, 2),
+    "pairs": ([200, 129], [700, 5], [50, 0], 1, 2),
+    "single": ([300, 20], [257, 640], [0, 20], 1, 1),
+    "three heads": ([50, 90, 3], [1000, 3, 129], [0, 90, 0], 1, 3),
+    "long": ([64], [9000], [64], 2, 2),
+}
+
+
+@gpu
+@pytest.mark.parametrize("max_keys", [1300, 3500, 40000])
+@pytest.mark.parametrize("max_q", [1, 12, 70, 128])
+@pytest.mark.parametrize("name", SHARED_OUT)
+def test_attend_shared_out(pkg, gpu_lib, name, max_q, max_keys):
+    """Clusters of CTAs share out the keys, be there fewer than CTAs, none, or more units than clusters; a bad entry among
+    the others is skipped. The same call gives the same bits."""
+    q, ext, kv, kvh, group = SHARED_OUT[name]
+    rng = np.random.default_rng(len(name) + 40)
+    h = kvh * group
+    c = Caches(rng, ext, kvh, -(-max(ext) // 8) * 8)
+    x, starts = poisoned_rows(rng, [max(a, b) for a, b in zip(q, kv)], (h + 2 * kvh) * 64)
+    seqs = [dict(q_start=s, q_len=a, kv_start=s, kv_len=b) for s, a, b in zip(starts, q, kv)]
+    want = plain_attend(x, seqs, c, list(range(len(q))), kvh, group, 0.125, True)
+    first = None
+    for bad in ([], [dict(q_start=0, q_len=5, kv_start=-1, kv_len=7)]):
+        for _ in range(2):
+            O, L = attend(gpu_lib, x, table(pkg, bad + seqs, c, [None] * len(bad) + list(range(len(q)))), len(bad + seqs), kvh,
+                          group, 0.125, max_q, max_keys)
+            assert (gpu_lib.d1_kv4_error() != 0) == bool(bad)
+            check_attend(O, L, want, h)
+            if not bad:
+                assert first is None or torch.equal(O, first)
+                first = O
+
+
 @gpu
 @pytest.mark.parametrize("max_q", HINTS)
 def test_lse_of_few_keys(pkg, gpu_lib, max_q):
