@@ -463,14 +463,15 @@ __global__ void __launch_bounds__(R_WARPS * 32, NT == 1 ? 4 : 2) k_kv4_attn_rows
 //              codes loaded straight into their registers, a tile ahead; 2200 with two warps to a tile, in turn.)
 //   9, 14      MMA issuers of warpgroups 0 and 1, one thread each: S = Q K^T (both in shared memory), O += P V (P in
 //              TMEM). Warp 9 also keeps the TMEM. (One issuer for both: each warpgroup then waits for the other's P.)
-// The softmax warps take 192 registers, the others 64.
+// The softmax warps take 200 registers, the others 56 (four documents of 2048 rows over 4096 keys: 253.5 us; 256.7 with
+// 192 and 64, 254 with 208 and 48, 272 with 184 and 72).
 // TMEM (512 columns), warpgroup w at 256 w: S in 128 columns, P in 64, O in 64. Both warpgroups' columns share the lanes,
-// so that a packed unit is joined by the first reading the second's O.
+// so that a packed unit is joined by each reading the other's O.
 constexpr int TQ = 128, TKV = 128, T_QSLOTS = 2, T_STAGES = 4, T_RAW_STAGES = 3, T_EXPANDERS = 128, T_THREADS = 512;
 constexpr int T_QT_BYTES = TQ * 128, T_KV_BYTES = TKV * 128;
 constexpr int T_RAW_V = TKV * 32, T_RAW_KP = 2 * TKV * 32, T_RAW_VP = T_RAW_KP + TKV * 2, T_RAW_BYTES = T_RAW_VP + TKV * 2;
 constexpr int T_ENTRIES = 256;  // of the table of units
-constexpr int T_SOFTMAX_REGS = 192, T_OTHER_REGS = 64;
+constexpr int T_SOFTMAX_REGS = 200, T_OTHER_REGS = 56;
 static_assert(T_SOFTMAX_REGS + T_OTHER_REGS <= 2 * 128, "what the launch of 512 threads, 128 registers each, has");
 constexpr uint32_t T_TMEM_COLS = 512, T_WG_COLS = 256, T_P_COL = TKV, T_O_COL = TKV + TKV / 2;
 enum : int {
@@ -609,9 +610,8 @@ struct Unit {
     }
     __device__ int head(int w) const { return h + (mode == kPair ? w : 0); }
     __device__ int rows(const Kv4Args& a, int w) const { return mode == kPacked ? q_len * a.group : q_len - row0(w); }
-    // key tiles that warpgroup w takes: all, or of a packed unit every other one; warpgroup 0, which finishes the unit, has
-    // the fewer where their number is odd, unless there is only one
-    __device__ int first_of(int w) const { return mode != kPacked ? 0 : tiles() > 1 ? 1 - w : w; }
+    // key tiles that warpgroup w takes: all, or of a packed unit every other one, from w
+    __device__ int first_of(int w) const { return mode == kPacked ? w : 0; }
     __device__ int tiles_of(int w) const {
         return mode == kPacked ? (tiles() - first_of(w) + 1) / 2 : w < q_tiles() ? tiles() : 0;
     }
