@@ -21,34 +21,35 @@ constexpr int kMaxGridZ = 65535;
 __device__ __forceinline__ void table_error() { atomicExch(&g_kv4_err, kErrTable); }
 
 // ------------------------------------------------------------------------------------------------ append, load
-// Bound by HBM. 8 lanes per vector of 64 dimensions (8 elements, one word of codes a lane), 4 consecutive rows of one kv
-// head per warp, so that a warp's codes are one 128-byte run of the cache. A CTA takes 32 rows of (K or V, kv head) for
-// each of PER to a thread, whose loads go out together. Append: 8 where that still occupies every SM twice, otherwise 2
-// (32 x 4096 rows, 8 kv heads: 78 us with 8, 85 with 4, 91 with 2, and 53 at the copy rate; one prefix of 1025 rows: 3.8,
-// 2.9 and 2.5 us). Load: 4 (56, 57 and 66 us with 4, 8 and 2, and 53 at the copy rate).
-constexpr int A_STEP = 32;
+// Bound by HBM, append in a small call by issue slots as well. Append: 4 lanes per vector of 64 dimensions (twice 8
+// elements, two words of codes a lane; the parameter's arithmetic, which every lane does, was a third of it with 8 lanes: 78
+// us), 8 consecutive rows of one kv head per warp; a CTA takes 64 rows of (K or V, kv head) for each of PER to a thread,
+// whose loads go out together: 4 where that still occupies every SM twice, otherwise 1 (32 x 4096 rows, 8 kv heads: 62 us
+// with 4, 69 with 2, 83 with 8, and 53 at the copy rate; one prefix of 1025 rows: 2.5 us). Load: 8 lanes per vector, 4 rows
+// to a thread (56, 57 and 66 us with 4, 8 and 2, and 53 at the copy rate).
+constexpr int A_ROWS = 64, A_STEP = 32;
 
 __device__ __forceinline__ bool append_ok(const D1Kv4Seq& s) {
     return s.kv_start >= 0 && s.kv_len >= 0 && kv4_seq_ok(s) && (long long)s.ext_len + s.kv_len <= s.ext_cap;
 }
 
-// One vector's word of codes (this lane's 8 elements) and parameter. round(x / step) without a division per element:
+// Words of codes of one vector (this lane's twice 8 elements of it; four lanes a vector) and its parameter. round(x / step) without a division per element:
 // t = x * (1 / step) is within 2^-18 of the quotient q, |q| < 15.6. As x has 11 significant bits and step 7, q either is
 // k + 1/2 exactly or at least 2^-13 away from it; 768 + t, whose last place is 2^-14, is therefore 768 + k + 1/2 in the
 // first case and on q's side of it in the second, and rounds as q does. (hi - lo) / 15 is rounded correctly, since whole
 // multiples of 15 are common: one step of correction after the product with 1 / 15.
-__device__ __forceinline__ void quantise8(const uint4& raw, uint32_t& word, uint32_t& par) {
-    const __half2* x2 = reinterpret_cast<const __half2*>(&raw);
+__device__ __forceinline__ void quantise16(const uint4 (&raw)[2], uint32_t (&word)[2], uint32_t& par) {
+    const __half2* x2 = reinterpret_cast<const __half2*>(raw);
     __half2 mn = __float2half2_rn(0.f), mx = mn;  // the range, with zero in it; NaN stays
 #pragma unroll
-    for (int i = 0; i < 4; i++) {
+    for (int i = 0; i < 8; i++) {
         mn = __hmin2_nan(mn, x2[i]);
         mx = __hmax2_nan(mx, x2[i]);
     }
     __half2 ends = __halves2half2(__hneg(__hmin_nan(__low2half(mn), __high2half(mn))),
                                   __hmax_nan(__low2half(mx), __high2half(mx)));  // (-lo, hi)
 #pragma unroll
-    for (int o = 1; o < 8; o <<= 1) ends = __hmax2_nan(ends, __shfl_xor_sync(D1_FULL_MASK, ends, o));
+    for (int o = 1; o < 4; o <<= 1) ends = __hmax2_nan(ends, __shfl_xor_sync(D1_FULL_MASK, ends, o));
     const float nlo = __low2float(ends), hi = __high2float(ends), range = hi + nlo;
     constexpr float kFifteenth = 1.f / 15.f;
     float want = range * kFifteenth;
@@ -64,20 +65,23 @@ __device__ __forceinline__ void quantise8(const uint4& raw, uint32_t& word, uint
     if (step > 4096.f) top = min(15, __float2int_rd(__fdiv_rn(65504.f, step)));
     const int least = kBias + max(-top, -zero), most = kBias + min(top, 15 - zero);
     const uint64_t inv2 = f2_pack(inv, inv);
-    uint32_t w = 0;
 #pragma unroll
-    for (int i = 0; i < 4; i++) {
-        const float2 f = __half22float2(x2[i]);
-        float a, b;
-        f2_unpack(f2_add(f2_fma(f2_pack(f.x, f.y), inv2, f2_pack(768.f, 768.f)), f2_pack(12582912.f, 12582912.f)), a, b);
-        // the biases go out of all eight places together
-        w += (uint32_t)max(least, min(most, __float_as_int(a))) << (4 * i);
-        w += (uint32_t)max(least, min(most, __float_as_int(b))) << (16 + 4 * i);
+    for (int k = 0; k < 2; k++) {
+        uint32_t w = 0;
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const float2 f = __half22float2(x2[4 * k + i]);
+            float a, b;
+            f2_unpack(f2_add(f2_fma(f2_pack(f.x, f.y), inv2, f2_pack(768.f, 768.f)), f2_pack(12582912.f, 12582912.f)), a, b);
+            // the biases go out of all eight places together
+            w += (uint32_t)max(least, min(most, __float_as_int(a))) << (4 * i);
+            w += (uint32_t)max(least, min(most, __float_as_int(b))) << (16 + 4 * i);
+        }
+        word[k] = w + (uint32_t)(zero - kBias) * 0x11111111u;
     }
-    word = w + (uint32_t)(zero - kBias) * 0x11111111u;
     par = (uint32_t)__half_as_ushort(__float2half_rn(step)) | (uint32_t)zero;
     if (!(range <= 131008.f)) {  // NaN or an infinity among them: a NaN step
-        word = 0;
+        word[0] = word[1] = 0;
         par = 0x7e00u;
     }
 }
@@ -86,7 +90,7 @@ template <int PER>
 __global__ void __launch_bounds__(256) k_kv4_append(const __half* __restrict__ K, const __half* __restrict__ V,
                                                     int ldkv, const D1Kv4Seq* __restrict__ seqs, int n_seqs) {
     pdl_entry();
-    const int sub = threadIdx.x & 7, row = threadIdx.x >> 3, g = blockIdx.y >> 1;
+    const int sub = threadIdx.x & 3, row = threadIdx.x >> 2, g = blockIdx.y >> 1;
     const bool is_v = blockIdx.y & 1;
     for (int sq = blockIdx.z; sq < n_seqs; sq += gridDim.z) {
         const D1Kv4Seq s = seqs[sq];
@@ -98,21 +102,27 @@ __global__ void __launch_bounds__(256) k_kv4_append(const __half* __restrict__ K
         const size_t at = (size_t)g * s.ext_cap + s.ext_len;
         uint32_t* codes = reinterpret_cast<uint32_t*>(is_v ? s.v4 : s.k4) + at * 8 + sub;
         uint16_t* pars = reinterpret_cast<uint16_t*>(is_v ? s.vp : s.kp) + at;
-        for (int r0 = blockIdx.x * (A_STEP * PER); r0 < s.kv_len; r0 += gridDim.x * (A_STEP * PER)) {
-            uint4 raw[PER];
+        for (int r0 = blockIdx.x * (A_ROWS * PER); r0 < s.kv_len; r0 += gridDim.x * (A_ROWS * PER)) {
+            uint4 raw[PER][2];
 #pragma unroll
             for (int i = 0; i < PER; i++) {
-                const int r = r0 + i * A_STEP + row;
-                raw[i] = r < s.kv_len ? __ldcs(reinterpret_cast<const uint4*>(src + (size_t)r * ldkv)) : make_uint4(0, 0, 0, 0);
+                const int r = r0 + i * A_ROWS + row;
+                raw[i][0] = raw[i][1] = make_uint4(0, 0, 0, 0);
+                if (r < s.kv_len) {
+                    const uint4* x = reinterpret_cast<const uint4*>(src + (size_t)r * ldkv);
+                    raw[i][0] = __ldcs(x);
+                    raw[i][1] = __ldcs(x + 4);
+                }
             }
 #pragma unroll
             for (int i = 0; i < PER; i++) {
-                if (r0 + i * A_STEP >= s.kv_len) break;
-                const int r = r0 + i * A_STEP + row;
-                uint32_t word, par;
-                quantise8(raw[i], word, par);
+                if (r0 + i * A_ROWS >= s.kv_len) break;
+                const int r = r0 + i * A_ROWS + row;
+                uint32_t word[2], par;
+                quantise16(raw[i], word, par);
                 if (r < s.kv_len) {
-                    codes[(size_t)r * 8] = word;
+                    codes[(size_t)r * 8] = word[0];
+                    codes[(size_t)r * 8 + 4] = word[1];
                     if (sub == 0) pars[r] = (uint16_t)par;
                 }
             }
@@ -362,8 +372,8 @@ bool bad_rows(const void* K, const void* V, int ldkv, int kv_heads) {
     return !K || !V || (((uintptr_t)K | (uintptr_t)V) & 15) || ldkv % 8 || ldkv < kv_heads * 64;
 }
 
-dim3 row_grid(int max_rows, int per, int kv_heads, int n_seqs) {
-    const int rows = A_STEP * per, x = max_rows <= rows ? 1 : max_rows > 4096 * rows ? 4096 : (max_rows - 1) / rows + 1;
+dim3 row_grid(int max_rows, int rows, int kv_heads, int n_seqs) {
+    const int x = max_rows <= rows ? 1 : max_rows > 4096 * rows ? 4096 : (max_rows - 1) / rows + 1;
     return dim3(x, kv_heads * 2, n_seqs < kMaxGridZ ? n_seqs : kMaxGridZ);
 }
 
@@ -373,11 +383,11 @@ extern "C" int d1_kv4_append(const d1_half* K, const d1_half* V, int ldkv, const
                              int max_rows, int kv_heads, cudaStream_t st) {
     if (n_seqs <= 0) return n_seqs == 0 ? 0 : -1;
     if (!seqs || max_rows < 0 || kv_heads <= 0 || kv_heads > 4096 || bad_rows(K, V, ldkv, kv_heads)) return -1;
-    const dim3 g8 = row_grid(max_rows, 8, kv_heads, n_seqs);
-    if ((long long)g8.x * g8.y * g8.z >= 2 * 148)
-        launch_pdl(k_kv4_append<8>, g8, 256, 0, st, K, V, ldkv, seqs, n_seqs);
+    const dim3 g4 = row_grid(max_rows, 4 * A_ROWS, kv_heads, n_seqs);
+    if ((long long)g4.x * g4.y * g4.z >= 2 * 148)
+        launch_pdl(k_kv4_append<4>, g4, 256, 0, st, K, V, ldkv, seqs, n_seqs);
     else
-        launch_pdl(k_kv4_append<2>, row_grid(max_rows, 2, kv_heads, n_seqs), 256, 0, st, K, V, ldkv, seqs, n_seqs);
+        launch_pdl(k_kv4_append<1>, row_grid(max_rows, A_ROWS, kv_heads, n_seqs), 256, 0, st, K, V, ldkv, seqs, n_seqs);
     return (int)cudaGetLastError();
 }
 
@@ -385,7 +395,7 @@ extern "C" int d1_kv4_load(const D1Kv4Seq* seqs, int n_seqs, int max_rows, int k
                            int ldkv, cudaStream_t st) {
     if (n_seqs <= 0) return n_seqs == 0 ? 0 : -1;
     if (!seqs || max_rows < 0 || kv_heads <= 0 || kv_heads > 4096 || bad_rows(K, V, ldkv, kv_heads)) return -1;
-    launch_pdl(k_kv4_load<4>, row_grid(max_rows, 4, kv_heads, n_seqs), 256, 0, st, seqs, n_seqs, K, V, ldkv);
+    launch_pdl(k_kv4_load<4>, row_grid(max_rows, 4 * A_STEP, kv_heads, n_seqs), 256, 0, st, seqs, n_seqs, K, V, ldkv);
     return (int)cudaGetLastError();
 }
 
