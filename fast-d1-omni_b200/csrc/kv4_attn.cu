@@ -1255,6 +1255,8 @@ __global__ void __launch_bounds__(256, 2) k_kv4_mass_rows(const Kv4Args a) {
     __shared__ uint32_t same[8];        // and which are of this mass array
     pdl_entry();
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, r = lane >> 2, t = lane & 3, g = blockIdx.y;
+    const int q_first = r / a.group, h_first = g * a.group + r % a.group, q_step = 8 / a.group, h_step = 8 % a.group;
+    const int h_end = (g + 1) * a.group;
     for (int sq = blockIdx.z; sq < a.n_seqs; sq += gridDim.z) {
         const D1Kv4Seq s = a.seqs[sq];
         if (!s.mass) continue;
@@ -1331,7 +1333,7 @@ __global__ void __launch_bounds__(256, 2) k_kv4_mass_rows(const Kv4Args a) {
                         const int2 p = peers[32 * i + __ffs(left) - 1];
                         any = true;
                         const uint32_t n_rows = (uint32_t)p.y * (uint32_t)a.group;
-                        int q = p.x + r / a.group, h = g * a.group + r % a.group;  // of the packed row fetched next
+                        int q = p.x + q_first, h = h_first;  // of the packed row fetched next
                         uint4 n0, n1;
                         float nl;
                         auto fetch = [&](uint32_t row) {
@@ -1343,9 +1345,9 @@ __global__ void __launch_bounds__(256, 2) k_kv4_mass_rows(const Kv4Args a) {
                                 n1 = __ldg(src + 1);
                                 nl = __ldg(a.lse + (size_t)h * a.lse_ld + q);
                             }
-                            q += 8 / a.group;
-                            h += 8 % a.group;
-                            if (h >= (g + 1) * a.group) {
+                            q += q_step;
+                            h += h_step;
+                            if (h >= h_end) {
                                 h -= a.group;
                                 q++;
                             }
