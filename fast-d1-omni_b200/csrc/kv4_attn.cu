@@ -70,11 +70,11 @@ __device__ __forceinline__ void ex2_fma2(float x0, float x1, float& p0, float& p
 // Bound: the issue slots (about 800 instructions a tile, half of them for the expansion of codes). Tried and dropped: the
 // codes as fp16 subnormals (code * 2^-24 or * 2^-20, no subtraction), with zeros and steps taken care of by the sums: an
 // eighth fewer instructions, but the MMA aligns its fp32 sums to the operands' exponent, and their last 10 bits are lost.
-constexpr int R_KEYS = 64, R_WARPS = 4, R_CLUSTER = 8, R_LD = 68;  // padded row of the joining buffers (floats)
+constexpr int R_KEYS = 64, R_CLUSTER = 8, R_LD = 68;  // padded row of the joining buffers (floats)
 
-template <int NT>
+template <int NT, int W>
 constexpr int rows_smem() {
-    return (R_WARPS + 1) * 8 * NT * (R_LD + 2) * 4;
+    return (W + 1) * 8 * NT * (R_LD + 2) * 4;
 }
 
 __device__ __forceinline__ uint32_t movmatrix_trans(uint32_t x) {
@@ -96,16 +96,16 @@ __device__ __forceinline__ float4 ld_cluster_f32x4(uint32_t addr) {
     return v;
 }
 
-template <int NT>
-__global__ void __launch_bounds__(R_WARPS * 32, NT == 1 ? 4 : 2) k_kv4_attn_rows(const Kv4Args a) {
+template <int NT, int W>
+__global__ void __launch_bounds__(W * 32, (NT == 1 ? 16 : 8) / W) k_kv4_attn_rows(const Kv4Args a) {
     extern __shared__ __align__(16) float r_smem[];
     constexpr int NR = 8 * NT;
     float* sO = r_smem;                               // [warp][NR][R_LD]
-    float* cO = sO + R_WARPS * NR * R_LD;             // [NR][R_LD]: the CTA's sum, read by the cluster
+    float* cO = sO + W * NR * R_LD;             // [NR][R_LD]: the CTA's sum, read by the cluster
     float* sM = cO + NR * R_LD;                       // [warp][NR]
-    float* cM = sM + R_WARPS * NR;                    // [NR]
+    float* cM = sM + W * NR;                    // [NR]
     float* sL = cM + NR;                              // [warp][NR]
-    float* cL = sL + R_WARPS * NR;                    // [NR]
+    float* cL = sL + W * NR;                    // [NR]
     pdl_entry();
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, r = lane >> 2, t = lane & 3, g = blockIdx.y;
     const int rank = (int)cluster_ctarank(), ranks = a.ranks;
@@ -169,7 +169,7 @@ __global__ void __launch_bounds__(R_WARPS * 32, NT == 1 ? 4 : 2) k_kv4_attn_rows
             };
             int tile = tile0 + warp;
             if (tile < tile1 && tile < ext_tiles) fetch_k(tile);
-            for (; tile < tile1; tile += R_WARPS) {
+            for (; tile < tile1; tile += W) {
                 const bool ext = tile < ext_tiles;
                 const int key0 = (ext ? tile : tile - ext_tiles) * R_KEYS;
                 const int left = (ext ? s.ext_len : s.kv_len) - key0;  // keys of this tile: min(left, 64), at least 1
@@ -229,7 +229,7 @@ __global__ void __launch_bounds__(R_WARPS * 32, NT == 1 ? 4 : 2) k_kv4_attn_rows
                                           sc[nt][i][2 * hf], sc[nt][i][2 * hf + 1]);
                         }
                     }
-                    if (tile + R_WARPS < tile1 && tile + R_WARPS < ext_tiles) fetch_k(tile + R_WARPS);
+                    if (tile + W < tile1 && tile + W < ext_tiles) fetch_k(tile + W);
                 } else {
                     const __half* kr = a.K + (size_t)(s.kv_start + key0) * a.ldkv + g * 64 + 16 * t;
 #pragma unroll
@@ -372,8 +372,8 @@ __global__ void __launch_bounds__(R_WARPS * 32, NT == 1 ? 4 : 2) k_kv4_attn_rows
                     make_uint2(pack_h2(x.x * il, x.y * il), pack_h2(x.z * il, x.w * il));
                 if (a.lse && d == 0) a.lse[(size_t)h * a.lse_ld + q] = tiles ? (M + log2f(L)) * kLn2 : -INFINITY;
             };
-            const int warps = min(R_WARPS, tile1 - tile0);  // those with tiles
-            for (int i = tid; i < NR * 16; i += R_WARPS * 32) {
+            const int warps = min(W, tile1 - tile0);  // those with tiles
+            for (int i = tid; i < NR * 16; i += W * 32) {
                 const int row = i >> 4, d = (i & 15) * 4;
                 if (base + row >= n_rows) break;
                 float M = -INFINITY, L = 0.f;
@@ -406,7 +406,7 @@ __global__ void __launch_bounds__(R_WARPS * 32, NT == 1 ? 4 : 2) k_kv4_attn_rows
             __syncwarp();
             cluster_sync();
             const int parts = tiles == 0 ? 0 : (tiles - 1) / per + 1;  // CTAs with tiles
-            for (int i = rank * R_WARPS * 32 + tid; i < NR * 16; i += ranks * R_WARPS * 32) {
+            for (int i = rank * W * 32 + tid; i < NR * 16; i += ranks * W * 32) {
                 const int row = i >> 4, d = (i & 15) * 4;
                 if (base + row >= n_rows) break;
                 float cm[R_CLUSTER], cl[R_CLUSTER];
@@ -1897,27 +1897,54 @@ int launch_clusters(void (*kernel)(KP...), dim3 grid, int block, size_t smem, in
     return (int)cudaGetLastError();
 }
 
+template <int NT, int W>
+bool rows_opt_in() {
+    static unsigned long long done = 0;
+    return smem_opt_in(k_kv4_attn_rows<NT, W>, rows_smem<NT, W>(), &done);
+}
+
+template <int NT, int W>
+int launch_rows_ranks(Kv4Args& a, long long x, int kv_heads, int z, int ranks, cudaStream_t st) {
+    if (!rows_opt_in<NT, W>()) return -1;
+    a.ranks = ranks;
+    return launch_clusters(k_kv4_attn_rows<NT, W>, dim3((unsigned)x * ranks, kv_heads, z), W * 32, rows_smem<NT, W>(), ranks, st,
+                           (const Kv4Args)a);
+}
+
+template <int NT, int W>
+int rows_clusters_at_once() {
+    static int found[64][R_CLUSTER + 1];
+    if (!rows_opt_in<NT, W>()) return 0;
+    return clusters_at_once(k_kv4_attn_rows<NT, W>, W * 32, rows_smem<NT, W>(), R_CLUSTER, found);
+}
+
 template <int NT>
 int launch_rows(Kv4Args& a, int max_q, int max_keys, int kv_heads, cudaStream_t st) {
-    static unsigned long long done = 0;
-    if (!smem_opt_in(k_kv4_attn_rows<NT>, rows_smem<NT>(), &done)) return -1;
     long long x = ((long long)max_q * a.group + 8 * NT - 1) / (8 * NT);
     x = x < 1 ? 1 : x > 65536 ? 65536 : x;
     const int z = a.n_seqs < 65535 ? a.n_seqs : 65535;
     // CTAs to a cluster: as many as are resident at once, and no more than the keys give a tile to every warp (16
     // sequences of 8 rows, 4096 keys, 2 CTAs to an SM: 24 us with 2, 33 with 1, 31 with 4 and 46 with 8; one token over
-    // 4097 keys: 8.5 us with 8, 11, 17 and 27 with 4, 2 and 1)
+    // 4097 keys, 4 warps to a CTA: 8.5 us with 8, 11, 17 and 27 with 4, 2 and 1)
     int ranks = R_CLUSTER;
     const long long tiles = ((long long)max_keys + R_KEYS - 1) / R_KEYS, slots = 148 * (NT == 1 ? 4 : 2);
     const long long ctas = x * kv_heads * z;
-    while (ranks > 1 && ((ranks / 2) * R_WARPS >= tiles || ctas * ranks > slots)) ranks /= 2;
+    while (ranks > 1 && ((ranks / 2) * 4 >= tiles || ctas * ranks > slots)) ranks /= 2;
     // where they leave more than a quarter of the room empty and the keys are long, twice as many, the rest of them as room
     // comes free (10, 20 and 40 tokens over 8192 to 16384 keys: 32, 72 and 123 us, otherwise 40, 82 and 164; but of 16
     // tiles a CTA 10 x 16 rows over 4096 keys: 31 us, otherwise 28; and of a fuller GPU, 32 tokens over 16384: 103 and 97)
     if (ranks < R_CLUSTER && ctas * ranks * 4 < slots * 3 && tiles >= 2 * ranks * 24) ranks *= 2;
-    a.ranks = ranks;
-    return launch_clusters(k_kv4_attn_rows<NT>, dim3((unsigned)x * ranks, kv_heads, z), R_WARPS * 32, rows_smem<NT>(), ranks, st,
-                           (const Kv4Args)a);
+    // more warps to a CTA where there are tiles for them and the GPU holds all of these clusters at once (one token: over 4097
+    // keys 6.8 us with 16 warps, 7.4 with 8, 8.3 with 4; over 60000 24, 31 and 48; two tokens, whose 16 clusters of 16 warps
+    // do not fit: over 4500 keys 8.3 with 8, 12.3 with 16)
+    if (ranks == R_CLUSTER) {
+        constexpr int MOST = NT == 1 ? 16 : 8;
+        if (NT == 1 && tiles > 8 * R_CLUSTER && ctas <= rows_clusters_at_once<NT, MOST>())
+            return launch_rows_ranks<NT, MOST>(a, x, kv_heads, z, ranks, st);
+        if (tiles > 4 * R_CLUSTER && ctas <= rows_clusters_at_once<NT, 8>())
+            return launch_rows_ranks<NT, 8>(a, x, kv_heads, z, ranks, st);
+    }
+    return launch_rows_ranks<NT, 4>(a, x, kv_heads, z, ranks, st);
 }
 
 // Q as [row][head][64], in boxes of the group's heads of `most` / group rows: the packed rows of a tile in their order, in
