@@ -1067,12 +1067,20 @@ __global__ void __launch_bounds__(T_THREADS, 1)
                 for (int e = 0; e < 4; e++) rs2[e] = f2_pack(0.f, 0.f);
                 uint32_t pr[TKV / 2];
 #pragma unroll
-                for (int i = 0; i < TKV / 2; i++) {
-                    float x0, x1;
-                    f2_unpack(f2_fma(f2_pack(__uint_as_float(sr[2 * i]), __uint_as_float(sr[2 * i + 1])), sc2, nm2), x0, x1);
-                    const float p0 = ex2(x0), p1 = ex2(x1);
-                    rs2[i & 3] = f2_add(rs2[i & 3], f2_pack(p0, p1));
-                    pr[i] = pack_h2(p0, p1);
+                for (int c64 = 0; c64 < 2; c64++) {
+                    if (c64 == 1 && n <= 64) {  // none of these keys is there
+#pragma unroll
+                        for (int i = 32; i < 64; i++) pr[i] = 0;
+                        break;
+                    }
+#pragma unroll
+                    for (int i = 32 * c64; i < 32 * c64 + 32; i++) {
+                        float x0, x1;
+                        f2_unpack(f2_fma(f2_pack(__uint_as_float(sr[2 * i]), __uint_as_float(sr[2 * i + 1])), sc2, nm2), x0, x1);
+                        const float p0 = ex2(x0), p1 = ex2(x1);
+                        rs2[i & 3] = f2_add(rs2[i & 3], f2_pack(p0, p1));
+                        pr[i] = pack_h2(p0, p1);
+                    }
                 }
                 if (c > 0) {  // P V of the tile before has read the P columns
                     if (!(ok = __all_sync(D1_FULL_MASK, mbar_wait(bar(B_ODONE + w), (c - 1) & 1, abort_flag)))) break;
