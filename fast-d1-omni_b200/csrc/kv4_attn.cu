@@ -464,7 +464,7 @@ __global__ void __launch_bounds__(W * 32, (NT == 1 ? 16 : 8) / W) k_kv4_attn_row
 //   9, 14      MMA issuers of warpgroups 0 and 1, one thread each: S = Q K^T (both in shared memory), O += P V (P in
 //              TMEM). Warp 9 also keeps the TMEM. (One issuer for both: each warpgroup then waits for the other's P.)
 // The softmax warps take 200 registers, the others 56 (four documents of 2048 rows over 4096 keys: 253.5 us; 256.7 with
-// 192 and 64, 254 with 208 and 48, 272 with 184 and 72).
+// 192 and 64, 254 with 208 and 48, 272 with 184 and 72; 251.5 now).
 // TMEM (512 columns), warpgroup w at 256 w: S in 128 columns, P in 64, O in 64. Both warpgroups' columns share the lanes,
 // so that a packed unit is joined by each reading the other's O.
 constexpr int TQ = 128, TKV = 128, T_QSLOTS = 2, T_STAGES = 4, T_RAW_STAGES = 3, T_EXPANDERS = 128, T_THREADS = 512;
@@ -1058,9 +1058,10 @@ __global__ void __launch_bounds__(T_THREADS, 1)
                         tmem_st8(tO + o8 * 8, o);
                     }
                 }
-                // P = 2^(s * scale - m), two scores at a time, and the row's sum in fp32. (An eighth of the exponentials on the
-                // FMA pipe: documents 258 -> 253 us with a polynomial of degree 3, whose 7.5e-5 showed in the log-sum-exp;
-                // 259 with degree 5.)
+                // P = 2^(s * scale - m), two scores at a time, and the row's sum in fp32; nothing for the upper half of a tile
+                // without keys there (26 x 176 rows over 7 keys 18.4 -> 17.5 us; in quarters 17.3, but documents 252 -> 256).
+                // (An eighth of the exponentials on the FMA pipe: documents 258 -> 253 us with a polynomial of degree 3, whose
+                // 7.5e-5 showed in the log-sum-exp; 259 with degree 5.)
                 const uint64_t sc2 = f2_pack(a.scale_log2, a.scale_log2), nm2 = f2_pack(-m_use, -m_use);
                 uint64_t rs2[4];
 #pragma unroll
