@@ -896,13 +896,24 @@ __global__ void __launch_bounds__(T_THREADS, 1)
                     if (!(ok = mbar_wait(bar(B_QFULL + qs), (qi / T_QSLOTS) & 1, abort_flag))) return;
                     const uint64_t dq = smem_desc_k128(smem_u32(sQ + qs * 2 * T_QT_BYTES) + (un.mode == kPacked ? 0 : w * T_QT_BYTES));
                     auto kv_addr = [&](int j) { return smem_u32(sKV + ((ki + j) % T_STAGES) * 2 * T_KV_BYTES); };
-                    auto kv_ready = [&](int j) {
-                        return mbar_wait(bar(B_KVFULL + (ki + j) % T_STAGES), ((ki + j) / T_STAGES) & 1, abort_flag);
+                    // Sees its tiles up to j full, one after the other (wait: or only those that are, at once). Both issuers see
+                    // every tile and give B_KVEMPTY an arrival for each, so that no stage's phase passes unseen: by its parity
+                    // a phase cannot be told from the one two before it. A tile without MMAs of this issuer goes back at once.
+                    int seen = 0;
+                    auto see = [&](int j, bool wait) {
+                        for (; seen <= j; seen++) {
+                            const int x = ki + seen, st = x % T_STAGES;
+                            if (!(wait ? mbar_wait(bar(B_KVFULL + st), (x / T_STAGES) & 1, abort_flag)
+                                       : mbar_test(bar(B_KVFULL + st), (x / T_STAGES) & 1)))
+                                return false;
+                            if (mine == 0 || (step == 2 && (seen & 1) != w)) mbar_arrive(bar(B_KVEMPTY + st));
+                        }
+                        return true;
                     };
                     // S of its i-th tile, once the softmax has read the one before
                     auto issue_s = [&](int i) {
                         const int c = cnt + i;
-                        if (!kv_ready(first + i * step)) return false;
+                        if (!see(first + i * step, true)) return false;
                         if (c > 0 && !mbar_wait(bar(B_SFREE + w), (c - 1) & 1, abort_flag)) return false;
                         tc_fence_after();
                         const uint64_t dk = smem_desc_k128(kv_addr(first + i * step));
@@ -911,16 +922,16 @@ __global__ void __launch_bounds__(T_THREADS, 1)
                         tc_commit(bar(B_SFULL + w));
                         return true;
                     };
-                    const bool both = un.mode != kPacked && un.q_tiles() == 2;  // the other issuer's MMAs read the tiles, too
                     if (mine > 0) ok = issue_s(0);
                     for (int i = 0; i < mine && ok; i++) {
                         const int j = first + i * step, c = cnt + i;
                         // the next S computes while the softmax works on tile i; where its keys are late, P V goes first (it
                         // frees a stage that they may be waiting for)
                         bool s_next = i + 1 == mine;
+                        const int next = s_next ? nt - 1 : j + step;  // meanwhile it sees the tiles up to its next, or the last ones
                         const uint64_t t0 = globaltimer_ns();
                         while (true) {
-                            if (!s_next && mbar_test(bar(B_KVFULL + (ki + j + step) % T_STAGES), ((ki + j + step) / T_STAGES) & 1)) {
+                            if (see(next, false) && !s_next) {
                                 if (!(ok = issue_s(i + 1))) break;
                                 s_next = true;
                             }
@@ -940,11 +951,11 @@ __global__ void __launch_bounds__(T_THREADS, 1)
                             tc_mma_f16_ts(tO, tP + k * 8, dv + k * (2048 >> 4), IDESC_O, (i | k) != 0);
                         tc_commit(bar(B_ODONE + w));
                         tc_commit(bar(B_KVEMPTY + (ki + j) % T_STAGES));
-                        if (!both) tc_commit(bar(B_KVEMPTY + (ki + j) % T_STAGES));
                         if (!s_next && !(ok = issue_s(i + 1))) break;
                     }
                     if (!ok) return;
                     tc_commit(bar(B_QEMPTY + qs));
+                    if (!(ok = see(nt - 1, true))) return;
                     ki += nt;
                     qi++;
                     cnt += mine;

@@ -802,3 +802,41 @@ def test_step_captured_and_on_two_streams(pkg, gpu_lib, max_q):
     for a, b in zip((steps[0].o1, steps[0].l1, steps[0].o2, steps[0].l2, steps[0].c.mass), want[2]):
         assert torch.equal(a.nan_to_num(9), b.nan_to_num(9))
     assert gpu_lib.d1_kv4_error() == 0
+
+
+# ------------------------------------------------------------------------------------------------ units after units
+# (queries, cached keys, own rows, kv heads, group): more units than CTAs, so that a CTA goes from one to the next
+UNITS = {
+    # heads without a partner, blocks of 256 rows and what is left of them: a block with rows for one warpgroup alone, then
+    # one with rows for both, whose keys are cached, own, or both
+    "one warpgroup, then both": ([300] * 10, [1000, 0, 1000, 130, 999, 0, 520, 1000, 3, 1000],
+                                 [300, 700, 0, 300, 300, 1, 0, 700, 300, 0], 16, 1),
+    "one warpgroup, then packed": ([300, 129, 100, 7, 290, 260, 90, 300, 128, 40] * 3, [1000, 300, 700, 0, 600, 129] * 5,
+                                   [0, 0, 300, 7, 129, 1, 700, 640, 0, 40] * 3, 16, 1),
+    "three heads": ([280 + 7 * (i % 5) if i % 3 else 40 for i in range(40)], [1000 * (i % 2) + i for i in range(40)],
+                    [(0, 300, 700)[i % 3] for i in range(40)], 3, 3),
+}
+
+
+@gpu
+@pytest.mark.parametrize("exact_hint", [True, False])
+@pytest.mark.parametrize("name", UNITS)
+def test_attend_units_in_turn(pkg, gpu_lib, name, exact_hint):
+    """CTAs that take unit after unit of every kind, at their full number and, by a hint just above 64 packed rows, fewer:
+    right, and the same bits each time."""
+    q, ext, kv, kvh, group = UNITS[name]
+    n, h = len(q), kvh * group
+    rng = np.random.default_rng(len(name) + 70)
+    c = Caches(rng, ext, kvh, -(-max(ext) // 8) * 8)
+    x, starts = poisoned_rows(rng, [max(a, b) for a, b in zip(q, kv)], (h + 2 * kvh) * 64)
+    seqs = [dict(q_start=s, q_len=a, kv_start=s, kv_len=b) for s, a, b in zip(starts, q, kv)]
+    want = plain_attend(x, seqs, c, list(range(n)), kvh, group, 0.125, True)
+    tab, d, first = table(pkg, seqs, c, range(n)), torch.from_numpy(x).cuda(), None
+    for _ in range(4):
+        O, L = attend(gpu_lib, d, tab, n, kvh, group, 0.125, max(q) if exact_hint else 64 // group + 1,
+                      max(a + b for a, b in zip(ext, kv)))
+        assert gpu_lib.d1_kv4_error() == 0
+        if first is None:
+            check_attend(O, L, want, h)
+            first = O, L
+        assert torch.equal(O, first[0]) and torch.equal(L, first[1])
