@@ -486,8 +486,8 @@ enum : int {
     B_OFREE = B_ODONE + 2,           // [w]: O has been read (8 warps of a packed unit, otherwise 4, twice)
     B_RAWFULL = B_OFREE + 2,         // [raw stage]: a tile's codes and parameters are in shared memory
     B_RAWEMPTY = B_RAWFULL + T_RAW_STAGES,  // [raw stage] (4 warps)
-    B_OWN = B_RAWEMPTY + T_RAW_STAGES,  // a partial tile of own rows has landed
-    B_JOIN = B_OWN + 1,              // a packed unit's maxima and sums are in shared memory, its O's complete (8 warps)
+    B_OWN = B_RAWEMPTY + T_RAW_STAGES,  // [stage]: a partial tile of own rows has landed
+    B_JOIN = B_OWN + T_STAGES,       // a packed unit's maxima and sums are in shared memory, its O's complete (8 warps)
     B_DRAIN = B_JOIN + 1,            // [issuer]
     T_NBARS = B_DRAIN + 2
 };
@@ -683,6 +683,7 @@ __global__ void __launch_bounds__(T_THREADS, 1)
         for (int i = 0; i < T_STAGES; i++) {
             mbar_init(bar(B_KVFULL + i), T_EXPANDERS);
             mbar_init(bar(B_KVEMPTY + i), 2);
+            mbar_init(bar(B_OWN + i), 1);
         }
         for (int w = 0; w < 2; w++) {
             mbar_init(bar(B_SFULL + w), 1);
@@ -696,7 +697,6 @@ __global__ void __launch_bounds__(T_THREADS, 1)
             mbar_init(bar(B_RAWFULL + i), 1);
             mbar_init(bar(B_RAWEMPTY + i), T_EXPANDERS / 32);
         }
-        mbar_init(bar(B_OWN), 1);
         mbar_init(bar(B_JOIN), 8);
         *abort_flag = 0;
         fence_mbar_init();
@@ -792,7 +792,9 @@ __global__ void __launch_bounds__(T_THREADS, 1)
         } else if (warp >= 10 && warp < 14) {
             // ------------------------------------------------------------------ expanding
             const int lt = (warp - 10) * 32 + lane;
-            int ri = 0, ki = 0, oi = 0;  // cached tiles, tiles, and partial tiles of own rows so far
+            int ri = 0, ki = 0;  // cached tiles and tiles so far
+            uint32_t own = 0;    // of each stage, the parity of its next partial tile of own rows
+            int waiting = -1;    // the stage of one whose copies are awaited
             bool ok = true;
             auto unit = [&](int u) {
                 find_unit(u);
@@ -848,7 +850,8 @@ __global__ void __launch_bounds__(T_THREADS, 1)
                     // own rows: a whole tile by TMA. Rows behind the sequence's end are others', or zeros behind the buffer's:
                     // their scores are masked, and their values, which P = 0 multiplies, are overwritten with zeros
                     const int row0 = un.kv_start + (un.first() + j - un.all_ext_tiles()) * TKV;
-                    const uint32_t landed = bar(n >= TKV ? B_KVFULL + st : B_OWN);
+                    // (a barrier to each stage, so that it is armed again only when every thread has seen its phase before)
+                    const uint32_t landed = bar((n >= TKV ? B_KVFULL : B_OWN) + st);
                     if (lt == 0) {
                         mbar_arrive_expect_tx(landed, 2 * T_KV_BYTES);
                         tma_load_2d(smem_u32(dK), &tmK, g * 64, row0, landed);
@@ -858,8 +861,10 @@ __global__ void __launch_bounds__(T_THREADS, 1)
                         if (lt != 0) mbar_arrive(landed);
                         continue;
                     }
-                    if (!(ok = __all_sync(D1_FULL_MASK, mbar_wait(landed, oi & 1, abort_flag)))) return;
-                    oi++;
+                    waiting = st;
+                    if (!(ok = __all_sync(D1_FULL_MASK, mbar_wait(landed, (own >> st) & 1, abort_flag)))) return;
+                    waiting = -1;
+                    own ^= 1u << st;
                     for (int c = n * 8 + lt; c < TKV * 8; c += T_EXPANDERS)
                         *reinterpret_cast<uint4*>(dK + T_KV_BYTES + c * 16) = make_uint4(0, 0, 0, 0);
                     fence_async_smem_cta();
@@ -874,7 +879,8 @@ __global__ void __launch_bounds__(T_THREADS, 1)
                 }
             }
             if (!ok && lane == 0) record_err(a.err, abort_flag, kErrWaitEmpty);
-            if (lt == 0 && !ok) mbar_wait_timed2(bar(B_OWN), oi & 1);  // copies still in flight land before the CTA exits
+            if (lt == 0 && waiting >= 0)  // copies still in flight (only after an abort) land before the CTA exits
+                mbar_wait_timed2(bar(B_OWN + waiting), (own >> waiting) & 1);
             if (lt == 0)
                 for (int i = ki > T_STAGES ? ki - T_STAGES : 0; i < ki; i++)
                     if (!mbar_wait_timed2(bar(B_KVFULL + i % T_STAGES), (i / T_STAGES) & 1)) break;

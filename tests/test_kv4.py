@@ -815,6 +815,9 @@ UNITS = {
                                    [0, 0, 300, 7, 129, 1, 700, 640, 0, 40] * 3, 16, 1),
     "three heads": ([280 + 7 * (i % 5) if i % 3 else 40 for i in range(40)], [1000 * (i % 2) + i for i in range(40)],
                     [(0, 300, 700)[i % 3] for i in range(40)], 3, 3),
+    # partial tiles of own rows one after the other, with nothing cached before them
+    "own rows only": ([60 - i % 20 for i in range(300)], [0] * 300, [60 - i % 20 for i in range(300)], 4, 2),
+    "few own rows": ([40 + i % 9 for i in range(300)], [128 * (i % 5 == 0) for i in range(300)], [1 + i % 130 for i in range(300)], 4, 2),
 }
 
 
