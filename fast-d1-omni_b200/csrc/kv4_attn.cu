@@ -794,7 +794,6 @@ __global__ void __launch_bounds__(T_THREADS, 1)
             const int lt = (warp - 10) * 32 + lane;
             int ri = 0, ki = 0;  // cached tiles and tiles so far
             uint32_t own = 0;    // of each stage, the parity of its next partial tile of own rows
-            int waiting = -1;    // the stage of one whose copies are awaited
             bool ok = true;
             auto unit = [&](int u) {
                 find_unit(u);
@@ -861,9 +860,7 @@ __global__ void __launch_bounds__(T_THREADS, 1)
                         if (lt != 0) mbar_arrive(landed);
                         continue;
                     }
-                    waiting = st;
                     if (!(ok = __all_sync(D1_FULL_MASK, mbar_wait(landed, (own >> st) & 1, abort_flag)))) return;
-                    waiting = -1;
                     own ^= 1u << st;
                     for (int c = n * 8 + lt; c < TKV * 8; c += T_EXPANDERS)
                         *reinterpret_cast<uint4*>(dK + T_KV_BYTES + c * 16) = make_uint4(0, 0, 0, 0);
@@ -879,8 +876,8 @@ __global__ void __launch_bounds__(T_THREADS, 1)
                 }
             }
             if (!ok && lane == 0) record_err(a.err, abort_flag, kErrWaitEmpty);
-            if (lt == 0 && waiting >= 0)  // copies still in flight (only after an abort) land before the CTA exits
-                mbar_wait_timed2(bar(B_OWN + waiting), (own >> waiting) & 1);
+            if (lt == 0 && !ok)  // copies still in flight land before the CTA exits
+                mbar_wait_timed2(bar(B_OWN + ki % T_STAGES), (own >> ki % T_STAGES) & 1);
             if (lt == 0)
                 for (int i = ki > T_STAGES ? ki - T_STAGES : 0; i < ki; i++)
                     if (!mbar_wait_timed2(bar(B_KVFULL + i % T_STAGES), (i / T_STAGES) & 1)) break;
