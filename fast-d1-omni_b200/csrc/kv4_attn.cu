@@ -1017,12 +1017,12 @@ __global__ void __launch_bounds__(T_THREADS, 1)
             for (int j = 0; j < nt; j++) {
                 const int c = cnt + j;
                 if (!(ok = __all_sync(D1_FULL_MASK, mbar_wait(bar(B_SFULL + w), c & 1, abort_flag)))) break;
-                if (idle) {  // in step with the others: their P of the tile before must be complete
-                    if (c > 0 && !(ok = __all_sync(D1_FULL_MASK, mbar_wait(bar(B_PFULL + w), (c - 1) & 1, abort_flag)))) break;
-                    if (lane == 0) {
-                        mbar_arrive(bar(B_SFREE + w));
-                        mbar_arrive(bar(B_PFULL + w));
-                    }
+                if (idle) {
+                    // in step with the others, through every phase of B_ODONE: a wait for the last one alone could pass on the
+                    // parity of the one before it, and O would be given back while the other warpgroup still reads it
+                    if (lane == 0) mbar_arrive(bar(B_SFREE + w));
+                    if (c > 0 && !(ok = __all_sync(D1_FULL_MASK, mbar_wait(bar(B_ODONE + w), (c - 1) & 1, abort_flag)))) break;
+                    if (lane == 0) mbar_arrive(bar(B_PFULL + w));
                     continue;
                 }
                 tc_fence_after();

@@ -818,6 +818,9 @@ UNITS = {
     # partial tiles of own rows one after the other, with nothing cached before them
     "own rows only": ([60 - i % 20 for i in range(300)], [0] * 300, [60 - i % 20 for i in range(300)], 4, 2),
     "few own rows": ([40 + i % 9 for i in range(300)], [128 * (i % 5 == 0) for i in range(300)], [1 + i % 130 for i in range(300)], 4, 2),
+    # full packed units, which both warpgroups read, before and after blocks that leave some warps without rows
+    "warps without rows": ([(64, 130, 64, 1, 165, 200)[i % 6] for i in range(60)], [(900, 300, 129, 640, 260, 0)[i % 6] for i in range(60)],
+                           [(0, 1, 300, 0, 0, 129)[i % 6] for i in range(60)], 4, 2),
 }
 
 
