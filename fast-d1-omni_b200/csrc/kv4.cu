@@ -30,7 +30,8 @@ __device__ __forceinline__ void table_error() { atomicExch(&g_kv4_err, kErrTable
 constexpr int A_ROWS = 64, A_STEP = 32;
 
 __device__ __forceinline__ bool append_ok(const D1Kv4Seq& s) {
-    return s.kv_start >= 0 && s.kv_len >= 0 && kv4_seq_ok(s) && (long long)s.ext_len + s.kv_len <= s.ext_cap;
+    return (s.kv_len == 0 || (s.kv_start >= 0 && s.kv_len > 0)) && kv4_seq_ok(s) &&
+           (long long)s.ext_len + s.kv_len <= s.ext_cap;
 }
 
 // Words of codes of one vector (this lane's twice 8 elements of it; four lanes a vector) and its parameter. round(x / step) without a division per element:

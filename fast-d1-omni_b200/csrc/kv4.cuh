@@ -25,9 +25,9 @@ __device__ __forceinline__ bool kv4_seq_ok(const D1Kv4Seq& s) {
     return kv4_cache_ok(s.ext_len, s.ext_cap, s.k4, s.v4, s.kp, s.vp);
 }
 
-// Rows [start, start + len) lie inside [0, rows).
+// Rows [start, start + len) lie inside [0, rows); none do, wherever they start.
 __device__ __forceinline__ bool rows_ok(int start, int len, int rows) {
-    return start >= 0 && len >= 0 && (long long)start + len <= rows;
+    return len == 0 || (start >= 0 && len > 0 && (long long)start + len <= rows);
 }
 
 __device__ __forceinline__ uint32_t h2_sub(uint32_t a, uint32_t b) {

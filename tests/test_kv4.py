@@ -804,6 +804,37 @@ def test_step_captured_and_on_two_streams(pkg, gpu_lib, max_q):
     assert gpu_lib.d1_kv4_error() == 0
 
 
+@gpu
+@pytest.mark.parametrize("max_q", HINTS)
+def test_step_with_all_rows_cached(pkg, gpu_lib, max_q):
+    """A server's step: rows appended, counted in ext_len, and kv_len = 0 with kv_start left where they were; the attention
+    is called without K and V. Nor does it matter where a sequence without query rows starts."""
+    rng = np.random.default_rng(31)
+    kvh, group, rows, ext = 2, 2, [5, 0, 130, 33, 1], [3, 9, 200, 64, 0]
+    h, n, total = kvh * group, 5, [a + b for a, b in zip(rows, ext)]
+    c = Caches(rng, ext, kvh, 336)
+    x, starts = poisoned_rows(rng, rows, (h + 2 * kvh) * 64)
+    T, ld, d, lib = len(x), x.shape[1], torch.from_numpy(x).cuda(), gpu_lib
+    seqs = [dict(q_start=s, q_len=m, kv_start=s, kv_len=m) for s, m in zip(starts, rows)]
+    k, v = d[:, h * 64:].data_ptr(), d[:, (h + kvh) * 64:].data_ptr()
+    assert lib.d1_kv4_append(k, v, ld, P(table(pkg, seqs, c, range(n))), n, max(rows), kvh, ST()) == 0
+    c.lens, c.host = total, c.back()
+    seqs = [dict(s, kv_len=0) for s in seqs]
+    seqs[1].update(q_start=10 ** 6, kv_start=-7)
+    tab = table(pkg, seqs, c, range(n), mass=True)
+    O, L = torch.full((T, h * 64), 7.0, dtype=torch.float16, device="cuda"), torch.full((h, T), 7.0, device="cuda")
+    assert lib.d1_flash_attn_kv4(P(d), ld, None, None, 0, P(O), h * 64, P(L), T, P(tab), n, max_q, max(total), h, group, 0.125,
+                                 T, 0, ST()) == 0
+    assert lib.d1_kv4_mass(P(d), ld, P(L), T, P(tab), n, max_q, max(total), h, group, 0.125, 0, T, ST()) == 0
+    assert lib.d1_kv4_append(k, v, ld, P(tab), n, max(rows), kvh, ST()) == 0 and lib.d1_kv4_error() == 0
+    seqs[1].update(q_start=0, kv_start=0)
+    check_attend(O, L, plain_attend(x, seqs, c, range(n), kvh, group, 0.125, True), h)
+    lse = L.cpu().numpy()
+    M, tol = plain_mass(x, lse, seqs, c, range(n), kvh, group, 0.125)
+    got = c.mass.double().cpu().numpy()
+    assert all((np.abs(got - M) <= tol)[i, :, :m].all() for i, m in enumerate(total))
+
+
 # ------------------------------------------------------------------------------------------------ units after units
 # (queries, cached keys, own rows, kv heads, group): more units than CTAs, so that a CTA goes from one to the next
 UNITS = {
