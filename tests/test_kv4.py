@@ -554,6 +554,37 @@ def test_mass_of_rows_that_add_nothing(pkg, gpu_lib, max_q):
     assert gpu_lib.d1_kv4_error() == 0
 
 
+@gpu
+def test_more_sequences_than_a_grid(pkg, gpu_lib):
+    """Beyond 65535 sequences a CTA takes one after the other: long sums first, then short ones."""
+    rng = np.random.default_rng(15)
+    kvh, group, n = 1, 2, 65535 + 24
+    h, at = kvh * group, list(range(24)) + list(range(65535, n))
+    q = [61 - i % 7 if i < 24 else 1 + i % 9 for i in range(48)]
+    c = Caches(rng, [30 + i for i in range(48)], kvh, 80)
+    x, starts = poisoned_rows(rng, q, (h + 2 * kvh) * 64)
+    lse = (2 + rng.standard_normal((h, len(x)))).astype(np.float32)
+    seqs = [dict(q_start=s, q_len=m, kv_start=0, kv_len=0) for s, m in zip(starts, q)]
+    some = bytes(table(pkg, seqs, c, range(48), mass=True).cpu().numpy())
+    tab = bytearray(64 * n)
+    for i, j in enumerate(at):
+        tab[64 * j:64 * j + 64] = some[64 * i:64 * i + 64]
+    tab = torch.frombuffer(tab, dtype=torch.uint8).cuda()
+    d, l = torch.from_numpy(x).cuda(), torch.from_numpy(lse).cuda()
+    M, T = plain_mass(x, lse, seqs, c, range(48), kvh, group, 0.125)
+    want = plain_attend(x, seqs, c, range(48), kvh, group, 0.125, True)
+    for _ in range(3):
+        c.mass.fill_(5)
+        assert gpu_lib.d1_kv4_mass(P(d), d.shape[1], P(l), len(x), P(tab), n, max(q), 80, h, group, 0.125, 0, len(x), ST()) == 0
+        got = c.mass.double().cpu().numpy()
+        for i, e in enumerate(c.lens):
+            assert (got[i, :, e:] == 5).all() and (np.abs(got[i, :, :e] - M[i, :, :e]) <= T[i, :, :e]).all()
+    for max_q in (1, 30, 61):
+        O, L = attend(gpu_lib, d, tab, n, kvh, group, 0.125, max_q, 80)
+        check_attend(O, L, want, h)
+    assert gpu_lib.d1_kv4_error() == 0
+
+
 # ------------------------------------------------------------------------------------------------ evict
 @gpu
 @pytest.mark.parametrize("lens,keep,recent,kvh", [([1], [1], [0], 1), ([9, 0, 100], [3, 5, 0], [0, 1, 4], 2),
