@@ -28,6 +28,11 @@ __device__ __forceinline__ float fmax_nan(float a, float b) {  // NaN if either 
     asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
     return d;
 }
+__device__ __forceinline__ float fmin_nan(float a, float b) {
+    float d;
+    asm("min.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
+    return d;
+}
 __device__ __forceinline__ uint64_t f2_mul(uint64_t a, uint64_t b) {
     uint64_t d;
     asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
@@ -36,9 +41,9 @@ __device__ __forceinline__ uint64_t f2_mul(uint64_t a, uint64_t b) {
 
 // 2^x of two numbers without the SFU: x = n + f, n whole by adding and taking away 1.5 * 2^23 (the sum's low bits, with
 // 127 added, are 2^n's exponent), |f| <= 1/2, 2^f by a polynomial of degree 5 fitted here for the smallest relative error,
-// 2.1e-7 evaluated in fp32. x below -126.5 gives 0; NaN stays.
+// 2.1e-7 evaluated in fp32. x below -126.5 gives 0, above 127.5 infinity; NaN stays.
 __device__ __forceinline__ void ex2_fma2(float x0, float x1, float& p0, float& p1) {
-    const uint64_t x = f2_pack(fmax_nan(x0, -127.f), fmax_nan(x1, -127.f));
+    const uint64_t x = f2_pack(fmin_nan(fmax_nan(x0, -127.f), 128.f), fmin_nan(fmax_nan(x1, -127.f), 128.f));
     const uint64_t t = f2_add(x, f2_pack(12583039.f, 12583039.f));
     const uint64_t f = f2_fma(f2_add(t, f2_pack(-12583039.f, -12583039.f)), f2_pack(-1.f, -1.f), x);
     auto c2 = [](float c) { return f2_pack(c, c); };

@@ -585,6 +585,30 @@ def test_more_sequences_than_a_grid(pkg, gpu_lib):
     assert gpu_lib.d1_kv4_error() == 0
 
 
+@gpu
+@pytest.mark.parametrize("max_q", [1, 64])
+def test_mass_of_a_foreign_lse(pkg, gpu_lib, max_q):
+    """An lse far from the scores, in each column of a piece of 32: e^80 is a number, e^95 is infinite, NaN stays, e^-120 and
+    lse = inf add nothing. Scores are 0 here, and the 63 other columns add 1 each: a sum is off by at most 2^-22 of an
+    exponential, 80 * 2^-23 of its exponent and 64 additions."""
+    rng = np.random.default_rng(16)
+    c = Caches(rng, [130], 1, 136)
+    d = torch.zeros(32, 128, dtype=torch.float16, device="cuda")
+    tab = table(pkg, [dict(q_start=0, q_len=32)], c, [0], mass=True)
+    for at in range(32):
+        for v, want in ((-80.0, math.exp(80)), (-95.0, INF), (-1e9, INF), (-1e30, INF), (120.0, 63.0), (INF, 63.0), (-INF, 63.0),
+                        (np.nan, np.nan)):
+            lse = torch.zeros(2, 32, device="cuda")
+            lse[at % 2, at // 2] = v
+            assert gpu_lib.d1_kv4_mass(P(d), 128, P(lse), 32, P(tab), 1, max_q, 130, 2, 2, 0.125, 0, 32, ST()) == 0
+            got = c.mass[0, 0, :130].double().cpu().numpy()
+            if math.isfinite(want):
+                assert (np.abs(got - want) <= (2.0 ** -22 + 80 * 2.0 ** -23 + 64 * 2.0 ** -24) * want).all(), (at, v, got[0])
+            else:
+                assert np.array_equal(got, np.full(130, want), equal_nan=True), (at, v, got[0])
+    assert gpu_lib.d1_kv4_error() == 0
+
+
 # ------------------------------------------------------------------------------------------------ evict
 @gpu
 @pytest.mark.parametrize("lens,keep,recent,kvh", [([1], [1], [0], 1), ([9, 0, 100], [3, 5, 0], [0, 1, 4], 2),
