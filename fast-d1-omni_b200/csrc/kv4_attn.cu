@@ -1285,7 +1285,6 @@ __global__ void __launch_bounds__(256, 2) k_kv4_mass_rows(const Kv4Args a) {
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, r = lane >> 2, t = lane & 3, g = blockIdx.y;
     const int q_first = r / a.group, h_first = g * a.group + r % a.group, q_step = 8 / a.group, h_step = 8 % a.group;
     const int h_end = (g + 1) * a.group;
-    bool used = false;  // the list has been written before, maybe for another sequence
     for (int sq = blockIdx.z; sq < a.n_seqs; sq += gridDim.z) {
         const D1Kv4Seq s = a.seqs[sq];
         if (!s.mass) continue;
@@ -1297,8 +1296,7 @@ __global__ void __launch_bounds__(256, 2) k_kv4_mass_rows(const Kv4Args a) {
         // lists sequences b0 .. b0 + 255; whether one before sq, which then takes the mass array, is among them
         auto list = [&](int b0) {
             if (listed == b0) return false;
-            if (used) __syncthreads();  // the list has been read
-            used = true;
+            if (listed >= 0) __syncthreads();  // the list has been read
             listed = b0;
             const int j = b0 + tid;
             bool mine = false, before = false;
@@ -1419,6 +1417,7 @@ __global__ void __launch_bounds__(256, 2) k_kv4_mass_rows(const Kv4Args a) {
                     if (any && t == 0 && key < s.ext_len) mass[key] = a.accumulate ? mass[key] + v : v;
                 }
         }
+        if (sq + (int)gridDim.z < a.n_seqs) __syncthreads();  // the list has been read, before the next sequence's is written
     }
 }
 
