@@ -1273,7 +1273,7 @@ __global__ void __launch_bounds__(T_THREADS, 1)
 // ------------------------------------------------------------------------------------------------ mass, few rows
 // S^T = K Q^T on m16n8k16: a warp holds 16 * MT keys as A operands (whole numbers code - zero, as above) and goes over the
 // packed query rows 8 at a time, adding exp(s - lse) into its keys' sums; four lanes share a key at the end. The sequences
-// that share a mass array are taken by the first of them, in the table's order. What bounds it are latencies: of the table,
+// that share a mass array are taken by the first of them whose cache is in order, in the table's order. What bounds it are latencies: of the table,
 // of the codes (both at once where the table has 256 entries at most), and of 8 rows after 8 rows.
 template <int MT>
 __global__ void __launch_bounds__(256, 2) k_kv4_mass_rows(const Kv4Args a) {
@@ -1293,7 +1293,8 @@ __global__ void __launch_bounds__(256, 2) k_kv4_mass_rows(const Kv4Args a) {
             continue;
         }
         int listed = -1;  // which 256 sequences the list holds
-        // lists sequences b0 .. b0 + 255; whether one before sq, which then takes the mass array, is among them
+        // lists sequences b0 .. b0 + 255; whether one before sq with a cache in order, which then takes the mass array, is
+        // among them
         auto list = [&](int b0) {
             if (listed == b0) return false;
             if (listed >= 0) __syncthreads();  // the list has been read
@@ -1303,7 +1304,7 @@ __global__ void __launch_bounds__(256, 2) k_kv4_mass_rows(const Kv4Args a) {
             if (j < a.n_seqs) {
                 const D1Kv4Seq p = a.seqs[j];
                 mine = p.mass == s.mass;
-                before = mine && j < sq;
+                before = mine && j < sq && kv4_seq_ok(p);
                 if (mine && (!kv4_seq_ok(p) || p.k4 != s.k4 || p.ext_len != s.ext_len || p.ext_cap != s.ext_cap ||
                              !rows_ok(p.q_start, p.q_len, a.q_rows))) {
                     atomicExch(a.err, kErrTable);
@@ -1456,7 +1457,7 @@ enum : int {
 
 // What the roles need of up to M_SEQS sequences, in shared memory: units (key tiles of 128 of the caches that belong to a
 // sequence, for each kv head) before each, query rows, cached keys, and the next sequence of the same mass array. The
-// sequences that share a mass array belong to the first of them, whose cache they must share, too.
+// sequences that share a mass array belong to the first of them whose cache is in order, which they must share, too.
 constexpr int M_SEQS = 256;
 struct MassTable {
     const float* mass[M_SEQS];
@@ -1485,7 +1486,7 @@ __device__ __forceinline__ void build_mass_table(const Kv4Args& a, MassTable& tb
             bool owner = true;
             int first = i, next = n;
             for (int j = 0; j < i && owner; j++)
-                if (tb.mass[j] == s.mass) {
+                if (tb.mass[j] == s.mass && kv4_seq_ok(a.seqs[j])) {
                     owner = false;
                     first = j;
                 }

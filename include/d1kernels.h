@@ -414,8 +414,9 @@ int d1_flash_attn_kv4(const d1_half* Q, int ldq, const d1_half* K, const d1_half
 /* extension — the attention weight that every cached key received: for every kv head g and key k of a sequence's cache
  *   mass[g][k] (+)= sum over its rows q and the heads h of g of exp(scale * Q[q] . K[k] - lse[h][q])
  * with lse as d1_flash_attn_kv4 gave it (-inf: the row adds nothing, whatever its Q holds). accumulate = 0 overwrites
- * mass[g][0 .. ext_len-1], 1 adds to it. Sequences with the same `mass` must share their cache; their weights are added
- * up in the table's order, always in the same order for the same call. max_q, max_len: the longest q_len and ext_len
+ * mass[g][0 .. ext_len-1], 1 adds to it. Sequences with the same `mass` must share their cache (one that does not share
+ * that of the first of them whose cache is in order is refused); their weights are added up in the table's order, always
+ * in the same order for the same call. max_q, max_len: the longest q_len and ext_len
  * (see above). */
 int d1_kv4_mass(const d1_half* Q, int ldq, const float* lse, int lse_ld, const D1Kv4Seq* seqs, int n_seqs, int max_q,
                 int max_len, int heads, int group, float scale, int accumulate, int q_rows, cudaStream_t stream);

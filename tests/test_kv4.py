@@ -696,6 +696,33 @@ def test_bad_entries_are_skipped(pkg, gpu_lib, max_q):
 
 
 @gpu
+@pytest.mark.parametrize("max_q", HINTS)
+def test_bad_entries_of_a_shared_mass(pkg, gpu_lib, max_q):
+    """An entry that is skipped takes none of those with it that share its mass array, be it before or behind them."""
+    rng = np.random.default_rng(17)
+    kvh, group, q = 2, 2, [9, 70, 33, 5]
+    h = kvh * group
+    c = Caches(rng, [140, 40], kvh, 144)
+    x, starts = poisoned_rows(rng, q, h * 64)
+    lse = (2 + rng.standard_normal((h, len(x)))).astype(np.float32)
+    d, l = torch.from_numpy(x).cuda(), torch.from_numpy(lse).cuda()
+    good, of = [dict(q_start=s, q_len=m) for s, m in zip(starts, q)], [0, 0, 1, 0]
+    for at in (0, 1, 3):
+        keep = [i for i in range(4) if i != at]
+        M, T = plain_mass(x, lse, [good[i] for i in keep], c, [of[i] for i in keep], kvh, group, 0.125)
+        for bad in (dict(ext_len=145), dict(k4=None), dict(ext_cap=140), dict(q_len=len(x) + 1), dict(kp=c.dev["kp"].data_ptr() + 2)):
+            seqs = [dict(s) for s in good]
+            seqs[at].update(bad)
+            c.mass.fill_(7)
+            assert gpu_lib.d1_kv4_mass(P(d), d.shape[1], P(l), len(x), P(table(pkg, seqs, c, of, mass=True)), 4, max_q, 140, h, group,
+                                       0.125, 0, len(x), ST()) == 0
+            assert gpu_lib.d1_kv4_error() != 0
+            got = c.mass.double().cpu().numpy()
+            for i, e in enumerate((140, 40)):
+                assert (got[i, :, e:] == 7).all() and (np.abs(got[i, :, :e] - M[i, :, :e]) <= T[i, :, :e]).all(), (at, bad, i)
+
+
+@gpu
 def test_evict_bad_items_are_skipped(pkg, gpu_lib):
     rng = np.random.default_rng(7)
     c, d = Caches(rng, [40, 40], 2), Caches(rng, [0, 0], 2, 24)
