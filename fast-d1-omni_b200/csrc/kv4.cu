@@ -218,7 +218,8 @@ __global__ void __launch_bounds__(E_THREADS, E_PER_SM) k_kv4_evict(const D1Kv4Ev
         const int len = it->len, cap = it->cap, dst_cap = it->dst_cap;
         const int keep = min(it->keep, len), recent = min(it->recent, keep);
         if (it->keep < 0 || it->recent < 0 || !kv4_cache_ok(len, cap, it->k4, it->v4, it->kp, it->vp) ||
-            (len > 0 && !it->mass) || !kv4_cache_ok(keep, dst_cap, it->dst_k4, it->dst_v4, it->dst_kp, it->dst_vp)) {
+            (len > 0 && !it->mass) || !kv4_cache_ok(keep, dst_cap, it->dst_k4, it->dst_v4, it->dst_kp, it->dst_vp) ||
+            (((uintptr_t)it->mass | (uintptr_t)it->dst_mass | (uintptr_t)it->kept) & 3)) {
             if (tid == 0) table_error();
             continue;
         }
@@ -383,7 +384,7 @@ dim3 row_grid(int max_rows, int rows, int kv_heads, int n_seqs) {
 extern "C" int d1_kv4_append(const d1_half* K, const d1_half* V, int ldkv, const D1Kv4Seq* seqs, int n_seqs,
                              int max_rows, int kv_heads, cudaStream_t st) {
     if (n_seqs <= 0) return n_seqs == 0 ? 0 : -1;
-    if (!seqs || max_rows < 0 || kv_heads <= 0 || kv_heads > 4096 || bad_rows(K, V, ldkv, kv_heads)) return -1;
+    if (!seqs || ((uintptr_t)seqs & 7) || max_rows < 0 || kv_heads <= 0 || kv_heads > 4096 || bad_rows(K, V, ldkv, kv_heads)) return -1;
     const dim3 g4 = row_grid(max_rows, 4 * A_ROWS, kv_heads, n_seqs);
     if ((long long)g4.x * g4.y * g4.z >= 2 * 148)
         launch_pdl(k_kv4_append<4>, g4, 256, 0, st, K, V, ldkv, seqs, n_seqs);
@@ -395,14 +396,14 @@ extern "C" int d1_kv4_append(const d1_half* K, const d1_half* V, int ldkv, const
 extern "C" int d1_kv4_load(const D1Kv4Seq* seqs, int n_seqs, int max_rows, int kv_heads, d1_half* K, d1_half* V,
                            int ldkv, cudaStream_t st) {
     if (n_seqs <= 0) return n_seqs == 0 ? 0 : -1;
-    if (!seqs || max_rows < 0 || kv_heads <= 0 || kv_heads > 4096 || bad_rows(K, V, ldkv, kv_heads)) return -1;
+    if (!seqs || ((uintptr_t)seqs & 7) || max_rows < 0 || kv_heads <= 0 || kv_heads > 4096 || bad_rows(K, V, ldkv, kv_heads)) return -1;
     launch_pdl(k_kv4_load<4>, row_grid(max_rows, 4 * A_STEP, kv_heads, n_seqs), 256, 0, st, seqs, n_seqs, K, V, ldkv);
     return (int)cudaGetLastError();
 }
 
 extern "C" int d1_kv4_evict(const D1Kv4Evict* items, int n_items, int max_len, int kv_heads, cudaStream_t st) {
     if (n_items <= 0) return n_items == 0 ? 0 : -1;
-    if (!items || kv_heads <= 0 || kv_heads > 4096 || max_len < 0) return -1;
+    if (!items || ((uintptr_t)items & 7) || kv_heads <= 0 || kv_heads > 4096 || max_len < 0) return -1;
     static unsigned long long done = 0;  // the shared-memory opt-in is per device
     int dev = 0;
     cudaGetDevice(&dev);

@@ -1288,7 +1288,7 @@ __global__ void __launch_bounds__(256, 2) k_kv4_mass_rows(const Kv4Args a) {
     for (int sq = blockIdx.z; sq < a.n_seqs; sq += gridDim.z) {
         const D1Kv4Seq s = a.seqs[sq];
         if (!s.mass) continue;
-        if (!kv4_seq_ok(s)) {
+        if (!kv4_seq_ok(s) || ((uintptr_t)s.mass & 3)) {
             if (tid == 0) atomicExch(a.err, kErrTable);
             continue;
         }
@@ -1494,7 +1494,7 @@ __device__ __forceinline__ void build_mass_table(const Kv4Args& a, MassTable& tb
                 if (tb.mass[j] == s.mass) next = j;
             tb.next[i] = next;
             const D1Kv4Seq& o = a.seqs[first];
-            const bool bad = !kv4_seq_ok(s);
+            const bool bad = !kv4_seq_ok(s) || ((uintptr_t)s.mass & 3);
             if (bad || !rows_ok(s.q_start, s.q_len, a.q_rows) ||
                 (!owner && (o.k4 != s.k4 || o.ext_len != s.ext_len || o.ext_cap != s.ext_cap))) {
                 atomicExch(a.err, kErrTable);
@@ -2072,6 +2072,7 @@ extern "C" int d1_flash_attn_kv4(const d1_half* Q, int ldq, const d1_half* K, co
     if (ldq < heads * 64 || ldo < heads * 64 || (kv_rows > 0 && ldkv < heads / group * 64)) return -1;
     if ((((uintptr_t)Q | (uintptr_t)K | (uintptr_t)V | (uintptr_t)O) & 15) || (ldq | ldkv | ldo) % 8) return -1;
     if (lse && lse_ld < q_rows) return -1;
+    if (((uintptr_t)lse & 3) || ((uintptr_t)seqs & 7)) return -1;
     Kv4Args a = {};
     a.Q = Q;
     a.K = K;
@@ -2108,7 +2109,7 @@ extern "C" int d1_kv4_mass(const d1_half* Q, int ldq, const float* lse, int lse_
     if (heads <= 0 || group <= 0 || heads % group || heads / group > 4096 || q_rows < 0 || !(scale > 0.f)) return -1;
     if (max_q < 0 || max_len < 0) return -1;
     if (!seqs || (q_rows > 0 && (!Q || !lse)) || ldq < heads * 64 || lse_ld < q_rows) return -1;
-    if (((uintptr_t)Q & 15) || ldq % 8) return -1;
+    if (((uintptr_t)Q & 15) || ldq % 8 || ((uintptr_t)lse & 3) || ((uintptr_t)seqs & 7)) return -1;
     Kv4Args a = {};
     a.Q = Q;
     a.lse = const_cast<float*>(lse);

@@ -346,10 +346,10 @@ int d1_gemm_noalloc_error(void);
  * and stands for (code - zero) * step, which fp16 holds exactly: |x - value| <= step / 2 (step, beside 65504). A vector
  * with a NaN or an infinity reads as NaN in every element.
  *
- * ext_cap must be a multiple of 8, at most 2^30, and the four pointers 16-byte aligned; ext_cap = 0 with null pointers
- * is a sequence without a cache. The tables below are read on the device when the kernel runs. An entry that breaks
- * these rules or reaches outside the rows that the call names is skipped, its outputs left as they were, and
- * d1_kv4_error() tells. No rows (q_len or kv_len 0) reach nowhere, whatever their start.
+ * ext_cap must be a multiple of 8, at most 2^30, and the four pointers 16-byte aligned (mass, dst_mass and kept: 4 bytes);
+ * ext_cap = 0 with null pointers is a sequence without a cache. The tables below, 8-byte aligned, are read on the device
+ * when the kernel runs. An entry that breaks these rules or reaches outside the rows that the call names is skipped, its
+ * outputs left as they were, and d1_kv4_error() tells. No rows (q_len or kv_len 0) reach nowhere, whatever their start.
  * The launchers keep no state and no workspace: calls on several streams, and captured ones, do not affect each other
  * as long as what they write does not overlap. */
 typedef struct D1Kv4Seq {

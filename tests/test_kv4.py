@@ -180,6 +180,20 @@ def test_refusals(pkg):
     assert ev(n=0) == 0
 
 
+def test_refusals_of_alignment(pkg):
+    """Tables off 8 bytes and log-sum-exps off 4 are refused before anything is launched."""
+    lib, A = pkg.lib(), 1 << 20  # never dereferenced
+    for at in (1, 2, 4):
+        assert lib.d1_kv4_append(A, A, 128, A + at, 1, 1, 2, None) == -1
+        assert lib.d1_kv4_load(A + at, 1, 1, 2, A, A, 128, None) == -1
+        assert lib.d1_kv4_evict(A + at, 1, 1, 2, None) == -1
+        for lse, seqs in ((A, A + at), (A + at % 4, A)):
+            if lse == seqs:
+                continue
+            assert lib.d1_flash_attn_kv4(A, 128, A, A, 64, A, 128, lse, 9, seqs, 1, 1, 1, 2, 2, 0.125, 9, 9, None) == -1
+            assert lib.d1_kv4_mass(A, 128, lse, 9, seqs, 1, 1, 1, 2, 2, 0.125, 0, 9, None) == -1
+
+
 # ------------------------------------------------------------------------------------------------ append, load
 def special_vectors():
     """Vectors at the format's borders."""
@@ -720,6 +734,41 @@ def test_bad_entries_of_a_shared_mass(pkg, gpu_lib, max_q):
             got = c.mass.double().cpu().numpy()
             for i, e in enumerate((140, 40)):
                 assert (got[i, :, e:] == 7).all() and (np.abs(got[i, :, :e] - M[i, :, :e]) <= T[i, :, :e]).all(), (at, bad, i)
+
+
+@gpu
+@pytest.mark.parametrize("off", [1, 2, 3])
+def test_masses_off_four_bytes_are_refused(pkg, gpu_lib, off):
+    """mass, dst_mass and kept off 4 bytes: the entry is skipped and reported, the others are computed."""
+    rng = np.random.default_rng(18)
+    c, d = Caches(rng, [140, 40], 2, 144), Caches(rng, [0, 0], 2, 24)
+    x, starts = poisoned_rows(rng, [9, 70], 4 * 64)
+    lse = (2 + rng.standard_normal((4, len(x)))).astype(np.float32)
+    dx, l = torch.from_numpy(x).cuda(), torch.from_numpy(lse).cuda()
+    seqs = [dict(q_start=s, q_len=m) for s, m in zip(starts, (9, 70))]
+    M, T = plain_mass(x, lse, seqs, c, [0, 1], 2, 2, 0.125)
+    for max_q in HINTS:
+        c.mass.fill_(7)
+        tab = table(pkg, [dict(seqs[0], mass=c.mass[0].data_ptr() + off), seqs[1]], c, [0, 1], mass=True)
+        assert gpu_lib.d1_kv4_mass(P(dx), dx.shape[1], P(l), len(x), P(tab), 2, max_q, 140, 4, 2, 0.125, 0, len(x), ST()) == 0
+        assert gpu_lib.d1_kv4_error() != 0
+        got = c.mass.double().cpu().numpy()
+        assert (got[0] == 7).all() and (np.abs(got - M) <= T)[1, :, :40].all()
+    mass, kept = torch.rand(2, 2, 144, device="cuda"), torch.zeros(2, 2, 24, dtype=torch.int32, device="cuda")
+    for bad in (dict(mass=P(mass) + off), dict(dst_mass=P(d.mass) + off), dict(kept=P(kept) + off)):
+        arr = (pkg.abi.Kv4Evict * 2)()
+        for i, e in enumerate(arr):
+            e.len, e.cap, e.keep, e.recent, e.dst_cap, e.mass = 40, c.cap, 20, 2, d.cap, mass[i].data_ptr()
+            e.dst_mass, e.kept = d.mass[i].data_ptr(), kept[i].data_ptr()
+            for k in c.dev:
+                setattr(e, k, c.dev[k][i].data_ptr())
+                setattr(e, "dst_" + k, d.dev[k][i].data_ptr())
+        for k, v in bad.items():
+            setattr(arr[0], k, v)
+        items = torch.frombuffer(bytearray(bytes(arr)), dtype=torch.uint8).cuda()
+        d.dev["kp"].fill_(77)
+        assert gpu_lib.d1_kv4_evict(P(items), 2, 40, 2, ST()) == 0 and gpu_lib.d1_kv4_error() != 0
+        assert (d.dev["kp"][0] == 77).all() and (d.dev["kp"][1, :, :20] != 77).all()
 
 
 @gpu
