@@ -9,6 +9,7 @@ using namespace d1;
 namespace {
 
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
+constexpr int kMaxHeads = 0x7fffffff / 64;  // their columns are counted in 32 bits
 constexpr float kLazyRescale = 8.f;  // log2: how far scores may exceed the reference of a running softmax
 
 struct Kv4Args {
@@ -2064,7 +2065,8 @@ extern "C" int d1_flash_attn_kv4(const d1_half* Q, int ldq, const d1_half* K, co
                                  int max_keys, int heads, int group, float scale, int q_rows, int kv_rows,
                                  cudaStream_t st) {
     if (n_seqs <= 0) return n_seqs == 0 ? 0 : -1;
-    if (heads <= 0 || group <= 0 || heads % group || heads / group > 4096 || q_rows < 0 || kv_rows < 0 || !(scale > 0.f))
+    if (heads <= 0 || heads > kMaxHeads || group <= 0 || heads % group || heads / group > 4096 || q_rows < 0 ||
+        kv_rows < 0 || !(scale > 0.f))
         return -1;
     if (max_q < 0 || max_keys < 0) return -1;
     if (q_rows == 0) return 0;
@@ -2106,7 +2108,9 @@ extern "C" int d1_kv4_mass(const d1_half* Q, int ldq, const float* lse, int lse_
                            int max_q, int max_len, int heads, int group, float scale, int accumulate, int q_rows,
                            cudaStream_t st) {
     if (n_seqs <= 0) return n_seqs == 0 ? 0 : -1;
-    if (heads <= 0 || group <= 0 || heads % group || heads / group > 4096 || q_rows < 0 || !(scale > 0.f)) return -1;
+    if (heads <= 0 || heads > kMaxHeads || group <= 0 || heads % group || heads / group > 4096 || q_rows < 0 ||
+        !(scale > 0.f))
+        return -1;
     if (max_q < 0 || max_len < 0) return -1;
     if (!seqs || (q_rows > 0 && (!Q || !lse)) || ldq < heads * 64 || lse_ld < q_rows) return -1;
     if (((uintptr_t)Q & 15) || ldq % 8 || ((uintptr_t)lse & 3) || ((uintptr_t)seqs & 7)) return -1;

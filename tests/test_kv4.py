@@ -966,6 +966,20 @@ def test_step_with_all_rows_cached(pkg, gpu_lib, max_q):
     assert all((np.abs(got - M) <= tol)[i, :, :m].all() for i, m in enumerate(total))
 
 
+@gpu
+@pytest.mark.parametrize("heads,group", [(2 ** 25, 2 ** 13), (2 ** 26, 2 ** 14), (2 ** 30, 2 ** 20)])
+def test_heads_beyond_32_bits_are_refused(pkg, gpu_lib, heads, group):
+    """64 columns a head would not be countable in 32 bits: refused, whatever the leading dimension."""
+    tab, d = table(pkg, [dict(q_len=0)]), torch.zeros(8, 64, dtype=torch.float16, device="cuda")
+    lse = torch.zeros(8, device="cuda")
+    for max_q in (1, 5000):
+        assert gpu_lib.d1_flash_attn_kv4(P(d), 64, None, None, 0, P(d), 64, None, 0, P(tab), 1, max_q, 1, heads, group, 0.125, 1, 0,
+                                         ST()) == -1
+        assert gpu_lib.d1_kv4_mass(P(d), 64, P(lse), 8, P(tab), 1, max_q, 1, heads, group, 0.125, 0, 1, ST()) == -1
+    torch.cuda.synchronize()
+    assert gpu_lib.d1_kv4_error() == 0
+
+
 # ------------------------------------------------------------------------------------------------ units after units
 # (queries, cached keys, own rows, kv heads, group): more units than CTAs, so that a CTA goes from one to the next
 UNITS = {
