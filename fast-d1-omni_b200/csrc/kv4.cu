@@ -384,9 +384,12 @@ dim3 row_grid(int max_rows, int rows, int kv_heads, int n_seqs) {
 extern "C" int d1_kv4_append(const d1_half* K, const d1_half* V, int ldkv, const D1Kv4Seq* seqs, int n_seqs,
                              int max_rows, int kv_heads, cudaStream_t st) {
     if (n_seqs <= 0) return n_seqs == 0 ? 0 : -1;
-    if (!seqs || ((uintptr_t)seqs & 7) || max_rows < 0 || kv_heads <= 0 || kv_heads > 4096 || bad_rows(K, V, ldkv, kv_heads)) return -1;
+    if (!seqs || ((uintptr_t)seqs & 7) || max_rows < 0 || kv_heads <= 0 || kv_heads > 4096 || bad_rows(K, V, ldkv, kv_heads))
+        return -1;
+    const int sms = sm_count();
+    if (!sms) return -1;
     const dim3 g4 = row_grid(max_rows, 4 * A_ROWS, kv_heads, n_seqs);
-    if ((long long)g4.x * g4.y * g4.z >= 2 * 148)
+    if ((long long)g4.x * g4.y * g4.z >= 2 * sms)
         launch_pdl(k_kv4_append<4>, g4, 256, 0, st, K, V, ldkv, seqs, n_seqs);
     else
         launch_pdl(k_kv4_append<1>, row_grid(max_rows, A_ROWS, kv_heads, n_seqs), 256, 0, st, K, V, ldkv, seqs, n_seqs);
@@ -396,7 +399,8 @@ extern "C" int d1_kv4_append(const d1_half* K, const d1_half* V, int ldkv, const
 extern "C" int d1_kv4_load(const D1Kv4Seq* seqs, int n_seqs, int max_rows, int kv_heads, d1_half* K, d1_half* V,
                            int ldkv, cudaStream_t st) {
     if (n_seqs <= 0) return n_seqs == 0 ? 0 : -1;
-    if (!seqs || ((uintptr_t)seqs & 7) || max_rows < 0 || kv_heads <= 0 || kv_heads > 4096 || bad_rows(K, V, ldkv, kv_heads)) return -1;
+    if (!seqs || ((uintptr_t)seqs & 7) || max_rows < 0 || kv_heads <= 0 || kv_heads > 4096 || bad_rows(K, V, ldkv, kv_heads))
+        return -1;
     launch_pdl(k_kv4_load<4>, row_grid(max_rows, 4 * A_STEP, kv_heads, n_seqs), 256, 0, st, seqs, n_seqs, K, V, ldkv);
     return (int)cudaGetLastError();
 }
@@ -404,6 +408,8 @@ extern "C" int d1_kv4_load(const D1Kv4Seq* seqs, int n_seqs, int max_rows, int k
 extern "C" int d1_kv4_evict(const D1Kv4Evict* items, int n_items, int max_len, int kv_heads, cudaStream_t st) {
     if (n_items <= 0) return n_items == 0 ? 0 : -1;
     if (!items || ((uintptr_t)items & 7) || kv_heads <= 0 || kv_heads > 4096 || max_len < 0) return -1;
+    const int sms = sm_count();
+    if (!sms) return -1;
     static unsigned long long done = 0;  // the shared-memory opt-in is per device
     int dev = 0;
     cudaGetDevice(&dev);
@@ -415,7 +421,7 @@ extern "C" int d1_kv4_evict(const D1Kv4Evict* items, int n_items, int max_len, i
     // parts to occupy the GPU, at most 8 (each finds the threshold again), of no less than 64 rows were every key kept
     const int z = n_items < kMaxGridZ ? n_items : kMaxGridZ;
     const long long heads = (long long)kv_heads * z, most = max_len > 448 ? 8 : (max_len + 63) / 64;
-    long long parts = E_PER_SM * 148 / heads;
+    long long parts = E_PER_SM * sms / heads;
     parts = parts > most ? most : parts;
     launch_pdl(k_kv4_evict, dim3(parts < 1 ? 1 : (unsigned)parts, kv_heads, z), E_THREADS, E_SMEM, st, items, n_items);
     return (int)cudaGetLastError();

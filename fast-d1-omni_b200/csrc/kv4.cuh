@@ -13,6 +13,16 @@ constexpr int kKv4MaxRows = 1 << 30;  // of a cache: row counters that step by a
 // Device address of the error word on the current device, or NULL.
 int* kv4_err_addr();
 
+// SMs of the current device, or 0.
+inline int sm_count() {
+    static int sms[64] = {};
+    int dev = 0;
+    cudaGetDevice(&dev);
+    if (!sms[dev & 63] && cudaDeviceGetAttribute(&sms[dev & 63], cudaDevAttrMultiProcessorCount, dev) != cudaSuccess)
+        return 0;
+    return sms[dev & 63];
+}
+
 __device__ __forceinline__ bool kv4_cache_ok(int len, int cap, const void* k4, const void* v4, const void* kp,
                                              const void* vp) {
     if (len < 0 || len > cap || cap > kKv4MaxRows || (cap & 7)) return false;

@@ -1871,15 +1871,6 @@ bool smem_opt_in(F* kernel, int bytes, unsigned long long* done) {
     return true;
 }
 
-int sm_count() {
-    static int sms[64] = {};
-    int dev = 0;
-    cudaGetDevice(&dev);
-    if (!sms[dev & 63] && cudaDeviceGetAttribute(&sms[dev & 63], cudaDevAttrMultiProcessorCount, dev) != cudaSuccess)
-        return 0;
-    return sms[dev & 63];
-}
-
 // How many clusters of `ranks` CTAs (1, 2, 4 or 8) of a kernel the GPU holds at once: the GPCs' sizes decide (of 8 CTAs, one
 // to an SM, fewer than 148 / 8). Found on the first call for a device and kept in `found`, the kernel's own.
 template <typename F>
@@ -1958,7 +1949,9 @@ int launch_rows(Kv4Args& a, int max_q, int max_keys, int kv_heads, cudaStream_t 
     // sequences of 8 rows, 4096 keys, 2 CTAs to an SM: 24 us with 2, 33 with 1, 31 with 4 and 46 with 8; one token over
     // 4097 keys, 4 warps to a CTA: 8.5 us with 8, 11, 17 and 27 with 4, 2 and 1)
     int ranks = R_CLUSTER;
-    const long long tiles = ((long long)max_keys + R_KEYS - 1) / R_KEYS, slots = 148 * (NT == 1 ? 4 : 2);
+    const int sms = sm_count();
+    if (!sms) return -1;
+    const long long tiles = ((long long)max_keys + R_KEYS - 1) / R_KEYS, slots = sms * (NT == 1 ? 4 : 2);
     const long long ctas = x * kv_heads * z;
     while (ranks > 1 && ((ranks / 2) * 4 >= tiles || ctas * ranks > slots)) ranks /= 2;
     // where they leave more than a quarter of the room empty and the keys are long, twice as many, the rest of them as room
@@ -2132,7 +2125,8 @@ extern "C" int d1_kv4_mass(const d1_half* Q, int ldq, const float* lse, int lse_
     // 20 us and 17 on mma.sync, 17 and 19 where they share 4 caches; 96 rows 19 and 19, 16 and 22; 192 rows 21 and 32, 21
     // and 38
     if ((long long)max_q * group > 64 && group <= MQ && q_rows > 0 && n_seqs <= M_SEQS) return launch_mass_tc(a, max_q, max_len, st);
-    const int z = n_seqs < 65535 ? n_seqs : 65535, kv_heads = heads / group;
+    const int z = n_seqs < 65535 ? n_seqs : 65535, kv_heads = heads / group, sms = sm_count();
+    if (!sms) return -1;
     auto blocks = [&](int keys) {
         const long long x = ((long long)max_len + keys - 1) / keys;
         return (unsigned)(x < 1 ? 1 : x > 65536 ? 65536 : x);
@@ -2140,7 +2134,7 @@ extern "C" int d1_kv4_mass(const d1_half* Q, int ldq, const float* lse, int lse_
     // 32 keys to a warp up to about two waves of CTAs, then 64, whose expansion the rows share out better (8 rows, one cache
     // of 8000 keys: 4.3 us and 5.0 with 64; 16 caches of 1200: 9.7 and 10.2; 16 of 8000: 43 and 33; 24 rows, 16 sequences
     // on 4 caches of 1200: 14 and 22)
-    if ((long long)blocks(256) * kv_heads * z <= 5 * 148)
+    if ((long long)blocks(256) * kv_heads * z <= 5 * sms)
         launch_pdl(k_kv4_mass_rows<2>, dim3(blocks(256), kv_heads, z), 256, 0, st, a);
     else
         launch_pdl(k_kv4_mass_rows<4>, dim3(blocks(512), kv_heads, z), 256, 0, st, a);
