@@ -1446,7 +1446,10 @@ enum : int {
     MB_KFULL = 0,                    // [2] the unit's keys
     MB_KEMPTY = MB_KFULL + 2,        // [2]
     MB_QFULL = MB_KEMPTY + 2,        // [stage]
-    MB_QEMPTY = MB_QFULL + M_STAGES, // [stage]: read by the MMA (1), and its lse by 16 warps
+    // [stage] the tile has been read: its lse by 16 warps, which wait for S, and so for the MMA, before they arrive. (A
+    // loader looks at every third tile's phase only. As the warps arrive tile after tile, the phase of the stage's use
+    // before is then over, and the parity that it waits on is not that one's.)
+    MB_QEMPTY = MB_QFULL + M_STAGES,
     MB_SFULL = MB_QEMPTY + M_STAGES, // [buffer] S of a tile is in TMEM
     MB_SFREE = MB_SFULL + 2,         // [buffer] (16 warps)
     MB_SUM = MB_SFREE + 2,           // [2] the other warpgroups' sums are in shared memory (12 warps)
@@ -1598,7 +1601,7 @@ __global__ void __launch_bounds__(M_THREADS, 1) k_kv4_mass_tc(const __grid_const
         }
         for (int i = 0; i < M_STAGES; i++) {
             mbar_init(bar(MB_QFULL + i), 32);
-            mbar_init(bar(MB_QEMPTY + i), 1 + 4 * M_WGS);
+            mbar_init(bar(MB_QEMPTY + i), 4 * M_WGS);
         }
         for (int i = 0; i < M_LOADERS; i++) mbar_init(bar(MB_LANDED + i), 1);
         mbar_init(bar(MB_DRAIN), 1);
@@ -1758,7 +1761,6 @@ __global__ void __launch_bounds__(M_THREADS, 1) k_kv4_mass_tc(const __grid_const
                     for (int k = 0; k < 4; k++)
                         tc_mma_f16(tmem + w * MQ, smem_desc_k128(k_addr + k * 32), smem_desc_k128(q_addr + k * 32), idesc, k != 0);
                     tc_commit(bar(MB_SFULL + w));
-                    tc_commit(bar(MB_QEMPTY + st));
                 }
                 __syncwarp();
             }
