@@ -388,8 +388,8 @@ static_assert(sizeof(D1Kv4Evict) == 112 && offsetof(D1Kv4Evict, k4) == 24, "D1Kv
 
 /* extension — stores the own rows of every sequence behind its cached ones: rows kv_start .. kv_start + kv_len - 1 of
  * K and V (fp16, kv_heads * 64 columns, row pitch ldkv) at cache rows ext_len .. ext_len + kv_len - 1, which must fit
- * ext_cap. The caller then counts them in ext_len. max_rows: the longest kv_len, by which the grid is chosen (results
- * do not depend on it). K, V 16-byte aligned, ldkv a multiple of 8. */
+ * ext_cap. The caller then counts them in ext_len, and sets their mass to 0 before d1_kv4_mass adds to it. max_rows: the
+ * longest kv_len, by which the grid is chosen (results do not depend on it). K, V 16-byte aligned, ldkv a multiple of 8. */
 int d1_kv4_append(const d1_half* K, const d1_half* V, int ldkv, const D1Kv4Seq* seqs, int n_seqs, int max_rows,
                   int kv_heads, cudaStream_t stream);
 

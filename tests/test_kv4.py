@@ -980,6 +980,62 @@ def test_heads_beyond_32_bits_are_refused(pkg, gpu_lib, heads, group):
     assert gpu_lib.d1_kv4_error() == 0
 
 
+@gpu
+@pytest.mark.parametrize("max_q", HINTS)
+def test_server_loop(pkg, gpu_lib, max_q):
+    """A bounded cache over three steps: append, the new keys' weights set to 0 by the caller, attention, weights added up
+    over the steps, eviction into the other cache."""
+    rng = np.random.default_rng(32)
+    kvh, group, keep, lib = 2, 2, 64, gpu_lib
+    h, n, lens, rows = kvh * group, 2, [150, 0], [40, 70]
+    a, b = Caches(rng, lens, kvh, 240), Caches(rng, [0, 0], kvh, 240)
+    a.mass[:] = float("nan")
+    for i, m in enumerate(lens):
+        a.mass[i, :, :m] = 0
+    sums, tols = np.zeros((n, kvh, 240)), np.zeros((n, kvh, 240))
+    for step in range(3):
+        x, starts = poisoned_rows(rng, rows, (h + 2 * kvh) * 64)
+        d, T = torch.from_numpy(x).cuda(), len(x)
+        k, v, ld = d[:, h * 64:].data_ptr(), d[:, (h + kvh) * 64:].data_ptr(), x.shape[1]
+        seqs = [dict(q_start=s, q_len=m, kv_start=s, kv_len=m) for s, m in zip(starts, rows)]
+        assert lib.d1_kv4_append(k, v, ld, P(table(pkg, seqs, a, range(n))), n, max(rows), kvh, ST()) == 0
+        for i in range(n):
+            a.mass[i, :, a.lens[i]:a.lens[i] + rows[i]] = 0
+        a.lens, a.host = [p + q for p, q in zip(a.lens, rows)], a.back()
+        tab = table(pkg, [dict(s, kv_len=0) for s in seqs], a, range(n), mass=True)
+        O, L = torch.zeros(T, h * 64, dtype=torch.float16, device="cuda"), torch.zeros(h, T, device="cuda")
+        assert lib.d1_flash_attn_kv4(P(d), ld, None, None, 0, P(O), h * 64, P(L), T, P(tab), n, max_q, max(a.lens), h, group, 0.125,
+                                     T, 0, ST()) == 0
+        assert lib.d1_kv4_mass(P(d), ld, P(L), T, P(tab), n, max_q, max(a.lens), h, group, 0.125, 1, T, ST()) == 0
+        arr = (pkg.abi.Kv4Evict * n)()
+        for i, e in enumerate(arr):
+            e.len, e.cap, e.keep, e.recent, e.dst_cap = a.lens[i], a.cap, keep, 8, b.cap
+            e.mass, e.dst_mass = a.mass[i].data_ptr(), b.mass[i].data_ptr()
+            for f in a.dev:
+                setattr(e, f, a.dev[f][i].data_ptr())
+                setattr(e, "dst_" + f, b.dev[f][i].data_ptr())
+        items = torch.frombuffer(bytearray(bytes(arr)), dtype=torch.uint8).cuda()
+        assert lib.d1_kv4_evict(P(items), n, max(a.lens), kvh, ST()) == 0 and lib.d1_kv4_error() == 0
+        own = [dict(s, kv_len=0) for s in seqs]
+        want = plain_attend(x, own, a, range(n), kvh, group, 0.125, True)
+        M, tol = plain_mass(x, L.cpu().numpy(), own, a, range(n), kvh, group, 0.125)
+        got, moved, back = a.mass.cpu().numpy(), b.mass.cpu().numpy(), b.back()
+        nsum, ntol = np.zeros_like(sums), np.zeros_like(tols)
+        for i, m in enumerate(a.lens):
+            r = slice(starts[i], starts[i] + rows[i])
+            assert (np.abs(O.double().cpu().numpy()[r] - want[0][r]) <= want[2][r]).all()
+            all_, t = sums[i, :, :m] + M[i, :, :m], tols[i, :, :m] + tol[i, :, :m]
+            t += 2.0 ** -24 * all_  # the addition
+            assert (np.abs(got[i, :, :m] - all_) <= t).all()
+            for g in range(kvh):
+                at = keep_set(got[i, g, :m], keep, 8)
+                assert (moved[i, g, :len(at)] == got[i, g, at]).all() and (back["k4"][i, g, :len(at)] == a.host["k4"][i, g, at]).all()
+                nsum[i, g, :len(at)], ntol[i, g, :len(at)] = all_[g, at], t[g, at]
+        sums, tols = nsum, ntol
+        b.lens = [min(keep, m) for m in a.lens]
+        a, b = b, a
+
+
 # ------------------------------------------------------------------------------------------------ units after units
 # (queries, cached keys, own rows, kv heads, group): more units than CTAs, so that a CTA goes from one to the next
 UNITS = {
