@@ -21,7 +21,8 @@ constexpr int kMaxGridZ = 65535;
 __device__ __forceinline__ void table_error() { atomicExch(&g_kv4_err, kErrTable); }
 
 // ------------------------------------------------------------------------------------------------ append, load
-// Bound by HBM, append in a small call by issue slots as well. Append: 4 lanes per vector of 64 dimensions (twice 8
+// Bound by HBM; append as much by the wait for its rows and by issue slots (0.66 of them while the SMs are busy, 8 ragged
+// caches of up to 4096 rows: 14 us, and 10.5 at the copy rate). Append: 4 lanes per vector of 64 dimensions (twice 8
 // elements, two words of codes a lane; the parameter's arithmetic, which every lane does, was a third of it with 8 lanes: 78
 // us), 8 consecutive rows of one kv head per warp; a CTA takes 64 rows of (K or V, kv head) for each of PER to a thread,
 // whose loads go out together: 4 where that still occupies every SM twice, otherwise 1 (32 x 4096 rows, 8 kv heads: 62 us
@@ -34,11 +35,12 @@ __device__ __forceinline__ bool append_ok(const D1Kv4Seq& s) {
            (long long)s.ext_len + s.kv_len <= s.ext_cap;
 }
 
-// Words of codes of one vector (this lane's twice 8 elements of it; four lanes a vector) and its parameter. round(x / step) without a division per element:
-// t = x * (1 / step) is within 2^-18 of the quotient q, |q| < 15.6. As x has 11 significant bits and step 7, q either is
-// k + 1/2 exactly or at least 2^-13 away from it; 768 + t, whose last place is 2^-14, is therefore 768 + k + 1/2 in the
-// first case and on q's side of it in the second, and rounds as q does. (hi - lo) / 15 is rounded correctly, since whole
-// multiples of 15 are common: one step of correction after the product with 1 / 15.
+// Words of codes of one vector (this lane's twice 8 elements of it; four lanes a vector) and its parameter.
+// round(x / step) without a division per element: t = x * (1 / step) is within 2^-18 of the quotient q, |q| < 15.6. As x
+// has 11 significant bits and step 7, q either is k + 1/2 exactly or at least 2^-13 away from it; 768 + t, whose last place
+// is 2^-14, is therefore 768 + k + 1/2 in the first case and on q's side of it in the second, and rounds as q does.
+// (hi - lo) / 15 is rounded correctly, since whole multiples of 15 are common: one step of correction after the product
+// with 1 / 15.
 __device__ __forceinline__ void quantise16(const uint4 (&raw)[2], uint32_t (&word)[2], uint32_t& par) {
     const __half2* x2 = reinterpret_cast<const __half2*>(raw);
     __half2 mn = __float2half2_rn(0.f), mx = mn;  // the range, with zero in it; NaN stays

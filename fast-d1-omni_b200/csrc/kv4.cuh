@@ -65,6 +65,8 @@ __device__ __forceinline__ void kv4_zero(uint32_t par2, uint32_t& z0, uint32_t& 
 __device__ __forceinline__ uint32_t kv4_step2(uint32_t par2) { return par2 & 0xfff0fff0u; }
 __device__ __forceinline__ float kv4_step(uint32_t par) { return __half2float(__ushort_as_half(par & 0xfff0u)); }
 
+// The expansion of 4-bit weights by or-ing codes into the mantissa of 1024 (Kim et al., "Who Says Elephants Can't Run:
+// Bringing Large Scale MoE Models into Cloud Scale Production", 2022), here with 64 for the upper nibbles.
 // A word's eight codes as fp16 pairs of (code - zero): out[i] holds the codes at bits 4i (low half) and 16 + 4i (high
 // half). A code at bits 0-3 of a half, or-ed into the fp16 pattern of 1024, is 1024 + code; at bits 4-7, into that of
 // 64, it is 64 + code; the differences are whole numbers in -15 .. 15, exact. One shift for the upper two codes.

@@ -73,9 +73,12 @@ __device__ __forceinline__ void ex2_fma2(float x0, float x1, float& p0, float& p
 // the values are (code - zero) * step, exact in fp16. Row r of the j-th m tile is dimension 8r + 2j, row r + 8 dimension
 // 8r + 2j + 1, so that a lane ends with dimensions 8r .. 8r+7 of packed rows 2t and 2t + 1. P^T turns from the result's
 // layout into the B operand's by movmatrix.
-// Bound: the issue slots (about 800 instructions a tile, half of them for the expansion of codes). Tried and dropped: the
-// codes as fp16 subnormals (code * 2^-24 or * 2^-20, no subtraction), with zeros and steps taken care of by the sums: an
-// eighth fewer instructions, but the MMA aligns its fp32 sums to the operands' exponent, and their last 10 bits are lost.
+// Bound: latency, and unequal sequences. 32 tokens over 8346 to 16151 keys, 89 us: the SMs are busy for 0.81 of the time and
+// issue in 0.52 of those cycles (about 800 instructions a tile, half of them for the expansion of codes), 16 warps an SM
+// waiting for each other's results and for memory. Of 9 to 64 packed rows the time is about five times that of the bytes
+// (16 x 32 packed rows over 8000 keys: 55 us). Tried and dropped: the codes as fp16 subnormals (code * 2^-24 or * 2^-20, no
+// subtraction), with zeros and steps taken care of by the sums: an eighth fewer instructions, but the MMA aligns its fp32
+// sums to the operands' exponent, and their last 10 bits are lost.
 constexpr int R_KEYS = 64, R_CLUSTER = 8, R_LD = 68;  // padded row of the joining buffers (floats)
 
 template <int NT, int W>
@@ -272,8 +275,9 @@ __global__ void __launch_bounds__(W * 32, (NT == 1 ? 16 : 8) / W) k_kv4_attn_row
                 }
                 // ---- running softmax, in the exp2 domain. The scores are taken against the reference m as it was before
                 // this tile; only where one exceeds it by more than 2^8 (and in the first tile) does m move, and what was
-                // summed so far is rescaled: P stays below 2^8, well inside fp16. P^T as B operands: keys 16i + 2t,
-                // 16i + 2t + 1 and 8 above
+                // summed so far is rescaled: P stays below 2^8, well inside fp16, to which it is rounded for the product with
+                // V, as in the fp16 attention; the row's sum is of P in fp32 (O is 2.4e-4 to 2.9e-4 off, and 2.1e-4 by its own
+                // rounding alone). P^T as B operands: keys 16i + 2t, 16i + 2t + 1 and 8 above
                 uint32_t pb[NT][4][2];
 #pragma unroll
                 for (int nt = 0; nt < NT; nt++) {
@@ -470,7 +474,7 @@ __global__ void __launch_bounds__(W * 32, (NT == 1 ? 16 : 8) / W) k_kv4_attn_row
 //   9, 14      MMA issuers of warpgroups 0 and 1, one thread each: S = Q K^T (both in shared memory), O += P V (P in
 //              TMEM). Warp 9 also keeps the TMEM. (One issuer for both: each warpgroup then waits for the other's P.)
 // The softmax warps take 200 registers, the others 56 (four documents of 2048 rows over 4096 keys: 253.5 us; 256.7 with
-// 192 and 64, 254 with 208 and 48, 272 with 184 and 72; 251.5 now).
+// 192 and 64, 254 with 208 and 48, 272 with 184 and 72; 252.5 now).
 // TMEM (512 columns), warpgroup w at 256 w: S in 128 columns, P in 64, O in 64. Both warpgroups' columns share the lanes,
 // so that a packed unit is joined by each reading the other's O.
 constexpr int TQ = 128, TKV = 128, T_QSLOTS = 2, T_STAGES = 4, T_RAW_STAGES = 3, T_EXPANDERS = 128, T_THREADS = 512;
@@ -1078,8 +1082,9 @@ __global__ void __launch_bounds__(T_THREADS, 1)
                         tmem_st8(tO + o8 * 8, o);
                     }
                 }
-                // P = 2^(s * scale - m), two scores at a time, and the row's sum in fp32; nothing for the upper half of a tile
-                // without keys there (26 x 176 rows over 7 keys 18.4 -> 17.5 us; in quarters 17.3, but documents 252 -> 256).
+                // P = 2^(s * scale - m), two scores at a time, and the row's sum in fp32. For the MMA, whose operands have 16
+                // bits, P is rounded to fp16 (O is 2.9e-4 off, and 2.1e-4 by its own rounding alone). Nothing for the upper
+                // half of a tile without keys there (26 x 176 rows over 7 keys 18.4 -> 17.5 us; in quarters 17.3, but documents 252 -> 256).
                 // (An eighth of the exponentials on the FMA pipe: documents 258 -> 253 us with a polynomial of degree 3, whose
                 // 7.5e-5 showed in the log-sum-exp; 259 with degree 5.)
                 const uint64_t sc2 = f2_pack(a.scale_log2, a.scale_log2), nm2 = f2_pack(-m_use, -m_use);
@@ -1432,7 +1437,7 @@ __global__ void __launch_bounds__(256, 2) k_kv4_mass_rows(const Kv4Args a) {
 //   0-15       four warpgroups share every tile (two of its eight 32-column pieces each): S from TMEM, where the next
 //              tile's S is computed meanwhile, exp2(s * scale - lse), summed in fp32; one pair of exponentials in eight on
 //              the FMA pipe. At the unit's end three pass their sums to the first through shared memory. (Two documents of
-//              2048 rows over 8192 keys: 77 us. Compared while it took 91: 98 with two warpgroups and the next piece's
+//              2048 rows over 8192 keys: 78 us. Compared while it took 91: 98 with two warpgroups and the next piece's
 //              load on its way, 97 with both pieces loaded at once, 93 without the FMA pipe, 94 and 99 with a quarter and
 //              three eighths there)
 //   16, 18, 19 loaders: the keys' codes, expanded; query tiles by TMA from a view of [row][head][64], always whole; the

@@ -416,8 +416,9 @@ int d1_flash_attn_kv4(const d1_half* Q, int ldq, const d1_half* K, const d1_half
  * with lse as d1_flash_attn_kv4 gave it (-inf: the row adds nothing, whatever its Q holds). accumulate = 0 overwrites
  * mass[g][0 .. ext_len-1], 1 adds to it. Sequences with the same `mass` must share their cache (one that does not share
  * that of the first of them whose cache is in order is refused); their weights are added up in the table's order, always
- * in the same order for the same call. max_q, max_len: the longest q_len and ext_len
- * (see above). */
+ * in the same order for the same call. Above 256 sequences a call uses the kernel for few rows however many there
+ * are, which takes 1.5 times as long and more from q_len * group = 192 on: split such a call, with accumulate = 1
+ * where a part adds to a mass array of the one before. max_q, max_len: the longest q_len and ext_len (see above). */
 int d1_kv4_mass(const d1_half* Q, int ldq, const float* lse, int lse_ld, const D1Kv4Seq* seqs, int n_seqs, int max_q,
                 int max_len, int heads, int group, float scale, int accumulate, int q_rows, cudaStream_t stream);
 
