@@ -1084,7 +1084,8 @@ __global__ void __launch_bounds__(T_THREADS, 1)
                 }
                 // P = 2^(s * scale - m), two scores at a time, and the row's sum in fp32. For the MMA, whose operands have 16
                 // bits, P is rounded to fp16 (O is 2.9e-4 off, and 2.1e-4 by its own rounding alone). Nothing for the upper
-                // half of a tile without keys there (26 x 176 rows over 7 keys 18.4 -> 17.5 us; in quarters 17.3, but documents 252 -> 256).
+                // half of a tile without keys there (26 x 176 rows over 7 keys 18.4 -> 17.5 us; in quarters 17.3, but
+                // documents 252 -> 256).
                 // (An eighth of the exponentials on the FMA pipe: documents 258 -> 253 us with a polynomial of degree 3, whose
                 // 7.5e-5 showed in the log-sum-exp; 259 with degree 5.)
                 const uint64_t sc2 = f2_pack(a.scale_log2, a.scale_log2), nm2 = f2_pack(-m_use, -m_use);
@@ -1279,8 +1280,8 @@ __global__ void __launch_bounds__(T_THREADS, 1)
 // ------------------------------------------------------------------------------------------------ mass, few rows
 // S^T = K Q^T on m16n8k16: a warp holds 16 * MT keys as A operands (whole numbers code - zero, as above) and goes over the
 // packed query rows 8 at a time, adding exp(s - lse) into its keys' sums; four lanes share a key at the end. The sequences
-// that share a mass array are taken by the first of them whose cache is in order, in the table's order. What bounds it are latencies: of the table,
-// of the codes (both at once where the table has 256 entries at most), and of 8 rows after 8 rows.
+// that share a mass array are taken by the first of them whose cache is in order, in the table's order. What bounds it are
+// latencies: of the table, of the codes (both at once where the table has 256 entries at most), and of 8 rows after 8 rows.
 template <int MT>
 __global__ void __launch_bounds__(256, 2) k_kv4_mass_rows(const Kv4Args a) {
     constexpr int KEYS = 16 * MT * 8;   // of a CTA of 8 warps
